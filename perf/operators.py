@@ -204,7 +204,7 @@ def prepare(case, seed):
             down, down_scales = _weights(gen, H, I)
             state.layers.append({"stream": _rows(gen, M, H, case["type"]), "gu": gu, "gu_scales": gu_scales, "down": down, "down_scales": down_scales,
                                  "weight": _channel(gen, H), "after": _channel(gen, H) if case["after"] else None, "gate": _gate(gen, case, H),
-                                 "stream_out": empty((M, H), _TYPES[case["type"]])})
+                                 "branch": empty((M, H), torch.float32), "stream_out": empty((M, H), _TYPES[case["type"]])})
     torch.cuda.synchronize()
     if own:
         _hold(state)
@@ -282,7 +282,7 @@ def _run_block(case, layer):
         return _residual(stream, branch, layer["after"], layer["gate"]).to(_TYPES[case["type"]])
     from rknpu2_matmul_open_amd import ops
     ops.mx4_ffn_block(layer["gu_ws"], layer["gu_w"], layer["down_ws"], layer["down_w"], layer["stream"], weight=layer["weight"], after=layer["after"],
-                      gate=layer["gate"], residual_scale=_SCALE, branch_scale=1.0, eps=_EPS, stream_out=layer["stream_out"])
+                      gate=layer["gate"], residual_scale=_SCALE, branch_scale=1.0, eps=_EPS, branch=layer["branch"], stream_out=layer["stream_out"])
     return layer["stream_out"]
 
 
