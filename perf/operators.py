@@ -16,6 +16,7 @@ from memory and not from a cache that the previous call filled.
 
 In the plain form a product's weights are decoded in the call: the codes and scales are what a program holds.
 """
+import ctypes
 import math
 
 import torch
@@ -25,6 +26,7 @@ own = False
 _TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 _SIZE = {"f32": 4, "f16": 2, "bf16": 2}
 _EPS = 1e-6
+_SCALE = 0.75  # of the residual stream
 
 # The largest drawn case costs what the largest listed one does.
 _MOST_PRODUCTS = 4096 * 4096 * 14336
@@ -211,84 +213,77 @@ def prepare(case, seed):
     return state
 
 
+def _address(x):
+    return ctypes.c_void_p(x.data_ptr() if x is not None else None)
+
+
 def _hold(state):
-    """The handles that a program keeps: weights of each layer, one workspace for all that have the same shape."""
-    from rknpu2_matmul_open_amd import ops
-    s, case = _session(), state.case
-    if case["kind"] == "linear":
-        ws = ops.MX4Workspace(s, case["M"], case["K"], case["N"])
-        state.handles.append(ws)
+    """What a program keeps: handles (weights of each layer, one workspace for all layers of a shape) and its calls' arguments."""
+    from rknpu2_matmul_open_amd import capi, ops
+    s, case, M = _session(), state.case, state.case["M"]
+    lib, kind = s.lib, {"f32": capi.MX4_F32, "f16": capi.MX4_F16, "bf16": capi.MX4_BF16}
+
+    def held(handle):
+        state.handles.append(handle)
+        return handle
+
+    if case["kind"] == "quant":
+        K = case["K"]
         for layer in state.layers:
-            layer["w"] = ops.MX4Weights.from_device(s, case["K"], case["N"], layer["codes"].data_ptr(), layer["scales"].data_ptr())
-            layer["ws"] = ws
-            state.handles.append(layer["w"])
-    elif case["kind"] == "block":
-        M, H, I = case["M"], case["H"], case["I"]
-        gu_ws, down_ws = ops.MX4Workspace(s, M, H, 2 * I), ops.MX4Workspace(s, M, I, H)
-        state.handles += [gu_ws, down_ws]
+            x, codes, scales, values = (_address(layer[k]) for k in ("x", "codes", "scales", "values"))
+            layer["calls"] = [(lib.rk_npu_mx4_quantize_device, (s.ctx, kind[case["type"]], M, K, x, K, codes, scales)),
+                              (lib.rk_npu_mx4_dequantize_device, (s.ctx, capi.MX4_F32, M, K, codes, scales, values, K))]
+    elif case["kind"] == "linear":
+        K, N = case["K"], case["N"]
+        ws = held(ops.MX4Workspace(s, M, K, N))
         for layer in state.layers:
-            layer["gu_w"] = ops.MX4Weights.from_device(s, H, 2 * I, layer["gu"].data_ptr(), layer["gu_scales"].data_ptr(), gate_up=True)
-            layer["down_w"] = ops.MX4Weights.from_device(s, I, H, layer["down"].data_ptr(), layer["down_scales"].data_ptr())
-            layer["gu_ws"], layer["down_ws"] = gu_ws, down_ws
-            state.handles += [layer["gu_w"], layer["down_w"]]
+            w = held(ops.MX4Weights.from_device(s, K, N, layer["codes"].data_ptr(), layer["scales"].data_ptr()))
+            layer["calls"] = [(lib.rk_npu_mx4_run_device, (ws.h, w.h, M, kind[case["type"]], _address(layer["x"]), K, kind[case["out"]],
+                                                           _address(layer["y"]), N))]
+    else:
+        D = case["D"] if case["kind"] == "norm" else case["H"]
+        if case["kind"] == "block":
+            gu_ws, down_ws = held(ops.MX4Workspace(s, M, D, 2 * case["I"])), held(ops.MX4Workspace(s, M, case["I"], D))
+        for layer in state.layers:
+            a = layer["args"] = capi.BlockNormArgs()
+            lib.rk_npu_block_norm_args_init(ctypes.byref(a), M, D)
+            a.eps, a.residual_scale = _EPS, _SCALE
+            a.residual_type = kind[case["stream"] if case["kind"] == "norm" else case["type"]]
+            a.gate_type = kind[case["type"]]
+            a.residual_ld = a.branch_ld = a.residual_out_ld = D
+            a.gate_ld = D if case["gate"] == "full" else 0
+            a.residual, a.gate, a.residual_out = _address(layer["stream"]), _address(layer["gate"]), _address(layer["stream_out"])
+            a.weight, a.branch_weight = _address(layer["weight"]), _address(layer["after"])
+            if case["kind"] == "norm":
+                a.branch_type = a.y_type = kind[case["type"]]
+                a.branch, a.y, a.y_ld = _address(layer["branch"]), _address(layer["y"]), D
+                layer["calls"] = [(lib.rk_npu_block_norm_device, (s.ctx, ctypes.byref(a)))]
+            else:
+                a.branch_type = capi.MX4_F32
+                gu = held(ops.MX4Weights.from_device(s, D, 2 * case["I"], layer["gu"].data_ptr(), layer["gu_scales"].data_ptr(), gate_up=True))
+                down = held(ops.MX4Weights.from_device(s, case["I"], D, layer["down"].data_ptr(), layer["down_scales"].data_ptr()))
+                layer["calls"] = [(lib.rk_npu_mx4_run_ffn_block_device, (gu_ws.h, gu.h, down_ws.h, down.h, ctypes.byref(a), _address(layer["branch"]), None))]
 
 
 # ---- one pass ------------------------------------------------------------------------------
 
 
 def run(state):
-    case = state.case
-    return [{"quant": _run_quant, "linear": _run_linear, "norm": _run_norm, "block": _run_block}[case["kind"]](case, layer) for layer in state.layers]
+    return [_run_layer(state.case, layer) for layer in state.layers]
 
 
-def _run_quant(case, layer):
-    if not own:
-        codes, scales = _encode(layer["x"])
-        return {"scales": scales, "values": _decode(codes, scales, case["K"])}
-    from rknpu2_matmul_open_amd import ops
-    s = _session()
-    ops.mx4_quantize(s, layer["x"], layer["codes"], layer["scales"])
-    ops.mx4_dequantize(s, layer["codes"], layer["scales"], layer["values"])
-    return {"scales": layer["scales"], "values": layer["values"]}
-
-
-def _run_linear(case, layer):
-    if not own:
-        x = _decode(*_encode(layer["x"]), case["K"])
-        return (x @ _decode(layer["codes"], layer["scales"], case["K"]).t()).to(_TYPES[case["out"]])
-    layer["ws"].run(layer["w"], layer["x"], layer["y"])
-    return layer["y"]
-
-
-def _run_norm(case, layer):
-    if not own:
-        r = _residual(layer["stream"].float(), layer["branch"].float(), layer["after"], layer["gate"])
-        return {"stream": r.to(_TYPES[case["stream"]]), "y": _rms(r, layer["weight"]).to(_TYPES[case["type"]])}
-    from rknpu2_matmul_open_amd import ops
-    ops.block_norm(_session(), layer["stream"], layer["branch"], after=layer["after"], gate=layer["gate"], residual_scale=_SCALE, branch_scale=1.0,
-                   weight=layer["weight"], eps=_EPS, stream_out=layer["stream_out"], y=layer["y"])
-    return {"stream": layer["stream_out"], "y": layer["y"]}
-
-
-def _run_block(case, layer):
-    if not own:
-        H, I = case["H"], case["I"]
-        stream = layer["stream"].float()
-        x = _decode(*_encode(_rms(stream, layer["weight"])), H)
-        both = x @ _decode(layer["gu"], layer["gu_scales"], H).t()
-        gate, up = both[:, :I], both[:, I:]
-        middle = _decode(*_encode(gate / (1 + torch.exp(-gate)) * up), I)
-        branch = (middle @ _decode(layer["down"], layer["down_scales"], I).t())
-        return _residual(stream, branch, layer["after"], layer["gate"]).to(_TYPES[case["type"]])
-    from rknpu2_matmul_open_amd import ops
-    ops.mx4_ffn_block(layer["gu_ws"], layer["gu_w"], layer["down_ws"], layer["down_w"], layer["stream"], weight=layer["weight"], after=layer["after"],
-                      gate=layer["gate"], residual_scale=_SCALE, branch_scale=1.0, eps=_EPS, branch=layer["branch"], stream_out=layer["stream_out"])
-    return layer["stream_out"]
+def _run_layer(case, layer):
+    if own:
+        for call, args in layer["calls"]:
+            if call(*args):
+                raise RuntimeError("%s failed" % call.__name__)
+        return {"quant": lambda: {"scales": layer["scales"], "values": layer["values"]}, "linear": lambda: layer["y"],
+                "norm": lambda: {"stream": layer["stream_out"], "y": layer["y"]}, "block": lambda: layer["stream_out"]}[case["kind"]]()
+    return {"quant": _plain_quant, "linear": _plain_linear, "norm": _plain_norm, "block": _plain_block}[case["kind"]](case, layer)
 
 
 # ---- the plain forms -----------------------------------------------------------------------
 
-_SCALE = 0.75  # of the residual stream
 _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
@@ -327,6 +322,32 @@ def _rms(x, weight):
 def _residual(stream, branch, after, gate):
     branch = branch if after is None else _rms(branch, after)
     return _SCALE * stream + (branch if gate is None else branch * gate.float())
+
+
+def _plain_quant(case, layer):
+    codes, scales = _encode(layer["x"])
+    return {"scales": scales, "values": _decode(codes, scales, case["K"])}
+
+
+def _plain_linear(case, layer):
+    x = _decode(*_encode(layer["x"]), case["K"])
+    return (x @ _decode(layer["codes"], layer["scales"], case["K"]).t()).to(_TYPES[case["out"]])
+
+
+def _plain_norm(case, layer):
+    r = _residual(layer["stream"].float(), layer["branch"].float(), layer["after"], layer["gate"])
+    return {"stream": r.to(_TYPES[case["stream"]]), "y": _rms(r, layer["weight"]).to(_TYPES[case["type"]])}
+
+
+def _plain_block(case, layer):
+    H, I = case["H"], case["I"]
+    stream = layer["stream"].float()
+    x = _decode(*_encode(_rms(stream, layer["weight"])), H)
+    both = x @ _decode(layer["gu"], layer["gu_scales"], H).t()
+    gate, up = both[:, :I], both[:, I:]
+    middle = _decode(*_encode(gate / (1 + torch.exp(-gate)) * up), I)
+    branch = middle @ _decode(layer["down"], layer["down_scales"], I).t()
+    return _residual(stream, branch, layer["after"], layer["gate"]).to(_TYPES[case["type"]])
 
 
 # ---- the definitions in 64 bits, apart from the above --------------------------------------
