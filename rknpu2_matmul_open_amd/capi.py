@@ -393,6 +393,43 @@ _PROTOTYPES = {
 }
 
 EXPORTED_SYMBOLS = tuple(_PROTOTYPES)
+
+
+# rk_npu_mx4.h
+MX4_F32, MX4_F16, MX4_BF16 = 0, 1, 2
+
+
+class MX4WeightConfig(C.Structure):
+    _fields_ = [("K", C.c_int), ("N", C.c_int), ("gate_up", C.c_int)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rows", C.c_int), ("D", C.c_int), ("residual_type", C.c_int), ("branch_type", C.c_int),
+                ("gate_type", C.c_int), ("y_type", C.c_int), ("eps", C.c_float), ("residual_scale", C.c_float), ("branch_scale", C.c_float),
+                ("residual", P), ("branch", P), ("gate", P), ("branch_weight", P), ("weight", P), ("residual_out", P), ("y", P), ("staged", P),
+                ("residual_ld", C.c_int64), ("branch_ld", C.c_int64), ("gate_ld", C.c_int64), ("residual_out_ld", C.c_int64), ("y_ld", C.c_int64)]
+
+
+_MX4_PROTOTYPES = {
+    "rk_npu_mx4_quantize_device": (C.c_int, [P, C.c_int, C.c_int64, C.c_int, P, C.c_int64, P, P]),
+    "rk_npu_mx4_dequantize_device": (C.c_int, [P, C.c_int, C.c_int64, C.c_int, P, P, P, C.c_int64]),
+    "rk_npu_mx4_weights_create": (P, [P, C.POINTER(MX4WeightConfig), P, P]),
+    "rk_npu_mx4_weights_create_device": (P, [P, C.POINTER(MX4WeightConfig), P, P]),
+    "rk_npu_mx4_weights_free": (None, [P]),
+    "rk_npu_mx4_weights_query": (C.c_int, [P, C.POINTER(MX4WeightConfig), C.POINTER(C.c_uint64)]),
+    "rk_npu_mx4_workspace_create": (P, [P, C.c_int, C.c_int, C.c_int]),
+    "rk_npu_mx4_workspace_free": (None, [P]),
+    "rk_npu_mx4_run_device": (C.c_int, [P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P, C.c_int64]),
+    "rk_npu_mx4_stage_device": (C.c_int, [P, C.c_int, C.c_int, P, C.c_int64]),
+    "rk_npu_mx4_run_staged_device": (C.c_int, [P, P, C.c_int, P, C.c_int64]),
+    "rk_npu_mx4_run_swiglu_device": (C.c_int, [P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P, C.c_int64]),
+    "rk_npu_mx4_run_ffn_device": (C.c_int, [P, P, P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P, C.c_int64]),
+    "rk_npu_block_norm_args_init": (None, [C.POINTER(BlockNormArgs), C.c_int, C.c_int]),
+    "rk_npu_block_norm_device": (C.c_int, [P, C.POINTER(BlockNormArgs)]),
+    "rk_npu_mx4_run_ffn_block_device": (C.c_int, [P, P, P, P, C.POINTER(BlockNormArgs), P, P]),
+}
+
+MX4_SYMBOLS = tuple(_MX4_PROTOTYPES)
 _LIB = None
 
 
@@ -413,7 +450,7 @@ def load_library():
             "%s is missing: build it with `python -m rknpu2_matmul_open_amd.build` "
             "(there is no CPU fallback)" % path)
     lib = C.CDLL(path)
-    for name, (restype, argtypes) in _PROTOTYPES.items():
+    for name, (restype, argtypes) in {**_PROTOTYPES, **_MX4_PROTOTYPES}.items():
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes

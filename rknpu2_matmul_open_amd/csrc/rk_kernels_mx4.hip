@@ -1,0 +1,202 @@
+// MX4 rows: quantization, reading back, staging as operand blocks, and the packing of weights.
+// All of them are bound by memory; nothing is kept between values but a block's largest magnitude.
+#include "rk_kernels_mx4.h"
+
+namespace {
+
+// ---- MX4 rows from values --------------------------------------------------------
+// Four lanes per block, eight values each: a wave reads and writes whole lines whatever the type.  The rows' blocks are
+// counted through from `first`, so that short rows fill the workgroups, too.
+constexpr int QUANT_UNITS = 4; // blocks of a quad of lanes; their loads go out together
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int K, int64_t ldx) {
+    const int KB = (K + 31) / 32, part = threadIdx.x & 3;
+    const int64_t blocks = rows * KB, first = (int64_t)blockIdx.x * (64 * QUANT_UNITS);
+    const bool dense = ldx == K && K % 32 == 0; // values follow one another
+    const int64_t row0 = dense ? 0 : first / KB;
+    const unsigned rest = (unsigned)(first - row0 * KB);
+    MxRaw<TYPE> raw[QUANT_UNITS];
+    int64_t at[QUANT_UNITS];
+#pragma unroll
+    for (int u = 0; u < QUANT_UNITS; ++u) {
+        at[u] = first + u * 64 + (threadIdx.x >> 2);
+        if (at[u] >= blocks) continue;
+        if (dense) {
+            raw[u] = mx_fetch8<TYPE>(x, at[u] * 32 + part * 8);
+        } else {
+            const unsigned t = rest + u * 64 + (threadIdx.x >> 2), r = t / (unsigned)KB;
+            const int k = (int)(t - r * KB) * 32 + part * 8;
+            const size_t i = (row0 + r) * ldx + k;
+            raw[u] = k + 8 <= K ? mx_fetch8<TYPE>(x, i) : mx_fetch_some<TYPE>(x, i, K - k);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < QUANT_UNITS; ++u) {
+        if (at[u] >= blocks) continue; // (the four lanes of a block together)
+        float v[8];
+        mx_unpack<TYPE>(raw[u], v);
+        const uint32_t scale = mx_scale(mx_top_of_quad(mx_top(v)));
+        *reinterpret_cast<u32_any*>(codes + at[u] * 16 + part * 4) = mx_codes(v, scale);
+        if (part == 0) scales[at[u]] = (uint8_t)scale;
+    }
+}
+
+// ---- and back --------------------------------------------------------------------
+__device__ __forceinline__ float mx_value(uint32_t code) { // e2m1: sign, two bits of exponent, one of mantissa
+    const uint32_t e = (code >> 1) & 3, m = code & 1;
+    const float size = e ? __uint_as_float(((e + 126) << 23) | (m << 22)) : 0.5f * (float)m;
+    return code & 8 ? -size : size;
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, void* y, int64_t rows, int K, int64_t ldy) {
+    const int KB = (K + 31) / 32, part = threadIdx.x & 3;
+    const int64_t blocks = rows * KB, first = (int64_t)blockIdx.x * (64 * QUANT_UNITS);
+    const bool dense = ldy == K && K % 32 == 0;
+    const int64_t row0 = dense ? 0 : first / KB;
+    const unsigned rest = (unsigned)(first - row0 * KB);
+    uint32_t w[QUANT_UNITS], s[QUANT_UNITS];
+#pragma unroll
+    for (int u = 0; u < QUANT_UNITS; ++u) {
+        const int64_t at = first + u * 64 + (threadIdx.x >> 2);
+        if (at >= blocks) continue;
+        w[u] = *reinterpret_cast<const u32_any*>(codes + at * 16 + part * 4);
+        s[u] = scales[at];
+    }
+#pragma unroll
+    for (int u = 0; u < QUANT_UNITS; ++u) {
+        const int64_t at = first + u * 64 + (threadIdx.x >> 2);
+        if (at >= blocks) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = s[u] == 255u ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(mx_value((w[u] >> (4 * e)) & 15u), (int)s[u] - 127);
+        if (dense) {
+            mx_store<TYPE, 8>(y, at * 32 + part * 8, v);
+        } else {
+            const unsigned t = rest + u * 64 + (threadIdx.x >> 2), r = t / (unsigned)KB;
+            const int k = (int)(t - r * KB) * 32 + part * 8;
+            const size_t i = (row0 + r) * ldy + k;
+            if (k + 8 <= K) {
+                mx_store<TYPE, 8>(y, i, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k + e < K) mx_store1<TYPE>(y, i + e, v[e]);
+            }
+        }
+    }
+}
+
+// ---- operand blocks from values --------------------------------------------------
+// A wave makes one piece of 16 rows x 128 k: lane (r, q) takes the 32 values of a block, so that the largest is found without
+// an exchange and the piece is stored as it lies, 1 KiB in a row; four waves, the four pieces that share scale dwords.
+template <int TYPE>
+__global__ __launch_bounds__(256) void mx4_stage_kernel(const void* x, uint8_t* codes, uint8_t* scales, int rows, int K, int64_t ldx) {
+    __shared__ uint8_t lds_scales[256];
+    const int KS = (int)rkh_mx4_ks(K), K4 = (int)rkh_mx4_k4(K);
+    const int lane = lane_id(), wave = wave_id();
+    const int rb = blockIdx.x / K4, k4 = blockIdx.x - rb * K4, ks = k4 * 4 + wave;
+    const int m = rb * 16 + (lane & 15), k0 = ks * 128 + (lane >> 4) * 32;
+    MxRaw<TYPE> raw[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const int k = k0 + c * 8;
+        const size_t i = (size_t)m * ldx + k;
+        if (m < rows && k + 8 <= K) raw[c] = mx_fetch8<TYPE>(x, i);
+        else raw[c] = mx_fetch_some<TYPE>(x, i, m < rows ? K - k : 0);
+    }
+    float v[4][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        mx_unpack<TYPE>(raw[c], v[c]);
+        top = max(top, mx_top(v[c]));
+    }
+    const uint32_t scale = mx_scale(top);
+    v4i w;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) w[c] = (int)mx_codes(v[c], scale);
+    if (ks < KS) *reinterpret_cast<v4i*>(codes + ((size_t)rb * KS + ks) * 1024 + lane * 16) = w;
+    lds_scales[lane * 4 + wave] = (uint8_t)scale;
+    __syncthreads();
+    if (threadIdx.x < 64) reinterpret_cast<uint32_t*>(scales)[((size_t)rb * K4 + k4) * 64 + threadIdx.x] = reinterpret_cast<const uint32_t*>(lds_scales)[threadIdx.x];
+}
+
+// ---- weights ---------------------------------------------------------------------
+// One thread per 16 bytes of operand blocks, then per scale byte; places without a column, and blocks beyond K, are zero.
+__global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* codes, const uint8_t* scales, uint8_t* dst, uint8_t* dst_scales, int K, int N,
+                                                       int gate_up, size_t pieces, size_t bytes) {
+    const int KB = (K + 31) / 32, KS = (int)rkh_mx4_ks(K), K4 = (int)rkh_mx4_k4(K);
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < pieces) {
+        const size_t piece = i >> 6;
+        const int lane = (int)(i & 63), rb = (int)(piece / KS), b = (int)(piece - (size_t)rb * KS) * 4 + (lane >> 4);
+        const int n = mx_column(rb * 16 + (lane & 15), N, gate_up);
+        v4i w = {0, 0, 0, 0};
+        if (n >= 0 && b < KB) w = *reinterpret_cast<const v4i_any*>(codes + ((size_t)n * KB + b) * 16);
+        *reinterpret_cast<v4i*>(dst + i * 16) = w;
+    }
+    if (i < bytes) {
+        const size_t group = i >> 8;
+        const int lane = (int)(i >> 2) & 63, rb = (int)(group / K4), b = (int)(group - (size_t)rb * K4) * 16 + (int)(i & 3) * 4 + (lane >> 4);
+        const int n = mx_column(rb * 16 + (lane & 15), N, gate_up);
+        dst_scales[i] = n >= 0 && b < KB ? scales[(size_t)n * KB + b] : 0;
+    }
+}
+
+} // namespace
+
+extern "C" {
+
+int rkh_mx4_quantize(void* stream, int type, int64_t rows, int K, const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales) {
+    const int64_t blocks = rows * ((K + 31) / 32), groups = (blocks + 64 * QUANT_UNITS - 1) / (64 * QUANT_UNITS);
+    if (!groups) return RKH_OK;
+    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
+    mark((hipStream_t)stream, "mx4_quantize_kernel");
+    mx_with_type(type, [&](auto t) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_quantize_kernel<decltype(t)::value>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, x,
+                           codes, scales, rows, K, ldx);
+    });
+    RKH_CHECK(hipGetLastError());
+    return RKH_OK;
+}
+
+int rkh_mx4_dequantize(void* stream, int type, int64_t rows, int K, const uint8_t* codes, const uint8_t* scales, void* y, int64_t ldy) {
+    const int64_t blocks = rows * ((K + 31) / 32), groups = (blocks + 64 * QUANT_UNITS - 1) / (64 * QUANT_UNITS);
+    if (!groups) return RKH_OK;
+    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
+    mark((hipStream_t)stream, "mx4_dequantize_kernel");
+    mx_with_type(type, [&](auto t) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_dequantize_kernel<decltype(t)::value>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream,
+                           codes, scales, y, rows, K, ldy);
+    });
+    RKH_CHECK(hipGetLastError());
+    return RKH_OK;
+}
+
+int rkh_mx4_stage(void* stream, int type, int rows, int K, const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales) {
+    if (!rows) return RKH_OK;
+    const int64_t groups = ((int64_t)rows + 15) / 16 * rkh_mx4_k4(K);
+    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
+    mark((hipStream_t)stream, "mx4_stage_kernel");
+    mx_with_type(type, [&](auto t) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_stage_kernel<decltype(t)::value>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, x, codes,
+                           scales, rows, K, ldx);
+    });
+    RKH_CHECK(hipGetLastError());
+    return RKH_OK;
+}
+
+int rkh_mx4_pack(void* stream, const uint8_t* codes, const uint8_t* scales, int K, int N, int gate_up, uint8_t* dst, uint8_t* dst_scales) {
+    const int64_t columns = rkh_mx4_columns(N, gate_up);
+    const size_t pieces = rkh_mx4_code_bytes(columns, K) / 16, bytes = rkh_mx4_scale_bytes(columns, K);
+    const size_t groups = ((pieces > bytes ? pieces : bytes) + 255) / 256;
+    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
+    hipLaunchKernelGGL(mx4_pack_kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, codes, scales, dst, dst_scales, K, N, gate_up,
+                       pieces, bytes);
+    RKH_CHECK(hipGetLastError());
+    return RKH_OK;
+}
+
+} // extern "C"

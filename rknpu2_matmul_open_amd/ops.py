@@ -378,3 +378,161 @@ class MoeW8:
         if self.w:
             lib.rk_npu_moe_w8_weights_free(self.w)
             self.w = None
+
+
+# ---- MX4 layers and the block norm: rows are tensors on the device ---------------------------
+# Anything with data_ptr(), shape, stride() and dtype that lies on the context's device (a torch tensor); the calls enqueue on
+# the context's stream, which the caller orders against its own (rk_npu_hip_stream).
+
+_MX4_TYPES = {"torch.float32": capi.MX4_F32, "torch.float16": capi.MX4_F16, "torch.bfloat16": capi.MX4_BF16}
+
+
+def _mx4_rows(x, columns=None):
+    """(element type, address, row stride) of a 2-d tensor whose rows are contiguous."""
+    kind = _MX4_TYPES.get(str(x.dtype))
+    if kind is None:
+        raise TypeError("rows of float32, float16 or bfloat16: got %s" % x.dtype)
+    if len(x.shape) != 2 or (columns is not None and x.shape[1] != columns) or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("contiguous rows%s: got shape %s, strides %s" % ("" if columns is None else " of %d values" % columns, tuple(x.shape), x.stride()))
+    return kind, C.c_void_p(x.data_ptr()), max(x.stride(0), x.shape[1]) if x.shape[0] <= 1 else x.stride(0)
+
+
+def _mx4_bytes(x, rows, width, what):
+    if str(x.dtype) != "torch.uint8" or tuple(x.shape) != (rows, width) or not x.is_contiguous():
+        raise ValueError("%s: contiguous uint8 of shape %s, got %s %s" % (what, (rows, width), x.dtype, tuple(x.shape)))
+    return C.c_void_p(x.data_ptr())
+
+
+def mx4_quantize(session, x, codes, scales):
+    """MX4 rows of x [rows, K]: codes uint8 [rows, 16 * ceil(K / 32)], scales uint8 [rows, ceil(K / 32)]."""
+    kind, p, ld = _mx4_rows(x)
+    rows, K = x.shape
+    blocks = -(-K // 32)
+    check(session.lib.rk_npu_mx4_quantize_device(session.ctx, kind, rows, K, p, ld, _mx4_bytes(codes, rows, 16 * blocks, "codes"),
+                                                 _mx4_bytes(scales, rows, blocks, "scales")), "mx4_quantize")
+
+
+def mx4_dequantize(session, codes, scales, y):
+    """The values of MX4 rows, rounded to y's type."""
+    kind, p, ld = _mx4_rows(y)
+    rows, K = y.shape
+    blocks = -(-K // 32)
+    check(session.lib.rk_npu_mx4_dequantize_device(session.ctx, kind, rows, K, _mx4_bytes(codes, rows, 16 * blocks, "codes"),
+                                                   _mx4_bytes(scales, rows, blocks, "scales"), p, ld), "mx4_dequantize")
+
+
+class MX4Weights:
+    """MX4 weights [N, K] (gate_up: N = 2F, the gate's rows first) from host arrays, or from_device from device addresses."""
+
+    def __init__(self, session, K, N, codes, scales, gate_up=False, on_device=False):
+        self.lib, self.K, self.N, self.gate_up = session.lib, K, N, gate_up
+        create = self.lib.rk_npu_mx4_weights_create_device if on_device else self.lib.rk_npu_mx4_weights_create
+        config = capi.MX4WeightConfig(K, N, 1 if gate_up else 0)
+        self.h = create(session.domain, C.byref(config), codes if on_device else ptr(codes), scales if on_device else ptr(scales))
+        if not self.h:
+            raise ValueError("rk_npu_mx4_weights_create failed")
+
+    @classmethod
+    def from_device(cls, session, K, N, codes, scales, gate_up=False):
+        return cls(session, K, N, codes, scales, gate_up, on_device=True)
+
+    def close(self):
+        if self.h:
+            self.lib.rk_npu_mx4_weights_free(self.h)
+            self.h = None
+
+
+class MX4Workspace:
+    """Workspace for up to max_rows rows of K values and weights of up to N columns (gate / up: 2F)."""
+
+    def __init__(self, session, max_rows, K, N):
+        self.lib, self.K = session.lib, K
+        self.h = self.lib.rk_npu_mx4_workspace_create(session.domain, max_rows, K, N)
+        if not self.h:
+            raise ValueError("rk_npu_mx4_workspace_create failed")
+
+    def _run(self, call, weights, a, c, columns):
+        kind, p, ld = _mx4_rows(a, self.K)
+        c_kind, c_p, c_ld = _mx4_rows(c, columns)
+        if c.shape[0] != a.shape[0]:
+            raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
+        check(call(self.h, weights.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4 run")
+
+    def run(self, weights, a, c):
+        self._run(self.lib.rk_npu_mx4_run_device, weights, a, c, weights.N)
+
+    def run_swiglu(self, weights, a, c):
+        self._run(self.lib.rk_npu_mx4_run_swiglu_device, weights, a, c, weights.N // 2)
+
+    def stage(self, a):
+        kind, p, ld = _mx4_rows(a, self.K)
+        check(self.lib.rk_npu_mx4_stage_device(self.h, a.shape[0], kind, p, ld), "mx4 stage")
+
+    def run_staged(self, weights, c):
+        kind, p, ld = _mx4_rows(c, weights.N // 2 if weights.gate_up else weights.N)
+        check(self.lib.rk_npu_mx4_run_staged_device(self.h, weights.h, kind, p, ld), "mx4 run_staged")
+
+    def close(self):
+        if self.h:
+            self.lib.rk_npu_mx4_workspace_free(self.h)
+            self.h = None
+
+
+def mx4_ffn(gu_ws, gate_up, down_ws, down, a, c):
+    kind, p, ld = _mx4_rows(a, gu_ws.K)
+    c_kind, c_p, c_ld = _mx4_rows(c, down.N)
+    if c.shape[0] != a.shape[0]:
+        raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
+    check(gu_ws.lib.rk_npu_mx4_run_ffn_device(gu_ws.h, gate_up.h, down_ws.h, down.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4_ffn")
+
+
+def _channel(w, D, what):
+    if w is None:
+        return None
+    if str(w.dtype) != "torch.float32" or tuple(w.shape) != (D,) or not w.is_contiguous():
+        raise ValueError("%s: contiguous float32 [%d], got %s %s" % (what, D, w.dtype, tuple(w.shape)))
+    return w.data_ptr()
+
+
+def _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, staged):
+    """rk_npu_block_norm_args of tensors, the branch's type and stride included."""
+    rows, D = stream.shape
+    a = capi.BlockNormArgs(struct_size=C.sizeof(capi.BlockNormArgs), rows=rows, D=D, eps=eps, residual_scale=residual_scale, branch_scale=branch_scale)
+    a.residual_type, a.residual, a.residual_ld = _mx4_rows(stream)
+
+    def alike(x, what):
+        if tuple(x.shape) != (rows, D):
+            raise ValueError("%s: shape %s, the stream's is %s" % (what, tuple(x.shape), (rows, D)))
+        return _mx4_rows(x)
+    if branch is not None:
+        a.branch_type, a.branch, a.branch_ld = alike(branch, "branch")
+    if gate is not None:
+        a.gate_type, a.gate, a.gate_ld = _mx4_rows(gate.reshape(1, D)) if len(gate.shape) == 1 else alike(gate, "gate")
+        if len(gate.shape) == 1:
+            a.gate_ld = 0
+    a.branch_weight, a.weight = _channel(after, D, "after"), _channel(weight, D, "weight")
+    if stream_out is not None:
+        kind, a.residual_out, a.residual_out_ld = alike(stream_out, "stream_out")
+        if kind != a.residual_type:
+            raise TypeError("stream_out: the stream's type")
+    if y is not None:
+        a.y_type, a.y, a.y_ld = alike(y, "y")
+    a.staged = staged.h if staged is not None else None
+    return a
+
+
+def block_norm(session, stream, branch=None, after=None, gate=None, residual_scale=1.0, branch_scale=1.0, weight=None, eps=1e-6,
+               stream_out=None, y=None, staged=None):
+    """The norms around a block (rk_npu_block_norm_device): stream, branch [rows, D]; after (behind the block) and weight (before the
+    next one) float32 [D]; gate [D] or [rows, D]."""
+    a = _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, staged)
+    check(session.lib.rk_npu_block_norm_device(session.ctx, C.byref(a)), "block_norm")
+
+
+def mx4_ffn_block(gu_ws, gate_up, down_ws, down, stream, branch, weight=None, after=None, gate=None, residual_scale=1.0, branch_scale=1.0,
+                  eps=1e-6, stream_out=None, y=None, next_weight=None):
+    """A gated FFN block on the residual stream (rk_npu_mx4_run_ffn_block_device); branch receives the FFN's output."""
+    a = _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, None)
+    a.branch = None
+    check(gu_ws.lib.rk_npu_mx4_run_ffn_block_device(gu_ws.h, gate_up.h, down_ws.h, down.h, C.byref(a), C.c_void_p(branch.data_ptr()),
+                                                    _channel(next_weight, stream.shape[1], "next_weight")), "mx4_ffn_block")

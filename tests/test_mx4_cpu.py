@@ -1,0 +1,118 @@
+"""The MX4 boundary without a GPU: the header, the exports and their bindings, refusals that come ahead of any device work, and what
+the dispatch decides, which is arithmetic."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+
+from rknpu2_matmul_open_amd import capi
+from tests import mx4_reference as ref
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+INC = os.path.join(ROOT, "include")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return capi.load_library()
+
+
+def test_header_compiles_as_c99(tmp_path):
+    src = tmp_path / "h.c"
+    src.write_text('#include "rk_npu_mx4.h"\nint main(void) { return 0; }\n')
+    subprocess.check_call(["gcc", "-std=c99", "-pedantic", "-Wall", "-Werror", "-I", INC, "-c", str(src), "-o", str(tmp_path / "o.o")])
+
+
+def test_library_exports_what_the_header_declares(lib):
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(INC, "rk_npu_mx4.h")).read(), flags=re.S)
+    declared = set(re.findall(r"\b(rk_npu_[a-z0-9_]+)\s*\(", text))
+    assert len(declared) >= 15
+    assert all(hasattr(lib, n) for n in declared)
+    assert set(capi.MX4_SYMBOLS) == declared
+
+
+def test_struct_layouts_match_the_c_compiler(tmp_path):
+    lines, want = [], []
+    for name, cls in (("rk_npu_mx4_weight_config", capi.MX4WeightConfig), ("rk_npu_block_norm_args", capi.BlockNormArgs)):
+        lines.append('printf("%%zu\\n", sizeof(%s));' % name)
+        want.append(C.sizeof(cls))
+        for field, _ in cls._fields_:
+            lines.append('printf("%%zu\\n", offsetof(%s, %s));' % (name, field))
+            want.append(getattr(cls, field).offset)
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "rk_npu_mx4.h"\nint main(void) { %s return 0; }\n' % " ".join(lines))
+    subprocess.check_call(["gcc", "-I", INC, str(src), "-o", str(tmp_path / "s")])
+    got = [int(x) for x in subprocess.check_output([str(tmp_path / "s")]).split()]
+    assert got == want
+
+
+def test_refusals_without_a_context(lib):
+    some = C.c_void_p(4096)
+    bad = capi.RK_NPU_ERR_PARAM
+    assert lib.rk_npu_mx4_quantize_device(None, 0, 1, 32, some, 32, some, some) == bad
+    assert lib.rk_npu_mx4_dequantize_device(None, 0, 1, 32, some, some, some, 32) == bad
+    assert lib.rk_npu_mx4_run_device(None, None, 1, 0, some, 32, 0, some, 32) == bad
+    assert lib.rk_npu_mx4_run_swiglu_device(None, None, 1, 0, some, 32, 0, some, 32) == bad
+    assert lib.rk_npu_mx4_stage_device(None, 1, 0, some, 32) == bad
+    assert lib.rk_npu_mx4_run_staged_device(None, None, 0, some, 32) == bad
+    assert lib.rk_npu_mx4_run_ffn_device(None, None, None, None, 1, 0, some, 32, 0, some, 32) == bad
+    args = capi.BlockNormArgs()
+    lib.rk_npu_block_norm_args_init(C.byref(args), 3, 64)
+    assert (args.struct_size, args.rows, args.D) == (C.sizeof(args), 3, 64)
+    assert (args.residual_scale, args.branch_scale) == (1.0, 1.0) and abs(args.eps - 1e-6) < 1e-12
+    assert lib.rk_npu_block_norm_device(None, C.byref(args)) == bad
+    assert lib.rk_npu_mx4_run_ffn_block_device(None, None, None, None, C.byref(args), some, None) == bad
+    assert lib.rk_npu_mx4_weights_query(None, None, None) == bad
+    config = capi.MX4WeightConfig(32, 32, 0)
+    assert not lib.rk_npu_mx4_weights_create(None, C.byref(config), some, some)
+    assert not lib.rk_npu_mx4_workspace_create(None, 1, 32, 32)
+    lib.rk_npu_mx4_weights_free(None)
+    lib.rk_npu_mx4_workspace_free(None)
+
+
+def _route(lib, M, N, K, swiglu):
+    out = [C.c_int(0) for _ in range(4)]
+    lib.rkh_mx4_route(M, N, K, swiglu, *[C.byref(x) for x in out])
+    return [x.value for x in out]
+
+
+@pytest.mark.parametrize("swiglu", [0, 1])
+def test_route_covers_every_row_and_column_and_its_scratch_is_what_the_parts_need(lib, swiglu):
+    lib.rkh_mx4_scratch_bytes.restype = C.c_size_t
+    rng = np.random.default_rng(3)
+    for _ in range(3000):
+        M, N, K = (int(np.exp(rng.uniform(0, np.log(top)))) for top in (9000, 40000, 40000))
+        kernel, rows, columns, parts = _route(lib, M, N, K, swiglu)
+        assert rows > 0 and columns % 16 == 0 and 1 <= parts <= max(1, -(-K // 512)), (M, N, K)
+        if kernel == 0:
+            assert M <= rows and parts == 1
+        else:
+            assert rows % 32 == 0 and columns % 32 == 0
+            assert not swiglu or columns % 128 == 0 # whole gate / up pairs in each wave
+        places = 2 * (-(-N // 32) * 32) if swiglu else -(-N // 32) * 32
+        tiles = -(-M // rows) * -(-places // columns)
+        want = tiles * parts * rows * columns * 4 if parts > 1 else 0
+        assert lib.rkh_mx4_scratch_bytes(M, N, K, swiglu) == want, (M, N, K)
+
+
+def test_reference_of_the_format():
+    """The oracle itself: its codes are what the definition says at every border between two values and beside it."""
+    borders = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]
+    down = [0, 1, 1, 2, 2, 4, 4]    # ties: 0 | 0.5 -> 0, 0.5 | 1 -> 1, 1 | 1.5 -> 1, 1.5 | 2 -> 2, 2 | 3 -> 2, 3 | 4 -> 4, 4 | 6 -> 4
+    x = np.zeros((1, 32))
+    x[0, 0] = 4.0                   # scale 1
+    x[0, 1:8] = borders
+    x[0, 8:15] = np.nextafter(borders, 10)
+    x[0, 15:22] = np.nextafter(borders, 0)
+    got = ref.round_trip(x)[0]
+    assert list(got[1:8]) == down
+    assert list(got[8:15]) == [0.5, 1, 1.5, 2, 3, 4, 6]
+    assert list(got[15:22]) == [0, 0.5, 1, 1.5, 2, 3, 4]
+    assert ref.quantize(np.full((1, 32), 7.99))[1][0, 0] == 127 and ref.round_trip(np.full((1, 32), 7.99))[0, 0] == 6
+    codes, scales = ref.exact_rows(np.random.default_rng(1), 5, 70)
+    again = ref.quantize(ref.values(codes, scales, 70))
+    live = ref.values(codes, scales, 96).reshape(5, 96)
+    assert np.array_equal(again[1], scales) and np.array_equal(ref.values(*again, 96), live)
