@@ -1,8 +1,9 @@
 """Static check of the hand-placed waits of the inline-assembly load kernels.
 
-    python -m rknpu2_matmul_open_amd.audit_waits            # compiles the two units to assembly and checks them
+    python -m rknpu2_matmul_open_amd.audit_waits            # compiles the units to assembly and checks them
 
-gemm_wk_kernel and gemm_stream_kernel issue their loop loads from inline assembly and place
+gemm_wk_kernel and gemm_stream_kernel issue their loop loads from inline assembly (the MX4 tile kernels their
+products, and loads to LDS, which the last two rules are about) and place
 every s_waitcnt by hand; the compiler believes the destination registers of such a load hold
 their value as soon as the asm statement has executed.  The kernels are correct only if, in the
 code the compiler actually produced, nothing reads or overwrites such a register between the
@@ -40,7 +41,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-UNITS = ["rk_kernels_gemm.hip", "rk_kernels_stream.hip"]
+UNITS = ["rk_kernels_gemm.hip", "rk_kernels_stream.hip", "rk_kernels_mx4_gemm.hip"]
 
 _VM_LOAD = re.compile(r"^\s*(global_load|buffer_load|flat_load|scratch_load)")
 _ASM_VLOAD = re.compile(r"^\s*global_load_dwordx?(\d*)\s+(v\[\d+:\d+\]|v\d+)\s*,")
@@ -48,19 +49,20 @@ _ASM_DSREAD = re.compile(r"^\s*ds_read_b(\d+)\s+(v\[\d+:\d+\]|v\d+)\s*,")
 _VMCNT = re.compile(r"vmcnt\((\d+)\)")
 _LGKMCNT = re.compile(r"lgkmcnt\((\d+)\)")
 _DS_OP = re.compile(r"^\s*ds_")
-_REG = re.compile(r"\bv\[(\d+):(\d+)\]|\bv(\d+)\b")
+_REG = re.compile(r"\b([va])\[(\d+):(\d+)\]|\b([va])(\d+)\b")
 _LABEL = re.compile(r"^(\.LBB\d+_\d+):")
 _BRANCH = re.compile(r"^\s*s_cbranch_\w+\s+(\.LBB\d+_\d+)|^\s*s_branch\s+(\.LBB\d+_\d+)")
+
+
+_ACC = 1000 # accumulation registers follow the others in the numbers below
 
 
 def _regs(operand_text):
     """Vector registers named in a piece of assembly text, as a set of numbers."""
     out = set()
-    for a, b, c in _REG.findall(operand_text):
-        if c:
-            out.add(int(c))
-        else:
-            out.update(range(int(a), int(b) + 1))
+    for half, lo, hi, one_half, one in _REG.findall(operand_text):
+        base = _ACC if "a" in (half, one_half) else 0
+        out.update(range(base + int(lo or one), base + int(hi or one) + 1))
     return out
 
 
@@ -276,7 +278,7 @@ def audit_function(name, lines):
     return violations
 
 
-def audit_text(asm_text, only=("gemm_wk_kernel", "gemm_wk_big_kernel", "gemm_stream_kernel")):
+def audit_text(asm_text, only=("gemm_wk_kernel", "gemm_wk_big_kernel", "gemm_stream_kernel", "mx4_tile_kernel", "mx4_big_kernel")):
     """Violations in every kernel of an assembly file whose (mangled) name contains one of `only`."""
     violations, checked = [], 0
     lines = asm_text.splitlines() + [".Lfunc_end:"]

@@ -116,8 +116,8 @@ __device__ __forceinline__ uint32_t mx_top_of_quad(uint32_t top) {
 }
 
 // Byte offsets of block b of row m in operand blocks.
-__device__ __forceinline__ size_t mx_code_at(int m, int b, int KS) {
-    return ((size_t)(m >> 4) * KS + (b >> 2)) * 1024 + (m & 15) * 16 + (b & 3) * 256;
+__device__ __forceinline__ size_t mx_code_at(int m, int b, int K4) {
+    return ((size_t)(m >> 4) * K4 * 4 + (b >> 2)) * 1024 + (m & 15) * 16 + (b & 3) * 256;
 }
 __device__ __forceinline__ size_t mx_scale_at(int m, int b, int K4) {
     return ((size_t)(m >> 4) * K4 + (b >> 4)) * 256 + (m & 15) * 4 + (b & 3) * 64 + ((b >> 2) & 3);

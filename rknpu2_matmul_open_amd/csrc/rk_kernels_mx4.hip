@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* code
 template <int TYPE>
 __global__ __launch_bounds__(256) void mx4_stage_kernel(const void* x, uint8_t* codes, uint8_t* scales, int rows, int K, int64_t ldx) {
     __shared__ uint8_t lds_scales[256];
-    const int KS = (int)rkh_mx4_ks(K), K4 = (int)rkh_mx4_k4(K);
+    const int K4 = (int)rkh_mx4_k4(K);
     const int lane = lane_id(), wave = wave_id();
     const int rb = blockIdx.x / K4, k4 = blockIdx.x - rb * K4, ks = k4 * 4 + wave;
     const int m = rb * 16 + (lane & 15), k0 = ks * 128 + (lane >> 4) * 32;
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void mx4_stage_kernel(const void* x, uint8_t* 
     v4i w;
 #pragma unroll
     for (int c = 0; c < 4; ++c) w[c] = (int)mx_codes(v[c], scale);
-    if (ks < KS) *reinterpret_cast<v4i*>(codes + ((size_t)rb * KS + ks) * 1024 + lane * 16) = w;
+    *reinterpret_cast<v4i*>(codes + ((size_t)rb * K4 * 4 + ks) * 1024 + lane * 16) = w;
     lds_scales[lane * 4 + wave] = (uint8_t)scale;
     __syncthreads();
     if (threadIdx.x < 64) reinterpret_cast<uint32_t*>(scales)[((size_t)rb * K4 + k4) * 64 + threadIdx.x] = reinterpret_cast<const uint32_t*>(lds_scales)[threadIdx.x];
@@ -127,11 +127,11 @@ __global__ __launch_bounds__(256) void mx4_stage_kernel(const void* x, uint8_t* 
 // One thread per 16 bytes of operand blocks, then per scale byte; places without a column, and blocks beyond K, are zero.
 __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* codes, const uint8_t* scales, uint8_t* dst, uint8_t* dst_scales, int K, int N,
                                                        int gate_up, size_t pieces, size_t bytes) {
-    const int KB = (K + 31) / 32, KS = (int)rkh_mx4_ks(K), K4 = (int)rkh_mx4_k4(K);
+    const int KB = (K + 31) / 32, K4 = (int)rkh_mx4_k4(K);
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i < pieces) {
         const size_t piece = i >> 6;
-        const int lane = (int)(i & 63), rb = (int)(piece / KS), b = (int)(piece - (size_t)rb * KS) * 4 + (lane >> 4);
+        const int lane = (int)(i & 63), rb = (int)(piece / (K4 * 4)), b = (int)(piece - (size_t)rb * K4 * 4) * 4 + (lane >> 4);
         const int n = mx_column(rb * 16 + (lane & 15), N, gate_up);
         v4i w = {0, 0, 0, 0};
         if (n >= 0 && b < KB) w = *reinterpret_cast<const v4i_any*>(codes + ((size_t)n * KB + b) * 16);

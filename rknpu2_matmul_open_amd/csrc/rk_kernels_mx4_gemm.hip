@@ -4,6 +4,8 @@
 // The weights are the FIRST operand: lane (r, q) = (l % 16, l / 16) of a 16 x 16 accumulator owns activation row r and four of the
 // tile's weight rows, which the packing has made the consecutive columns 8 q + 4 h .. + 3 of a block of 32 (h: the first or the
 // second tile of the block).
+#include <algorithm>
+
 #include "rk_kernels_mx4.h"
 
 namespace {
@@ -14,6 +16,36 @@ typedef __attribute__((address_space(3))) uint8_t* mx_lds_ptr;
 template <int STEP> __device__ __forceinline__ v4f mx_mfma(const v4i& w, const v4i& a, const v4f& sum, uint32_t ws, uint32_t as) {
     const v8i w8 = {w.x, w.y, w.z, w.w, 0, 0, 0, 0}, a8 = {a.x, a.y, a.z, a.w, 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, a8, sum, 4, 4, STEP, (int)ws, STEP, (int)as);
+}
+
+// The same as an asm statement, for the tiles: the sums stay in one place (of products that it knows the compiler moved 256 sums
+// between registers and spilled others).  What the compiler then does not order: a vector instruction that writes an operand has
+// to be two wait states ahead of the product -- here LDS reads alone write them --, and one that reads a sum waits for the last
+// products, at the end of the loop.
+// ACC: the sum is in the accumulation half of the registers.  (256 of them take all of it; with none to spare the compiler kept
+// some on the move, so a few live in the other half.)
+template <int STEP, bool ACC> __device__ __forceinline__ void mx_mfma_in_place(const v4i& w, const v4i& a, v4f& sum, uint32_t ws, uint32_t as) {
+    if constexpr (ACC)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%c5,%c5,0] op_sel_hi:[%c6,%c6,0] cbsz:4 blgp:4"
+                     : "+a"(sum) : "v"(w), "v"(a), "v"(ws), "v"(as), "n"(STEP & 1), "n"(STEP >> 1));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%c5,%c5,0] op_sel_hi:[%c6,%c6,0] cbsz:4 blgp:4"
+                     : "+v"(sum) : "v"(w), "v"(a), "v"(ws), "v"(as), "n"(STEP & 1), "n"(STEP >> 1));
+}
+// ... of which there is no sum yet
+template <int STEP, bool ACC> __device__ __forceinline__ void mx_mfma_first(const v4i& w, const v4i& a, v4f& sum, uint32_t ws, uint32_t as) {
+    if constexpr (ACC)
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[%c5,%c5,0] op_sel_hi:[%c6,%c6,0] cbsz:4 blgp:4"
+                     : "=&a"(sum) : "v"(w), "v"(a), "v"(ws), "v"(as), "n"(STEP & 1), "n"(STEP >> 1));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel:[%c5,%c5,0] op_sel_hi:[%c6,%c6,0] cbsz:4 blgp:4"
+                     : "=&v"(sum) : "v"(w), "v"(a), "v"(ws), "v"(as), "n"(STEP & 1), "n"(STEP >> 1));
+}
+// The sum as it is at this point, where it is: what keeps the compiler from fetching all sums ahead of the first one's store, and
+// from putting anything but products between two of them.
+template <bool ACC> __device__ __forceinline__ void mx_settled(v4f& sum) {
+    if constexpr (ACC) asm volatile("" : "+a"(sum));
+    else asm volatile("" : "+v"(sum));
 }
 
 __device__ __forceinline__ float mx_silu(float gate, float up) { return __fmul_rn(silu_poly(gate), up); }
@@ -40,7 +72,7 @@ __device__ __forceinline__ void mx_put_rows(const rkh_mx4_gemm_args& g, int m, i
     top = max(top, (uint32_t)__shfl_xor((int)top, 32));
     const uint32_t scale = mx_scale(top);
     if (!live) return;
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.C) + mx_code_at(m, block, (int)rkh_mx4_ks(g.N)) + (lane >> 4) * 4) = mx_codes(v, scale);
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.C) + mx_code_at(m, block, (int)rkh_mx4_k4(g.N)) + (lane >> 4) * 4) = mx_codes(v, scale);
     if (lane < 16) g.c_scale[mx_scale_at(m, block, (int)rkh_mx4_k4(g.N))] = (uint8_t)scale;
 }
 
@@ -68,7 +100,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void mx4_few_kernel(rkh_mx4_gemm_ar
 #pragma unroll
         for (int j = 0; j < CN; ++j) {
             const int col = min(col0 + j, cols - 1);
-            const uint8_t* src = g.W + ((size_t)col * KS + group * 4) * 1024 + lane * 16;
+            const uint8_t* src = g.W + ((size_t)col * K4 + group) * 4096 + lane * 16;
 #pragma unroll
             for (int s = 0; s < 4; ++s) w[s][j] = *reinterpret_cast<const v4i*>(src + (group * 4 + s < KS ? s * 1024 : 0));
             ws[j] = reinterpret_cast<const uint32_t*>(g.w_scale)[((size_t)col * K4 + group) * 64 + lane];
@@ -128,7 +160,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void mx4_few_kernel(rkh_mx4_gemm_ar
                     a[s][i] = live && group * 4 + s < KS ? *reinterpret_cast<const v4i*>(lds + ((size_t)((group * 4 + s) * 4 + q) * g.M + r) * 16) : v4i{0, 0, 0, 0};
             } else {
                 const int rb = min(i, rblocks - 1);
-                const uint8_t* src = g.A + ((size_t)rb * KS + group * 4) * 1024 + lane * 16;
+                const uint8_t* src = g.A + ((size_t)rb * K4 + group) * 4096 + lane * 16;
 #pragma unroll
                 for (int s = 0; s < 4; ++s) a[s][i] = *reinterpret_cast<const v4i*>(src + (group * 4 + s < KS ? s * 1024 : 0));
                 as[i] = reinterpret_cast<const uint32_t*>(g.a_scale)[((size_t)rb * K4 + group) * 64 + lane];
@@ -188,17 +220,17 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void mx4_few_kernel(rkh_mx4_gemm_ar
 
 // ---- tiles ---------------------------------------------------------------------------
 // Tiles of 32 RM rows x 32 CN places by four waves (two by two), RM x CN accumulators each.  A step is 128 k: every operand of the tile is 1 KiB,
-// copied global -> LDS directly (no registers) NBUF - 1 steps ahead, and read into registers one step ahead of its products.
-// The scales of four steps are 256 bytes per operand, copied two groups ahead and read one step ahead.
+// copied global -> LDS directly (no registers) D steps ahead, and read into registers one step ahead of its products.  Four steps
+// are a group, whose scales are 256 bytes per operand, copied two groups ahead.  K ends with a group: pieces beyond it are zeros.
 //
 // The copies are inline assembly (they write no register; the compiler, which would put every LDS read behind ALL copies in
 // flight, does not see them), and what orders them is explicit:
-//  * the copies of step s + NBUF - 1 are issued in step s, into the buffer of step s - 1: its last reads were issued in step
-//    s - 2 and waited for by the first products of step s - 1, ahead of the barrier that ended it;
+//  * the copies of step s + D are issued in step s, into the buffer of step s - 1 (the ring has D + 1): its last reads were issued in step
+//    s - 2 and waited for by the products of step s - 1, ahead of the barrier that ended it;
 //  * step s reads the operands of step s + 1; the wait in front of the barrier that ends step s - 1 has left no copy of that step in
 //    flight (vector memory loads complete in order, wait_for() counts what was issued since);
-//  * the scales of group g + 2, issued in the first step of group g, overwrite those of group g, which were read in the last
-//    step of group g - 1.
+//  * the scales of group g + 2, issued in the second step of group g, overwrite those of group g, which were read in the last
+//    step of group g - 1 and waited for by the products of the first step of group g, ahead of the barrier that ended it.
 // Copies beyond the part's K bring its last step again, for the count; nothing reads them.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm" // m0 is set and clobbered on purpose below
@@ -208,172 +240,304 @@ __device__ __forceinline__ void mx_copy(const uint8_t* base, unsigned off, uint3
 }
 #pragma clang diagnostic pop
 
-template <int RM, int CN, int NBUF> struct MxTile {
+// HALVES: groups that the ring holds.
+template <int RM, int CN, int HALVES> struct MxTile {
     static constexpr int AB = 2 * RM, WB = 2 * CN;               // operands of a step
     static constexpr int COPIES = (AB + WB) / 4;                 // 1 KiB copies of a wave per step
     static constexpr int SCALE_COPIES = (AB + WB) / 4;           // 1 KiB copies of four operands' scales, of all waves
     static constexpr int SC = (SCALE_COPIES + 3) / 4;            // ... of a wave per group
-    static constexpr int D = NBUF - 1, UNR = 8;                  // look-ahead; steps of an unrolled trip
+    static constexpr int D = 4 * HALVES - 1;                     // look-ahead
     static constexpr int BUF = (AB + WB) * 1024, SBUF = (AB + WB) * 256;
-    static constexpr int SCALES_OFF = NBUF * BUF, LDS = SCALES_OFF + 2 * SBUF;
-    static_assert(RM % 2 == 0 && CN % 2 == 0 && UNR % NBUF == 0 && LDS <= 160 * 1024, "");
-    // loads of a wave issued in the last `steps` steps up to step t of a trip
-    static constexpr int issued(int t, int steps) {
+    static constexpr int SCALES_OFF = 4 * HALVES * BUF, LDS = SCALES_OFF + 2 * SBUF;
+    static_assert(RM % 2 == 0 && CN % 2 == 0 && (HALVES == 1 || HALVES == 2) && LDS <= 160 * 1024, "");
+    // the copies of step t + 2 of a group have landed: what a wave has issued in the D - 2 steps up to step t
+    static constexpr int wait_for(int t) {
         int n = 0;
-        for (int s = 0; s < steps; ++s) n += COPIES + ((t - s + 8) % 4 == 0 ? SC : 0);
+        for (int s = 0; s < D - 2; ++s) n += COPIES + ((t - s + 8) % 4 == 1 ? SC : 0);
         return n;
     }
-    static constexpr int wait_for(int t) { return issued(t, D - 2); } // the copies of step t + 2 have landed
-    static_assert(D >= 3 && D - 2 <= 5, "a group's scales are older than what wait_for leaves in flight");
+    static_assert(D - 2 <= 5, "a group's scales, issued in the sixth step ahead, are older than what wait_for leaves in flight");
 };
 
-template <int RM, int CN, int NBUF, bool SWIGLU>
-__global__ __launch_bounds__(256) void mx4_tile_kernel(rkh_mx4_gemm_args g, int mblocks, int nblocks, int parts) {
-    using S = MxTile<RM, CN, NBUF>;
+// Where a tile lies: column sweeps over groups of row blocks, so that concurrently running tiles share weights in L2.
+__device__ __forceinline__ void mx_place(unsigned tile, unsigned mblocks, unsigned nblocks, int& mblk, int& nblk) {
+    constexpr unsigned GM = 4;
+    const unsigned per_group = GM * nblocks, grp = tile / per_group, first_m = grp * GM, gm = min(mblocks - first_m, GM);
+    const unsigned in_group = tile - grp * per_group, col = in_group / gm;
+    mblk = __builtin_amdgcn_readfirstlane((int)(first_m + in_group - col * gm));
+    nblk = __builtin_amdgcn_readfirstlane((int)col);
+}
+
+// The jobs of a launch: tiles, or parts of them where K is split (all tiles' first parts, then all second ones, ..).  `halves`: from tile `skip` on every
+// tile is two jobs, its upper and its lower half of rows.
+struct MxJobs {
+    int mblocks, nblocks, parts; // of whole tiles
+    int jobs, skip;
+    bool halves;
+    __device__ __forceinline__ void place(int job, int& mblk, int& nblk, int& kpart) const {
+        const unsigned j = (unsigned)xcd_remap(job, jobs);
+        // (quotients of uniform values come out of vector registers)
+        if (halves) {
+            mx_place(skip + (j >> 1), mblocks, nblocks, mblk, nblk);
+            mblk = 2 * mblk + (j & 1), kpart = 0;
+        } else {
+            const unsigned tiles = (unsigned)mblocks * nblocks;
+            kpart = parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(j / tiles));
+            mx_place(j - kpart * tiles, mblocks, nblocks, mblk, nblk);
+        }
+    }
+    __device__ __forceinline__ unsigned partial(int job) const { // [tile][part] of a split job's sums
+        const unsigned j = (unsigned)xcd_remap(job, jobs), tiles = (unsigned)mblocks * nblocks;
+        return (j % tiles) * parts + j / tiles;
+    }
+};
+
+// Multiplies jobs job, job + stride, ...  Their steps follow one another: the copies that run ahead of a tile's end are the next
+// tile's first, and land while the tile is converted and stored.
+template <int RM, int CN, int HALVES, bool SWIGLU>
+__device__ __forceinline__ void mx_tiles(const rkh_mx4_gemm_args& g, uint8_t* lds, const MxJobs& of, int job, int stride) {
+    using S = MxTile<RM, CN, HALVES>;
     static_assert(!SWIGLU || CN % 4 == 0, "gate and up halves of blocks of 32 columns in one wave");
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    constexpr auto in_acc = [](int i) { return RM * CN < 64 || i < RM - 1; };
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave & 1, wn = wave >> 1;
-    const int KS = (int)rkh_mx4_ks(g.K), K4 = (int)rkh_mx4_k4(g.K);
+    const int K4 = (int)rkh_mx4_k4(g.K);
     const int cols = (int)rkh_mx4_columns(SWIGLU ? 2 * g.N : g.N, SWIGLU) / 16, rows = (g.M + 15) / 16; // operands that exist
 
-    // column sweeps over groups of row blocks, so that concurrently running tiles share weights in L2
-    constexpr unsigned GM = 4;
-    const unsigned tiles = mblocks * nblocks, job = xcd_remap(blockIdx.x, tiles * parts);
-    const unsigned kpart = job / tiles, tile = job - kpart * tiles;
-    const unsigned per_group = GM * nblocks, grp = tile / per_group, first_m = grp * GM, gm = min(mblocks - first_m, GM);
-    const unsigned in_group = tile - grp * per_group, nblk = in_group / gm, mblk = first_m + in_group - nblk * gm;
-
-    const int g0 = (int)((size_t)K4 * kpart / parts), g1 = (int)((size_t)K4 * (kpart + 1) / parts); // groups of 512 k
-    const int ks0 = g0 * 4, steps = min(g1 * 4, KS) - ks0, groups = g1 - g0;
-
-    // ---- sources: wave-uniform base pointers and a lane offset that advances with K
-    const uint8_t *a_src[RM / 2], *w_src[CN / 2];
-#pragma unroll
-    for (int c = 0; c < RM / 2; ++c) a_src[c] = g.A + ((size_t)min((int)mblk * S::AB + wave * (RM / 2) + c, rows - 1) * KS + ks0) * 1024;
-#pragma unroll
-    for (int c = 0; c < CN / 2; ++c) w_src[c] = g.W + ((size_t)min((int)nblk * S::WB + wave * (CN / 2) + c, cols - 1) * KS + ks0) * 1024;
+    // ---- sources: wave-uniform base pointers and a lane offset that advances with K.  Two streams, of steps and of groups of scales, each
+    // with the job that it has come to.
     const uint32_t base = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
     const uint32_t a_to = base + wave * (RM / 2) * 1024, w_to = base + (S::AB + wave * (CN / 2)) * 1024;
-    // scales: copy x brings those of operands 4 x .. 4 x + 3 of the tile (activations first)
+    const auto part_of = [&](int kpart, int& g0, int& groups) {
+        g0 = of.parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)((unsigned)(K4 * kpart) / of.parts));
+        groups = (of.parts == 1 ? K4 : __builtin_amdgcn_readfirstlane((int)((unsigned)(K4 * (kpart + 1)) / of.parts))) - g0;
+    };
+    const uint8_t *a_src[RM / 2], *w_src[CN / 2];
+    unsigned k_off = lane * 16, k_step = 1024;
+    int mblk_next = 0, nblk_next = 0, groups_next = 0; // of the job that the copies have come to
+    const auto steps_of = [&](int j) {
+        int kpart, g0;
+        of.place(j, mblk_next, nblk_next, kpart);
+        part_of(kpart, g0, groups_next);
+        const int mblk = mblk_next, nblk = nblk_next;
+#pragma unroll
+        for (int c = 0; c < RM / 2; ++c) a_src[c] = g.A + ((size_t)min(mblk * S::AB + wave * (RM / 2) + c, rows - 1) * K4 + g0) * 4096;
+#pragma unroll
+        for (int c = 0; c < CN / 2; ++c) w_src[c] = g.W + ((size_t)min(nblk * S::WB + wave * (CN / 2) + c, cols - 1) * K4 + g0) * 4096;
+        k_off = lane * 16;
+    };
+    // copy x of a group's scales brings those of operands 4 x .. 4 x + 3 of the tile (activations first)
     const uint8_t* s_src[S::SC];
     unsigned s_off[S::SC];
-    uint32_t s_to[S::SC];
+    int s_job = job, s_left = 0; // groups that are still to come of s_job
+    const auto scales_of = [&](int j) {
+        int mblk, nblk, kpart, g0;
+        of.place(j, mblk, nblk, kpart);
+        part_of(kpart, g0, s_left);
 #pragma unroll
-    for (int c = 0; c < S::SC; ++c) {
-        const int x = (c * 4 + wave) % S::SCALE_COPIES, op = x * 4 + (lane >> 4);
-        static_assert(S::AB % 4 == 0, "a copy's operands are of one kind");
-        const bool is_a = x * 4 < S::AB;
-        const int first_op = is_a ? (int)mblk * S::AB : (int)nblk * S::WB, limit = (is_a ? rows : cols) - 1;
-        const int at = min(first_op, limit);
-        s_src[c] = (is_a ? g.a_scale : g.w_scale) + ((size_t)at * K4 + g0) * 256;
-        s_off[c] = (unsigned)(min(first_op + op - (is_a ? 0 : S::AB), limit) - at) * (unsigned)K4 * 256 + (lane & 15) * 16;
-        s_to[c] = base + S::SCALES_OFF + x * 1024;
-    }
+        for (int c = 0; c < S::SC; ++c) {
+            const int x = (c * 4 + wave) % S::SCALE_COPIES, op = x * 4 + (lane >> 4);
+            static_assert(S::AB % 4 == 0, "a copy's operands are of one kind");
+            const bool is_a = x * 4 < S::AB;
+            const int first_op = is_a ? mblk * S::AB : nblk * S::WB, limit = (is_a ? rows : cols) - 1;
+            const int at = min(first_op, limit);
+            s_src[c] = (is_a ? g.a_scale : g.w_scale) + ((size_t)at * K4 + g0) * 256;
+            s_off[c] = (unsigned)(min(first_op + op - (is_a ? 0 : S::AB), limit) - at) * (unsigned)K4 * 256 + (lane & 15) * 16;
+        }
+    };
 
     v4f acc[RM][CN];
-    v4i a[2][RM], w[2][CN];
-    uint32_t as[2][RM], ws[2][CN];
+    v4i a[RM], w[2][CN];
+    uint32_t as[RM], ws[CN];
+    // places in LDS, from the half of the ring that the group lies in and the half of the scales'
+    uint32_t half = 0, s_half = 0;
+    const auto other = [&](uint32_t h) { return HALVES == 2 ? (uint32_t)(4 * S::BUF) - h : h; };
     const uint8_t* a_at = lds + wm * RM * 1024 + lane * 16;
     const uint8_t* w_at = lds + (S::AB + wn * CN) * 1024 + lane * 16;
     const uint8_t* as_at = lds + S::SCALES_OFF + wm * RM * 256 + lane * 4;
     const uint8_t* ws_at = lds + S::SCALES_OFF + (S::AB + wn * CN) * 256 + lane * 4;
 
-    int ahead = 0; // next step to copy
-    unsigned k_off = lane * 16;
-    const auto copy = [&](auto buf_tag, auto c_tag) {
-        constexpr int B = decltype(buf_tag)::value % NBUF, C = decltype(c_tag)::value;
-        if constexpr (C < RM / 2) mx_copy(a_src[C], k_off, a_to + B * S::BUF + C * 1024);
-        else mx_copy(w_src[C - RM / 2], k_off, w_to + B * S::BUF + (C - RM / 2) * 1024);
-        if constexpr (C == S::COPIES - 1) {
-            ++ahead;
-            k_off += ahead < steps ? 1024u : 0u;
-        }
+    const auto copy = [&](uint32_t to, auto buf_tag, auto c_tag) {
+        constexpr int B = decltype(buf_tag)::value % 4, C = decltype(c_tag)::value;
+        if constexpr (C < RM / 2) mx_copy(a_src[C], k_off, a_to + to + B * S::BUF + C * 1024);
+        else mx_copy(w_src[C - RM / 2], k_off, w_to + to + B * S::BUF + (C - RM / 2) * 1024);
+        if constexpr (C == S::COPIES - 1) k_off += k_step;
     };
-    int s_ahead = 0; // next group whose scales are to be copied
-    const auto copy_scales = [&](auto half_tag) {
+    const auto copy_scales = [&](uint32_t to) {
+        if (s_left == 0 && s_job + stride < of.jobs) scales_of(s_job += stride);
 #pragma unroll
-        for (int c = 0; c < S::SC; ++c) mx_copy(s_src[c], s_off[c] + (unsigned)min(s_ahead, groups - 1) * 256, s_to[c] + decltype(half_tag)::value * S::SBUF);
-        ++s_ahead;
+        for (int c = 0; c < S::SC; ++c) {
+            mx_copy(s_src[c], s_off[c], base + S::SCALES_OFF + to + (c * 4 + wave) % S::SCALE_COPIES * 1024);
+            s_off[c] += s_left > 1 ? 256 : 0;
+        }
+        s_left -= s_left > 0 ? 1 : 0;
     };
-    // item Y of what step T reads for the next one: weights, activations, then (from the first step of a group) scales
-    const auto read = [&](auto t_tag, auto y_tag) {
-        constexpr int T = decltype(t_tag)::value, Y = decltype(y_tag)::value, B = T % NBUF, P = T & 1, H = (T / 4) & 1;
-        if constexpr (Y < CN) w[P][Y] = *reinterpret_cast<const v4i*>(w_at + B * S::BUF + Y * 1024);
-        else if constexpr (Y < CN + RM) a[P][Y - CN] = *reinterpret_cast<const v4i*>(a_at + B * S::BUF + (Y - CN) * 1024);
-        else if constexpr (Y < 2 * CN + RM) ws[H][Y - CN - RM] = *reinterpret_cast<const uint32_t*>(ws_at + H * S::SBUF + (Y - CN - RM) * 256);
-        else as[H][Y - 2 * CN - RM] = *reinterpret_cast<const uint32_t*>(as_at + H * S::SBUF + (Y - 2 * CN - RM) * 256);
+    const auto read_a = [&](uint32_t from, auto t_tag, auto i_tag) {
+        constexpr int B = decltype(t_tag)::value % 4, I = decltype(i_tag)::value;
+        a[I] = *reinterpret_cast<const v4i*>(a_at + from + B * S::BUF + I * 1024);
     };
+    const auto read_w = [&](uint32_t from, auto t_tag, auto j_tag) {
+        constexpr int T = decltype(t_tag)::value, B = T % 4, J = decltype(j_tag)::value;
+        w[T & 1][J] = *reinterpret_cast<const v4i*>(w_at + from + B * S::BUF + J * 1024);
+    };
+    const auto read_as = [&](uint32_t from, int i) { as[i] = *reinterpret_cast<const uint32_t*>(as_at + from + i * 256); };
+    const auto read_ws = [&](uint32_t from, int j) { ws[j] = *reinterpret_cast<const uint32_t*>(ws_at + from + j * 256); };
 
     // ---- prologue
     using C0 = std::integral_constant<int, 0>;
-    using C1 = std::integral_constant<int, 1>;
-    copy_scales(C0{});
-    static_for<2>([&](auto b) { static_for<S::COPIES>([&](auto c) { copy(b, c); }); });
-    copy_scales(C1{});
-    static_for<S::D - 2>([&](auto b) { static_for<S::COPIES>([&](auto c) { copy(std::integral_constant<int, decltype(b)::value + 2>{}, c); }); });
-#pragma unroll
-    for (int t = 0; t < RM * CN; ++t) acc[t / CN][t % CN] = v4f{0, 0, 0, 0};
+    steps_of(job);
+    scales_of(job);
+    int mblk = mblk_next, nblk = nblk_next, groups = groups_next;
+    int c_job = job, c_left = groups * 4; // steps that are still to be copied of c_job
+    const auto copied = [&](int n) { // n steps more (never past a tile's last): the next ones are the next tile's, or nobody's
+        c_left -= n;
+        if (c_left == 0) {
+            if (c_job + stride < of.jobs) {
+                steps_of(c_job += stride);
+                c_left = groups_next * 4;
+            } else { // (the last step again, for the count of loads)
+                k_off -= k_step;
+                k_step = 0;
+            }
+        }
+    };
+    copy_scales(0);
+    static_for<2>([&](auto b) { static_for<S::COPIES>([&](auto c) { copy(0, b, c); }); });
+    copy_scales(S::SBUF);
+    static_for<S::D - 2>([&](auto b) {
+        constexpr int B = decltype(b)::value + 2;
+        if constexpr (B == 4) copied(4);
+        static_for<S::COPIES>([&](auto c) { copy(B / 4 * 4 * S::BUF, std::integral_constant<int, B>{}, c); });
+    });
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S::D - 2) * S::COPIES) : "memory"); // steps 0 and 1, both groups of scales
-    static_for<2 * (RM + CN)>([&](auto y) { read(C0{}, y); });
+    static_for<RM>([&](auto i) { read_a(0, C0{}, i); });
+    static_for<CN>([&](auto j) { read_w(0, C0{}, j); });
+#pragma unroll
+    for (int i = 0; i < RM; ++i) read_as(0, i);
+#pragma unroll
+    for (int j = 0; j < CN; ++j) read_ws(0, j);
 
-    const auto step = [&](auto t_tag) {
-        constexpr int T = decltype(t_tag)::value, P = T & 1, H = (T / 4) & 1, MF = RM * CN;
-        using Next = std::integral_constant<int, (T + 1) % S::UNR>;
-        constexpr int READS = (RM + CN) * (T % 4 == 3 ? 2 : 1), COPIES = S::COPIES, ITEMS = READS + COPIES;
-        if constexpr (T % 4 == 0) copy_scales(std::integral_constant<int, H>{});
+    const auto step = [&](auto t_tag, auto fresh_tag) { // FRESH: the sums start here
+        constexpr int T = decltype(t_tag)::value, MF = RM * CN;
+        using Next = std::integral_constant<int, T + 1>;
+        const uint32_t from = T == 3 ? other(half) : half, to = T == 0 ? other(half) : half, s_from = S::SBUF - s_half;
+        constexpr int COPIES = S::COPIES, ITEMS = CN + COPIES, BOTH = COPIES < CN ? COPIES : CN;
+        if constexpr (T == 1) {
+            copied(4); // (the fourth of a group in the step before)
+            copy_scales(s_half);
+        }
         static_for<MF>([&](auto x_tag) {
-            constexpr int X = decltype(x_tag)::value, I = X / CN, J = I & 1 ? CN - 1 - X % CN : X % CN;
-            acc[I][J] = mx_mfma<T % 4>(w[P][J], a[P][I], acc[I][J], ws[H][J], as[H][I]);
+            // (rows there and back, so that one operand stays; the last one forth, whose scales are then replaced in order)
+            constexpr int X = decltype(x_tag)::value, I = X / CN, J = (I & 1) && I < RM - 1 ? CN - 1 - X % CN : X % CN;
+            if constexpr (decltype(fresh_tag)::value && T == 0) mx_mfma_first<T, in_acc(I)>(w[T & 1][J], a[I], acc[I][J], ws[J], as[I]);
+            else mx_mfma_in_place<T, in_acc(I)>(w[T & 1][J], a[I], acc[I][J], ws[J], as[I]);
             constexpr int FROM = X * ITEMS / MF, TO = (X + 1) * ITEMS / MF;
-            static_for<TO - FROM>([&](auto z_tag) {
+            static_for<TO - FROM>([&](auto z_tag) { // copies and reads of weights in turn while there are both
                 constexpr int Z = FROM + decltype(z_tag)::value;
-                // copies and reads in turn while there are copies
-                if constexpr (Z < 2 * COPIES && (Z & 1) == 0) copy(std::integral_constant<int, T + S::D>{}, std::integral_constant<int, Z / 2>{});
-                else read(Next{}, std::integral_constant<int, (Z < 2 * COPIES ? Z / 2 : Z - COPIES)>{});
+                if constexpr (Z < 2 * BOTH ? (Z & 1) == 0 : COPIES > CN)
+                    copy(to, std::integral_constant<int, T + S::D>{}, std::integral_constant<int, Z < 2 * BOTH ? Z / 2 : Z - CN>{});
+                else read_w(from, Next{}, std::integral_constant<int, Z < 2 * BOTH ? Z / 2 : Z - COPIES>{});
             });
+            // what its last product has used is replaced by the next step's
+            if constexpr (X % CN == CN - 1) read_a(from, Next{}, std::integral_constant<int, I>{});
+            if constexpr (T == 3 && X % CN == CN - 1) read_as(s_from, I);
+            if constexpr (T == 3 && I == RM - 1) read_ws(s_from, J);
             __builtin_amdgcn_sched_barrier(0);
         });
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::wait_for(T)) : "memory");
     };
-    for (int s = 0; s < steps; s += S::UNR)
-        static_while<S::UNR>([&](auto t) {
-            if (s + decltype(t)::value >= steps) return false;
-            step(t);
-            return true;
-        });
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // a load to LDS must not outlive the workgroup
+    for (;;) {
+        const auto group = [&](auto fresh_tag) {
+            static_for<4>([&](auto t) { step(t, fresh_tag); });
+            half = other(half);
+            s_half = S::SBUF - s_half;
+        };
+        group(std::true_type{});
+        for (int n = 1; n < groups; ++n) group(std::false_type{});
+        // the last products have to be through
+        asm volatile("s_nop 7\n\ts_nop 7" ::: "memory");
 
-    // ---- epilogue
-    const int m_first = ((int)mblk * 2 + wm) * RM * 16 + (lane & 15), col_first = ((int)nblk * 2 + wn) * CN;
-    if (parts > 1) { // partial tile in accumulator order: [tile][part][wave][tile of 16 x 16][lane]
-        v4f* to = reinterpret_cast<v4f*>(g.scratch) + (((size_t)tile * parts + kpart) * 4 + wave) * (RM * CN * 64) + lane;
-#pragma unroll
-        for (int t = 0; t < RM * CN; ++t) to[t * 64] = acc[t / CN][t % CN];
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < RM; ++i) {
-        const int m = m_first + i * 16;
-        if constexpr (SWIGLU) {
-#pragma unroll
-            for (int j = 0; j < CN; j += 4) {
+        const int m0 = (mblk * 2 + wm) * RM * 16, m_first = m0 + (lane & 15), col_first = (nblk * 2 + wn) * CN;
+        if (of.parts > 1) { // partial tile in accumulator order: [tile][part][wave][tile of 16 x 16][lane]
+            v4f* to = reinterpret_cast<v4f*>(g.scratch) + ((size_t)of.partial(job) * 4 + wave) * (RM * CN * 64) + lane;
+            static_for<RM * CN>([&](auto t) {
+                mx_settled<in_acc(t() / CN)>(acc[t() / CN][t() % CN]);
+                to[t() * 64] = acc[t() / CN][t() % CN];
+            });
+        } else if (SWIGLU && g.out_type == RKH_MX4_ROWS) {
+            static_for<RM * CN / 4>([&](auto t) {
+                constexpr int i = t() / (CN / 4), j = t() % (CN / 4) * 4;
+                const int m = m_first + i * 16, block = (col_first + j) / 4;
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = mx_silu(acc[i][j + (e >> 2)][e & 3], acc[i][j + 2 + (e >> 2)][e & 3]);
-                const int block = (col_first + j) / 4;
-                const bool live = m < g.M && block * 32 < g.N;
-                if (g.out_type == RKH_MX4_ROWS) mx_put_rows(g, m, block, live, v, lane);
-                else if (live) mx_put<8>(g, m, block * 32 + 8 * (lane >> 4), g.N, v);
-            }
+                for (int x = 0; x < 4; ++x) mx_settled<in_acc(i)>(acc[i][(j + x) % CN]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = mx_silu(acc[i][j + (e >> 2)][e & 3], acc[i][(j + 2 + (e >> 2)) % CN][e & 3]);
+                mx_put_rows(g, m, block, m < g.M && block * 32 < g.N, v, lane);
+            });
         } else {
+            constexpr int W = SWIGLU ? 4 : 2; // accumulators of a block of 32 columns
+            const bool whole = m0 + RM * 16 <= g.M && (col_first + CN) / W * 32 <= g.N;
+            mx_with_type(g.out_type, [&](auto type_tag) {
+                constexpr int TYPE = decltype(type_tag)::value;
+                using T = typename MxType<TYPE>::T;
+                const int n0 = col_first / W * 32 + 8 * (lane >> 4);
+                T* row = static_cast<T*>(g.C) + (size_t)m_first * g.ldc + n0;
+                const size_t rows16 = (size_t)16 * g.ldc;
+                const auto put = [&](auto whole_tag) {
+                    static_for<RM * CN / W>([&](auto t) {
+                        constexpr int i = t() / (CN / W), j = t() % (CN / W) * W;
+                        const int m = m_first + i * 16, n = n0 + j / W * 32;
+                        T* to = row + j / W * 32;
+                        if constexpr (j + W == CN) row += rows16;
+                        float v[8];
 #pragma unroll
-            for (int j = 0; j < CN; j += 2) {
-                float v[8];
+                        for (int x = 0; x < W; ++x) mx_settled<in_acc(i)>(acc[i][j + x]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = acc[i][j + (e >> 2)][e & 3];
-                if (m < g.M) mx_put<8>(g, m, (col_first + j) * 16 + 8 * (lane >> 4), g.N, v);
-            }
+                        for (int e = 0; e < 8; ++e) {
+                            v[e] = acc[i][j + (e >> 2)][e & 3];
+                            if constexpr (SWIGLU) v[e] = mx_silu(v[e], acc[i][(j + 2 + (e >> 2)) % CN][e & 3]);
+                        }
+                        if constexpr (decltype(whole_tag)::value) {
+                            mx_store<TYPE, 8>(to, 0, v);
+                        } else if (m < g.M) {
+                            if (n + 8 <= g.N) {
+                                mx_store<TYPE, 8>(to, 0, v);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    if (n + e < g.N) mx_store1<TYPE>(to, e, v[e]);
+                            }
+                        }
+                    });
+                };
+                if (whole) put(std::true_type{});
+                else put(std::false_type{});
+            });
         }
+        job += stride;
+        if (job >= of.jobs) break;
+        mblk = mblk_next, nblk = nblk_next, groups = groups_next; // (copies are less than a tile ahead)
+    }
+    // a load to LDS must not outlive the workgroup
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+template <int RM, int CN, int HALVES, bool SWIGLU>
+__global__ __launch_bounds__(256) void mx4_tile_kernel(rkh_mx4_gemm_args g, int mblocks, int nblocks, int parts) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    mx_tiles<RM, CN, HALVES, SWIGLU>(g, lds, MxJobs{mblocks, nblocks, parts, mblocks * nblocks * parts, 0, false}, blockIdx.x, gridDim.x);
+}
+
+// Whole tiles of 256 x 256 by one workgroup per compute unit, one after the other; what would be a last round for half of them or fewer goes as tiles of
+// 128 x 256, one each.
+template <bool SWIGLU>
+__global__ __launch_bounds__(256) void mx4_big_kernel(rkh_mx4_gemm_args g, int mblocks, int nblocks, int big) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int rest = mblocks * nblocks - big;
+    if ((int)blockIdx.x < big) mx_tiles<8, 8, 1, SWIGLU>(g, lds, MxJobs{mblocks, nblocks, 1, big, 0, false}, blockIdx.x, gridDim.x);
+    if ((int)blockIdx.x < 2 * rest) {
+        __syncthreads();
+        mx_tiles<4, 8, 1, SWIGLU>(g, lds, MxJobs{mblocks, nblocks, 1, 2 * rest, big, true}, blockIdx.x, 2 * rest);
     }
 }
 
@@ -385,10 +549,9 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(rkh_mx4_gemm_args g, int 
     const int tile = unit / UNITS, in_tile = unit - tile * UNITS;
     if (tile >= mblocks * nblocks) return;
     const int wave = in_tile / (RM * CN / W), u = in_tile % (RM * CN / W), i = u / (CN / W), j = u % (CN / W) * W;
-    constexpr unsigned GM = 4;
-    const unsigned per_group = GM * nblocks, grp = tile / per_group, first_m = grp * GM, gm = min(mblocks - first_m, GM);
-    const unsigned in_group = tile - grp * per_group, nblk = in_group / gm, mblk = first_m + in_group - nblk * gm;
-    const int m = (((int)mblk * 2 + (wave & 1)) * RM + i) * 16 + (lane & 15), col = ((int)nblk * 2 + (wave >> 1)) * CN + j;
+    int mblk, nblk;
+    mx_place(tile, mblocks, nblocks, mblk, nblk);
+    const int m = ((mblk * 2 + (wave & 1)) * RM + i) * 16 + (lane & 15), col = (nblk * 2 + (wave >> 1)) * CN + j;
 
     const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + ((size_t)tile * parts * 4 + wave) * (RM * CN * 64) + (i * CN + j) * 64 + lane;
     v4f s[W];
@@ -434,7 +597,7 @@ MxRoute mx_route(int M, int N, int K, int swiglu) {
         r.nblocks = (int)((cols + r.cn - 1) / r.cn);
         return r;
     }
-    static constexpr int SHAPES[][2] = {{8, 4}, {4, 4}, {2, 4}};
+    static constexpr int SHAPES[][2] = {{8, 8}, {8, 4}, {4, 4}, {2, 4}};
     for (const auto& s : SHAPES) {
         r.rm = s[0], r.cn = s[1];
         r.mblocks = (M + 32 * r.rm - 1) / (32 * r.rm);
@@ -468,17 +631,17 @@ int launch_few(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
     return RKH_OK;
 }
 
-template <int RM, int CN, int NBUF, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
-    constexpr int LDS = MxTile<RM, CN, NBUF>::LDS;
+template <int RM, int CN, int HALVES, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
+    constexpr int LDS = MxTile<RM, CN, HALVES>::LDS;
     static std::atomic<int> ready{0};
     if (!ready.load()) {
-        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_tile_kernel<RM, CN, NBUF, SWIGLU>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_tile_kernel<RM, CN, HALVES, SWIGLU>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
         ready.store(1);
     }
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
     if (tiles * r.parts > 0x7fffffff) return RKH_ERR_RUNTIME;
     mark(st, "mx4_tile_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_tile_kernel<RM, CN, NBUF, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks,
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_tile_kernel<RM, CN, HALVES, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks,
                        r.nblocks, r.parts);
     RKH_CHECK(hipGetLastError());
     if (r.parts > 1) {
@@ -487,6 +650,21 @@ template <int RM, int CN, int NBUF, bool SWIGLU> int launch_tiles(hipStream_t st
                            r.mblocks, r.nblocks, r.parts);
         RKH_CHECK(hipGetLastError());
     }
+    return RKH_OK;
+}
+
+template <bool SWIGLU> int launch_big(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
+    constexpr int LDS = MxTile<8, 8, 1>::LDS;
+    static std::atomic<int> ready{0};
+    if (!ready.load()) {
+        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_big_kernel<SWIGLU>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+        ready.store(1);
+    }
+    const int64_t tiles = (int64_t)r.mblocks * r.nblocks, left = tiles % MX_CUS, big = left <= MX_CUS / 2 ? tiles - left : tiles;
+    if (tiles > 0x3fffffff) return RKH_ERR_RUNTIME;
+    mark(st, "mx4_big_kernel");
+    hipLaunchKernelGGL(mx4_big_kernel<SWIGLU>, dim3((unsigned)(big ? std::min<int64_t>(big, MX_CUS) : 2 * left)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, (int)big);
+    RKH_CHECK(hipGetLastError());
     return RKH_OK;
 }
 
@@ -507,8 +685,8 @@ template <bool SWIGLU> int launch(hipStream_t st, const rkh_mx4_gemm_args& g) {
         }
     }
     if (mx_scratch(r) > (g.scratch ? g.scratch_bytes : 0)) r.parts = 1;
-    if (r.rm == 8) return launch_tiles<8, 4, 4, SWIGLU>(st, g, r);
-    return r.rm == 4 ? launch_tiles<4, 4, 4, SWIGLU>(st, g, r) : launch_tiles<2, 4, 8, SWIGLU>(st, g, r);
+    if (r.rm == 8) return r.cn == 8 ? launch_big<SWIGLU>(st, g, r) : launch_tiles<8, 4, 1, SWIGLU>(st, g, r);
+    return r.rm == 4 ? launch_tiles<4, 4, 1, SWIGLU>(st, g, r) : launch_tiles<2, 4, 2, SWIGLU>(st, g, r);
 }
 
 } // namespace

@@ -75,7 +75,7 @@ __device__ __forceinline__ void norm_out(const rkh_block_norm_args& a, int m, in
         const uint32_t scale = mx_scale(mx_top_of_quad(mx_top(r)));
         const int b = k >> 5;
         if (b * 32 < a.D) {
-            *reinterpret_cast<uint32_t*>(a.q + mx_code_at(m, b, (int)rkh_mx4_ks(a.D)) + (k & 31) / 2) = mx_codes(r, scale);
+            *reinterpret_cast<uint32_t*>(a.q + mx_code_at(m, b, (int)rkh_mx4_k4(a.D)) + (k & 31) / 2) = mx_codes(r, scale);
             if ((k & 31) == 0) a.q_scale[mx_scale_at(m, b, (int)rkh_mx4_k4(a.D))] = (uint8_t)scale;
         }
     }

@@ -9,10 +9,10 @@
  * b * 16 (value 2 i in the low half of byte i, value 2 i + 1 in the high one) and one scale byte.
  *
  * "Operand blocks" (activations in a workspace, weights): 1 KiB pieces of 16 rows x 128 k.  Piece (rb, ks) starts at
- * (rb * KS + ks) * 1024, KS = ceil(K / 128); inside it lane l = r + 16 q owns the 16 bytes at l * 16, the codes of block
+ * (4 K4 rb + ks) * 1024, K4 = ceil(K / 512); inside it lane l = r + 16 q owns the 16 bytes at l * 16, the codes of block
  * 4 ks + q of row 16 rb + r.  One 16-byte load per lane is an operand of v_mfma_scale_f32_16x16x128_f8f6f4, whose lane
  * (r, q) holds 32 consecutive k of one row: an MX block exactly, with its one scale.  The scales of four consecutive
- * pieces share a dword: (rb, ks, l) is byte ks % 4 of the dword ((rb * K4 + ks / 4) * 64 + l), K4 = ceil(KS / 4), and the
+ * pieces share a dword: (rb, ks, l) is byte ks % 4 of the dword ((rb * K4 + ks / 4) * 64 + l), and the
  * product takes the byte by its operand select.  Blocks beyond K hold zeros.
  *
  * Weights: the rows of the operand blocks are output columns, in an order that leaves each lane of an accumulator eight
@@ -33,7 +33,7 @@ enum rkh_mx4_type { RKH_MX4_F32 = 0, RKH_MX4_F16 = 1, RKH_MX4_BF16 = 2, RKH_MX4_
 static inline RKH_HD int64_t rkh_mx4_ks(int64_t K) { return (K + 127) / 128; }
 static inline RKH_HD int64_t rkh_mx4_k4(int64_t K) { return (K + 511) / 512; }
 /* Bytes of the operand blocks of `rows` rows, and of their scales. */
-static inline size_t rkh_mx4_code_bytes(int64_t rows, int64_t K) { return (size_t)((rows + 15) / 16 * rkh_mx4_ks(K)) * 1024; }
+static inline size_t rkh_mx4_code_bytes(int64_t rows, int64_t K) { return (size_t)((rows + 15) / 16 * rkh_mx4_k4(K)) * 4096; }
 static inline size_t rkh_mx4_scale_bytes(int64_t rows, int64_t K) { return (size_t)((rows + 15) / 16 * rkh_mx4_k4(K)) * 256; }
 /* Columns that the operand blocks of a weight matrix hold: N, or 2 * align32(F) for gate / up pairs. */
 static inline RKH_HD int64_t rkh_mx4_columns(int64_t N, int gate_up) { return gate_up ? 2 * rkh_align_up(N / 2, 32) : rkh_align_up(N, 32); }

@@ -116,3 +116,18 @@ def test_reference_of_the_format():
     again = ref.quantize(ref.values(codes, scales, 70))
     live = ref.values(codes, scales, 96).reshape(5, 96)
     assert np.array_equal(again[1], scales) and np.array_equal(ref.values(*again, 96), live)
+
+
+def test_audit_sees_sums_in_accumulation_registers():
+    """A product from asm whose sum is moved before it is through is reported, in either half of the registers."""
+    from rknpu2_matmul_open_amd import audit_waits
+
+    def kernel(behind):
+        return "\n".join(["_Z14mx4_big_kernelv:", "\tv_mov_b32_e32 v1, 0", ";;#ASMSTART",
+                          "\tv_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[8:11], v[12:15], a[4:7], v20, v21 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4",
+                          ";;#ASMEND"] + behind + ["\ts_endpgm", ".Lfunc_end0:"])
+    move = "\tv_accvgpr_read_b32 v30, a5"
+    assert len(audit_waits.audit_text(kernel([move]))[0]) == 1
+    assert len(audit_waits.audit_text(kernel(["\ts_nop 7", move]))[0]) == 1
+    assert audit_waits.audit_text(kernel(["\ts_nop 7", "\ts_nop 7", move])) == ([], 1)
+    assert audit_waits.audit_text(kernel(["\tv_accvgpr_read_b32 v30, a8"])) == ([], 1)
