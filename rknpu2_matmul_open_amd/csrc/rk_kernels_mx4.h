@@ -115,6 +115,29 @@ __device__ __forceinline__ uint32_t mx_top_of_quad(uint32_t top) {
     return max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, true)); // lanes 2 3 0 1
 }
 
+// ---- norms.  The sum of squares of a row has one order wherever it is made: eight values of a lane one after the other, 64 lanes
+// as a butterfly -- a segment of 512 values --, segments one after the other.
+__device__ __forceinline__ float mx_squares(const float (&v)[8], float sum) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+    return sum;
+}
+__device__ __forceinline__ float mx_segment_sum(float x) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
+    return x;
+}
+__device__ __forceinline__ float mx_sum_of_segments(const float* part, int segments) {
+    float sum = part[0];
+    for (int s = 1; s < segments; ++s) sum += part[s];
+    return sum;
+}
+__device__ __forceinline__ float mx_norm_factor(float sum, int D, float eps) { return 1.0f / sqrtf(sum / (float)D + eps); }
+__device__ __forceinline__ void mx_normed(float (&v)[8], float factor, bool weighted, const float (&weight)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = weighted ? v[e] * factor * weight[e] : v[e] * factor;
+}
+
 // Byte offsets of block b of row m in operand blocks.
 __device__ __forceinline__ size_t mx_code_at(int m, int b, int K4) {
     return ((size_t)(m >> 4) * K4 * 4 + (b >> 2)) * 1024 + (m & 15) * 16 + (b & 3) * 256;

@@ -50,18 +50,24 @@ template <bool ACC> __device__ __forceinline__ void mx_settled(v4f& sum) {
 
 __device__ __forceinline__ float mx_silu(float gate, float up) { return __fmul_rn(silu_poly(gate), up); }
 
-// N (4 or 8) consecutive columns from n on of row m, of which those below `end` exist.
-template <int N> __device__ __forceinline__ void mx_put(const rkh_mx4_gemm_args& g, int m, int n, int end, const float* v) {
+// N (4 or 8) consecutive values to where `to` points, of which `count` exist.  (Instructions that are not yet in the cache cost small
+// calls more than those that run: the part of a row's end is a loop.)
+template <int TYPE, int N> __device__ __forceinline__ void mx_put(void* to, int count, float (&v)[N]) {
+    if (count >= N) {
+        mx_store<TYPE, N>(to, 0, v);
+    } else {
+#pragma unroll 1
+        for (int e = 0; e < count; ++e) {
+            mx_store1<TYPE>(to, e, v[0]);
+#pragma unroll
+            for (int i = 0; i + 1 < N; ++i) v[i] = v[i + 1];
+        }
+    }
+}
+template <int N> __device__ __forceinline__ void mx_put(const rkh_mx4_gemm_args& g, int m, int n, float (&v)[N]) {
     mx_with_type(g.out_type, [&](auto t) {
         constexpr int TYPE = decltype(t)::value;
-        const size_t at = (size_t)m * g.ldc + n;
-        if (n + N <= end) {
-            mx_store<TYPE, N>(g.C, at, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (n + e < end) mx_store1<TYPE>(g.C, at + e, v[e]);
-        }
+        mx_put<TYPE, N>(static_cast<typename MxType<TYPE>::T*>(g.C) + (size_t)m * g.ldc + n, g.N - n, v);
     });
 }
 
@@ -78,117 +84,183 @@ __device__ __forceinline__ void mx_put_rows(const rkh_mx4_gemm_args& g, int m, i
 
 // ---- few rows ----------------------------------------------------------------------
 // One workgroup multiplies all rows with 16 * CN places; its waves split K in groups of 512 and are summed through LDS.  Every weight
-// byte is loaded once, straight into registers, a group (CN * 4 KiB per wave) ahead of its products.
-// FUSED: the rows are given as values, and every workgroup quantizes them for itself while its first weights are on their way.
-constexpr int FEW_FUSED_LDS = 64 * 1024;
+// byte is loaded once, straight into registers, NG groups of a wave together: all of its share unless K is very long.
+// FUSED: the rows are given as values, and every workgroup quantizes them for itself (2: norms them first), behind its first weights'
+// loads: those wait to leave for as long as the stream takes, the last of them almost to its end.  (Waves of their own that quantize have their
+// loads behind everyone's weights: 1 x 4096 -> 14336 7.6 -> 11.3 us.  A launch in front costs 3.)
+__host__ __device__ constexpr int few_row_bytes(int K4) { return K4 * (256 + 16 + 4); } // codes, scales, sums of squares
 
-template <int RM, int CN, int MAX_WAVES, bool SWIGLU, bool FUSED>
-__global__ __launch_bounds__(MAX_WAVES * 64) void mx4_few_kernel(rkh_mx4_gemm_args g, int per_wave) {
+struct MxFewRows { // the workgroup's rows in LDS
+    uint8_t* codes;  // block b of row r: 16 bytes at (b * M + r) * 16
+    uint8_t* scales; // a lane's four of a group: one dword
+    float* squares;  // [row][segment of 512]
+    int M, K4;
+    __device__ MxFewRows(uint8_t* lds, int rows, int k4)
+        : codes(lds), scales(lds + k4 * rows * 256), squares(reinterpret_cast<float*>(scales + k4 * rows * 16)), M(rows), K4(k4) {}
+    __device__ __forceinline__ void put(int r, int piece, const float (&v)[8]) const { // (four lanes of a block together)
+        const uint32_t scale = mx_scale(mx_top_of_quad(mx_top(v)));
+        const int b = piece >> 2;
+        *reinterpret_cast<uint32_t*>(codes + (b * M + r) * 16 + (piece & 3) * 4) = mx_codes(v, scale);
+        if ((piece & 3) == 0) scales[(((b >> 4) * M + r) * 4 + (b & 3)) * 4 + ((b >> 2) & 3)] = (uint8_t)scale;
+    }
+};
+
+// Quantizes the rows into `to` with `threads` threads; `between` runs behind the first loads.  A wave's 64 pieces of eight values are a segment of one
+// row.  K is a multiple of eight.  PIECES: of a thread, that are fetched ahead.
+template <int TYPE, int PIECES, bool NORM, class Between>
+__device__ __forceinline__ void mx_few_quantize(const rkh_mx4_gemm_args& g, const MxFewRows& to, int threads, Between&& between) {
+    const int per_row = to.K4 * 64, total = per_row * to.M, t = threadIdx.x;
+    const auto row_of = [&](int i) { return to.M == 1 ? 0 : (int)((unsigned)i / (unsigned)per_row); };
+    const auto fetch = [&](int i) {
+        const int r = row_of(i), k = (i - r * per_row) * 8;
+        MxRaw<TYPE> raw = {};
+        if (i < total && k < g.K) raw = mx_fetch8<TYPE>(g.x, (size_t)r * g.ldx + k);
+        return raw;
+    };
+    const auto weight_of = [&](int i) {
+        const int k = (i - row_of(i) * per_row) * 8;
+        MxRaw<RKH_MX4_F32> raw = {};
+        if (i < total && k < g.K) raw = mx_fetch8<RKH_MX4_F32>(g.x_weight, k);
+        return raw;
+    };
+    MxRaw<TYPE> raw[PIECES];
+    MxRaw<RKH_MX4_F32> weight[PIECES];
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) raw[u] = fetch(t + u * threads);
+    if (NORM && g.x_weight) {
+#pragma unroll
+        for (int u = 0; u < PIECES; ++u) weight[u] = weight_of(t + u * threads);
+    }
+    // (a wave's share of the rows would queue behind the weights of those that are ahead of it, and all wait for the last)
+    asm volatile("s_barrier" ::: "memory");
+    between();
+    const auto each = [&](auto&& f) { // f(piece, values, its place among those fetched ahead or -1)
+        static_for<PIECES>([&](auto u) {
+            if (t + u() * threads >= total) return;
+            float v[8];
+            mx_unpack<TYPE>(raw[u()], v);
+            f(t + u() * threads, v, u);
+        });
+#pragma unroll 1
+        for (int i = t + PIECES * threads; i < total; i += threads) {
+            float v[8];
+            mx_unpack<TYPE>(fetch(i), v);
+            f(i, v, std::integral_constant<int, -1>{});
+        }
+    };
+    if constexpr (NORM) {
+        each([&](int i, float (&v)[8], auto) {
+            const float sum = mx_segment_sum(mx_squares(v, 0.0f));
+            if (lane_id() == 0) to.squares[i >> 6] = sum;
+        });
+        __syncthreads();
+        each([&](int i, float (&v)[8], auto ahead) {
+            constexpr int U = decltype(ahead)::value;
+            const int r = row_of(i);
+            const float factor = mx_norm_factor(mx_sum_of_segments(to.squares + r * to.K4, to.K4), g.K, g.x_eps);
+            float w[8];
+            if (g.x_weight) {
+                if constexpr (U >= 0) mx_unpack<RKH_MX4_F32>(weight[U], w);
+                else mx_unpack<RKH_MX4_F32>(weight_of(i), w);
+            }
+            mx_normed(v, factor, g.x_weight != nullptr, w);
+            to.put(r, i - r * per_row, v);
+        });
+    } else {
+        each([&](int i, float (&v)[8], auto) {
+            const int r = row_of(i);
+            to.put(r, i - r * per_row, v);
+        });
+    }
+    __syncthreads();
+}
+
+// (Leading scalar arguments arrive in registers; the structure takes a round trip to memory, which its users here can wait for.
+// FUSED: a_scale is the rows' stride.)
+// X: the rows' type.
+template <int RM, int CN, int NG, int MAX_WAVES, bool SWIGLU, int FUSED, int X>
+__global__ __launch_bounds__(MAX_WAVES * 64, RM == 1 ? 4 : 1) void mx4_few_kernel(const uint8_t* W, const uint8_t* w_scale, const void* rows, const uint8_t* a_scale, int M, int N,
+                                                                                 int K, int per_wave, int workgroups, int waves, rkh_mx4_gemm_args g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     static_assert(!SWIGLU || CN == 4, "gate and up halves of a block of 32 columns");
     static_assert(!FUSED || RM == 1, "rows as given: up to 16");
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), waves = blockDim.x >> 6;
-    const int KS = (int)rkh_mx4_ks(g.K), K4 = (int)rkh_mx4_k4(g.K);
-    const int col0 = xcd_remap(blockIdx.x, gridDim.x) * CN; // first of the workgroup's operands of weights
-    const int cols = (int)rkh_mx4_columns(SWIGLU ? 2 * g.N : g.N, SWIGLU) / 16;
-    const int rblocks = (g.M + 15) / 16;
+    g.M = M, g.N = N, g.K = K;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+    const int KS = (int)rkh_mx4_ks(K), K4 = (int)rkh_mx4_k4(K);
+    const int col0 = xcd_remap(blockIdx.x, workgroups) * CN; // first of the workgroup's operands of weights
+    const int cols = (int)rkh_mx4_columns(SWIGLU ? 2 * N : N, SWIGLU) / 16;
     const int first = wave * per_wave, last = min(first + per_wave, K4); // groups of 512 k
 
-    v4i w[4][CN];
-    uint32_t ws[CN];
-    const auto load_w = [&](int group) {
+    v4i w[NG][4][CN], a[NG][4][RM];
+    uint32_t ws[NG][CN], as[NG][RM];
+    // (groups beyond the last: that one again, multiplied with nothing.  Pieces beyond K: the activations' are zeros, any weights will do)
+    const auto load = [&](int from, auto s0, auto s1) { // steps s0 .. s1 - 1 of each group, the scales behind the last
+        static_for<NG>([&](auto p_tag) {
+            constexpr int P = decltype(p_tag)::value;
+            const int group = min(from + P, K4 - 1);
 #pragma unroll
-        for (int j = 0; j < CN; ++j) {
-            const int col = min(col0 + j, cols - 1);
-            const uint8_t* src = g.W + ((size_t)col * K4 + group) * 4096 + lane * 16;
+            for (int s = s0(); s < s1(); ++s) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) w[s][j] = *reinterpret_cast<const v4i*>(src + (group * 4 + s < KS ? s * 1024 : 0));
-            ws[j] = reinterpret_cast<const uint32_t*>(g.w_scale)[((size_t)col * K4 + group) * 64 + lane];
-        }
-    };
-
-    if constexpr (FUSED) {
-        // Blocks b of row r: 16 bytes at (b * M + r) * 16; their scales behind them, so that a lane's four of a group are a dword.
-        uint8_t* lds_scales = lds + (size_t)KS * 4 * g.M * 16;
-        mx_with_type(g.x_type, [&](auto t) {
-            constexpr int TYPE = decltype(t)::value;
-            const int per_row = KS * 16, total = per_row * g.M; // pieces of eight values
-            const auto fetch = [&](int i) {
-                const int r = i / per_row, k = (i - r * per_row) * 8;
-                const size_t at = (size_t)r * g.ldx + k;
-                return k + 8 <= g.K ? mx_fetch8<TYPE>(g.x, at) : mx_fetch_some<TYPE>(g.x, at, g.K - k);
-            };
-            const auto put = [&](int i, const MxRaw<TYPE>& raw) {
-                const int r = i / per_row, piece = i - r * per_row, b = piece >> 2;
-                float v[8];
-                mx_unpack<TYPE>(raw, v);
-                const uint32_t scale = mx_scale(mx_top_of_quad(mx_top(v)));
-                *reinterpret_cast<uint32_t*>(lds + ((size_t)b * g.M + r) * 16 + (piece & 3) * 4) = mx_codes(v, scale);
-                if ((piece & 3) == 0) lds_scales[(((b >> 4) * g.M + r) * 4 + (b & 3)) * 4 + ((b >> 2) & 3)] = (uint8_t)scale;
-            };
-            int i = threadIdx.x;
-            MxRaw<TYPE> raw = {};
-            if (i < total) raw = fetch(i);
-            if (first < last) load_w(first);
-            for (; i < total; i += blockDim.x) {
-                MxRaw<TYPE> next = {};
-                if (i + (int)blockDim.x < total) next = fetch(i + blockDim.x);
-                put(i, raw);
-                raw = next;
+                for (int j = 0; j < CN; ++j)
+                    w[P][s][j] = *reinterpret_cast<const v4i*>(W + ((size_t)min(col0 + j, cols - 1) * K4 + group) * 4096 + (group * 4 + s < KS ? s * 1024 : 0) + lane * 16);
+                if constexpr (!FUSED) {
+#pragma unroll
+                    for (int i = 0; i < RM; ++i)
+                        a[P][s][i] = *reinterpret_cast<const v4i*>(static_cast<const uint8_t*>(rows) + ((size_t)min(i, (M - 1) >> 4) * K4 + group) * 4096 + s * 1024 + lane * 16);
+                }
+            }
+            if constexpr (s1() == 4) {
+#pragma unroll
+                for (int j = 0; j < CN; ++j) ws[P][j] = reinterpret_cast<const uint32_t*>(w_scale)[((size_t)min(col0 + j, cols - 1) * K4 + group) * 64 + lane];
+                if constexpr (!FUSED) {
+#pragma unroll
+                    for (int i = 0; i < RM; ++i) as[P][i] = reinterpret_cast<const uint32_t*>(a_scale)[((size_t)min(i, (M - 1) >> 4) * K4 + group) * 64 + lane];
+                }
             }
         });
-        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using S0 = std::integral_constant<int, 0>;
+    using S4 = std::integral_constant<int, 4>;
+    // what goes out ahead of the rows' quantization: half of the weights where they are many
+    using Ahead = std::integral_constant<int, CN * NG >= 4 ? 2 : 4>;
+    v4f* sums = reinterpret_cast<v4f*>(lds);
+    const MxFewRows staged(lds + waves * RM * CN * 1024, M, K4);
+    if constexpr (FUSED) {
+        g.x = rows;
+        g.ldx = (int64_t)reinterpret_cast<intptr_t>(a_scale);
+        mx_few_quantize<X, CN == 4 ? 1 : 2, FUSED == 2>(g, staged, waves * 64, [&]() { load(first, S0{}, Ahead{}); });
+        if constexpr (Ahead::value < 4) load(first, Ahead{}, S4{});
     } else {
-        if (first < last) load_w(first);
+        load(first, S0{}, S4{});
     }
 
     v4f acc[RM][CN];
 #pragma unroll
     for (int t = 0; t < RM * CN; ++t) acc[t / CN][t % CN] = v4f{0, 0, 0, 0};
-    for (int group = first; group < last; ++group) {
-        v4i a[4][RM];
-        uint32_t as[RM];
-#pragma unroll
-        for (int i = 0; i < RM; ++i) {
-            if constexpr (FUSED) {
-                const int r = lane & 15, q = lane >> 4;
-                const bool live = r < g.M;
-                const uint8_t* lds_scales = lds + (size_t)KS * 4 * g.M * 16;
-                as[i] = live ? *reinterpret_cast<const uint32_t*>(lds_scales + ((group * g.M + r) * 4 + q) * 4) : 0;
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-                    a[s][i] = live && group * 4 + s < KS ? *reinterpret_cast<const v4i*>(lds + ((size_t)((group * 4 + s) * 4 + q) * g.M + r) * 16) : v4i{0, 0, 0, 0};
-            } else {
-                const int rb = min(i, rblocks - 1);
-                const uint8_t* src = g.A + ((size_t)rb * K4 + group) * 4096 + lane * 16;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) a[s][i] = *reinterpret_cast<const v4i*>(src + (group * 4 + s < KS ? s * 1024 : 0));
-                as[i] = reinterpret_cast<const uint32_t*>(g.a_scale)[((size_t)rb * K4 + group) * 64 + lane];
-            }
-        }
-        v4i wc[4][CN];
-        uint32_t wsc[CN];
-#pragma unroll
-        for (int j = 0; j < CN; ++j) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) wc[s][j] = w[s][j];
-            wsc[j] = ws[j];
-        }
-        if (group + 1 < last) load_w(group + 1);
-        static_for<4>([&](auto s_tag) {
-            constexpr int S = decltype(s_tag)::value;
-            if (group * 4 + S < KS) {
+    const bool live = (lane & 15) < M;
+    for (int from = first;;) {
+        static_for<NG>([&](auto p_tag) {
+            constexpr int P = decltype(p_tag)::value;
+            const int group = from + P;
+            if (group >= last) return;
+            if constexpr (FUSED) as[P][0] = live ? *reinterpret_cast<const uint32_t*>(staged.scales + ((group * M + (lane & 15)) * 4 + (lane >> 4)) * 4) : 0;
+            static_for<4>([&](auto s_tag) {
+                constexpr int S = decltype(s_tag)::value;
+                if constexpr (FUSED)
+                    a[P][S][0] = live ? *reinterpret_cast<const v4i*>(staged.codes + (((group * 4 + S) * 4 + (lane >> 4)) * M + (lane & 15)) * 16) : v4i{0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < RM; ++i)
 #pragma unroll
-                    for (int j = 0; j < CN; ++j) acc[i][j] = mx_mfma<S>(wc[S][j], a[S][i], acc[i][j], wsc[j], as[i]);
-            }
+                    for (int j = 0; j < CN; ++j) acc[i][j] = mx_mfma<S>(w[P][S][j], a[P][S][i], acc[i][j], ws[P][j], as[P][i]);
+            });
         });
+        from += NG;
+        if (from >= last) break;
+        load(from, S0{}, S4{});
     }
 
     // the waves' sums, added in order: thread (tile, lane) takes the tile's place `lane`
-    v4f* sums = reinterpret_cast<v4f*>(lds);
-    if constexpr (FUSED) __syncthreads();
 #pragma unroll
     for (int t = 0; t < RM * CN; ++t) sums[(wave * RM * CN + t) * 64 + lane] = acc[t / CN][t % CN];
     __syncthreads();
@@ -197,8 +269,8 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void mx4_few_kernel(rkh_mx4_gemm_ar
             v4f s = sums[t * 64 + lane];
             for (int o = 1; o < waves; ++o) s += sums[(o * RM * CN + t) * 64 + lane];
             const int m = t / CN * 16 + (lane & 15), col = col0 + t % CN;
-            const float v[4] = {s.x, s.y, s.z, s.w};
-            if (m < g.M && col < cols) mx_put<4>(g, m, (col >> 1) * 32 + 8 * (lane >> 4) + 4 * (col & 1), g.N, v);
+            float v[4] = {s.x, s.y, s.z, s.w};
+            if (m < M && col < cols) mx_put<4>(g, m, (col >> 1) * 32 + 8 * (lane >> 4) + 4 * (col & 1), v);
         }
     } else {
         for (int i = wave; i < RM; i += waves) {
@@ -212,8 +284,8 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void mx4_few_kernel(rkh_mx4_gemm_ar
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = mx_silu(s[e >> 2][e & 3], s[2 + (e >> 2)][e & 3]);
             const int m = i * 16 + (lane & 15), block = col0 / 4;
-            if (g.out_type == RKH_MX4_ROWS) mx_put_rows(g, m, block, m < g.M, v, lane);
-            else if (m < g.M) mx_put<8>(g, m, block * 32 + 8 * (lane >> 4), g.N, v);
+            if (g.out_type == RKH_MX4_ROWS) mx_put_rows(g, m, block, m < M, v, lane);
+            else if (m < M) mx_put<8>(g, m, block * 32 + 8 * (lane >> 4), v);
         }
     }
 }
@@ -294,7 +366,7 @@ struct MxJobs {
 
 // Multiplies jobs job, job + stride, ...  Their steps follow one another: the copies that run ahead of a tile's end are the next
 // tile's first, and land while the tile is converted and stored.
-template <int RM, int CN, int HALVES, bool SWIGLU>
+template <int RM, int CN, int HALVES, bool SWIGLU, int OUT>
 __device__ __forceinline__ void mx_tiles(const rkh_mx4_gemm_args& g, uint8_t* lds, const MxJobs& of, int job, int stride) {
     using S = MxTile<RM, CN, HALVES>;
     static_assert(!SWIGLU || CN % 4 == 0, "gate and up halves of blocks of 32 columns in one wave");
@@ -463,55 +535,29 @@ __device__ __forceinline__ void mx_tiles(const rkh_mx4_gemm_args& g, uint8_t* ld
                 mx_settled<in_acc(t() / CN)>(acc[t() / CN][t() % CN]);
                 to[t() * 64] = acc[t() / CN][t() % CN];
             });
-        } else if (SWIGLU && g.out_type == RKH_MX4_ROWS) {
-            static_for<RM * CN / 4>([&](auto t) {
-                constexpr int i = t() / (CN / 4), j = t() % (CN / 4) * 4;
-                const int m = m_first + i * 16, block = (col_first + j) / 4;
-                float v[8];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) mx_settled<in_acc(i)>(acc[i][(j + x) % CN]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = mx_silu(acc[i][j + (e >> 2)][e & 3], acc[i][(j + 2 + (e >> 2)) % CN][e & 3]);
-                mx_put_rows(g, m, block, m < g.M && block * 32 < g.N, v, lane);
-            });
         } else {
             constexpr int W = SWIGLU ? 4 : 2; // accumulators of a block of 32 columns
-            const bool whole = m0 + RM * 16 <= g.M && (col_first + CN) / W * 32 <= g.N;
-            mx_with_type(g.out_type, [&](auto type_tag) {
-                constexpr int TYPE = decltype(type_tag)::value;
-                using T = typename MxType<TYPE>::T;
-                const int n0 = col_first / W * 32 + 8 * (lane >> 4);
-                T* row = static_cast<T*>(g.C) + (size_t)m_first * g.ldc + n0;
-                const size_t rows16 = (size_t)16 * g.ldc;
-                const auto put = [&](auto whole_tag) {
-                    static_for<RM * CN / W>([&](auto t) {
-                        constexpr int i = t() / (CN / W), j = t() % (CN / W) * W;
-                        const int m = m_first + i * 16, n = n0 + j / W * 32;
-                        T* to = row + j / W * 32;
-                        if constexpr (j + W == CN) row += rows16;
-                        float v[8];
+            const int n0 = col_first / W * 32 + 8 * (lane >> 4);
+            using T = typename MxType<OUT == RKH_MX4_ROWS ? RKH_MX4_F32 : OUT>::T;
+            T* row = static_cast<T*>(g.C) + (size_t)m_first * g.ldc + n0;
+            const size_t rows16 = (size_t)16 * g.ldc;
+            static_for<RM * CN / W>([&](auto t) {
+                constexpr int i = t() / (CN / W), j = t() % (CN / W) * W;
+                const int m = m_first + i * 16, n = n0 + j / W * 32;
+                float v[8];
 #pragma unroll
-                        for (int x = 0; x < W; ++x) mx_settled<in_acc(i)>(acc[i][j + x]);
+                for (int x = 0; x < W; ++x) mx_settled<in_acc(i)>(acc[i][j + x]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            v[e] = acc[i][j + (e >> 2)][e & 3];
-                            if constexpr (SWIGLU) v[e] = mx_silu(v[e], acc[i][(j + 2 + (e >> 2)) % CN][e & 3]);
-                        }
-                        if constexpr (decltype(whole_tag)::value) {
-                            mx_store<TYPE, 8>(to, 0, v);
-                        } else if (m < g.M) {
-                            if (n + 8 <= g.N) {
-                                mx_store<TYPE, 8>(to, 0, v);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    if (n + e < g.N) mx_store1<TYPE>(to, e, v[e]);
-                            }
-                        }
-                    });
-                };
-                if (whole) put(std::true_type{});
-                else put(std::false_type{});
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = acc[i][j + (e >> 2)][e & 3];
+                    if constexpr (SWIGLU) v[e] = mx_silu(v[e], acc[i][(j + 2 + (e >> 2)) % CN][e & 3]);
+                }
+                if constexpr (OUT == RKH_MX4_ROWS) {
+                    mx_put_rows(g, m, n >> 5, m < g.M && (n & ~31) < g.N, v, lane);
+                } else {
+                    if (m < g.M) mx_put<OUT, 8>(row + j / W * 32, g.N - n, v);
+                    if constexpr (j + W == CN) row += rows16;
+                }
             });
         }
         job += stride;
@@ -522,22 +568,22 @@ __device__ __forceinline__ void mx_tiles(const rkh_mx4_gemm_args& g, uint8_t* ld
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int RM, int CN, int HALVES, bool SWIGLU>
+template <int RM, int CN, int HALVES, bool SWIGLU, int OUT>
 __global__ __launch_bounds__(256) void mx4_tile_kernel(rkh_mx4_gemm_args g, int mblocks, int nblocks, int parts) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    mx_tiles<RM, CN, HALVES, SWIGLU>(g, lds, MxJobs{mblocks, nblocks, parts, mblocks * nblocks * parts, 0, false}, blockIdx.x, gridDim.x);
+    mx_tiles<RM, CN, HALVES, SWIGLU, OUT>(g, lds, MxJobs{mblocks, nblocks, parts, mblocks * nblocks * parts, 0, false}, blockIdx.x, gridDim.x);
 }
 
 // Whole tiles of 256 x 256 by one workgroup per compute unit, one after the other; what would be a last round for half of them or fewer goes as tiles of
 // 128 x 256, one each.
-template <bool SWIGLU>
+template <bool SWIGLU, int OUT>
 __global__ __launch_bounds__(256) void mx4_big_kernel(rkh_mx4_gemm_args g, int mblocks, int nblocks, int big) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int rest = mblocks * nblocks - big;
-    if ((int)blockIdx.x < big) mx_tiles<8, 8, 1, SWIGLU>(g, lds, MxJobs{mblocks, nblocks, 1, big, 0, false}, blockIdx.x, gridDim.x);
+    if ((int)blockIdx.x < big) mx_tiles<8, 8, 1, SWIGLU, OUT>(g, lds, MxJobs{mblocks, nblocks, 1, big, 0, false}, blockIdx.x, gridDim.x);
     if ((int)blockIdx.x < 2 * rest) {
         __syncthreads();
-        mx_tiles<4, 8, 1, SWIGLU>(g, lds, MxJobs{mblocks, nblocks, 1, 2 * rest, big, true}, blockIdx.x, 2 * rest);
+        mx_tiles<4, 8, 1, SWIGLU, OUT>(g, lds, MxJobs{mblocks, nblocks, 1, 2 * rest, big, true}, blockIdx.x, 2 * rest);
     }
 }
 
@@ -569,11 +615,11 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(rkh_mx4_gemm_args g, int 
         const int block = col / 4;
         const bool live = m < g.M && block * 32 < g.N;
         if (g.out_type == RKH_MX4_ROWS) mx_put_rows(g, m, block, live, v, lane);
-        else if (live) mx_put<8>(g, m, block * 32 + 8 * (lane >> 4), g.N, v);
+        else if (live) mx_put<8>(g, m, block * 32 + 8 * (lane >> 4), v);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = s[e >> 2][e & 3];
-        if (m < g.M) mx_put<8>(g, m, col * 16 + 8 * (lane >> 4), g.N, v);
+        if (m < g.M) mx_put<8>(g, m, col * 16 + 8 * (lane >> 4), v);
     }
 }
 
@@ -583,6 +629,7 @@ struct MxRoute {
     int rm, cn, parts, mblocks, nblocks; // few: 16 rm rows, 16 cn places of a workgroup
 };
 
+constexpr int MX_ROWS = 4;  // rows that the few-row kernel quantizes itself
 constexpr int MX_CUS = 256; // compute units that a launch is cut for
 
 MxRoute mx_route(int M, int N, int K, int swiglu) {
@@ -614,34 +661,51 @@ MxRoute mx_route(int M, int N, int K, int swiglu) {
 }
 size_t mx_scratch(const MxRoute& r) { return r.few || r.parts == 1 ? 0 : (size_t)r.mblocks * r.nblocks * r.parts * r.rm * r.cn * 4096; }
 
-template <int RM, int CN, int MAX_WAVES, bool SWIGLU, bool FUSED>
-int launch_few(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
-    const int K4 = (int)rkh_mx4_k4(g.K), per = (K4 + MAX_WAVES - 1) / MAX_WAVES, waves = (K4 + per - 1) / per;
-    const size_t sums = (size_t)waves * RM * CN * 1024, rows = FUSED ? (size_t)rkh_mx4_ks(g.K) * 4 * g.M * 16 + (size_t)K4 * g.M * 16 : 0;
-    const size_t bytes = sums > rows ? sums : rows;
+template <int RM, int CN, int NG, int MAX_WAVES, bool SWIGLU, int FUSED, int X>
+int launch_few_as(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r, int per, int waves) {
+    const int K4 = (int)rkh_mx4_k4(g.K);
+    const size_t bytes = (size_t)waves * RM * CN * 1024 + (FUSED ? (size_t)few_row_bytes(K4) * g.M : 0);
     static std::atomic<int> ready{0};
     if (!ready.load()) {
-        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_few_kernel<RM, CN, MAX_WAVES, SWIGLU, FUSED>),
+        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_few_kernel<RM, CN, NG, MAX_WAVES, SWIGLU, FUSED, X>),
                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         ready.store(1);
     }
     mark(st, "mx4_few_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_few_kernel<RM, CN, MAX_WAVES, SWIGLU, FUSED>), dim3(r.nblocks), dim3(waves * 64), bytes, st, g, per);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_few_kernel<RM, CN, NG, MAX_WAVES, SWIGLU, FUSED, X>), dim3(r.nblocks), dim3(waves * 64), bytes, st, g.W,
+                       g.w_scale, FUSED ? g.x : g.A, FUSED ? reinterpret_cast<const uint8_t*>((intptr_t)g.ldx) : g.a_scale, g.M, g.N, g.K, per, r.nblocks, waves, g);
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
 }
+template <int RM, int CN, int MAX_WAVES, bool SWIGLU, int FUSED> int launch_few(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
+    const int K4 = (int)rkh_mx4_k4(g.K), per = (K4 + MAX_WAVES - 1) / MAX_WAVES, waves = (K4 + per - 1) / per;
+    int rc = RKH_OK;
+    const auto as = [&](auto x) {
+        constexpr int X = decltype(x)::value;
+        if constexpr (RM * CN == 1) {
+            if (per > 1) {
+                rc = launch_few_as<RM, CN, 2, MAX_WAVES, SWIGLU, FUSED, X>(st, g, r, per, waves);
+                return;
+            }
+        }
+        rc = launch_few_as<RM, CN, 1, MAX_WAVES, SWIGLU, FUSED, X>(st, g, r, per, waves);
+    };
+    if constexpr (FUSED) mx_with_type(g.x_type, as);
+    else as(std::integral_constant<int, RKH_MX4_F32>{});
+    return rc;
+}
 
-template <int RM, int CN, int HALVES, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
+template <int RM, int CN, int HALVES, bool SWIGLU, int OUT> int launch_tiles(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
     constexpr int LDS = MxTile<RM, CN, HALVES>::LDS;
     static std::atomic<int> ready{0};
     if (!ready.load()) {
-        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_tile_kernel<RM, CN, HALVES, SWIGLU>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_tile_kernel<RM, CN, HALVES, SWIGLU, OUT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
         ready.store(1);
     }
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
     if (tiles * r.parts > 0x7fffffff) return RKH_ERR_RUNTIME;
     mark(st, "mx4_tile_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_tile_kernel<RM, CN, HALVES, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks,
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_tile_kernel<RM, CN, HALVES, SWIGLU, OUT>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks,
                        r.nblocks, r.parts);
     RKH_CHECK(hipGetLastError());
     if (r.parts > 1) {
@@ -653,40 +717,52 @@ template <int RM, int CN, int HALVES, bool SWIGLU> int launch_tiles(hipStream_t 
     return RKH_OK;
 }
 
-template <bool SWIGLU> int launch_big(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
+template <bool SWIGLU, int OUT> int launch_big(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
     constexpr int LDS = MxTile<8, 8, 1>::LDS;
     static std::atomic<int> ready{0};
     if (!ready.load()) {
-        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_big_kernel<SWIGLU>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_big_kernel<SWIGLU, OUT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
         ready.store(1);
     }
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks, left = tiles % MX_CUS, big = left <= MX_CUS / 2 ? tiles - left : tiles;
     if (tiles > 0x3fffffff) return RKH_ERR_RUNTIME;
     mark(st, "mx4_big_kernel");
-    hipLaunchKernelGGL(mx4_big_kernel<SWIGLU>, dim3((unsigned)(big ? std::min<int64_t>(big, MX_CUS) : 2 * left)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, (int)big);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_big_kernel<SWIGLU, OUT>), dim3((unsigned)(big ? std::min<int64_t>(big, MX_CUS) : 2 * left)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, (int)big);
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
+}
+
+template <bool SWIGLU, int OUT> int launch_shape(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
+    if (r.rm == 8) return r.cn == 8 ? launch_big<SWIGLU, OUT>(st, g, r) : launch_tiles<8, 4, 1, SWIGLU, OUT>(st, g, r);
+    return r.rm == 4 ? launch_tiles<4, 4, 1, SWIGLU, OUT>(st, g, r) : launch_tiles<2, 4, 2, SWIGLU, OUT>(st, g, r);
 }
 
 template <bool SWIGLU> int launch(hipStream_t st, const rkh_mx4_gemm_args& g) {
     MxRoute r = mx_route(g.M, g.N, g.K, SWIGLU);
     if (r.few) {
         if (!g.A) {
-            if constexpr (SWIGLU) return launch_few<1, 4, 8, true, true>(st, g, r);
-            else return r.cn == 1 ? launch_few<1, 1, 16, false, true>(st, g, r) : launch_few<1, 2, 16, false, true>(st, g, r);
+            if constexpr (SWIGLU) return g.x_norm ? launch_few<1, 4, 8, true, 2>(st, g, r) : launch_few<1, 4, 8, true, 1>(st, g, r);
+            else return r.cn == 1 ? launch_few<1, 1, 16, false, 1>(st, g, r) : launch_few<1, 2, 16, false, 1>(st, g, r);
         }
         if constexpr (SWIGLU) {
-            if (r.rm == 1) return launch_few<1, 4, 8, true, false>(st, g, r);
-            return launch_few<2, 4, 8, true, false>(st, g, r);
+            if (r.rm == 1) return launch_few<1, 4, 8, true, 0>(st, g, r);
+            return launch_few<2, 4, 8, true, 0>(st, g, r);
         } else {
-            if (r.rm == 1) return r.cn == 1 ? launch_few<1, 1, 16, false, false>(st, g, r) : launch_few<1, 2, 16, false, false>(st, g, r);
-            if (r.rm == 2) return r.cn == 1 ? launch_few<2, 1, 16, false, false>(st, g, r) : launch_few<2, 2, 8, false, false>(st, g, r);
-            return launch_few<4, 1, 8, false, false>(st, g, r);
+            if (r.rm == 1) return r.cn == 1 ? launch_few<1, 1, 16, false, 0>(st, g, r) : launch_few<1, 2, 16, false, 0>(st, g, r);
+            if (r.rm == 2) return r.cn == 1 ? launch_few<2, 1, 16, false, 0>(st, g, r) : launch_few<2, 2, 8, false, 0>(st, g, r);
+            return launch_few<4, 1, 8, false, 0>(st, g, r);
         }
     }
     if (mx_scratch(r) > (g.scratch ? g.scratch_bytes : 0)) r.parts = 1;
-    if (r.rm == 8) return r.cn == 8 ? launch_big<SWIGLU>(st, g, r) : launch_tiles<8, 4, 1, SWIGLU>(st, g, r);
-    return r.rm == 4 ? launch_tiles<4, 4, 1, SWIGLU>(st, g, r) : launch_tiles<2, 4, 2, SWIGLU>(st, g, r);
+    // (partial tiles have no type)
+    switch (r.parts > 1 ? RKH_MX4_F32 : g.out_type) {
+    case RKH_MX4_F16: return launch_shape<SWIGLU, RKH_MX4_F16>(st, g, r);
+    case RKH_MX4_BF16: return launch_shape<SWIGLU, RKH_MX4_BF16>(st, g, r);
+    case RKH_MX4_ROWS:
+        if constexpr (SWIGLU) return launch_shape<SWIGLU, RKH_MX4_ROWS>(st, g, r);
+        return RKH_ERR_RUNTIME;
+    default: return launch_shape<SWIGLU, RKH_MX4_F32>(st, g, r);
+    }
 }
 
 } // namespace
@@ -699,8 +775,10 @@ int rkh_mx4_gemm(void* stream, const rkh_mx4_gemm_args* args) {
     return args->swiglu ? launch<true>((hipStream_t)stream, *args) : launch<false>((hipStream_t)stream, *args);
 }
 int rkh_mx4_takes_rows(int M, int N, int K, int swiglu) {
+    // Every workgroup quantizes all rows: up to 16384 values (1 x 14336 -> 4096 7.2 us, with a launch of its own in front 9.1; 4 x 4096 -> 14336
+    // 8.8 and 9.7; 4 x 14336 -> 4096 11.5 and 9.1), in whole pieces of eight.
     (void)N, (void)swiglu;
-    return M <= 4 && rkh_mx4_ks(K) * 4 * M * 16 + rkh_mx4_k4(K) * M * 16 <= FEW_FUSED_LDS;
+    return M <= MX_ROWS && K % 8 == 0 && (int64_t)M * K <= 16384;
 }
 void rkh_mx4_route(int M, int N, int K, int swiglu, int* kernel, int* rows, int* columns, int* parts) {
     const MxRoute r = mx_route(M, N, K, swiglu);

@@ -1,24 +1,12 @@
 // The norms around a block: z = rms(branch) * w_b, r' = a r + b gate z, y = rms(r') * w, one row per workgroup.
-// Bound by memory: every value is read and written once.  A row lives in registers between its two sums of squares.
+// Bound by memory for many rows, by the round trips of one workgroup for few: everything that a row needs is loaded at once, weights and gate
+// included, and the row lives in registers between its two sums of squares.
 #include "rk_kernels_mx4.h"
 
 namespace {
 
-constexpr int NORM_MAX_WAVES = 16;
-
-// Sum over the workgroup, the same in every thread.  The waves' sums are added in order; `part` takes turns between calls.
-__device__ __forceinline__ float norm_sum(float x, float* part) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) x += __shfl_xor(x, off);
-    const int waves = blockDim.x >> 6;
-    if (waves == 1) return x;
-    if (lane_id() == 0) part[wave_id()] = x;
-    __syncthreads();
-    float sum = part[0];
-    for (int w = 1; w < waves; ++w) sum += part[w];
-    return sum;
-}
-__device__ __forceinline__ float norm_factor(float sum, int D, float eps) { return 1.0f / sqrtf(sum / (float)D + eps); }
+constexpr int NORM_MAX_THREADS = 1024;
+constexpr int NORM_SEGMENTS = 2 * NORM_MAX_THREADS / 64; // of 512 values, that registers hold
 
 __device__ __forceinline__ void norm_load(int type, const void* p, size_t i, int count, float (&v)[8]) {
     mx_with_type(type, [&](auto t) { mx_load8<decltype(t)::value>(p, i, count, v); });
@@ -36,133 +24,113 @@ __device__ __forceinline__ void norm_store(int type, void* p, size_t i, int coun
     });
 }
 
-// z of eight values of the branch, without the gate
-__device__ __forceinline__ void norm_branch(const rkh_block_norm_args& a, int k, int count, float factor, float (&v)[8]) {
-    if (!a.branch_weight) return;
-    float w[8];
-    mx_load8<RKH_MX4_F32>(a.branch_weight, k, count, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * factor * w[e];
-}
 // r' of eight values, from z and the stream's
-__device__ __forceinline__ void norm_join(const rkh_block_norm_args& a, int m, int k, int count, const float (&z)[8], float (&r)[8]) {
-    float g[8];
-    if (a.gate) norm_load(a.gate_type, a.gate, (size_t)m * a.gate_row_stride + k, count, g);
+__device__ __forceinline__ void norm_join(const rkh_block_norm_args& a, const float (&z)[8], const float (&gate)[8], float (&r)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float gated = a.gate ? z[e] * g[e] : z[e];
-        r[e] = fmaf(a.residual_scale, r[e], a.branch_scale * gated);
-    }
-}
-__device__ __forceinline__ float norm_squares(const float (&v)[8], float sum) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
-    return sum;
+    for (int e = 0; e < 8; ++e) r[e] = fmaf(a.residual_scale, r[e], a.branch_scale * (a.gate ? z[e] * gate[e] : z[e]));
 }
 // the normed values to wherever they go
-__device__ __forceinline__ void norm_out(const rkh_block_norm_args& a, int m, int k, int count, float factor, float (&r)[8]) {
-    if (a.weight) {
-        float w[8];
-        mx_load8<RKH_MX4_F32>(a.weight, k, count, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] = r[e] * factor * w[e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) r[e] *= factor;
-    }
+__device__ __forceinline__ void norm_out(const rkh_block_norm_args& a, int m, int k, const float (&r)[8]) {
+    const int count = a.D - k;
     if (a.y && count > 0) norm_store(a.y_type, a.y, (size_t)m * a.ld_y + k, count, r);
     if (a.q) { // (values beyond D are zeros; a block's four lanes come here together)
         const uint32_t scale = mx_scale(mx_top_of_quad(mx_top(r)));
-        const int b = k >> 5;
+        const int b = k >> 5, K4 = (int)rkh_mx4_k4(a.D);
         if (b * 32 < a.D) {
-            *reinterpret_cast<uint32_t*>(a.q + mx_code_at(m, b, (int)rkh_mx4_k4(a.D)) + (k & 31) / 2) = mx_codes(r, scale);
-            if ((k & 31) == 0) a.q_scale[mx_scale_at(m, b, (int)rkh_mx4_k4(a.D))] = (uint8_t)scale;
+            *reinterpret_cast<uint32_t*>(a.q + mx_code_at(m, b, K4) + (k & 31) / 2) = mx_codes(r, scale);
+            if ((k & 31) == 0) a.q_scale[mx_scale_at(m, b, K4)] = (uint8_t)scale;
         }
     }
 }
 
 // CHUNKS pieces of eight values per thread.
 template <int CHUNKS>
-__global__ __launch_bounds__(1024) void block_norm_kernel(rkh_block_norm_args a) {
-    __shared__ float part[2][NORM_MAX_WAVES];
-    const int m = blockIdx.x, t = threadIdx.x, step = blockDim.x * 8;
-    float r[CHUNKS][8], z[CHUNKS][8];
+__global__ __launch_bounds__(NORM_MAX_THREADS) void block_norm_kernel(rkh_block_norm_args a) {
+    __shared__ float part[2][NORM_SEGMENTS];
+    const int m = blockIdx.x, waves = blockDim.x >> 6, segments = (a.D + 511) / 512;
+    float r[CHUNKS][8], z[CHUNKS][8], gate[CHUNKS][8], wb[CHUNKS][8], w[CHUNKS][8];
+    const auto at = [&](int c) { return (c * (int)blockDim.x + (int)threadIdx.x) * 8; };
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-        const int k = c * step + t * 8;
-        norm_load(a.stream_type, a.stream, (size_t)m * a.ld_stream + k, a.D - k, r[c]);
-        if (a.branch) norm_load(a.branch_type, a.branch, (size_t)m * a.ld_branch + k, a.D - k, z[c]);
+        const int k = at(c), count = a.D - k;
+        norm_load(a.stream_type, a.stream, (size_t)m * a.ld_stream + k, count, r[c]);
+        if (a.branch) norm_load(a.branch_type, a.branch, (size_t)m * a.ld_branch + k, count, z[c]);
+        if (a.gate) norm_load(a.gate_type, a.gate, (size_t)m * a.gate_row_stride + k, count, gate[c]);
+        if (a.branch_weight) mx_load8<RKH_MX4_F32>(a.branch_weight, k, count, wb[c]);
+        if (a.weight) mx_load8<RKH_MX4_F32>(a.weight, k, count, w[c]);
     }
-    if (a.branch) {
-        float factor = 1.0f;
-        if (a.branch_weight) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) sum = norm_squares(z[c], sum);
-            factor = norm_factor(norm_sum(sum, part[0]), a.D, a.eps);
-        }
+    // the factor of the values' norm: one part per segment, chunk c of wave v holds segment c * waves + v
+    const auto factor_of = [&](const float (&v)[CHUNKS][8], float* sums) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
-            const int k = c * step + t * 8;
-            norm_branch(a, k, a.D - k, factor, z[c]);
-            norm_join(a, m, k, a.D - k, z[c], r[c]);
+            const float sum = mx_segment_sum(mx_squares(v[c], 0.0f));
+            if (lane_id() == 0) sums[c * waves + wave_id()] = sum;
         }
+        __syncthreads();
+        return mx_norm_factor(mx_sum_of_segments(sums, segments), a.D, a.eps);
+    };
+    if (a.branch) {
+        if (a.branch_weight) {
+            const float factor = factor_of(z, part[0]);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) mx_normed(z[c], factor, true, wb[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) norm_join(a, z[c], gate[c], r[c]);
     }
     if (a.stream_out) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-            const int k = c * step + t * 8;
-            if (k < a.D) norm_store(a.stream_type, a.stream_out, (size_t)m * a.ld_stream_out + k, a.D - k, r[c]);
-        }
+        for (int c = 0; c < CHUNKS; ++c)
+            if (at(c) < a.D) norm_store(a.stream_type, a.stream_out, (size_t)m * a.ld_stream_out + at(c), a.D - at(c), r[c]);
     }
     if (!a.y && !a.q) return;
-    float sum = 0.0f;
+    const float factor = factor_of(r, part[1]);
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) sum = norm_squares(r[c], sum);
-    const float factor = norm_factor(norm_sum(sum, part[1]), a.D, a.eps);
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) norm_out(a, m, c * step + t * 8, a.D - c * step - t * 8, factor, r[c]);
+    for (int c = 0; c < CHUNKS; ++c) {
+        mx_normed(r[c], factor, a.weight != nullptr, w[c]);
+        norm_out(a, m, at(c), r[c]);
+    }
 }
 
 // Rows that do not fit into registers are read up to three times; nothing is written before the last pass, so that the
 // stream may be updated in place here, too.
-__global__ __launch_bounds__(1024) void block_norm_long_kernel(rkh_block_norm_args a) {
-    __shared__ float part[2][NORM_MAX_WAVES];
-    const int m = blockIdx.x, step = blockDim.x * 8;
-    float branch_factor = 1.0f;
-    if (a.branch && a.branch_weight) {
-        float sum = 0.0f;
-        for (int k = threadIdx.x * 8; k < a.D; k += step) {
-            float z[8];
-            norm_load(a.branch_type, a.branch, (size_t)m * a.ld_branch + k, a.D - k, z);
-            sum = norm_squares(z, sum);
+__global__ __launch_bounds__(NORM_MAX_THREADS) void block_norm_long_kernel(rkh_block_norm_args a) {
+    extern __shared__ float parts[]; // one per segment
+    const int m = blockIdx.x, step = blockDim.x * 8, segments = (a.D + 511) / 512;
+    const auto factor_of = [&](auto&& values) {
+        __syncthreads(); // (the parts are read no more)
+        for (int k = threadIdx.x * 8; k < segments * 512; k += step) {
+            float v[8];
+            values(k, v);
+            const float sum = mx_segment_sum(mx_squares(v, 0.0f));
+            if (lane_id() == 0) parts[k >> 9] = sum;
         }
-        branch_factor = norm_factor(norm_sum(sum, part[0]), a.D, a.eps);
-    }
+        __syncthreads();
+        return mx_norm_factor(mx_sum_of_segments(parts, segments), a.D, a.eps);
+    };
+    const auto branch = [&](int k, float (&z)[8]) { norm_load(a.branch_type, a.branch, (size_t)m * a.ld_branch + k, a.D - k, z); };
+    const float branch_factor = a.branch && a.branch_weight ? factor_of(branch) : 1.0f;
     const auto joined = [&](int k, float (&r)[8]) {
         norm_load(a.stream_type, a.stream, (size_t)m * a.ld_stream + k, a.D - k, r);
-        if (a.branch) {
-            float z[8];
-            norm_load(a.branch_type, a.branch, (size_t)m * a.ld_branch + k, a.D - k, z);
-            norm_branch(a, k, a.D - k, branch_factor, z);
-            norm_join(a, m, k, a.D - k, z, r);
+        if (!a.branch) return;
+        float z[8], w[8], gate[8];
+        branch(k, z);
+        if (a.branch_weight) {
+            mx_load8<RKH_MX4_F32>(a.branch_weight, k, a.D - k, w);
+            mx_normed(z, branch_factor, true, w);
         }
+        if (a.gate) norm_load(a.gate_type, a.gate, (size_t)m * a.gate_row_stride + k, a.D - k, gate);
+        norm_join(a, z, gate, r);
     };
-    float factor = 1.0f;
-    if (a.y || a.q) {
-        float sum = 0.0f;
-        for (int k = threadIdx.x * 8; k < a.D; k += step) {
-            float r[8];
-            joined(k, r);
-            sum = norm_squares(r, sum);
-        }
-        factor = norm_factor(norm_sum(sum, part[1]), a.D, a.eps);
-    }
+    const float factor = a.y || a.q ? factor_of(joined) : 1.0f;
     for (int k = threadIdx.x * 8; k < rkh_align_up(a.D, 32); k += step) { // (whole blocks: their lanes stay together)
-        float r[8];
+        float r[8], w[8];
         joined(k, r);
         if (a.stream_out && k < a.D) norm_store(a.stream_type, a.stream_out, (size_t)m * a.ld_stream_out + k, a.D - k, r);
-        if (a.y || a.q) norm_out(a, m, k, a.D - k, factor, r);
+        if (!a.y && !a.q) continue;
+        if (a.weight) mx_load8<RKH_MX4_F32>(a.weight, k, a.D - k, w);
+        mx_normed(r, factor, a.weight != nullptr, w);
+        norm_out(a, m, k, r);
     }
 }
 
@@ -171,14 +139,19 @@ __global__ __launch_bounds__(1024) void block_norm_long_kernel(rkh_block_norm_ar
 extern "C" int rkh_block_norm(void* stream, const rkh_block_norm_args* args) {
     const rkh_block_norm_args& a = *args;
     if (!a.rows) return RKH_OK;
-    const int64_t pieces = rkh_align_up(a.D, 32) / 8; // of eight values
-    // two pieces per thread once a row fills four waves
-    const int chunks = pieces <= 256 ? 1 : 2;
-    int threads = (int)rkh_align_up((pieces + chunks - 1) / chunks, 64);
+    const int64_t segments = (a.D + 511) / 512; // a wave's pieces
+    // two pieces per thread once a row fills eight waves, or four where there are rows enough to fill the compute units
+    const int chunks = segments <= NORM_MAX_THREADS / 64 ? 1 : 2;
+    const int64_t threads = (segments + chunks - 1) / chunks * 64;
     mark((hipStream_t)stream, "block_norm_kernel");
-    if (threads > 1024) hipLaunchKernelGGL(block_norm_long_kernel, dim3(a.rows), dim3(1024), 0, (hipStream_t)stream, a);
-    else if (chunks == 1) hipLaunchKernelGGL(block_norm_kernel<1>, dim3(a.rows), dim3(threads), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(block_norm_kernel<2>, dim3(a.rows), dim3(threads), 0, (hipStream_t)stream, a);
+    if (threads > NORM_MAX_THREADS) {
+        // (one float per segment: 16 KiB for the longest rows there are)
+        hipLaunchKernelGGL(block_norm_long_kernel, dim3(a.rows), dim3(NORM_MAX_THREADS), (size_t)segments * 4, (hipStream_t)stream, a);
+    } else if (chunks == 1) {
+        hipLaunchKernelGGL(block_norm_kernel<1>, dim3(a.rows), dim3((unsigned)threads), 0, (hipStream_t)stream, a);
+    } else {
+        hipLaunchKernelGGL(block_norm_kernel<2>, dim3(a.rows), dim3((unsigned)threads), 0, (hipStream_t)stream, a);
+    }
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
 }

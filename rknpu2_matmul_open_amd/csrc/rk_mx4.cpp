@@ -365,16 +365,6 @@ int rk_npu_mx4_run_ffn_block_device(rk_npu_mx4_workspace* ws, const rk_npu_mx4_w
     std::lock_guard<std::mutex> submit(ctx->submit_mutex);
     ws->staged = down_ws->staged = 0;
     if (!a->rows) return RK_NPU_OK;
-    rkh_block_norm_args before{}; // h, straight to the first product's rows
-    before.rows = a->rows;
-    before.D = a->D;
-    before.stream_type = a->residual_type;
-    before.eps = a->eps;
-    before.stream = a->residual;
-    before.ld_stream = a->residual_ld;
-    before.weight = a->weight;
-    before.q = ws->codes.as<>();
-    before.q_scale = ws->scales.as<>();
     rkh_mx4_gemm_args g = product(ws, gate_up, a->rows), d = product(down_ws, down, a->rows);
     to_middle(g, down_ws);
     d.out_type = a->branch_type;
@@ -383,7 +373,27 @@ int rk_npu_mx4_run_ffn_block_device(rk_npu_mx4_workspace* ws, const rk_npu_mx4_w
     rkh_block_norm_args after = norm_args(a);
     after.branch = branch;
     after.weight = next_weight;
-    rc = rkh_block_norm(ctx->stream, &before);
+    if (rkh_mx4_takes_rows(g.M, g.N, g.K, 1)) { // h is made where it is multiplied
+        g.A = nullptr;
+        g.x = a->residual;
+        g.ldx = a->residual_ld;
+        g.x_type = a->residual_type;
+        g.x_norm = 1;
+        g.x_weight = a->weight;
+        g.x_eps = a->eps;
+    } else {
+        rkh_block_norm_args before{}; // h, straight to the first product's rows
+        before.rows = a->rows;
+        before.D = a->D;
+        before.stream_type = a->residual_type;
+        before.eps = a->eps;
+        before.stream = a->residual;
+        before.ld_stream = a->residual_ld;
+        before.weight = a->weight;
+        before.q = ws->codes.as<>();
+        before.q_scale = ws->scales.as<>();
+        rc = rkh_block_norm(ctx->stream, &before);
+    }
     if (!rc) rc = rkh_mx4_gemm(ctx->stream, &g);
     if (!rc) rc = rkh_mx4_gemm(ctx->stream, &d);
     if (!rc) rc = rkh_block_norm(ctx->stream, &after);

@@ -54,6 +54,9 @@ typedef struct rkh_mx4_gemm_args {
     const void* x;         /* rows of values that the few-row kernel quantizes itself             */
     int64_t ldx;
     int x_type;
+    int x_norm;            /* (SwiGLU) normed first: x / sqrt(mean(x^2) + x_eps) * x_weight       */
+    const float* x_weight; /* or NULL                                                             */
+    float x_eps;
     int M, N, K;           /* N: columns of the result (SwiGLU: F)                                */
     int swiglu;
     int out_type;          /* rkh_mx4_type                                                        */
