@@ -41,7 +41,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-UNITS = ["rk_kernels_gemm.hip", "rk_kernels_stream.hip", "rk_kernels_mx4_gemm.hip"]
+UNITS = ["rk_kernels_gemm.hip", "rk_kernels_stream.hip", "rk_kernels_mx4_gemm.hip", "rk_kernels_mx4_swiglu.hip"]
 
 _VM_LOAD = re.compile(r"^\s*(global_load|buffer_load|flat_load|scratch_load)")
 _ASM_VLOAD = re.compile(r"^\s*global_load_dwordx?(\d*)\s+(v\[\d+:\d+\]|v\d+)\s*,")

@@ -13,27 +13,20 @@ def quantize(x):
     v = np.zeros((rows, blocks * 32))
     v[:, :K] = x
     v = v.reshape(rows, blocks, 32)
-    codes = np.zeros((rows, blocks, 32), np.uint8)
-    scales = np.zeros((rows, blocks), np.uint8)
-    with np.errstate(invalid="ignore"):
-        most = np.abs(v).max(axis=2)
-    for r in range(rows):
-        for b in range(blocks):
-            if not np.isfinite(v[r, b]).all():
-                scales[r, b] = 255
-                continue
-            e = -127
-            if most[r, b] > 0:
-                e = max(-127, int(np.frexp(most[r, b])[1]) - 1 - 2)
-            scales[r, b] = e + 127
-            size = np.abs(v[r, b]) / 2.0 ** e
-            # the nearest value; of two equally near ones the even code
-            far = np.abs(size[:, None] - VALUES[None, :])
-            near = far.min(axis=1, keepdims=True)
-            tied = far == near
-            even = tied & (np.arange(8) % 2 == 0)[None, :]
-            pick = np.where(even.any(axis=1), even.argmax(axis=1), tied.argmax(axis=1))
-            codes[r, b] = pick + 8 * np.signbit(v[r, b])
+    bad = ~np.isfinite(v).all(axis=2)
+    v[bad] = 0
+    most = np.abs(v).max(axis=2)
+    e = np.where(most > 0, np.maximum(-127, np.frexp(most)[1] - 1 - 2), -127)
+    scales = np.where(bad, 255, e + 127).astype(np.uint8)
+    size = np.abs(v) / (2.0 ** e)[:, :, None]
+    # the nearest value; of two equally near ones the even code
+    pick, near = np.zeros(size.shape, np.uint8), np.full(size.shape, np.inf)
+    for code, value in enumerate(VALUES):
+        far = np.abs(size - value)
+        take = (far < near) | ((far == near) & (code % 2 == 0))
+        pick[take], near = code, np.minimum(far, near)
+    codes = pick + 8 * np.signbit(v).astype(np.uint8)
+    codes[bad] = 0
     packed = codes[:, :, 0::2] | (codes[:, :, 1::2] << 4)
     return packed.reshape(rows, blocks * 16).astype(np.uint8), scales
 

@@ -168,6 +168,20 @@ class Layer:
         self.w.close()
 
 
+def test_the_shapes_take_every_kernel(sess):
+    """The lists of sizes below reach every shape of tile, halves of the largest ones, K in parts and both ways to the few-row kernel."""
+    taken = {route(sess, M, N, K)[:3] + (route(sess, M, N, K)[3] > 1,) for M, N, K in SHAPES}
+    assert {(0, 16, 16, False), (0, 32, 16, False), (0, 32, 32, False), (0, 64, 16, False)} <= taken
+    assert {t[:3] for t in taken if t[0]} == {(1, a, b) for a, b in ((256, 256), (128, 128), (64, 128), (128, 64), (64, 64))}
+    assert any(t[3] for t in taken)
+    big = [(M, N) for M, N, K in SHAPES if route(sess, M, N, K)[:3] == (1, 256, 256)]
+    tiles = {-(-M // 256) * -(-N // 256) for M, N in big}
+    assert any(t > 256 and 0 < t % 256 <= 128 for t in tiles) # chains with halves behind ...
+    assert any(t % 256 > 128 for t in tiles)                   # ... a round of whole tiles
+    swiglu = {route(sess, M, F, K, 1)[:3] for M, F, K in SWIGLU} | {route(sess, M, F, H, 1)[:3] for M, H, F in FFN}
+    assert {(0, 16, 64), (0, 32, 64), (1, 64, 128), (1, 128, 128), (1, 256, 256)} <= swiglu
+
+
 def route(sess, M, N, K, swiglu=0):
     out = [C.c_int(0) for _ in range(4)]
     sess.lib.rkh_mx4_route(M, N, K, swiglu, *[C.byref(x) for x in out])
@@ -176,7 +190,8 @@ def route(sess, M, N, K, swiglu=0):
 
 SHAPES = [(1, 1, 1), (1, 32, 32), (1, 33, 31), (1, 129, 500), (2, 64, 513), (3, 200, 4096), (4, 1999, 2050), (5, 100, 128), (16, 4100, 640), (16, 48, 14336),
           (17, 65, 129), (32, 4100, 300), (33, 70, 1100), (61, 1999, 2050), (64, 96, 8192), (65, 31, 33), (65, 300, 8200), (100, 1000, 520), (128, 4096, 512), (129, 257, 1536),
-          (130, 11008, 256), (256, 512, 7000), (257, 4096, 96), (300, 12400, 160), (515, 6000, 700), (1025, 2100, 1030), (2048, 4096, 512)]
+          (130, 11008, 256), (256, 512, 7000), (257, 4096, 96), (300, 12400, 160), (515, 6000, 700), (1025, 2100, 1030), (2048, 4096, 512),
+          (20, 17000, 300), (2100, 5900, 700), (4100, 5000, 520)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -318,14 +333,18 @@ def test_weights_from_device_arrays_that_quantize_wrote(sess):
 
 
 def swiglu_bound(gate, up, K, a, g_values, u_values):
-    """How far fp32 sums, the polynomial exponential (below 2^-20 relative) and the products may take silu(gate) * up."""
+    """How far fp32 sums, the exponential, the reciprocal (together below 2^-20 relative) and the products may take silu(gate) * up."""
     eg = K * 2.0 ** -24 * (np.abs(a) @ np.abs(g_values).T)
     eu = K * 2.0 ** -24 * (np.abs(a) @ np.abs(u_values).T)
     s = np.abs(ref.silu(gate))
     return 1.1 * eg * (np.abs(up) + eu) + s * eu + 2.0 ** -19 * s * np.abs(up) + 1e-30
 
 
-@pytest.mark.parametrize("M,F,K", [(1, 64, 96), (1, 33, 512), (3, 300, 4100), (16, 500, 640), (31, 70, 1000), (33, 96, 300), (100, 350, 1500), (300, 1000, 520)])
+SWIGLU = [(1, 64, 96), (1, 33, 512), (3, 300, 4100), (16, 500, 640), (31, 70, 1000), (33, 96, 300), (100, 350, 1500), (300, 1000, 520), (200, 7000, 200),
+          (500, 14300, 130)]
+
+
+@pytest.mark.parametrize("M,F,K", SWIGLU)
 def test_swiglu(sess, M, F, K):
     rng = np.random.default_rng(M + F + K)
     layer = Layer(sess, rng, 2 * F, K, gate_up=True, make=ordinary)
@@ -347,7 +366,32 @@ def test_swiglu(sess, M, F, K):
     layer.close()
 
 
-FFN = [(1, 512, 700), (4, 96, 64), (13, 300, 333), (32, 640, 1000), (40, 130, 257), (150, 512, 900), (300, 1024, 1600)]
+@pytest.mark.parametrize("M", [1, 20, 70, 300])
+def test_swiglu_of_far_gates(sess, M):
+    """One-hot rows: the sums are single products, exact, over the whole range of the exponential.  16 roundings or ulps around it."""
+    K = F = 512
+    rng = np.random.default_rng(M)
+    gate = np.zeros((F, K))
+    up = np.zeros((F, K))
+    at = np.arange(F)
+    gate[at, at] = np.tile([0, 0.5, -0.5, 1, -1.5, 4, -6, 12, -24, 48, -64, 96, -96, 128, -192, 1024], F // 16)
+    up[at, at] = rng.choice([1.0, -2.0, 0.5], F)
+    w = ops.MX4Weights(sess, K, 2 * F, *ref.quantize(np.concatenate([gate, up])), gate_up=True)
+    x = np.zeros((M, K))
+    pick = rng.integers(0, K, M)
+    x[np.arange(M), pick] = 1.0
+    ws, d, c = ops.MX4Workspace(sess, M, K, 2 * F), device(x, "f32"), torch.zeros((M, F), device="cuda")
+    ready()
+    ws.run_swiglu(w, d, c)
+    done(sess)
+    with np.errstate(over="ignore"):
+        want = ref.silu(x @ gate.T) * (x @ up.T)
+    assert (np.abs(host(c) - want) <= 16 * 2.0 ** -24 * np.abs(want) + 1e-36).all()
+    ws.close()
+    w.close()
+
+
+FFN = [(1, 512, 700), (4, 96, 64), (13, 300, 333), (32, 640, 1000), (40, 130, 257), (150, 512, 900), (300, 1024, 1600), (500, 130, 14300)]
 
 
 @pytest.mark.parametrize("M,H,F", FFN)
