@@ -9,36 +9,39 @@ namespace {
 // counted through from `first`, so that short rows fill the workgroups, too.
 constexpr int QUANT_UNITS = 4; // blocks of a quad of lanes; their loads go out together
 
-template <int TYPE>
+// DENSE: the values follow one another, and rows are whole blocks.  (As two branches of one kernel the loads waited for each other:
+// 4096 x 14336 bf16 49 us.)
+template <int TYPE, bool DENSE>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int K, int64_t ldx) {
     const int KB = (K + 31) / 32, part = threadIdx.x & 3;
     const int64_t blocks = rows * KB, first = (int64_t)blockIdx.x * (64 * QUANT_UNITS);
-    const bool dense = ldx == K && K % 32 == 0; // values follow one another
-    const int64_t row0 = dense ? 0 : first / KB;
+    const int mine = threadIdx.x >> 2, live = (int)min(blocks - first, (int64_t)(64 * QUANT_UNITS)); // units of this workgroup
+    const int64_t row0 = DENSE ? 0 : first / KB;
     const unsigned rest = (unsigned)(first - row0 * KB);
     MxRaw<TYPE> raw[QUANT_UNITS];
-    int64_t at[QUANT_UNITS];
 #pragma unroll
     for (int u = 0; u < QUANT_UNITS; ++u) {
-        at[u] = first + u * 64 + (threadIdx.x >> 2);
-        if (at[u] >= blocks) continue;
-        if (dense) {
-            raw[u] = mx_fetch8<TYPE>(x, at[u] * 32 + part * 8);
+        const int unit = u * 64 + mine;
+        if constexpr (DENSE) {
+            // (beyond the end: the last block again, which is not stored)
+            raw[u] = mx_fetch8<TYPE>(x, (first + min(unit, live - 1)) * 32 + part * 8);
         } else {
-            const unsigned t = rest + u * 64 + (threadIdx.x >> 2), r = t / (unsigned)KB;
+            const unsigned t = rest + min(unit, live - 1), r = t / (unsigned)KB;
             const int k = (int)(t - r * KB) * 32 + part * 8;
             const size_t i = (row0 + r) * ldx + k;
-            raw[u] = k + 8 <= K ? mx_fetch8<TYPE>(x, i) : mx_fetch_some<TYPE>(x, i, K - k);
+            if (k + 8 <= K) raw[u] = mx_fetch8<TYPE>(x, i);
+            else raw[u] = mx_fetch_some<TYPE>(x, i, K - k);
         }
     }
 #pragma unroll
     for (int u = 0; u < QUANT_UNITS; ++u) {
-        if (at[u] >= blocks) continue; // (the four lanes of a block together)
+        const int unit = u * 64 + mine;
         float v[8];
         mx_unpack<TYPE>(raw[u], v);
         const uint32_t scale = mx_scale(mx_top_of_quad(mx_top(v)));
-        *reinterpret_cast<u32_any*>(codes + at[u] * 16 + part * 4) = mx_codes(v, scale);
-        if (part == 0) scales[at[u]] = (uint8_t)scale;
+        if (unit >= live) continue;
+        *reinterpret_cast<u32_any*>(codes + (first + unit) * 16 + part * 4) = mx_codes(v, scale);
+        if (part == 0) scales[first + unit] = (uint8_t)scale;
     }
 }
 
@@ -155,8 +158,8 @@ int rkh_mx4_quantize(void* stream, int type, int64_t rows, int K, const void* x,
     if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
     mark((hipStream_t)stream, "mx4_quantize_kernel");
     mx_with_type(type, [&](auto t) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_quantize_kernel<decltype(t)::value>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, x,
-                           codes, scales, rows, K, ldx);
+        const auto kernel = K % 32 == 0 && (ldx == K || rows == 1) ? mx4_quantize_kernel<decltype(t)::value, true> : mx4_quantize_kernel<decltype(t)::value, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, x, codes, scales, rows, K, ldx);
     });
     RKH_CHECK(hipGetLastError());
     return RKH_OK;

@@ -695,16 +695,24 @@ MxRoute mx_route(int M, int N, int K, int swiglu) {
 }
 size_t mx_scratch(const MxRoute& r) { return r.few || r.parts == 1 ? 0 : (size_t)r.mblocks * r.nblocks * r.parts * r.rm * r.cn * 4096; }
 
+// More than 64 KiB of LDS for a kernel, once per device; `opted_in` is the kernel's own.
+int mx_allow_lds(const void* kernel, std::atomic<bool> (&opted_in)[64], int bytes) {
+    int dev = 0;
+    RKH_CHECK(hipGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return RKH_ERR_RUNTIME;
+    if (!opted_in[dev].load(std::memory_order_acquire)) {
+        RKH_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        opted_in[dev].store(true, std::memory_order_release);
+    }
+    return RKH_OK;
+}
+
 template <int RM, int CN, int NG, int MAX_WAVES, bool SWIGLU, int FUSED, int X>
 int launch_few_as(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r, int per, int waves) {
     const int K4 = (int)rkh_mx4_k4(g.K);
     const size_t bytes = (size_t)waves * RM * CN * 1024 + (FUSED ? (size_t)few_row_bytes(K4) * g.M : 0);
-    static std::atomic<int> ready{0};
-    if (!ready.load()) {
-        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_few_kernel<RM, CN, NG, MAX_WAVES, SWIGLU, FUSED, X>),
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        ready.store(1);
-    }
+    static std::atomic<bool> opted_in[64] = {};
+    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&mx4_few_kernel<RM, CN, NG, MAX_WAVES, SWIGLU, FUSED, X>), opted_in, 160 * 1024)) return rc;
     mark(st, "mx4_few_kernel");
     hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_few_kernel<RM, CN, NG, MAX_WAVES, SWIGLU, FUSED, X>), dim3(r.nblocks), dim3(waves * 64), bytes, st, g.W,
                        g.w_scale, FUSED ? g.x : g.A, FUSED ? reinterpret_cast<const uint8_t*>((intptr_t)g.ldx) : g.a_scale, g.M, g.N, g.K, per, r.nblocks, waves, g);
@@ -731,11 +739,8 @@ template <int RM, int CN, int MAX_WAVES, bool SWIGLU, int FUSED> int launch_few(
 
 template <int RM, int CN, int HALVES, bool SWIGLU, int OUT> int launch_tiles(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
     constexpr int LDS = MxTile<RM, CN, HALVES>::LDS;
-    static std::atomic<int> ready{0};
-    if (!ready.load()) {
-        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_tile_kernel<RM, CN, HALVES, SWIGLU, OUT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-        ready.store(1);
-    }
+    static std::atomic<bool> opted_in[64] = {};
+    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&mx4_tile_kernel<RM, CN, HALVES, SWIGLU, OUT>), opted_in, LDS)) return rc;
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
     if (tiles * r.parts > 0x7fffffff) return RKH_ERR_RUNTIME;
     mark(st, "mx4_tile_kernel");
@@ -753,11 +758,8 @@ template <int RM, int CN, int HALVES, bool SWIGLU, int OUT> int launch_tiles(hip
 
 template <bool SWIGLU, int OUT> int launch_big(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r) {
     constexpr int LDS = MxTile<8, 8, 1>::LDS;
-    static std::atomic<int> ready{0};
-    if (!ready.load()) {
-        RKH_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&mx4_big_kernel<SWIGLU, OUT>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-        ready.store(1);
-    }
+    static std::atomic<bool> opted_in[64] = {};
+    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&mx4_big_kernel<SWIGLU, OUT>), opted_in, LDS)) return rc;
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks, left = tiles % MX_CUS, big = left <= MX_CUS / 2 ? tiles - left : tiles;
     if (tiles > 0x3fffffff) return RKH_ERR_RUNTIME;
     mark(st, "mx4_big_kernel");

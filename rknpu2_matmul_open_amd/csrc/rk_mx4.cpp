@@ -248,9 +248,10 @@ rk_npu_mx4_workspace* rk_npu_mx4_workspace_create(rk_npu_iommu_domain* domain, i
     ws->rows = max_rows;
     ws->K = K;
     ws->N = N;
-    // the most that any call of up to so many rows splits into, so that a result does not depend on the workspace's size
+    // the most that any call of up to so many rows splits K into (no more than 16384 rows do: 128 tiles of 128), so that a result
+    // does not depend on the workspace's size
     size_t scratch = 0;
-    for (int64_t rows = 1; rows < max_rows + 16 && rows <= 8192; rows += 16)
+    for (int64_t rows = 1; rows < max_rows + 16 && rows <= 16384; rows += 16)
         for (int swiglu = 0; swiglu < (N % 2 ? 1 : 2); ++swiglu)
             scratch = std::max(scratch, rkh_mx4_scratch_bytes((int)std::min<int64_t>(rows + 15, max_rows), swiglu ? N / 2 : N, K, swiglu));
     std::lock_guard<std::mutex> lock(domain->ctx->submit_mutex);
