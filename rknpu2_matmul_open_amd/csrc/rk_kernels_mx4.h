@@ -13,6 +13,7 @@ namespace {
 typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef int v2i_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
 
 template <int TYPE> struct MxType;
 template <> struct MxType<RKH_MX4_F32> { using T = float; };

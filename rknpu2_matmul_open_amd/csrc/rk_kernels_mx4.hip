@@ -52,41 +52,59 @@ __device__ __forceinline__ float mx_value(uint32_t code) { // e2m1: sign, two bi
     return code & 8 ? -size : size;
 }
 
-template <int TYPE>
+// A lane makes 16 bytes of a row, so that a wave stores 1 KiB in a row.  STREAM: with streaming stores, for results that the caches would not
+// hold: written the usual way, 32 bytes apart, the 235 MB of 4096 x 14336 fp32 values were still on their way to memory when the next launch read its
+// rows (quantization and reading back together 87 -> 68 us; streaming stores of half lines, 16 bytes of every 32: 124).
+constexpr size_t STREAM_FROM = (size_t)64 << 20; // a quarter of the memory-side cache
+
+template <int TYPE, bool STREAM>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, void* y, int64_t rows, int K, int64_t ldy) {
-    const int KB = (K + 31) / 32, part = threadIdx.x & 3;
+    constexpr int V = TYPE == RKH_MX4_F32 ? 4 : 8, LANES = 32 / V; // values of a lane, lanes of a block
+    constexpr int PASSES = 64 * QUANT_UNITS * LANES / 256;
+    const int KB = (K + 31) / 32, part = threadIdx.x % LANES, mine = threadIdx.x / LANES;
     const int64_t blocks = rows * KB, first = (int64_t)blockIdx.x * (64 * QUANT_UNITS);
-    const bool dense = ldy == K && K % 32 == 0;
+    const int live = (int)min(blocks - first, (int64_t)(64 * QUANT_UNITS));
+    const bool dense = K % 32 == 0 && (ldy == K || rows == 1);
     const int64_t row0 = dense ? 0 : first / KB;
     const unsigned rest = (unsigned)(first - row0 * KB);
-    uint32_t w[QUANT_UNITS], s[QUANT_UNITS];
+    uint32_t w[PASSES], s[PASSES];
 #pragma unroll
-    for (int u = 0; u < QUANT_UNITS; ++u) {
-        const int64_t at = first + u * 64 + (threadIdx.x >> 2);
-        if (at >= blocks) continue;
-        w[u] = *reinterpret_cast<const u32_any*>(codes + at * 16 + part * 4);
+    for (int u = 0; u < PASSES; ++u) { // (beyond the end: the last block again, which is not stored)
+        const int64_t at = first + min(u * (256 / LANES) + mine, live - 1);
+        if constexpr (V == 4) w[u] = *reinterpret_cast<const u16_any*>(codes + at * 16 + part * 2);
+        else w[u] = *reinterpret_cast<const u32_any*>(codes + at * 16 + part * 4);
         s[u] = scales[at];
     }
 #pragma unroll
-    for (int u = 0; u < QUANT_UNITS; ++u) {
-        const int64_t at = first + u * 64 + (threadIdx.x >> 2);
-        if (at >= blocks) continue;
-        float v[8];
+    for (int u = 0; u < PASSES; ++u) {
+        const int unit = u * (256 / LANES) + mine;
+        if (unit >= live) continue;
+        float v[V];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = s[u] == 255u ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(mx_value((w[u] >> (4 * e)) & 15u), (int)s[u] - 127);
+        for (int e = 0; e < V; ++e) v[e] = s[u] == 255u ? __uint_as_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(mx_value((w[u] >> (4 * e)) & 15u), (int)s[u] - 127);
+        size_t i;
+        int count = V;
         if (dense) {
-            mx_store<TYPE, 8>(y, at * 32 + part * 8, v);
+            i = (size_t)(first + unit) * 32 + part * V;
         } else {
-            const unsigned t = rest + u * 64 + (threadIdx.x >> 2), r = t / (unsigned)KB;
-            const int k = (int)(t - r * KB) * 32 + part * 8;
-            const size_t i = (row0 + r) * ldy + k;
-            if (k + 8 <= K) {
-                mx_store<TYPE, 8>(y, i, v);
-            } else {
+            const unsigned t = rest + unit, r = t / (unsigned)KB;
+            const int k = (int)(t - r * KB) * 32 + part * V;
+            i = (row0 + r) * ldy + k;
+            count = K - k;
+        }
+        if (count >= V) {
+            using T = typename MxType<TYPE>::T;
+            typedef T vec __attribute__((ext_vector_type(V)));
+            vec x;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (k + e < K) mx_store1<TYPE>(y, i + e, v[e]);
-            }
+            for (int e = 0; e < V; ++e) x[e] = (T)v[e];
+            v4i_any* to = reinterpret_cast<v4i_any*>(static_cast<uint8_t*>(y) + i * sizeof(T));
+            if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(v4i, x), to);
+            else *to = __builtin_bit_cast(v4i, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (e < count) mx_store1<TYPE>(y, i + e, v[e]);
         }
     }
 }
@@ -171,8 +189,10 @@ int rkh_mx4_dequantize(void* stream, int type, int64_t rows, int K, const uint8_
     if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
     mark((hipStream_t)stream, "mx4_dequantize_kernel");
     mx_with_type(type, [&](auto t) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_dequantize_kernel<decltype(t)::value>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream,
-                           codes, scales, y, rows, K, ldy);
+        constexpr int TYPE = decltype(t)::value;
+        const bool streams = (size_t)rows * K * sizeof(typename MxType<TYPE>::T) > STREAM_FROM;
+        const auto kernel = streams ? mx4_dequantize_kernel<TYPE, true> : mx4_dequantize_kernel<TYPE, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, codes, scales, y, rows, K, ldy);
     });
     RKH_CHECK(hipGetLastError());
     return RKH_OK;

@@ -153,6 +153,21 @@ def test_many_short_rows(sess):
     assert np.array_equal(host(y)[some], ref.round_trip(host(x)[some]))
 
 
+@pytest.mark.parametrize("kind,rows,K,pad", [("f32", 1030, 17000, 0), ("bf16", 2100, 16500, 3)])
+def test_results_larger_than_the_caches(sess, kind, rows, K, pad):
+    """Values of more than 64 MiB are written with other stores."""
+    codes, scales = ref.exact_rows(np.random.default_rng(rows), 37, K)
+    pick = np.random.default_rng(1).integers(0, 37, rows)
+    y, buf = poisoned(rows, K, kind, K + pad)
+    dc, ds = device(codes[pick]), device(scales[pick])
+    ready()
+    ops.mx4_dequantize(sess, dc, ds, y)
+    done(sess)
+    want = torch.from_numpy(ref.values(codes, scales, K).astype(np.float32)).to(TYPES[kind]).to("cuda")[torch.from_numpy(pick).to("cuda")]
+    assert torch.equal(y, want)
+    assert (buf[rows * (K + pad):] == 77).all() and (pad == 0 or (buf[:rows * (K + pad)].view(rows, K + pad)[:, K:] == 77).all())
+
+
 # ---- products ----------------------------------------------------------------------------
 
 
