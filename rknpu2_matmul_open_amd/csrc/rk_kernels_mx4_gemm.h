@@ -648,9 +648,9 @@ struct MxRoute {
 constexpr int MX_ROWS = 4;  // rows that the few-row kernel quantizes itself
 constexpr int MX_CUS = 256; // compute units that a launch is cut for
 
-// The shapes of tiles and what a group of 512 k takes in each, us, when every compute unit has one, and a tile's conversion: from 4096 x 4096 x 4096
-// (256 x 256: 32 us), 2048 x 4096 x 4096 (128 x 256, halves of the former: 19.9; 256 x 128 takes the same and had no sizes of its own), 1024 x 4096 x 4096 (128 x 128: 11.7), 512 x 4096 x 14336
-// (128 x 64: 20.7, 64 x 128: 21.0), 256 x 4096 x 4096 (64 x 64: 6.3).
+// The shapes of tiles, what a group of 512 k takes in each when every compute unit has one, and a tile's conversion, us: from 4096 x 4096 x 4096
+// (256 x 256: 32 us), 2048 x 4096 x 4096 (128 x 256, halves of the former: 19.9; 256 x 128 takes the same and had no sizes of its own), 1024 x 4096 x
+// 4096 (128 x 128: 11.7), 512 x 4096 x 14336 (128 x 64: 20.7, 64 x 128: 21.0), 256 x 4096 x 4096 (64 x 64: 6.3).
 struct MxShape { int rm, cn; float group, end; };
 constexpr MxShape MX_SHAPES[] = {{8, 8, 3.4f, 1.8f}, {4, 4, 1.05f, 0.5f}, {2, 4, 0.63f, 0.3f}, {4, 2, 0.62f, 0.3f}, {2, 2, 0.4f, 0.2f}};
 constexpr float MX_HALF_GROUP = 2.0f;                     // of 128 x 256
@@ -763,7 +763,8 @@ template <bool SWIGLU, int OUT> int launch_big(hipStream_t st, const rkh_mx4_gem
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks, left = tiles % MX_CUS, big = left <= MX_CUS / 2 ? tiles - left : tiles;
     if (tiles > 0x3fffffff) return RKH_ERR_RUNTIME;
     mark(st, "mx4_big_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_big_kernel<SWIGLU, OUT>), dim3((unsigned)(big ? std::min<int64_t>(big, MX_CUS) : 2 * left)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, (int)big);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_big_kernel<SWIGLU, OUT>), dim3((unsigned)(big ? std::min<int64_t>(big, MX_CUS) : 2 * left)), dim3(256), LDS,
+                       st, g, r.mblocks, r.nblocks, (int)big);
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
 }

@@ -21,6 +21,8 @@ void rkh_mx4_route(int M, int N, int K, int swiglu, int* kernel, int* rows, int*
     *columns = r.few ? 16 * r.cn : 32 * r.cn;
     *parts = r.parts;
 }
+// (mx_route: K in parts of four groups or more, a part for each compute unit at most, tiles of up to 128 x 128)
+size_t rkh_mx4_scratch_most(int max_rows, int K) { return max_rows > 16 && rkh_mx4_k4(K) >= 8 ? (size_t)MX_CUS * 128 * 128 * 4 : 0; }
 size_t rkh_mx4_scratch_bytes(int M, int N, int K, int swiglu) { return mx_scratch(mx_route(M, N, K, swiglu)); }
 
 } // extern "C"

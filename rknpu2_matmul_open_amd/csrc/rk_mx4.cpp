@@ -44,8 +44,9 @@ Span values(const void* p, int type, int64_t rows, int64_t ld, int64_t width) {
 }
 // Pointer and stride of rows of values: aligned to the type, no row on the next one, and all of it addressable.
 bool valid_rows(const void* p, int type, int64_t rows, int64_t ld, int64_t width) {
+    if (rows == 0) return valid_type(type); // (an empty tensor may have no address)
     return valid_type(type) && p && reinterpret_cast<uintptr_t>(p) % type_bytes(type) == 0 && ld >= width && ld <= (INT64_C(1) << 40) &&
-           (rows == 0 || ld <= (INT64_C(1) << 56) / rows);
+           ld <= (INT64_C(1) << 56) / rows;
 }
 
 rk_npu_mx4_weights* create_weights(rk_npu_iommu_domain* domain, const rk_npu_mx4_weight_config* config, const uint8_t* codes, const uint8_t* scales,
@@ -207,7 +208,9 @@ rkh_block_norm_args norm_args(const rk_npu_block_norm_args* a) {
 extern "C" {
 
 int rk_npu_mx4_quantize_device(rk_npu_ctx* ctx, int type, int64_t rows, int K, const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales) {
-    if (!ctx || rows < 0 || rows > INT64_C(1) << 40 || !valid_length(K) || !valid_rows(x, type, rows, ldx, K) || !codes || !scales) return RK_NPU_ERR_PARAM;
+    if (!ctx || rows < 0 || rows > INT64_C(1) << 40 || !valid_length(K) || !valid_rows(x, type, rows, ldx, K) ||
+        (rows && (!codes || !scales)))
+        return RK_NPU_ERR_PARAM;
     const int64_t blocks = (K + 31) / 32;
     const Span in = values(x, type, rows, ldx, K), c(codes, rows, blocks * 16, blocks * 16), s(scales, rows, blocks, blocks);
     if (rows * blocks > (INT64_C(1) << 38) || c.meets(in) || s.meets(in) || c.meets(s)) return RK_NPU_ERR_PARAM;
@@ -216,7 +219,9 @@ int rk_npu_mx4_quantize_device(rk_npu_ctx* ctx, int type, int64_t rows, int K, c
 }
 
 int rk_npu_mx4_dequantize_device(rk_npu_ctx* ctx, int type, int64_t rows, int K, const uint8_t* codes, const uint8_t* scales, void* y, int64_t ldy) {
-    if (!ctx || rows < 0 || rows > INT64_C(1) << 40 || !valid_length(K) || !valid_rows(y, type, rows, ldy, K) || !codes || !scales) return RK_NPU_ERR_PARAM;
+    if (!ctx || rows < 0 || rows > INT64_C(1) << 40 || !valid_length(K) || !valid_rows(y, type, rows, ldy, K) ||
+        (rows && (!codes || !scales)))
+        return RK_NPU_ERR_PARAM;
     const int64_t blocks = (K + 31) / 32;
     const Span out = values(y, type, rows, ldy, K), c(codes, rows, blocks * 16, blocks * 16), s(scales, rows, blocks, blocks);
     if (rows * blocks > (INT64_C(1) << 38) || c.meets(out) || s.meets(out)) return RK_NPU_ERR_PARAM;
@@ -248,12 +253,8 @@ rk_npu_mx4_workspace* rk_npu_mx4_workspace_create(rk_npu_iommu_domain* domain, i
     ws->rows = max_rows;
     ws->K = K;
     ws->N = N;
-    // the most that any call of up to so many rows splits K into (no more than 16384 rows do: 128 tiles of 128), so that a result
-    // does not depend on the workspace's size
-    size_t scratch = 0;
-    for (int64_t rows = 1; rows < max_rows + 16 && rows <= 16384; rows += 16)
-        for (int swiglu = 0; swiglu < (N % 2 ? 1 : 2); ++swiglu)
-            scratch = std::max(scratch, rkh_mx4_scratch_bytes((int)std::min<int64_t>(rows + 15, max_rows), swiglu ? N / 2 : N, K, swiglu));
+    // what any of the calls may ask for, so that a result does not depend on the workspace's sizes
+    const size_t scratch = rkh_mx4_scratch_most(max_rows, K);
     std::lock_guard<std::mutex> lock(domain->ctx->submit_mutex);
     // (zeros: blocks beyond K are read and never written by the SwiGLU epilogue)
     if (ws->codes.alloc(ws->owner, rkh_mx4_code_bytes(max_rows, K), true) || ws->scales.alloc(ws->owner, rkh_mx4_scale_bytes(max_rows, K), true) ||
@@ -335,7 +336,7 @@ int rk_npu_block_norm_device(rk_npu_ctx* ctx, const rk_npu_block_norm_args* a) {
     int rc = check_norm(a, a->branch != nullptr);
     if (rc) return rc;
     rk_npu_mx4_workspace* ws = a->staged;
-    if ((!a->residual_out && !a->y && !ws) || norm_overlaps(a, nullptr, nullptr)) return RK_NPU_ERR_PARAM;
+    if ((a->rows && !a->residual_out && !a->y && !ws) || norm_overlaps(a, nullptr, nullptr)) return RK_NPU_ERR_PARAM;
     if (ws && (ws->owner.ctx != ctx || ws->owner.ctx_id != ctx->id)) return RK_NPU_ERR_DOMAIN;
     if (ws && (a->D != ws->K || a->rows > ws->rows)) return RK_NPU_ERR_PARAM;
     std::atomic_flag none = ATOMIC_FLAG_INIT;
@@ -357,8 +358,8 @@ int rk_npu_mx4_run_ffn_block_device(rk_npu_mx4_workspace* ws, const rk_npu_mx4_w
     int rc = check_ffn(ws, gate_up, down_ws, down);
     if (!rc) rc = check_norm(a, true);
     if (rc) return rc;
-    if (a->branch || a->staged || (!a->residual_out && !a->y) || !valid_rows(branch, a->branch_type, a->rows, a->branch_ld, a->D) || a->D != ws->K || a->D != down->config.N || a->rows > ws->rows || a->rows > down_ws->rows ||
-        reinterpret_cast<uintptr_t>(next_weight) % 4 || norm_overlaps(a, branch, next_weight))
+    if (a->branch || a->staged || (a->rows && !a->residual_out && !a->y) || !valid_rows(branch, a->branch_type, a->rows, a->branch_ld, a->D) ||
+        a->D != ws->K || a->D != down->config.N || a->rows > ws->rows || a->rows > down_ws->rows || reinterpret_cast<uintptr_t>(next_weight) % 4 || norm_overlaps(a, branch, next_weight))
         return RK_NPU_ERR_PARAM;
     BusyLock lock(ws->busy), down_lock(down_ws->busy);
     if (!lock || !down_lock) return RK_NPU_ERR_BUSY;

@@ -73,6 +73,8 @@ int rkh_mx4_takes_rows(int M, int N, int K, int swiglu);
  * workgroup and the parts that K is split into.  N as in the args. */
 void rkh_mx4_route(int M, int N, int K, int swiglu, int* kernel, int* rows, int* columns, int* parts);
 size_t rkh_mx4_scratch_bytes(int M, int N, int K, int swiglu);
+/* ... and the most that any product of up to max_rows rows of K values needs. */
+size_t rkh_mx4_scratch_most(int max_rows, int K);
 
 typedef struct rkh_block_norm_args {
     int rows, D;
@@ -88,6 +90,7 @@ typedef struct rkh_block_norm_args {
     int64_t ld_stream, ld_branch, gate_row_stride, ld_stream_out, ld_y;
     uint8_t* q;            /* operand blocks of the normed rows, or NULL                          */
     uint8_t* q_scale;
+    int first;             /* (a launch's first row; the launcher's own)                           */
 } rkh_block_norm_args;
 int rkh_block_norm(void* stream, const rkh_block_norm_args* args);
 

@@ -387,9 +387,15 @@ class MoeW8:
 _MX4_TYPES = {"torch.float32": capi.MX4_F32, "torch.float16": capi.MX4_F16, "torch.bfloat16": capi.MX4_BF16}
 
 
+def _on_device(x):
+    if not getattr(x, "is_cuda", True):
+        raise ValueError("a tensor on the device is needed, this one lies on %s" % x.device)
+
+
 def _mx4_rows(x, columns=None):
     """(element type, address, row stride) of a 2-d tensor whose rows are contiguous."""
     kind = _MX4_TYPES.get(str(x.dtype))
+    _on_device(x)
     if kind is None:
         raise TypeError("rows of float32, float16 or bfloat16: got %s" % x.dtype)
     if len(x.shape) != 2 or (columns is not None and x.shape[1] != columns) or (x.shape[1] > 1 and x.stride(1) != 1):
@@ -398,6 +404,7 @@ def _mx4_rows(x, columns=None):
 
 
 def _mx4_bytes(x, rows, width, what):
+    _on_device(x)
     if str(x.dtype) != "torch.uint8" or tuple(x.shape) != (rows, width) or not x.is_contiguous():
         raise ValueError("%s: contiguous uint8 of shape %s, got %s %s" % (what, (rows, width), x.dtype, tuple(x.shape)))
     return C.c_void_p(x.data_ptr())
@@ -489,6 +496,7 @@ def mx4_ffn(gu_ws, gate_up, down_ws, down, a, c):
 def _channel(w, D, what):
     if w is None:
         return None
+    _on_device(w)
     if str(w.dtype) != "torch.float32" or tuple(w.shape) != (D,) or not w.is_contiguous():
         raise ValueError("%s: contiguous float32 [%d], got %s %s" % (what, D, w.dtype, tuple(w.shape)))
     return w.data_ptr()
@@ -533,6 +541,6 @@ def mx4_ffn_block(gu_ws, gate_up, down_ws, down, stream, branch, weight=None, af
                   eps=1e-6, stream_out=None, y=None, next_weight=None):
     """A gated FFN block on the residual stream (rk_npu_mx4_run_ffn_block_device); branch receives the FFN's output."""
     a = _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, None)
-    a.branch = None
+    a.branch = None # (an output here)
     check(gu_ws.lib.rk_npu_mx4_run_ffn_block_device(gu_ws.h, gate_up.h, down_ws.h, down.h, C.byref(a), C.c_void_p(branch.data_ptr()),
                                                     _channel(next_weight, stream.shape[1], "next_weight")), "mx4_ffn_block")

@@ -139,6 +139,21 @@ def test_staged_rows_are_the_quantized_y(sess, rows, D):
     w.close()
 
 
+def test_rows_of_more_than_one_launch(sess):
+    """A launch holds 2^31 threads at most: rows before and behind that line are what they are on their own."""
+    rows, D = (1 << 25) + 9, 2
+    x = torch.full((rows, D), 3.0, dtype=torch.float16, device="cuda")
+    near = slice((1 << 25) - 5, rows)
+    x[near] = device(np.random.default_rng(2).standard_normal((14, D)), "f16")
+    y, alone = torch.zeros_like(x), torch.zeros((14, D), dtype=torch.float16, device="cuda")
+    ready()
+    ops.block_norm(sess, x, y=y)
+    ops.block_norm(sess, x[near], y=alone)
+    done(sess)
+    assert torch.equal(y[near], alone) and alone.abs().min() > 0
+    assert (y[:near.start] == 1).all()
+
+
 def test_refusals(sess):
     rows, D = 4, 64
     buf = torch.ones(8 * rows * D, device="cuda")

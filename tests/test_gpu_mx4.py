@@ -502,7 +502,79 @@ def test_captured_block_replays_what_the_eager_call_gives(sess, M):
         h.close()
 
 
+def test_two_captured_graphs_share_workspaces(sess):
+    """Two graphs on the same workspaces, replayed in turn with eager calls between them: each stages its own rows."""
+    rng = np.random.default_rng(4)
+    M, H, N = 70, 640, 200
+    layers = [Layer(sess, rng, N, H, make=ordinary) for _ in range(2)]
+    ws = ops.MX4Workspace(sess, M, H, N)
+    xs = [device(rng.standard_normal((M, H)), "f16") for _ in range(2)]
+    outs = [torch.zeros((M, N), device="cuda") for _ in range(4)]
+
+    def call(k, to):
+        ws.stage(xs[k])
+        ws.run_staged(layers[k].w, to)
+    ready()
+    graphs = []
+    for k in range(2):
+        call(k, outs[2 + k])
+        done(sess)
+        assert sess.lib.rk_npu_hip_capture_begin(sess.ctx) == 0
+        call(k, outs[k])
+        graphs.append(sess.lib.rk_npu_hip_capture_end(sess.ctx))
+        assert graphs[-1]
+    for k in (0, 1, 1, 0, 1, 0, 0):
+        outs[k].zero_()
+        ready()
+        assert sess.lib.rk_npu_hip_graph_launch(sess.ctx, graphs[k]) == 0
+        call(1 - k, outs[3 - k])
+        done(sess)
+        assert np.array_equal(host(outs[k]), host(outs[2 + k])) and np.abs(host(outs[k])).max() > 0
+    for graph in graphs:
+        sess.lib.rk_npu_hip_graph_free(graph)
+    for h in layers + [ws]:
+        h.close()
+
+
+def test_offsets_beyond_32_bits(sess):
+    """More than 2^32 values in a quantization and in a product's result: the last rows are right, and reading back finds them."""
+    rng = np.random.default_rng(9)
+    rows, K = 140000, 32768
+    last = device(rng.standard_normal((3, K)), "bf16")
+    x = torch.zeros((rows, K), dtype=torch.bfloat16, device="cuda")
+    x[-3:] = last
+    codes, scales = torch.full((rows, K // 2), 0x11, dtype=torch.uint8, device="cuda"), torch.zeros((rows, K // 32), dtype=torch.uint8, device="cuda")
+    ready()
+    ops.mx4_quantize(sess, x, codes, scales)
+    done(sess)
+    x[-3:] = 0
+    ready()
+    ops.mx4_dequantize(sess, codes, scales, x)
+    done(sess)
+    assert np.array_equal(host(x[-3:]), ref.round_trip(host(last)))
+    assert not codes[:-3].any() and not x[:-3].any()
+    del x, codes, scales
+    M, N = 140000, 32000
+    layer = Layer(sess, rng, N, 32)
+    a = ref.values(*ref.exact_rows(rng, 64, 32), 32)
+    d = device(np.tile(a, (-(-M // 64), 1))[:M], "bf16")
+    ws, c = ops.MX4Workspace(sess, M, 32, N), torch.full((M, N), 77.0, dtype=torch.bfloat16, device="cuda")
+    ready()
+    ws.run(layer.w, d, c)
+    done(sess)
+    want = torch.from_numpy(a @ layer.values.T).to(torch.bfloat16).to("cuda")
+    for at in (0, 67072, 134208, M - 64):
+        assert torch.equal(c[at:at + 64], want.roll(-(at % 64), 0)), at
+    ws.close()
+    layer.close()
+
+
 def test_zero_rows_write_nothing(sess):
+    nothing = torch.zeros((0, 96), device="cuda")
+    none = torch.zeros((0, 48), dtype=torch.uint8, device="cuda"), torch.zeros((0, 3), dtype=torch.uint8, device="cuda")
+    ops.mx4_quantize(sess, nothing, *none)
+    ops.mx4_dequantize(sess, *none, nothing)
+    ops.block_norm(sess, nothing, y=nothing.clone())
     rng = np.random.default_rng(1)
     layer = Layer(sess, rng, 64, 96)
     ws = ops.MX4Workspace(sess, 8, 96, 64)

@@ -81,7 +81,7 @@ def _route(lib, M, N, K, swiglu):
 
 @pytest.mark.parametrize("swiglu", [0, 1])
 def test_route_covers_every_row_and_column_and_its_scratch_is_what_the_parts_need(lib, swiglu):
-    lib.rkh_mx4_scratch_bytes.restype = C.c_size_t
+    lib.rkh_mx4_scratch_bytes.restype = lib.rkh_mx4_scratch_most.restype = C.c_size_t
     rng = np.random.default_rng(3)
     for _ in range(3000):
         M, N, K = (int(np.exp(rng.uniform(0, np.log(top)))) for top in (9000, 40000, 40000))
@@ -96,6 +96,7 @@ def test_route_covers_every_row_and_column_and_its_scratch_is_what_the_parts_nee
         tiles = -(-M // rows) * -(-places // columns)
         want = tiles * parts * rows * columns * 4 if parts > 1 else 0
         assert lib.rkh_mx4_scratch_bytes(M, N, K, swiglu) == want, (M, N, K)
+        assert want <= lib.rkh_mx4_scratch_most(M, K), (M, N, K)
 
 
 def test_reference_of_the_format():
@@ -131,3 +132,26 @@ def test_audit_sees_sums_in_accumulation_registers():
     assert len(audit_waits.audit_text(kernel(["\ts_nop 7", move]))[0]) == 1
     assert audit_waits.audit_text(kernel(["\ts_nop 7", "\ts_nop 7", move])) == ([], 1)
     assert audit_waits.audit_text(kernel(["\tv_accvgpr_read_b32 v30, a8"])) == ([], 1)
+
+
+def test_wrappers_refuse_host_tensors_and_odd_layouts():
+    import torch
+
+    from rknpu2_matmul_open_amd import ops
+    with pytest.raises(ValueError):
+        ops._mx4_rows(torch.zeros(4, 32))
+    with pytest.raises(ValueError):
+        ops._channel(torch.zeros(32), 32, "weight")
+
+    class OnDevice:  # (what the wrappers look at)
+        def __init__(self, t):
+            self.t, self.dtype, self.shape, self.is_cuda = t, t.dtype, t.shape, True
+            self.stride, self.data_ptr = t.stride, t.data_ptr
+    kind, _, ld = ops._mx4_rows(OnDevice(torch.zeros(4, 40, dtype=torch.bfloat16)[:, :32]))
+    assert (kind, ld) == (capi.MX4_BF16, 40)
+    assert ops._mx4_rows(OnDevice(torch.zeros(1, 32)))[2] == 32
+    for bad in (torch.zeros(4, 32).t(), torch.zeros(32), torch.zeros(4, 64)[:, ::2]):
+        with pytest.raises(ValueError):
+            ops._mx4_rows(OnDevice(bad))
+    with pytest.raises(TypeError):
+        ops._mx4_rows(OnDevice(torch.zeros(4, 32, dtype=torch.float64)))
