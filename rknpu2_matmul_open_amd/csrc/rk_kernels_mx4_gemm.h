@@ -338,13 +338,32 @@ template <int RM, int CN, int HALVES> struct MxTile {
     static constexpr int BUF = (AB + WB) * 1024, SBUF = (AB + WB) * 256;
     static constexpr int SCALES_OFF = 4 * HALVES * BUF, LDS = SCALES_OFF + 2 * SBUF;
     static_assert(RM % 2 == 0 && CN % 2 == 0 && (HALVES == 1 || HALVES == 2) && LDS <= 160 * 1024, "");
-    // the copies of step t + 2 of a group have landed: what a wave has issued in the D - 2 steps up to step t
-    static constexpr int wait_for(int t) {
+    // The copies of step t + 2 of a group have landed: what a wave has issued in the D - 2 steps up to step t.  FIRST: no group is ahead of this one; the
+    // prologue issues its scales earlier than a group would.
+    static constexpr int wait_for(int t, bool first) {
         int n = 0;
-        for (int s = 0; s < D - 2; ++s) n += COPIES + ((t - s + 8) % 4 == 1 ? SC : 0);
+        for (int s = 0; s < D - 2; ++s) n += COPIES + ((t - s + 8) % 4 == 1 && (!first || t - s >= 0) ? SC : 0);
         return n;
     }
-    static_assert(D - 2 <= 5, "a group's scales, issued in the sixth step ahead, are older than what wait_for leaves in flight");
+    // All of it counted out over the first groups: whatever a step reads has landed behind the wait that ends the step before.
+    static constexpr bool covers() {
+        constexpr int STEPS = 16;
+        int issued = 0, step_at[STEPS + 16] = {}, scales_at[STEPS / 4 + 4] = {};
+        scales_at[0] = issued += SC;
+        for (int s = 0; s < D; ++s) {
+            if (s == 2) scales_at[1] = issued += SC;
+            step_at[s] = issued += COPIES;
+        }
+        int landed = issued - (D - 2) * COPIES;
+        if (step_at[1] > landed || scales_at[1] > landed) return false;
+        for (int t = 0; t < STEPS; ++t) {
+            if (t % 4 == 1) scales_at[t / 4 + 2] = issued += SC;
+            step_at[t + D] = issued += COPIES;
+            landed = issued - wait_for(t % 4, t < 4);
+            if (step_at[t + 2] > landed || ((t + 1) % 4 == 3 && scales_at[t / 4 + 1] > landed)) return false;
+        }
+        return true;
+    }
 };
 
 // Where a tile lies: column sweeps over groups of row blocks, so that concurrently running tiles share weights in L2.
@@ -386,6 +405,7 @@ template <int RM, int CN, int HALVES, bool SWIGLU, int OUT>
 __device__ __forceinline__ void mx_tiles(const rkh_mx4_gemm_args& g, uint8_t* lds, const MxJobs& of, int job, int stride) {
     using S = MxTile<RM, CN, HALVES>;
     static_assert(!SWIGLU || CN % 4 == 0, "gate and up halves of blocks of 32 columns in one wave");
+    static_assert(S::covers(), "a step would read what has not landed");
     constexpr auto in_acc = [](int i) { return RM * CN < 64 || i < RM - 1; };
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave & 1, wn = wave >> 1;
     const int K4 = (int)rkh_mx4_k4(g.K);
@@ -531,7 +551,7 @@ __device__ __forceinline__ void mx_tiles(const rkh_mx4_gemm_args& g, uint8_t* ld
             if constexpr (T == 3 && I == RM - 1) read_ws(s_from, J);
             __builtin_amdgcn_sched_barrier(0);
         });
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::wait_for(T)) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::wait_for(T, decltype(fresh_tag)::value)) : "memory");
     };
     for (;;) {
         const auto group = [&](auto fresh_tag) {

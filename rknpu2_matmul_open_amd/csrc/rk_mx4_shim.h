@@ -1,7 +1,7 @@
 /*
  * rk_mx4_shim.h -- the C ABI between the host layer of the microscaled 4-bit (MX4) operators and of the block norm
- * (rk_mx4.cpp) and their kernels (rk_kernels_mx4.hip, rk_kernels_mx4_gemm.hip, rk_kernels_norm.hip).  Conventions as in
- * rk_hip_shim.h.
+ * (rk_mx4.cpp) and their kernels (rk_kernels_mx4.hip, rk_kernels_norm.hip; rk_kernels_mx4_gemm.h, in two units: rk_kernels_mx4_gemm.hip and
+ * rk_kernels_mx4_swiglu.hip).  Conventions as in rk_hip_shim.h.
  *
  * Device data layouts
  * -------------------
