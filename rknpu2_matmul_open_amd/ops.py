@@ -433,6 +433,9 @@ class MX4Weights:
 
     def __init__(self, session, K, N, codes, scales, gate_up=False, on_device=False):
         self.lib, self.K, self.N, self.gate_up = session.lib, K, N, gate_up
+        blocks = N * -(-K // 32)
+        if not on_device and any(x.dtype != np.uint8 or x.size != n or not x.flags.c_contiguous for x, n in ((codes, 16 * blocks), (scales, blocks))):
+            raise ValueError("contiguous uint8 of %d bytes of codes and %d scales: got %s and %s" % (16 * blocks, blocks, codes.shape, scales.shape))
         create = self.lib.rk_npu_mx4_weights_create_device if on_device else self.lib.rk_npu_mx4_weights_create
         config = capi.MX4WeightConfig(K, N, 1 if gate_up else 0)
         self.h = create(session.domain, C.byref(config), codes if on_device else ptr(codes), scales if on_device else ptr(scales))
@@ -454,6 +457,7 @@ class MX4Workspace:
 
     def __init__(self, session, max_rows, K, N):
         self.lib, self.K = session.lib, K
+        self.staged = 0 # rows that run_staged writes
         self.h = self.lib.rk_npu_mx4_workspace_create(session.domain, max_rows, K, N)
         if not self.h:
             raise ValueError("rk_npu_mx4_workspace_create failed")
@@ -464,6 +468,7 @@ class MX4Workspace:
         if c.shape[0] != a.shape[0]:
             raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
         check(call(self.h, weights.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4 run")
+        self.staged = 0
 
     def run(self, weights, a, c):
         self._run(self.lib.rk_npu_mx4_run_device, weights, a, c, weights.N)
@@ -474,9 +479,12 @@ class MX4Workspace:
     def stage(self, a):
         kind, p, ld = _mx4_rows(a, self.K)
         check(self.lib.rk_npu_mx4_stage_device(self.h, a.shape[0], kind, p, ld), "mx4 stage")
+        self.staged = a.shape[0]
 
     def run_staged(self, weights, c):
         kind, p, ld = _mx4_rows(c, weights.N // 2 if weights.gate_up else weights.N)
+        if c.shape[0] != self.staged:
+            raise ValueError("%d rows staged, %d out" % (self.staged, c.shape[0]))
         check(self.lib.rk_npu_mx4_run_staged_device(self.h, weights.h, kind, p, ld), "mx4 run_staged")
 
     def close(self):
@@ -491,6 +499,7 @@ def mx4_ffn(gu_ws, gate_up, down_ws, down, a, c):
     if c.shape[0] != a.shape[0]:
         raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
     check(gu_ws.lib.rk_npu_mx4_run_ffn_device(gu_ws.h, gate_up.h, down_ws.h, down.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4_ffn")
+    gu_ws.staged = down_ws.staged = 0
 
 
 def _channel(w, D, what):
@@ -535,6 +544,8 @@ def block_norm(session, stream, branch=None, after=None, gate=None, residual_sca
     next one) float32 [D]; gate [D] or [rows, D]."""
     a = _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, staged)
     check(session.lib.rk_npu_block_norm_device(session.ctx, C.byref(a)), "block_norm")
+    if staged is not None:
+        staged.staged = stream.shape[0]
 
 
 def mx4_ffn_block(gu_ws, gate_up, down_ws, down, stream, branch, weight=None, after=None, gate=None, residual_scale=1.0, branch_scale=1.0,
@@ -544,3 +555,4 @@ def mx4_ffn_block(gu_ws, gate_up, down_ws, down, stream, branch, weight=None, af
     a.branch = None # (an output here)
     check(gu_ws.lib.rk_npu_mx4_run_ffn_block_device(gu_ws.h, gate_up.h, down_ws.h, down.h, C.byref(a), C.c_void_p(branch.data_ptr()),
                                                     _channel(next_weight, stream.shape[1], "next_weight")), "mx4_ffn_block")
+    gu_ws.staged = down_ws.staged = 0

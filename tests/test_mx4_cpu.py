@@ -155,3 +155,28 @@ def test_wrappers_refuse_host_tensors_and_odd_layouts():
             ops._mx4_rows(OnDevice(bad))
     with pytest.raises(TypeError):
         ops._mx4_rows(OnDevice(torch.zeros(4, 32, dtype=torch.float64)))
+
+
+def test_wrappers_refuse_short_weights_and_results_of_other_rows_than_the_staged():
+    import torch
+
+    from rknpu2_matmul_open_amd import ops
+
+    class Session:  # (nothing is called before the checks)
+        lib = domain = None
+    for codes, scales in ((np.zeros((4, 31), np.uint8), np.zeros((4, 2), np.uint8)), (np.zeros((4, 32), np.uint8), np.zeros((4, 1), np.uint8)),
+                          (np.zeros((4, 32), np.int8), np.zeros((4, 2), np.uint8)), (np.zeros((4, 64), np.uint8)[:, ::2], np.zeros((4, 2), np.uint8))):
+        with pytest.raises(ValueError):
+            ops.MX4Weights(Session, 40, 4, codes, scales)
+    ws = ops.MX4Workspace.__new__(ops.MX4Workspace)
+    ws.K, ws.staged = 40, 5
+
+    class Weights:
+        N, gate_up = 64, False
+
+    class Out:
+        def __init__(self, t):
+            self.dtype, self.shape, self.is_cuda, self.stride, self.data_ptr = t.dtype, t.shape, True, t.stride, t.data_ptr
+    for rows in (4, 6, 0):
+        with pytest.raises(ValueError):
+            ws.run_staged(Weights, Out(torch.zeros(rows, 64)))
