@@ -8,7 +8,9 @@
  * All pointers are device pointers unless said otherwise; the calls enqueue on the context's stream and return, under the rules
  * for *_device calls in rk_npu_hip.h (rk_npu_hip_sync() waits, stream capture records them, a workspace is BUSY only while a
  * call enqueues).  Rows lie `ld` values apart (ld >= the row's length, any alignment of the element's size).  Calls of zero
- * rows do nothing.  An output may not overlap an input (RK_NPU_ERR_PARAM), except where it is said below.
+ * rows do nothing.  An output may not share a byte with an input or another output (RK_NPU_ERR_PARAM), except where it is said
+ * below.  Rows of one pitch in bytes may lie between each other's, as column slices of one buffer do; rows of different pitches
+ * are told apart by their ranges alone, first byte to last.
  *
  * MX4 rows
  *   code    bits 3 sign, 2..0 one of 0, 0.5, 1, 1.5, 2, 3, 4, 6

@@ -7,6 +7,7 @@
 #include "rk_host.h"
 #include "rk_mx4_shim.h"
 #include "rk_npu_mx4.h"
+#include "rk_rows.h"
 
 using namespace rkhost;
 
@@ -31,14 +32,6 @@ bool valid_type(int type) { return type >= RK_NPU_MX4_F32 && type <= RK_NPU_MX4_
 int64_t type_bytes(int type) { return type == RK_NPU_MX4_F32 ? 4 : 2; }
 bool valid_length(int K) { return K > 0 && K <= INT32_MAX / 1024; }
 
-// Memory that rows of `width` bytes, `pitch` apart, lie in.
-struct Span {
-    uintptr_t from = 0, to = 0;
-    Span() = default;
-    Span(const void* p, int64_t rows, int64_t pitch, int64_t width)
-        : from(reinterpret_cast<uintptr_t>(p)), to(p && rows > 0 ? from + (uintptr_t)((rows - 1) * pitch + width) : from) {}
-    bool meets(const Span& o) const { return from < o.to && o.from < to; }
-};
 Span values(const void* p, int type, int64_t rows, int64_t ld, int64_t width) {
     return Span(p, rows, ld * type_bytes(type), width * type_bytes(type));
 }

@@ -1,0 +1,150 @@
+"""GPU tests of MX4 and block norm calls that a program may make of them beyond the plain ones: operands that are slices of one buffer.
+
+Products of exact_rows are compared bit for bit; the other calls with the same call on buffers of their own.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from rknpu2_matmul_open_amd import capi, ops
+from tests import mx4_reference as ref
+from tests.test_gpu_mx4 import Layer, TYPES, device, done, host, ordinary, ready
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- column slices of one buffer ---------------------------------------------------------
+
+
+def halves(rows, left, right, kind="f32", gap=0):
+    """Two slices of one buffer of 77s, of `left` and `right` columns, and the buffer."""
+    buf = torch.full((rows, left + gap + right + 3), 77.0, dtype=TYPES[kind], device="cuda")
+    return buf[:, :left], buf[:, left + gap:left + gap + right], buf
+
+
+@pytest.mark.parametrize("M", [1, 3, 20, 200, 1100])
+@pytest.mark.parametrize("swap", [False, True])
+def test_product_between_the_slices_of_a_buffer(sess, M, swap):
+    """Rows and result as column slices of one buffer, either one first."""
+    rng = np.random.default_rng(M)
+    K, N = 520, 100
+    layer = Layer(sess, rng, N, K)
+    a = ref.values(*ref.exact_rows(rng, M, K), K)
+    ws = ops.MX4Workspace(sess, M, K, N)
+    first, second, buf = halves(M, *((N, K) if swap else (K, N)))
+    x, c = (second, first) if swap else (first, second)
+    x.copy_(device(a, "f32"))
+    ready()
+    ws.run(layer.w, x, c)
+    done(sess)
+    assert np.array_equal(host(c), a @ layer.values.T) and np.array_equal(host(x), a)
+    assert (host(buf)[:, K + N:] == 77).all()
+    # a result of another type in the same buffer: its pitch in bytes is the rows' own
+    as_half = buf.view(torch.float16)
+    at = 0 if swap else 2 * K
+    half = as_half[:, at:at + N]
+    ready()
+    ws.run(layer.w, x, half)
+    done(sess)
+    assert np.array_equal(host(half), torch.from_numpy(a @ layer.values.T).half().double().numpy()) and np.array_equal(host(x), a)
+    ws.close()
+    layer.close()
+
+
+@pytest.mark.parametrize("M,H,F", [(1, 64, 96), (5, 333, 260), (200, 512, 1000)])
+def test_ffn_calls_between_the_slices_of_a_buffer(sess, M, H, F):
+    rng = np.random.default_rng(M + H)
+    gu, dn = Layer(sess, rng, 2 * F, H, gate_up=True, make=ordinary), Layer(sess, rng, H, F, make=ordinary)
+    gws, dws = ops.MX4Workspace(sess, M, H, 2 * F), ops.MX4Workspace(sess, M, F, H)
+    value = device(rng.standard_normal((M, H)), "f32")
+    x, c, _ = halves(M, H, H)
+    x.copy_(value)
+    want, middle, want_middle = torch.zeros((M, H), device="cuda"), halves(M, H, F), torch.zeros((M, F), device="cuda")
+    middle[0].copy_(value)
+    branch, stream_out, _ = halves(M, H, H, gap=2)
+    y, want_out, want_y = torch.zeros((M, H), device="cuda"), torch.zeros((M, H), device="cuda"), torch.zeros((M, H), device="cuda")
+    ready()
+    ops.mx4_ffn(gws, gu.w, dws, dn.w, value, want)
+    ops.mx4_ffn(gws, gu.w, dws, dn.w, x, c)
+    gws.run_swiglu(gu.w, value, want_middle)
+    gws.run_swiglu(gu.w, middle[0], middle[1])
+    done(sess)
+    assert torch.equal(c, want) and torch.equal(x, value) and torch.equal(middle[1], want_middle) and want.abs().max() > 0
+    ops.mx4_ffn_block(gws, gu.w, dws, dn.w, value, want, stream_out=want_out, y=want_y)
+    ops.mx4_ffn_block(gws, gu.w, dws, dn.w, value, branch, stream_out=stream_out, y=y)
+    done(sess)
+    assert torch.equal(branch, want) and torch.equal(stream_out, want_out) and torch.equal(y, want_y)
+    for h in (gws, dws, gu, dn):
+        h.close()
+
+
+@pytest.mark.parametrize("rows,D", [(1, 40), (4, 64), (9, 4096), (3, 17000)])
+def test_norm_between_the_slices_of_a_buffer(sess, rows, D):
+    """Stream, branch, gate and both outputs as slices of one buffer, the stream in place in the second call."""
+    rng = np.random.default_rng(D)
+    buf = torch.zeros((rows, 5 * D + 1), device="cuda")
+    stream, branch, gate, out, y = (buf[:, i * D:(i + 1) * D] for i in range(5))
+    buf.copy_(device(rng.standard_normal((rows, 5 * D + 1)), "f32"))
+    apart = [t.clone() for t in (stream, branch, gate)]
+    want_out, want_y = torch.zeros((rows, D), device="cuda"), torch.zeros((rows, D), device="cuda")
+    ready()
+    ops.block_norm(sess, apart[0], apart[1], gate=apart[2], residual_scale=0.5, stream_out=want_out, y=want_y)
+    ops.block_norm(sess, stream, branch, gate=gate, residual_scale=0.5, stream_out=out, y=y)
+    done(sess)
+    assert torch.equal(out, want_out) and torch.equal(y, want_y)
+    assert all(torch.equal(t, was) for t, was in zip((stream, branch, gate), apart))
+    y.zero_()
+    ready()
+    ops.block_norm(sess, stream, branch, gate=gate, residual_scale=0.5, stream_out=stream, y=y)
+    done(sess)
+    assert torch.equal(stream, want_out) and torch.equal(y, want_y)
+
+
+def test_values_read_back_beside_their_codes(sess):
+    """A buffer that holds each row's codes and values next to each other is no MX4 matrix, but values between other values' rows are fine."""
+    rows, K = 6, 64
+    buf = torch.full((rows, 2 * K), 77.0, device="cuda")
+    codes, scales = torch.zeros((rows, 32), dtype=torch.uint8, device="cuda"), torch.zeros((rows, 2), dtype=torch.uint8, device="cuda")
+    buf[:, K:] = device(np.random.default_rng(3).standard_normal((rows, K)), "f32")
+    want = ref.round_trip(host(buf[:, K:]))
+    ready()
+    ops.mx4_quantize(sess, buf[:, K:], codes, scales)
+    ops.mx4_dequantize(sess, codes, scales, buf[:, :K])
+    done(sess)
+    assert np.array_equal(host(buf[:, :K]), want)
+
+
+def test_slices_that_share_a_column_are_refused(sess):
+    rng = np.random.default_rng(1)
+    K, N, M = 96, 64, 4
+    layer = Layer(sess, rng, N, K)
+    ws = ops.MX4Workspace(sess, M, K, N)
+    buf = torch.ones((M + 2, K + N), device="cuda")
+    ready()
+    for x, c in ((buf[:M, :K], buf[:M, K - 1:K + N - 1]), (buf[:M, N:], buf[:M, 1:N + 1]), (buf[:M, :K], buf[1:M + 1, K - 1:K + N - 1]),
+                 (buf[1:M + 1, N:], buf[:M, 1:N + 1])):
+        with pytest.raises(ops.RkError) as e:
+            ws.run(layer.w, x, c)
+        assert e.value.code == capi.RK_NPU_ERR_PARAM
+    # rows of two pitches in one range, though no byte is shared
+    flat = torch.ones(4096, device="cuda")
+    q = flat.data_ptr()
+    assert sess.lib.rk_npu_mx4_run_device(ws.h, layer.w.h, 2, 0, C.c_void_p(q), 512, 0, C.c_void_p(q + 4 * 100), 64) == capi.RK_NPU_ERR_PARAM
+    a = capi.BlockNormArgs()
+    sess.lib.rk_npu_block_norm_args_init(C.byref(a), 3, 64)
+    a.residual, a.residual_ld, a.residual_out, a.residual_out_ld, a.y, a.y_ld = q, 200, q + 4 * 64, 200, q + 4 * 127, 200
+    assert sess.lib.rk_npu_block_norm_device(sess.ctx, C.byref(a)) == capi.RK_NPU_ERR_PARAM
+    a.y = q + 4 * 128
+    assert sess.lib.rk_npu_block_norm_device(sess.ctx, C.byref(a)) == 0
+    done(sess)
+    # a weight of one row in the gap between rows: no output touches it
+    a.weight = q + 4 * 192
+    a.D = 8
+    assert sess.lib.rk_npu_block_norm_device(sess.ctx, C.byref(a)) == 0
+    a.weight = q + 4 * 135
+    assert sess.lib.rk_npu_block_norm_device(sess.ctx, C.byref(a)) == capi.RK_NPU_ERR_PARAM
+    done(sess)
+    ws.close()
+    layer.close()
