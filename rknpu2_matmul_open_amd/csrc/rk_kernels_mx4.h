@@ -15,6 +15,10 @@ typedef int v2i_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint16_t u16_any __attribute__((aligned(1)));
 
+// A launch holds fewer than 2^32 threads: of more, all but what is left modulo 2^32 never run, without an error.  Longer ones are cut into
+// pieces of so many workgroups of 256.
+constexpr int64_t MX_TOO_MANY_THREADS = INT64_C(1) << 32, MX_MOST_GROUPS = MX_TOO_MANY_THREADS / 2 / 256;
+
 template <int TYPE> struct MxType;
 template <> struct MxType<RKH_MX4_F32> { using T = float; };
 template <> struct MxType<RKH_MX4_F16> { using T = _Float16; };

@@ -1,5 +1,7 @@
 // MX4 rows: quantization, reading back, staging as operand blocks, and the packing of weights.
 // All of them are bound by memory; nothing is kept between values but a block's largest magnitude.
+#include <algorithm>
+
 #include "rk_kernels_mx4.h"
 
 namespace {
@@ -147,9 +149,9 @@ __global__ __launch_bounds__(256) void mx4_stage_kernel(const void* x, uint8_t* 
 // ---- weights ---------------------------------------------------------------------
 // One thread per 16 bytes of operand blocks, then per scale byte; places without a column, and blocks beyond K, are zero.
 __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* codes, const uint8_t* scales, uint8_t* dst, uint8_t* dst_scales, int K, int N,
-                                                       int gate_up, size_t pieces, size_t bytes) {
+                                                       int gate_up, size_t first, size_t pieces, size_t bytes) {
     const int KB = (K + 31) / 32, K4 = (int)rkh_mx4_k4(K);
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const size_t i = first + (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i < pieces) {
         const size_t piece = i >> 6;
         const int lane = (int)(i & 63), rb = (int)(piece / (K4 * 4)), b = (int)(piece - (size_t)rb * K4 * 4) * 4 + (lane >> 4);
@@ -171,28 +173,36 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* codes, con
 extern "C" {
 
 int rkh_mx4_quantize(void* stream, int type, int64_t rows, int K, const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales) {
-    const int64_t blocks = rows * ((K + 31) / 32), groups = (blocks + 64 * QUANT_UNITS - 1) / (64 * QUANT_UNITS);
-    if (!groups) return RKH_OK;
-    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
-    mark((hipStream_t)stream, "mx4_quantize_kernel");
+    if (!rows) return RKH_OK;
+    const int64_t KB = (K + 31) / 32, most = MX_MOST_GROUPS * 64 * QUANT_UNITS / KB; // rows of a launch
     mx_with_type(type, [&](auto t) {
-        const auto kernel = K % 32 == 0 && (ldx == K || rows == 1) ? mx4_quantize_kernel<decltype(t)::value, true> : mx4_quantize_kernel<decltype(t)::value, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, x, codes, scales, rows, K, ldx);
+        constexpr int TYPE = decltype(t)::value;
+        const auto kernel = K % 32 == 0 && (ldx == K || rows == 1) ? mx4_quantize_kernel<TYPE, true> : mx4_quantize_kernel<TYPE, false>;
+        for (int64_t first = 0; first < rows; first += most) {
+            const int64_t some = std::min(most, rows - first), groups = (some * KB + 64 * QUANT_UNITS - 1) / (64 * QUANT_UNITS);
+            mark((hipStream_t)stream, "mx4_quantize_kernel");
+            hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream,
+                               static_cast<const typename MxType<TYPE>::T*>(x) + first * ldx, codes + first * KB * 16, scales + first * KB, some, K, ldx);
+        }
     });
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
 }
 
 int rkh_mx4_dequantize(void* stream, int type, int64_t rows, int K, const uint8_t* codes, const uint8_t* scales, void* y, int64_t ldy) {
-    const int64_t blocks = rows * ((K + 31) / 32), groups = (blocks + 64 * QUANT_UNITS - 1) / (64 * QUANT_UNITS);
-    if (!groups) return RKH_OK;
-    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
-    mark((hipStream_t)stream, "mx4_dequantize_kernel");
+    if (!rows) return RKH_OK;
+    const int64_t KB = (K + 31) / 32, most = MX_MOST_GROUPS * 64 * QUANT_UNITS / KB;
     mx_with_type(type, [&](auto t) {
         constexpr int TYPE = decltype(t)::value;
-        const bool streams = (size_t)rows * K * sizeof(typename MxType<TYPE>::T) > STREAM_FROM;
+        using T = typename MxType<TYPE>::T;
+        const bool streams = (size_t)rows * K * sizeof(T) > STREAM_FROM;
         const auto kernel = streams ? mx4_dequantize_kernel<TYPE, true> : mx4_dequantize_kernel<TYPE, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, codes, scales, y, rows, K, ldy);
+        for (int64_t first = 0; first < rows; first += most) {
+            const int64_t some = std::min(most, rows - first), groups = (some * KB + 64 * QUANT_UNITS - 1) / (64 * QUANT_UNITS);
+            mark((hipStream_t)stream, "mx4_dequantize_kernel");
+            hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, codes + first * KB * 16, scales + first * KB,
+                               static_cast<T*>(y) + first * ldy, some, K, ldy);
+        }
     });
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
@@ -200,12 +210,16 @@ int rkh_mx4_dequantize(void* stream, int type, int64_t rows, int K, const uint8_
 
 int rkh_mx4_stage(void* stream, int type, int rows, int K, const void* x, int64_t ldx, uint8_t* codes, uint8_t* scales) {
     if (!rows) return RKH_OK;
-    const int64_t groups = ((int64_t)rows + 15) / 16 * rkh_mx4_k4(K);
-    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
-    mark((hipStream_t)stream, "mx4_stage_kernel");
+    const int64_t K4 = rkh_mx4_k4(K), most = MX_MOST_GROUPS / K4 * 16;
     mx_with_type(type, [&](auto t) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_stage_kernel<decltype(t)::value>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, x, codes,
-                           scales, rows, K, ldx);
+        constexpr int TYPE = decltype(t)::value;
+        for (int64_t first = 0; first < rows; first += most) {
+            const int64_t some = std::min(most, rows - first), groups = (some + 15) / 16 * K4;
+            mark((hipStream_t)stream, "mx4_stage_kernel");
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_stage_kernel<TYPE>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream,
+                               static_cast<const typename MxType<TYPE>::T*>(x) + first * ldx, codes + rkh_mx4_code_bytes(first, K),
+                               scales + rkh_mx4_scale_bytes(first, K), (int)some, K, ldx);
+        }
     });
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
@@ -214,10 +228,10 @@ int rkh_mx4_stage(void* stream, int type, int rows, int K, const void* x, int64_
 int rkh_mx4_pack(void* stream, const uint8_t* codes, const uint8_t* scales, int K, int N, int gate_up, uint8_t* dst, uint8_t* dst_scales) {
     const int64_t columns = rkh_mx4_columns(N, gate_up);
     const size_t pieces = rkh_mx4_code_bytes(columns, K) / 16, bytes = rkh_mx4_scale_bytes(columns, K);
-    const size_t groups = ((pieces > bytes ? pieces : bytes) + 255) / 256;
-    if (groups > 0x7fffffff) return RKH_ERR_RUNTIME;
-    hipLaunchKernelGGL(mx4_pack_kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, codes, scales, dst, dst_scales, K, N, gate_up,
-                       pieces, bytes);
+    const int64_t groups = (int64_t)((std::max(pieces, bytes) + 255) / 256);
+    for (int64_t first = 0; first < groups; first += MX_MOST_GROUPS)
+        hipLaunchKernelGGL(mx4_pack_kernel, dim3((unsigned)std::min(MX_MOST_GROUPS, groups - first)), dim3(256), 0, (hipStream_t)stream, codes, scales, dst,
+                           dst_scales, K, N, gate_up, (size_t)first * 256, pieces, bytes);
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
 }

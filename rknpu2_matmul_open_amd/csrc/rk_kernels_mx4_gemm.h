@@ -730,6 +730,7 @@ int mx_allow_lds(const void* kernel, std::atomic<bool> (&opted_in)[64], int byte
 template <int RM, int CN, int NG, int MAX_WAVES, bool SWIGLU, int FUSED, int X>
 int launch_few_as(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r, int per, int waves) {
     const int K4 = (int)rkh_mx4_k4(g.K);
+    if ((int64_t)r.nblocks * waves * 64 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
     const size_t bytes = (size_t)waves * RM * CN * 1024 + (FUSED ? (size_t)few_row_bytes(K4) * g.M : 0);
     static std::atomic<bool> opted_in[64] = {};
     if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&mx4_few_kernel<RM, CN, NG, MAX_WAVES, SWIGLU, FUSED, X>), opted_in, 160 * 1024)) return rc;
@@ -762,7 +763,7 @@ template <int RM, int CN, int HALVES, bool SWIGLU, int OUT> int launch_tiles(hip
     static std::atomic<bool> opted_in[64] = {};
     if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&mx4_tile_kernel<RM, CN, HALVES, SWIGLU, OUT>), opted_in, LDS)) return rc;
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
-    if (tiles * r.parts > 0x7fffffff) return RKH_ERR_RUNTIME;
+    if (tiles * r.parts * 256 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
     mark(st, "mx4_tile_kernel");
     hipLaunchKernelGGL(HIP_KERNEL_NAME(mx4_tile_kernel<RM, CN, HALVES, SWIGLU, OUT>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks,
                        r.nblocks, r.parts);

@@ -148,3 +148,80 @@ def test_slices_that_share_a_column_are_refused(sess):
     done(sess)
     ws.close()
     layer.close()
+
+
+# ---- more blocks than one launch has threads for -------------------------------------------
+# A launch holds fewer than 2^32 threads.  Rows of one value keep the memory small: 17 bytes each as MX4 rows, 272 as operand blocks.
+
+
+def room():
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+
+
+def test_rows_of_more_blocks_than_a_launch_has_threads_for(sess):
+    """Quantization and reading back of more than 2^32 blocks: beside every multiple of 2^31, and at the end, rows are what they are."""
+    room()
+    rows = (1 << 32) + 300
+    near = [slice(0, 64)] + [slice((m << 31) - 64, (m << 31) + 64) for m in (1, 2)] + [slice(rows - 64, rows)]
+    rng = np.random.default_rng(2)
+    x = torch.ones((rows, 1), dtype=torch.float16, device="cuda")
+    for at in near:
+        x[at] = device(rng.standard_normal((at.stop - at.start, 1)), "f16")
+    codes, scales = torch.zeros((rows, 16), dtype=torch.uint8, device="cuda"), torch.zeros((rows, 1), dtype=torch.uint8, device="cuda")
+    ready()
+    ops.mx4_quantize(sess, x, codes, scales)
+    done(sess)
+    for at in near:
+        want = ref.quantize(host(x[at]))
+        assert np.array_equal(codes[at].cpu().numpy(), want[0]) and np.array_equal(scales[at].cpu().numpy(), want[1]), at
+    values = [host(x[at]) for at in near]
+    x.fill_(7)
+    ready()
+    ops.mx4_dequantize(sess, codes, scales, x)
+    done(sess)
+    for at, was in zip(near, values):
+        assert np.array_equal(host(x[at]), ref.round_trip(was)), at
+    for piece in x.view(-1).split(1 << 30): # the others are ones but for the slices above
+        assert int((piece != 1).sum()) <= 4 * 128
+    del x, codes, scales, piece
+    room()
+
+
+def test_staged_rows_of_more_blocks_than_a_launch_has_threads_for(sess):
+    room()
+    rows, w = (1 << 28) + 17, 1.5
+    weights = ops.MX4Weights(sess, 1, 1, *ref.quantize(np.array([[w]])))
+    ws = ops.MX4Workspace(sess, rows, 1, 1)
+    x = (torch.arange(rows, device="cuda") % 7 - 3).to(torch.float16).view(rows, 1) # (each is a code of its block's scale)
+    c = torch.full((rows, 1), 77.0, dtype=torch.float16, device="cuda")
+    ready()
+    ws.run(weights, x, c)
+    done(sess)
+    assert torch.equal(c, x * w)
+    ws.close()
+    weights.close()
+    del x, c
+    room()
+
+
+def test_weights_of_more_blocks_than_a_launch_has_threads_for(sess):
+    room()
+    N = (1 << 28) + 64
+    codes, scales = torch.zeros((N, 16), dtype=torch.uint8, device="cuda"), torch.full((N, 1), 127, dtype=torch.uint8, device="cuda")
+    codes[:, 0] = (torch.arange(N, device="cuda") % 15).to(torch.uint8)
+    ready()
+    weights = ops.MX4Weights.from_device(sess, 1, N, codes.data_ptr(), scales.data_ptr())
+    del scales
+    ws = ops.MX4Workspace(sess, 1, 1, N)
+    x, c = torch.full((1, 1), 2.0, device="cuda"), torch.full((1, N), 77.0, dtype=torch.float16, device="cuda")
+    ready()
+    ws.run(weights, x, c)
+    done(sess)
+    table = torch.from_numpy(2 * ref.SIGNED).half().to("cuda")
+    for k in range(0, N, 1 << 26):
+        assert torch.equal(c[0, k:k + (1 << 26)], table[codes[k:k + (1 << 26), 0].int()]), k
+    ws.close()
+    weights.close()
+    del codes, c, x
+    room()
