@@ -71,7 +71,10 @@ void rk_npu_mx4_workspace_free(rk_npu_mx4_workspace* workspace);
 int rk_npu_mx4_run_device(rk_npu_mx4_workspace* workspace, const rk_npu_mx4_weights* weights, int rows, int a_type, const void* A,
                           int64_t lda, int c_type, void* C, int64_t ldc);
 /* The same in two calls, for rows that several weights of one shape (or of a smaller N) multiply: stage quantizes A into the workspace, where
- * the rows stay until the next call but run_staged that uses the workspace; run_staged without staged rows: RK_NPU_ERR_PARAM. */
+ * the rows stay until the next call but run_staged that uses the workspace.  run_staged multiplies as many rows as the last call staged; where
+ * that is none, because nothing was staged or a call of zero rows was the last, it returns RK_NPU_ERR_PARAM and writes nothing: a program whose
+ * batches may be empty leaves it out for those.  A captured stage counts as a call when it is captured, and its replays put their own rows into the
+ * workspace: the products of those rows belong into the same graph. */
 int rk_npu_mx4_stage_device(rk_npu_mx4_workspace* workspace, int rows, int a_type, const void* A, int64_t lda);
 int rk_npu_mx4_run_staged_device(rk_npu_mx4_workspace* workspace, const rk_npu_mx4_weights* weights, int c_type, void* C, int64_t ldc);
 /* C[rows, F] = silu(A * gate) * (A * up), silu(x) = x / (1 + exp(-x)). */

@@ -457,7 +457,7 @@ class MX4Workspace:
 
     def __init__(self, session, max_rows, K, N):
         self.lib, self.K = session.lib, K
-        self.staged = 0 # rows that run_staged writes
+        self.staged = None # rows that run_staged writes; None: nothing is staged
         self.h = self.lib.rk_npu_mx4_workspace_create(session.domain, max_rows, K, N)
         if not self.h:
             raise ValueError("rk_npu_mx4_workspace_create failed")
@@ -468,7 +468,7 @@ class MX4Workspace:
         if c.shape[0] != a.shape[0]:
             raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
         check(call(self.h, weights.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4 run")
-        self.staged = 0
+        self.staged = None
 
     def run(self, weights, a, c):
         self._run(self.lib.rk_npu_mx4_run_device, weights, a, c, weights.N)
@@ -484,7 +484,9 @@ class MX4Workspace:
     def run_staged(self, weights, c):
         kind, p, ld = _mx4_rows(c, weights.N // 2 if weights.gate_up else weights.N)
         if c.shape[0] != self.staged:
-            raise ValueError("%d rows staged, %d out" % (self.staged, c.shape[0]))
+            raise ValueError("%s rows staged, %d out" % (self.staged, c.shape[0]))
+        if self.staged == 0:
+            return # (an empty batch; the C call knows staged rows only)
         check(self.lib.rk_npu_mx4_run_staged_device(self.h, weights.h, kind, p, ld), "mx4 run_staged")
 
     def close(self):
@@ -499,7 +501,7 @@ def mx4_ffn(gu_ws, gate_up, down_ws, down, a, c):
     if c.shape[0] != a.shape[0]:
         raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
     check(gu_ws.lib.rk_npu_mx4_run_ffn_device(gu_ws.h, gate_up.h, down_ws.h, down.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4_ffn")
-    gu_ws.staged = down_ws.staged = 0
+    gu_ws.staged = down_ws.staged = None
 
 
 def _channel(w, D, what):
@@ -555,4 +557,4 @@ def mx4_ffn_block(gu_ws, gate_up, down_ws, down, stream, branch, weight=None, af
     a.branch = None # (an output here)
     check(gu_ws.lib.rk_npu_mx4_run_ffn_block_device(gu_ws.h, gate_up.h, down_ws.h, down.h, C.byref(a), C.c_void_p(branch.data_ptr()),
                                                     _channel(next_weight, stream.shape[1], "next_weight")), "mx4_ffn_block")
-    gu_ws.staged = down_ws.staged = 0
+    gu_ws.staged = down_ws.staged = None

@@ -225,3 +225,40 @@ def test_weights_of_more_blocks_than_a_launch_has_threads_for(sess):
     weights.close()
     del codes, c, x
     room()
+
+
+# ---- empty batches -------------------------------------------------------------------------
+
+
+def test_batches_of_no_rows_go_through_every_wrapper(sess):
+    """What a program does with a batch, done with an empty one: no call fails, and the calls behind it are right."""
+    rng = np.random.default_rng(11)
+    H, F = 96, 64
+    gu, dn, layer = Layer(sess, rng, 2 * F, H, gate_up=True), Layer(sess, rng, H, F), Layer(sess, rng, 50, H)
+    gws, dws = ops.MX4Workspace(sess, 8, H, 2 * F), ops.MX4Workspace(sess, 8, F, H)
+    empty = lambda n: torch.zeros((0, n), device="cuda")  # noqa: E731
+    a = ref.values(*ref.exact_rows(rng, 3, H), H)
+    x, c = device(a, "f32"), torch.zeros((3, 50), device="cuda")
+    ready()
+    with pytest.raises(ValueError):
+        gws.run_staged(layer.w, empty(50)) # nothing staged yet
+    gws.run(layer.w, empty(H), empty(50))
+    gws.run_swiglu(gu.w, empty(H), empty(F))
+    ops.mx4_ffn(gws, gu.w, dws, dn.w, empty(H), empty(H))
+    ops.mx4_ffn_block(gws, gu.w, dws, dn.w, empty(H), empty(H), stream_out=empty(H))
+    with pytest.raises(ValueError):
+        gws.run_staged(layer.w, empty(50)) # run leaves nothing staged
+    for stage in (lambda rows: gws.stage(rows), lambda rows: ops.block_norm(sess, rows, staged=gws)):
+        stage(empty(H))
+        gws.run_staged(layer.w, empty(50))
+        gws.run_staged(gu.w, empty(F))
+        with pytest.raises(ValueError):
+            gws.run_staged(layer.w, c)
+        stage(x)
+        gws.run_staged(layer.w, c)
+    gws.stage(x)
+    gws.run_staged(layer.w, c)
+    done(sess)
+    assert np.array_equal(host(c), a @ layer.values.T)
+    for h in (gws, dws, gu, dn, layer):
+        h.close()
