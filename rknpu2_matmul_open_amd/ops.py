@@ -381,21 +381,29 @@ class MoeW8:
 
 
 # ---- MX4 layers and the block norm: rows are tensors on the device ---------------------------
-# Anything with data_ptr(), shape, stride() and dtype that lies on the context's device (a torch tensor); the calls enqueue on
-# the context's stream, which the caller orders against its own (rk_npu_hip_stream).
+# Anything with data_ptr(), shape, stride() and dtype that lies on the context's device (a torch tensor; one of another device is
+# refused); the calls enqueue on the context's stream, which the caller orders against its own (rk_npu_hip_stream).
 
 _MX4_TYPES = {"torch.float32": capi.MX4_F32, "torch.float16": capi.MX4_F16, "torch.bfloat16": capi.MX4_BF16}
 
 
-def _on_device(x):
+def _device_of(session):
+    return session.lib.rk_npu_hip_device(session.ctx)
+
+
+def _on_device(x, device=None):
+    """device: the context's ordinal, or None: any."""
     if not getattr(x, "is_cuda", True):
         raise ValueError("a tensor on the device is needed, this one lies on %s" % x.device)
+    index = getattr(getattr(x, "device", None), "index", None)
+    if device is not None and index is not None and index != device:
+        raise ValueError("a tensor on device %d is needed, where the context is: this one lies on %s" % (device, x.device))
 
 
-def _mx4_rows(x, columns=None):
+def _mx4_rows(x, columns=None, device=None):
     """(element type, address, row stride) of a 2-d tensor whose rows are contiguous."""
     kind = _MX4_TYPES.get(str(x.dtype))
-    _on_device(x)
+    _on_device(x, device)
     if kind is None:
         raise TypeError("rows of float32, float16 or bfloat16: got %s" % x.dtype)
     if len(x.shape) != 2 or (columns is not None and x.shape[1] != columns) or (x.shape[1] > 1 and x.stride(1) != 1):
@@ -403,8 +411,8 @@ def _mx4_rows(x, columns=None):
     return kind, C.c_void_p(x.data_ptr()), max(x.stride(0), x.shape[1]) if x.shape[0] <= 1 else x.stride(0)
 
 
-def _mx4_bytes(x, rows, width, what):
-    _on_device(x)
+def _mx4_bytes(x, rows, width, what, device=None):
+    _on_device(x, device)
     if str(x.dtype) != "torch.uint8" or tuple(x.shape) != (rows, width) or not x.is_contiguous():
         raise ValueError("%s: contiguous uint8 of shape %s, got %s %s" % (what, (rows, width), x.dtype, tuple(x.shape)))
     return C.c_void_p(x.data_ptr())
@@ -412,24 +420,26 @@ def _mx4_bytes(x, rows, width, what):
 
 def mx4_quantize(session, x, codes, scales):
     """MX4 rows of x [rows, K]: codes uint8 [rows, 16 * ceil(K / 32)], scales uint8 [rows, ceil(K / 32)]."""
-    kind, p, ld = _mx4_rows(x)
+    device = _device_of(session)
+    kind, p, ld = _mx4_rows(x, device=device)
     rows, K = x.shape
     blocks = -(-K // 32)
-    check(session.lib.rk_npu_mx4_quantize_device(session.ctx, kind, rows, K, p, ld, _mx4_bytes(codes, rows, 16 * blocks, "codes"),
-                                                 _mx4_bytes(scales, rows, blocks, "scales")), "mx4_quantize")
+    check(session.lib.rk_npu_mx4_quantize_device(session.ctx, kind, rows, K, p, ld, _mx4_bytes(codes, rows, 16 * blocks, "codes", device),
+                                                 _mx4_bytes(scales, rows, blocks, "scales", device)), "mx4_quantize")
 
 
 def mx4_dequantize(session, codes, scales, y):
     """The values of MX4 rows, rounded to y's type."""
-    kind, p, ld = _mx4_rows(y)
+    device = _device_of(session)
+    kind, p, ld = _mx4_rows(y, device=device)
     rows, K = y.shape
     blocks = -(-K // 32)
-    check(session.lib.rk_npu_mx4_dequantize_device(session.ctx, kind, rows, K, _mx4_bytes(codes, rows, 16 * blocks, "codes"),
-                                                   _mx4_bytes(scales, rows, blocks, "scales"), p, ld), "mx4_dequantize")
+    check(session.lib.rk_npu_mx4_dequantize_device(session.ctx, kind, rows, K, _mx4_bytes(codes, rows, 16 * blocks, "codes", device),
+                                                   _mx4_bytes(scales, rows, blocks, "scales", device), p, ld), "mx4_dequantize")
 
 
 class MX4Weights:
-    """MX4 weights [N, K] (gate_up: N = 2F, the gate's rows first) from host arrays, or from_device from device addresses."""
+    """MX4 weights [N, K] (gate_up: N = 2F, the gate's rows first) from host arrays, or from_device."""
 
     def __init__(self, session, K, N, codes, scales, gate_up=False, on_device=False):
         self.lib, self.K, self.N, self.gate_up = session.lib, K, N, gate_up
@@ -444,7 +454,11 @@ class MX4Weights:
 
     @classmethod
     def from_device(cls, session, K, N, codes, scales, gate_up=False):
-        return cls(session, K, N, codes, scales, gate_up, on_device=True)
+        """codes, scales: tensors as mx4_quantize fills them, or addresses of as many bytes, of which nothing can be checked."""
+        blocks = -(-K // 32)
+        p, q = (_mx4_bytes(x, N, width, what, _device_of(session)) if hasattr(x, "data_ptr") else x
+                for x, width, what in ((codes, 16 * blocks, "codes"), (scales, blocks, "scales")))
+        return cls(session, K, N, p, q, gate_up, on_device=True)
 
     def close(self):
         if self.h:
@@ -454,17 +468,18 @@ class MX4Weights:
 
 class MX4Workspace:
     """Workspace for up to max_rows rows of K values and weights of up to N columns (gate / up: 2F)."""
+    device = None # the context's
 
     def __init__(self, session, max_rows, K, N):
-        self.lib, self.K = session.lib, K
+        self.lib, self.K, self.device = session.lib, K, _device_of(session)
         self.staged = None # rows that run_staged writes; None: nothing is staged
         self.h = self.lib.rk_npu_mx4_workspace_create(session.domain, max_rows, K, N)
         if not self.h:
             raise ValueError("rk_npu_mx4_workspace_create failed")
 
     def _run(self, call, weights, a, c, columns):
-        kind, p, ld = _mx4_rows(a, self.K)
-        c_kind, c_p, c_ld = _mx4_rows(c, columns)
+        kind, p, ld = _mx4_rows(a, self.K, self.device)
+        c_kind, c_p, c_ld = _mx4_rows(c, columns, self.device)
         if c.shape[0] != a.shape[0]:
             raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
         check(call(self.h, weights.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4 run")
@@ -477,12 +492,12 @@ class MX4Workspace:
         self._run(self.lib.rk_npu_mx4_run_swiglu_device, weights, a, c, weights.N // 2)
 
     def stage(self, a):
-        kind, p, ld = _mx4_rows(a, self.K)
+        kind, p, ld = _mx4_rows(a, self.K, self.device)
         check(self.lib.rk_npu_mx4_stage_device(self.h, a.shape[0], kind, p, ld), "mx4 stage")
         self.staged = a.shape[0]
 
     def run_staged(self, weights, c):
-        kind, p, ld = _mx4_rows(c, weights.N // 2 if weights.gate_up else weights.N)
+        kind, p, ld = _mx4_rows(c, weights.N // 2 if weights.gate_up else weights.N, self.device)
         if c.shape[0] != self.staged:
             raise ValueError("%s rows staged, %d out" % (self.staged, c.shape[0]))
         if self.staged == 0:
@@ -496,40 +511,40 @@ class MX4Workspace:
 
 
 def mx4_ffn(gu_ws, gate_up, down_ws, down, a, c):
-    kind, p, ld = _mx4_rows(a, gu_ws.K)
-    c_kind, c_p, c_ld = _mx4_rows(c, down.N)
+    kind, p, ld = _mx4_rows(a, gu_ws.K, gu_ws.device)
+    c_kind, c_p, c_ld = _mx4_rows(c, down.N, gu_ws.device)
     if c.shape[0] != a.shape[0]:
         raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
     check(gu_ws.lib.rk_npu_mx4_run_ffn_device(gu_ws.h, gate_up.h, down_ws.h, down.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "mx4_ffn")
     gu_ws.staged = down_ws.staged = None
 
 
-def _channel(w, D, what):
+def _channel(w, D, what, device=None):
     if w is None:
         return None
-    _on_device(w)
+    _on_device(w, device)
     if str(w.dtype) != "torch.float32" or tuple(w.shape) != (D,) or not w.is_contiguous():
         raise ValueError("%s: contiguous float32 [%d], got %s %s" % (what, D, w.dtype, tuple(w.shape)))
     return w.data_ptr()
 
 
-def _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, staged):
+def _norm_args(device, stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, staged):
     """rk_npu_block_norm_args of tensors, the branch's type and stride included."""
     rows, D = stream.shape
     a = capi.BlockNormArgs(struct_size=C.sizeof(capi.BlockNormArgs), rows=rows, D=D, eps=eps, residual_scale=residual_scale, branch_scale=branch_scale)
-    a.residual_type, a.residual, a.residual_ld = _mx4_rows(stream)
+    a.residual_type, a.residual, a.residual_ld = _mx4_rows(stream, device=device)
 
     def alike(x, what):
         if tuple(x.shape) != (rows, D):
             raise ValueError("%s: shape %s, the stream's is %s" % (what, tuple(x.shape), (rows, D)))
-        return _mx4_rows(x)
+        return _mx4_rows(x, device=device)
     if branch is not None:
         a.branch_type, a.branch, a.branch_ld = alike(branch, "branch")
     if gate is not None:
-        a.gate_type, a.gate, a.gate_ld = _mx4_rows(gate.reshape(1, D)) if len(gate.shape) == 1 else alike(gate, "gate")
+        a.gate_type, a.gate, a.gate_ld = _mx4_rows(gate.reshape(1, D), device=device) if len(gate.shape) == 1 else alike(gate, "gate")
         if len(gate.shape) == 1:
             a.gate_ld = 0
-    a.branch_weight, a.weight = _channel(after, D, "after"), _channel(weight, D, "weight")
+    a.branch_weight, a.weight = _channel(after, D, "after", device), _channel(weight, D, "weight", device)
     if stream_out is not None:
         kind, a.residual_out, a.residual_out_ld = alike(stream_out, "stream_out")
         if kind != a.residual_type:
@@ -544,7 +559,7 @@ def block_norm(session, stream, branch=None, after=None, gate=None, residual_sca
                stream_out=None, y=None, staged=None):
     """The norms around a block (rk_npu_block_norm_device): stream, branch [rows, D]; after (behind the block) and weight (before the
     next one) float32 [D]; gate [D] or [rows, D]."""
-    a = _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, staged)
+    a = _norm_args(_device_of(session), stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, staged)
     check(session.lib.rk_npu_block_norm_device(session.ctx, C.byref(a)), "block_norm")
     if staged is not None:
         staged.staged = stream.shape[0]
@@ -553,8 +568,8 @@ def block_norm(session, stream, branch=None, after=None, gate=None, residual_sca
 def mx4_ffn_block(gu_ws, gate_up, down_ws, down, stream, branch, weight=None, after=None, gate=None, residual_scale=1.0, branch_scale=1.0,
                   eps=1e-6, stream_out=None, y=None, next_weight=None):
     """A gated FFN block on the residual stream (rk_npu_mx4_run_ffn_block_device); branch receives the FFN's output."""
-    a = _norm_args(stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, None)
+    a = _norm_args(gu_ws.device, stream, branch, after, gate, residual_scale, branch_scale, weight, eps, stream_out, y, None)
     a.branch = None # (an output here)
     check(gu_ws.lib.rk_npu_mx4_run_ffn_block_device(gu_ws.h, gate_up.h, down_ws.h, down.h, C.byref(a), C.c_void_p(branch.data_ptr()),
-                                                    _channel(next_weight, stream.shape[1], "next_weight")), "mx4_ffn_block")
+                                                    _channel(next_weight, stream.shape[1], "next_weight", gu_ws.device)), "mx4_ffn_block")
     gu_ws.staged = down_ws.staged = None

@@ -262,3 +262,29 @@ def test_batches_of_no_rows_go_through_every_wrapper(sess):
     assert np.array_equal(host(c), a @ layer.values.T)
     for h in (gws, dws, gu, dn, layer):
         h.close()
+
+
+# ---- weights from tensors --------------------------------------------------------------------
+
+
+def test_weights_from_tensors_on_the_device(sess):
+    """The tensors that quantization fills, or their addresses: the same weights.  Tensors too short are refused, not read past their end."""
+    rng = np.random.default_rng(12)
+    N, K = 70, 333
+    x = device(rng.standard_normal((N, K)), "f32")
+    codes, scales = torch.zeros((N, 176), dtype=torch.uint8, device="cuda"), torch.zeros((N, 11), dtype=torch.uint8, device="cuda")
+    eye = torch.eye(K, device="cuda")
+    ready()
+    ops.mx4_quantize(sess, x, codes, scales)
+    both = [ops.MX4Weights.from_device(sess, K, N, codes, scales), ops.MX4Weights.from_device(sess, K, N, codes.data_ptr(), scales.data_ptr())]
+    ws, outs = ops.MX4Workspace(sess, K, K, N), [torch.zeros((K, N), device="cuda") for _ in both]
+    ready()
+    for w, c in zip(both, outs):
+        ws.run(w, eye, c)
+    done(sess)
+    assert torch.equal(*outs) and np.array_equal(host(outs[0]).T, ref.round_trip(host(x)))
+    for bad in ((codes[:, :160], scales), (codes[1:], scales), (codes, scales[:, :10]), (codes.int(), scales), (codes.cpu(), scales)):
+        with pytest.raises(ValueError):
+            ops.MX4Weights.from_device(sess, K, N, *bad)
+    for h in both + [ws]:
+        h.close()
