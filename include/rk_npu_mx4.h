@@ -95,8 +95,8 @@ int rk_npu_mx4_run_ffn_device(rk_npu_mx4_workspace* workspace, const rk_npu_mx4_
  * computed in fp32 and rounded once per output; y is computed from r before its rounding.  Every part may be left out: branch NULL: r = residual
  * as it is (no scale, no gate); gate NULL: 1; weight NULL: 1; outputs NULL: not wanted, but one has to be.  residual_out may
  * be the residual's own buffer (same stride): the stream is then updated in place.  Rows of the gate lie gate_ld values
- * apart, 0: one row for all.  A NaN makes its row of y NaN; where the mean square is beyond
- * fp32, y is zero (NaN where r is infinite).
+ * apart, 0: one row for all.  A NaN makes its row of y NaN.  Squares are added in fp32, without scaling: where the sum of a row's
+ * is beyond fp32 (a root mean square of 1.8e19 / sqrt(D)), its normed values are zero (NaN where the row is infinite).
  * staged: a workspace of K = D that takes the normed rows as MX4, quantized from fp32, for rk_npu_mx4_run_staged_device.
  */
 typedef struct {

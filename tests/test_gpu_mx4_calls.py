@@ -288,3 +288,35 @@ def test_weights_from_tensors_on_the_device(sess):
             ops.MX4Weights.from_device(sess, K, N, *bad)
     for h in both + [ws]:
         h.close()
+
+
+# ---- the ends of the norm's range ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,D", [(1, 512), (4, 4096), (3, 20000)])
+def test_sums_of_squares_at_the_end_of_fp32(sess, rows, D):
+    """Rows whose sum of squares is just inside fp32 are normed, rows whose sum is just beyond are zero, in both norms."""
+    largest = 2.0 ** 64 / np.sqrt(D)  # D of its squares: 2^128
+    sign = np.where(np.arange(D) % 3 == 0, -1.0, 1.0)
+    inside, beyond = (np.tile(sign * largest * f, (rows, 1)) for f in (0.99, 1.01))
+    y, z = torch.full((rows, D), 7.0, device="cuda"), torch.full((rows, D), 7.0, device="cuda")
+    for values, want in ((inside, 1.0), (beyond, 0.0)):
+        stream = device(values, "f32")
+        nothing = torch.zeros_like(stream)
+        ones = torch.ones(D, device="cuda")
+        ready()
+        ops.block_norm(sess, stream, y=y)
+        ops.block_norm(sess, nothing, stream, after=ones, stream_out=z)
+        done(sess)
+        for got in (host(y), host(z)):
+            assert (np.abs(got - want * sign) <= (D / 2 + 8) * 2.0 ** -24).all()
+        if D == 512:
+            ws, w = ops.MX4Workspace(sess, rows, D, D), ops.MX4Weights(sess, D, D, *ref.quantize(np.eye(D)))
+            c = torch.full((rows, D), 7.0, device="cuda")
+            ready()
+            ops.block_norm(sess, stream, staged=ws)
+            ws.run_staged(w, c)
+            done(sess)
+            assert np.array_equal(host(c), ref.round_trip(host(y)))
+            ws.close()
+            w.close()
