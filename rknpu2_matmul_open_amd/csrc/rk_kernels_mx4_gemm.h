@@ -63,7 +63,8 @@ __device__ __forceinline__ float mx_silu(float gate, float up) {
     constexpr float L = 1.44269504088896f, L_REST = 1.92596299e-8f, LN2 = 0.693147180559945f; // log2 e = L + L_REST
     const float t = -gate * L, rest = fmaf(-gate, L_REST, fmaf(-gate, L, -t));
     const float power = __builtin_amdgcn_exp2f(t) * (fabsf(gate) < 128.0f ? fmaf(rest, LN2, 1.0f) : 1.0f); // (beyond: 0 or infinity)
-    return gate * __builtin_amdgcn_rcpf(1.0f + power) * up;
+    // (of a quarter: the reciprocal gives zero for what is 2^126 or more, where gate * reciprocal is still a normal number)
+    return 0.25f * gate * __builtin_amdgcn_rcpf(fmaf(0.25f, power, 0.25f)) * up;
 }
 
 // N (4 or 8) consecutive values to where `to` points, of which `count` exist.  (Instructions that are not yet in the cache cost small

@@ -320,3 +320,36 @@ def test_sums_of_squares_at_the_end_of_fp32(sess, rows, D):
             assert np.array_equal(host(c), ref.round_trip(host(y)))
             ws.close()
             w.close()
+
+
+# ---- SwiGLU where the quotient is small ------------------------------------------------------
+
+
+@pytest.mark.parametrize("M", [1, 20, 70, 300])
+def test_swiglu_where_the_exponential_is_near_the_end_of_fp32(sess, M):
+    """Gates of -79.5 .. -88.5, each an exact sum of products, with up to 2^100 behind them: silu is 1e-33 .. 3e-37, and none of it is lost.  Relative to it
+    16 roundings or ulps, as for other gates.  (From -88.73 on exp is beyond fp32, and silu with it.)"""
+    K, F = 64, 512
+    rng = np.random.default_rng(M)
+    gate, up = np.zeros((F, K)), np.zeros((F, K))
+    gate[:, 0] = -64
+    gate[:, 32] = rng.choice([-16, -24], F)
+    gate[:, 33] = rng.choice([0, -2, 2], F)
+    up[:, 0] = rng.choice([1.0, 2.0 ** 20, 2.0 ** 60, 2.0 ** 100], F)
+    codes, scales = ref.quantize(np.concatenate([gate, up]))
+    values = ref.values(codes, scales, K)
+    w = ops.MX4Weights(sess, K, 2 * F, codes, scales, gate_up=True)
+    x = np.zeros((M, K))
+    x[:, 0] = x[:, 32] = 1.0
+    x[::2, 33] = 0.25
+    x = ref.round_trip(x)
+    ws, d, c = ops.MX4Workspace(sess, M, K, 2 * F), device(x, "f32"), torch.zeros((M, F), device="cuda")
+    ready()
+    ws.run_swiglu(w, d, c)
+    done(sess)
+    g = x @ values[:F].T
+    want = ref.silu(g) * (x @ values[F:].T)
+    assert g.min() == -88.5 and g.max() == -79.5 and len(np.unique(g)) == 6 and (np.abs(want) > 2.0 ** -122).all()
+    assert (np.abs(host(c) - want) <= 16 * 2.0 ** -24 * np.abs(want)).all()
+    ws.close()
+    w.close()
