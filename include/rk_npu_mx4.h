@@ -70,14 +70,15 @@ void rk_npu_mx4_workspace_free(rk_npu_mx4_workspace* workspace);
 /* C[rows, N] = A[rows, K] as MX4 times the weights. */
 int rk_npu_mx4_run_device(rk_npu_mx4_workspace* workspace, const rk_npu_mx4_weights* weights, int rows, int a_type, const void* A,
                           int64_t lda, int c_type, void* C, int64_t ldc);
-/* The same in two calls, for rows that several weights of one shape (or of a smaller N) multiply: stage quantizes A into the workspace, where
- * the rows stay until the next call but run_staged that uses the workspace.  run_staged multiplies as many rows as the last call staged; where
- * that is none, because nothing was staged or a call of zero rows was the last, it returns RK_NPU_ERR_PARAM and writes nothing: a program whose
- * batches may be empty leaves it out for those.  A captured stage counts as a call when it is captured, and its replays put their own rows into the
- * workspace: the products of those rows belong into the same graph. */
+/* The same in two calls, for rows that several weights of one shape multiply (or of a smaller N; gate / up weights give what
+ * run_swiglu gives): stage quantizes A into the workspace, where the rows stay until the next call but run_staged that uses the
+ * workspace.  run_staged multiplies as many rows as the last call staged; where that is none, because nothing was staged or a call
+ * of zero rows was the last, it returns RK_NPU_ERR_PARAM and writes nothing: a program whose batches may be empty leaves it out for
+ * those.  A captured stage counts as a call when it is captured, and its replays put their own rows into the workspace: the
+ * products of those rows belong into the same graph. */
 int rk_npu_mx4_stage_device(rk_npu_mx4_workspace* workspace, int rows, int a_type, const void* A, int64_t lda);
 int rk_npu_mx4_run_staged_device(rk_npu_mx4_workspace* workspace, const rk_npu_mx4_weights* weights, int c_type, void* C, int64_t ldc);
-/* C[rows, F] = silu(A * gate) * (A * up), silu(x) = x / (1 + exp(-x)). */
+/* C[rows, F] = silu(A * gate) * (A * up), silu(x) = x / (1 + exp(-x)) in fp32: zero below -88.7, where exp leaves it. */
 int rk_npu_mx4_run_swiglu_device(rk_npu_mx4_workspace* workspace, const rk_npu_mx4_weights* gate_up, int rows, int a_type,
                                  const void* A, int64_t lda, int c_type, void* C, int64_t ldc);
 /* Gate / up product, SwiGLU and down product; the middle goes from the fp32 sums to MX4 rows in down_workspace and is not written
