@@ -2,7 +2,7 @@
 
     python -m rknpu2_matmul_open_amd.audit_waits            # compiles the units to assembly and checks them
 
-gemm_wk_kernel and gemm_stream_kernel issue their loop loads from inline assembly (the MX4 tile kernels their
+gemm_wk_kernel and gemm_stream_kernel issue their loop loads from inline assembly (the MX4 and G4 tile kernels their
 products, and loads to LDS, which the last two rules are about) and place
 every s_waitcnt by hand; the compiler believes the destination registers of such a load hold
 their value as soon as the asm statement has executed.  The kernels are correct only if, in the
@@ -28,7 +28,7 @@ with the same flags):
 
   * a product (v_mfma) from asm takes no part in the compiler's bookkeeping of hazards: no vector instruction may write one
     of its operands in the two wait states ahead of it, nor any other instruction read its result in the eleven behind it
-    (a product may: the hardware orders those).
+    (a product may: the hardware orders those; one of 32x32x16 halves in between counts for the eight that it takes to be issued).
 
 The check walks the control-flow graph of a kernel (basic blocks split at labels and branches):
 from every asm load it follows every path until the covering wait, carrying the number of loads
@@ -41,7 +41,8 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-UNITS = ["rk_kernels_gemm.hip", "rk_kernels_stream.hip", "rk_kernels_mx4_gemm.hip", "rk_kernels_mx4_swiglu.hip"]
+UNITS = ["rk_kernels_gemm.hip", "rk_kernels_stream.hip", "rk_kernels_mx4_gemm.hip", "rk_kernels_mx4_swiglu.hip",
+         "rk_kernels_g4_tile1.hip", "rk_kernels_g4_tile2.hip", "rk_kernels_g4_tile4.hip"]
 
 _VM_LOAD = re.compile(r"^\s*(global_load|buffer_load|flat_load|scratch_load)")
 _ASM_VLOAD = re.compile(r"^\s*global_load_dwordx?(\d*)\s+(v\[\d+:\d+\]|v\d+)\s*,")
@@ -194,6 +195,10 @@ _VALU = re.compile(r"^\s*v_(?!mfma_)")
 _READS_ALL = re.compile(r"^\s*(ds_write|global_store|buffer_store|scratch_store|global_load_lds|v_cmp)")
 
 
+# A product that takes eight passes to enter the matrix pipe: one behind another of the same wave is not issued before those are over.
+_EIGHT_PASSES = re.compile(r"^\s*v_mfma_f32_32x32x16_f16\b")
+
+
 def _operands(text):
     """(registers written, registers read) of an instruction, as far as the rules below need it."""
     parts = text.split(None, 1)
@@ -247,7 +252,7 @@ def _check_mfma(name, instrs, violations):
                     if not _MFMA.match(t) and (read | (written if _VALU.match(t) else set())) & result:
                         violations.append("%s: `%s` touches the result of `%s` %d wait states behind it" % (name, t.strip(), text.strip(), states))
                     nop = _NOP.match(t)
-                    states += 1 + (int(nop.group(1)) if nop else 0)
+                    states += 8 if _EIGHT_PASSES.match(t) else 1 + (int(nop.group(1)) if nop else 0)
                 j += 1
             if states < 11:
                 for nxt in succ:
@@ -278,7 +283,7 @@ def audit_function(name, lines):
     return violations
 
 
-def audit_text(asm_text, only=("gemm_wk_kernel", "gemm_wk_big_kernel", "gemm_stream_kernel", "mx4_tile_kernel", "mx4_big_kernel")):
+def audit_text(asm_text, only=("gemm_wk_kernel", "gemm_wk_big_kernel", "gemm_stream_kernel", "mx4_tile_kernel", "mx4_big_kernel", "g4_tile_kernel")):
     """Violations in every kernel of an assembly file whose (mangled) name contains one of `only`."""
     violations, checked = [], 0
     lines = asm_text.splitlines() + [".Lfunc_end:"]

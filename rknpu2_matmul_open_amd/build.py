@@ -16,7 +16,8 @@ CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "librk_npu_matmul.so")
 SOURCES = ["rk_kernels.hip", "rk_kernels_gemv.hip", "rk_kernels_gemm.hip", "rk_kernels_stream.hip", "rk_kernels_few.hip", "rk_core.cpp", "rk_quant_matmul.cpp", "rk_autotune.cpp", "rk_w4a8.cpp", "rk_w4a8_tune.cpp", "rk_i4.cpp",
-           "rk_moe_w8.cpp", "rk_kernels_mx4.hip", "rk_kernels_mx4_gemm.hip", "rk_kernels_mx4_swiglu.hip", "rk_kernels_norm.hip", "rk_mx4.cpp"]
+           "rk_moe_w8.cpp", "rk_kernels_mx4.hip", "rk_kernels_mx4_gemm.hip", "rk_kernels_mx4_swiglu.hip", "rk_kernels_norm.hip", "rk_mx4.cpp",
+           "rk_kernels_g4.hip", "rk_kernels_g4_tile1.hip", "rk_kernels_g4_tile2.hip", "rk_kernels_g4_tile4.hip", "rk_g4.cpp", "rk_kernels_heads.hip", "rk_heads.cpp"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -430,6 +430,35 @@ _MX4_PROTOTYPES = {
 }
 
 MX4_SYMBOLS = tuple(_MX4_PROTOTYPES)
+
+
+# rk_npu_g4.h, rk_npu_heads.h
+class G4WeightConfig(C.Structure):
+    _fields_ = [("K", C.c_int), ("N", C.c_int), ("group", C.c_int), ("gate_up", C.c_int), ("scale_type", C.c_int)]
+
+
+class HeadsArgs(C.Structure):
+    _fields_ = ([("struct_size", C.c_uint32)] + [(n, C.c_int) for n in ("rows", "head_dim", "q_heads", "k_heads", "type", "norm")] + [("eps", C.c_float)] +
+                [(n, P) for n in ("q_weight", "k_weight", "q", "k", "q_out", "k_out")] +
+                [(n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "q_out_row", "q_out_head", "k_out_row", "k_out_head")] +
+                [(n, C.c_int) for n in ("rotary_dim", "neighbours", "axes")] + [("positions", P), ("position_axis", C.c_int64), ("pair_axis", P), ("inv_freq", P),
+                 ("rotation_scale", C.c_float)])
+
+
+_G4_PROTOTYPES = {
+    "rk_npu_g4_weights_create": (P, [P, C.POINTER(G4WeightConfig), P, P, P]),
+    "rk_npu_g4_weights_create_device": (P, [P, C.POINTER(G4WeightConfig), P, P, P]),
+    "rk_npu_g4_weights_free": (None, [P]),
+    "rk_npu_g4_weights_query": (C.c_int, [P, C.POINTER(G4WeightConfig), C.POINTER(C.c_uint64)]),
+    "rk_npu_g4_workspace_create": (P, [P, C.c_int, C.c_int, C.c_int]),
+    "rk_npu_g4_workspace_free": (None, [P]),
+    "rk_npu_g4_run_device": (C.c_int, [P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P, C.c_int64]),
+    "rk_npu_g4_run_swiglu_device": (C.c_int, [P, P, C.c_int, C.c_int, P, C.c_int64, C.c_int, P, C.c_int64]),
+    "rk_npu_heads_args_init": (None, [C.POINTER(HeadsArgs), C.c_int, C.c_int]),
+    "rk_npu_heads_norm_rotate_device": (C.c_int, [P, C.POINTER(HeadsArgs)]),
+}
+
+G4_SYMBOLS = tuple(_G4_PROTOTYPES)
 _LIB = None
 
 
@@ -450,7 +479,7 @@ def load_library():
             "%s is missing: build it with `python -m rknpu2_matmul_open_amd.build` "
             "(there is no CPU fallback)" % path)
     lib = C.CDLL(path)
-    for name, (restype, argtypes) in {**_PROTOTYPES, **_MX4_PROTOTYPES}.items():
+    for name, (restype, argtypes) in {**_PROTOTYPES, **_MX4_PROTOTYPES, **_G4_PROTOTYPES}.items():
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes

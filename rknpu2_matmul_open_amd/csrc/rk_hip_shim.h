@@ -68,6 +68,9 @@ int rkh_device_count(void);
 int rkh_open(int device, void** stream_out, char* name_out, int name_len, int* cu_count,
              int* clock_khz);
 void rkh_close(int device, void* stream);
+/* Makes `device` the calling thread's current one for a while: returns what was, which leaving restores (-1: nothing to do). */
+int rkh_enter_device(int device);
+void rkh_leave_device(int before);
 int rkh_malloc(int device, void** ptr, size_t bytes);
 void rkh_free(int device, void* ptr);
 int rkh_host_alloc(void** ptr, size_t bytes); /* pinned staging */

@@ -113,6 +113,19 @@ private:
     Owner owner_;
 };
 
+// The context's device is the calling thread's current one for as long as this lives (kernels have attributes per device, and are
+// launched on the current one).
+class OnDevice {
+public:
+    explicit OnDevice(int device) : before_(rkh_enter_device(device)) {}
+    ~OnDevice() { rkh_leave_device(before_); }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+
+private:
+    int before_;
+};
+
 // Non-reentrancy guard of a workspace: try-lock semantics, BUSY on contention.
 class BusyLock {
 public:

@@ -1219,6 +1219,15 @@ void rkh_set_marker(rkh_marker_fn fn, void* user) {
     g_marker_on.store(fn != nullptr, std::memory_order_release);
 }
 
+int rkh_enter_device(int device) {
+    int before = -1;
+    if (hipGetDevice(&before) != hipSuccess || before == device || hipSetDevice(device) != hipSuccess) return -1;
+    return before;
+}
+void rkh_leave_device(int before) {
+    if (before >= 0) (void)hipSetDevice(before);
+}
+
 int rkh_malloc(int device, void** ptr, size_t bytes) {
     *ptr = nullptr;
     if (g_fail_malloc_after > 0 && --g_fail_malloc_after == 0) return RKH_ERR_NOMEM;

@@ -1,0 +1,324 @@
+// Tiles of G4 products: 64 RM rows x 128 places by four waves (two by two), each RM x 2 accumulators of 32 x 32.  Bound by the matrix pipes and what
+// has to be issued beside them.
+//
+// A step is 128 k.  Its activations (rows of 256 bytes), codes and scales are copied global -> LDS directly, two steps ahead of the products and one
+// ahead of the LDS reads:
+//  * a wave's activations of a step live in registers, 8 RM operands that both of its 32-place halves j multiply.  An operand's last product
+//    is one of half 1; behind it, it is replaced by the next step's;
+//  * codes become halves (code - zero) one operand at a time: those of half 1 behind the last products of half 0 that use the same registers, and those
+//    of half 0 of the next step behind the last ones of half 1.  So both ways of issue are used evenly;
+//  * a group's products start from zero, and its sum goes into the accumulators, times the scale, while the next group's run.
+// In half-time of step s (between the halves) a wave waits for its copies of step s + 1 and for its LDS reads, and meets the others: from
+// there on LDS holds step s + 1 for all, and nobody reads step s any more, whose place the copies of step s + 2 take.
+//
+// Places in LDS: a row's 128 bytes of 64 k are eight pieces of 16 bytes, of which piece c lies at place c ^ (row & 7); eight lanes then read
+// eight rows without a conflict, and a copy still fetches whole 128-byte lines.
+#ifndef RK_KERNELS_G4_TILE_H
+#define RK_KERNELS_G4_TILE_H
+
+#include <algorithm>
+
+#include "rk_kernels_g4.h"
+
+namespace {
+
+template <int RM, int GPB> struct G4Tile {
+    static constexpr int ROWS = 64 * RM, HALF = ROWS * 128; // bytes of 64 k
+    static constexpr int W_OFF = 2 * HALF, S_OFF = W_OFF + 8192, S_COPIES = GPB == 4 ? 2 : 1, BUF = S_OFF + S_COPIES * 1024, LDS = 2 * BUF;
+    static constexpr int COPIES = 4 * RM + 3; // of a wave and step: activations, codes, scales
+    static_assert(LDS <= 160 * 1024, "");
+};
+
+// What a step issues, as asm statements: they stay where they are written (of plain operations the compiler collects a step's sums, and its halves, in a
+// few places, and moves sums between the halves of the registers).  What it then does not order: a vector instruction that writes an operand has to be
+// two wait states ahead of the product; one that reads a sum eleven behind it, and a product in between counts for eight of them, which it
+// takes to issue behind another one.
+__device__ __forceinline__ void g4_product(const v4i& a, const v4i& w, v16f& sum) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(sum) : "a"(a), "v"(w));
+}
+__device__ __forceinline__ void g4_product_first(const v4i& a, const v4i& w, v16f& sum) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(sum) : "a"(a), "v"(w));
+}
+__device__ __forceinline__ void g4_add_scaled(float& acc, float sum, float scale) { asm volatile("v_fmac_f32_e32 %0, %1, %2" : "+v"(acc) : "v"(sum), "v"(scale)); }
+// g4_pair; `magic` is 0x64006400 in a vector register.  (One statement: between two of them the compiler puts a wait state for a hazard that these
+// instructions do not have.)  R = 2 leaves the codes, shifted by eight bits, in `upper` for R = 3.
+template <int R> __device__ __forceinline__ uint32_t g4_pair_here(uint32_t w, const G4Zero& z, uint32_t magic, uint32_t& upper) {
+    uint32_t v;
+    if constexpr (R == 0)
+        asm volatile("v_and_or_b32 %0, %1, %2, %3\n\tv_pk_add_f16 %0, %0, %4" : "=&v"(v) : "v"(w), "s"(0x000f000fu), "v"(magic), "v"(z.low));
+    else if constexpr (R == 2)
+        asm volatile("v_lshrrev_b32 %1, 8, %2\n\tv_and_or_b32 %0, %1, %3, %4\n\tv_pk_add_f16 %0, %0, %5"
+                     : "=&v"(v), "=&v"(upper) : "v"(w), "s"(0x000f000fu), "v"(magic), "v"(z.low));
+    else // (times 1/16)
+        asm volatile("v_and_or_b32 %0, %1, %2, %3\n\tv_pk_fma_f16 %0, %0, %4, %5"
+                     : "=&v"(v) : "v"(R == 1 ? w : upper), "s"(0x00f000f0u), "v"(magic), "s"(0x2c002c00u), "v"(z.high));
+    return v;
+}
+
+// Where a tile lies: column sweeps over groups of row blocks, so that concurrently running tiles share weights in L2.
+__device__ __forceinline__ void g4_place(unsigned tile, unsigned mblocks, unsigned nblocks, int& mblk, int& nblk) {
+    constexpr unsigned GM = 4;
+    const unsigned per_group = GM * nblocks, grp = tile / per_group, first_m = grp * GM, gm = min(mblocks - first_m, GM);
+    const unsigned in_group = tile - grp * per_group, col = in_group / gm;
+    mblk = __builtin_amdgcn_readfirstlane((int)(first_m + in_group - col * gm));
+    nblk = __builtin_amdgcn_readfirstlane((int)col);
+}
+
+// Two accumulators of 32 x 32 of rows m0 .. m0 + 31 and the 64 places from `unit` on to results.
+template <bool SWIGLU> __device__ __forceinline__ void g4_finish(const rkh_g4_args& g, int m0, int64_t unit, const float (&s0)[16], const float (&s1)[16], int lane) {
+    const int64_t n = SWIGLU ? unit * 32 + (lane & 31) : unit * 64 + 2 * (lane & 31);
+    if (n >= g.N) return;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int m = m0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        if (m >= g.M) continue;
+        float a = s0[e], b = s1[e];
+        if (g.exponents) {
+            const int ex = g.exponents[m];
+            a = __builtin_amdgcn_ldexpf(a, ex), b = __builtin_amdgcn_ldexpf(b, ex);
+        }
+        if constexpr (SWIGLU) {
+            const float v[1] = {mx_silu(a, b)};
+            g4_put<1>(g, m, n, v);
+        } else {
+            const float v[2] = {a, b};
+            g4_put<2>(g, m, n, v);
+        }
+    }
+}
+
+template <int RM, int GPB, bool SWIGLU>
+__global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+    using S = G4Tile<RM, GPB>;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave & 1, wn = wave >> 1;
+    const unsigned tiles = (unsigned)mblocks * nblocks, job = (unsigned)xcd_remap(blockIdx.x, (int)(tiles * parts));
+    const int part = parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(job / tiles));
+    const unsigned tile = job - part * tiles;
+    int mblk, nblk;
+    g4_place(tile, mblocks, nblocks, mblk, nblk);
+    const int KB = (int)rkh_g4_kb(g.K);
+    const int kb0 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * part / parts)), kb1 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * (part + 1) / parts));
+    const int64_t places = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU);
+
+    // ---- copies.  Wave-uniform addresses that advance by a step, lane offsets that stay.
+    const uint32_t base = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
+    const int m0 = mblk * S::ROWS;
+    const uint8_t* x_src = static_cast<const uint8_t*>(g.x) + ((size_t)m0 * g.ldx + (size_t)kb0 * 128) * 2;
+    unsigned x_off[2 * RM]; // of eight rows' 128 bytes; rows beyond M: the last one again
+#pragma unroll
+    for (int r = 0; r < 2 * RM; ++r) {
+        const int row = min(m0 + (wave * 2 * RM + r) * 8 + (lane >> 3), g.M - 1) - m0;
+        x_off[r] = (unsigned)row * (unsigned)g.ldx * 2 + ((lane & 7) ^ (lane >> 3)) * 16;
+    }
+    const uint8_t* w_src[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * 2 + i, places / 16 - 1) * KB + kb0) * 1024;
+    // (waves copy the same scales, or the same half of them, to one place)
+    const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_place = s_lane % (512 * GPB) / (4 * GPB);
+    const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)kb0 * places + (size_t)nblk * 128) * GPB * 4;
+    const unsigned s_off = (unsigned)min((int64_t)s_place, places - (int64_t)nblk * 128 - (GPB == 1 ? 4 : GPB == 2 ? 2 : 1)) * (4 * GPB);
+    const size_t s_step = (size_t)places * GPB * 4;
+    int ahead = kb1 - kb0; // steps that are still to be copied
+    const auto copy = [&](uint32_t to, auto c_tag) {
+        constexpr int C = decltype(c_tag)::value;
+        if constexpr (C < 4 * RM) {
+            constexpr int SUB = C / (2 * RM), R = C % (2 * RM);
+            mx_copy(x_src + SUB * 128, x_off[R], base + to + SUB * S::HALF + (wave * 2 * RM + R) * 1024);
+        } else if constexpr (C < 4 * RM + 2) {
+            mx_copy(w_src[C - 4 * RM], lane * 16, base + to + S::W_OFF + (wave * 2 + C - 4 * RM) * 1024);
+        } else {
+            mx_copy(s_src, s_off, base + to + S::S_OFF + (GPB == 4 ? (wave & 1) * 1024 : 0));
+        }
+    };
+    const auto copied = [&]() { // (behind the last step: that one again, which nobody reads)
+        if (--ahead > 0) {
+            x_src += 256;
+            w_src[0] += 1024, w_src[1] += 1024;
+            s_src += s_step;
+        }
+    };
+
+    // ---- LDS reads
+    uint32_t a_at[4]; // step s of a row's 64 k: s % 4
+#pragma unroll
+    for (int s = 0; s < 4; ++s) a_at[s] = (wm * RM * 32 + (lane & 31)) * 128 + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16);
+    const uint32_t w_at = S::W_OFF + wn * 4096 + (lane >> 4 & 1) * 2048 + (lane & 15) * 16 + (lane >> 5) * 256;
+    const uint32_t s_at = S::S_OFF + (wn * 64 + (lane >> 4 & 1) * 32 + (lane & 15)) * GPB * 4;
+    v4i a[RM][8], w[8];
+    v4i raw[2][2];
+    typedef uint32_t words __attribute__((ext_vector_type(GPB)));
+    words sd[2];
+    float scale[2][GPB];
+    const auto read_a = [&](uint32_t from, auto i_tag, auto s_tag) {
+        constexpr int I = decltype(i_tag)::value, ST = decltype(s_tag)::value;
+        a[I][ST] = *reinterpret_cast<const v4i*>(lds + from + a_at[ST & 3] + (ST >> 2) * S::HALF + I * 4096);
+    };
+    const auto read_w = [&](uint32_t from, auto j_tag) {
+        constexpr int J = decltype(j_tag)::value;
+        raw[J][0] = *reinterpret_cast<const v4i*>(lds + from + w_at + J * 1024);
+        raw[J][1] = *reinterpret_cast<const v4i*>(lds + from + w_at + J * 1024 + 512);
+    };
+    const auto read_s = [&](uint32_t from, auto j_tag) {
+        constexpr int J = decltype(j_tag)::value;
+        sd[J] = *reinterpret_cast<const words*>(lds + from + s_at + J * 64 * GPB);
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+
+    // ---- codes to operands: pair x (0..31) of a half's eight operands
+    G4Zero zero[2][GPB];
+    uint32_t magic, upper[2] = {0, 0};
+    asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(magic));
+    const auto decode = [&](auto j_tag, auto x_tag) {
+        constexpr int J = decltype(j_tag)::value, X = decltype(x_tag)::value, ST = X / 4, R = X % 4;
+        w[ST][R] = (int)g4_pair_here<R>((uint32_t)raw[J][ST & 1][ST >> 1], zero[J][ST * GPB / 8], magic, upper[J]);
+    };
+    const auto zeros_of = [&](auto j_tag) {
+        constexpr int J = decltype(j_tag)::value;
+#pragma unroll
+        for (int n = 0; n < GPB; ++n) zero[J][n].of(sd[J][n]);
+    };
+    const auto scale_of = [&](auto j_tag) {
+        constexpr int J = decltype(j_tag)::value;
+#pragma unroll
+        for (int n = 0; n < GPB; ++n) scale[J][n] = g4_scale(sd[J][n], g.scale_type);
+    };
+
+    // ---- prologue
+    static_for<S::COPIES>([&](auto c) { copy(0, c); });
+    copied();
+    static_for<S::COPIES>([&](auto c) { copy(S::BUF, c); });
+    copied();
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::COPIES) : "memory");
+    static_for<RM>([&](auto i) { static_for<8>([&](auto s) { read_a(0, i, s); }); });
+    read_w(0, I0{}), read_w(0, I1{});
+    read_s(0, I0{}), read_s(0, I1{});
+    zeros_of(I0{});
+    static_for<32>([&](auto x) { decode(I0{}, x); });
+
+    float acc[RM][2][16];
+    v16f sum[2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i) acc[i][0][e] = acc[i][1][e] = 0;
+        sum[0][e] = sum[1][e] = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < GPB; ++n) scale[0][n] = scale[1][n] = 0;
+
+    // ---- steps.  Slot t is product t of the step and what is issued behind it.
+    constexpr int L = 8 / GPB, GROUPS = 2 * RM * GPB, SLOTS = 16 * RM, MID = 8 * RM; // products of a group, groups and slots of a step
+    constexpr int DECODE_FROM = RM == 1 ? 4 : 1;                                     // (with RM = 1 the codes have just been read)
+    const auto fold = [&](auto g_tag, auto from_tag, auto to_tag) { // elements of group G's sum into the accumulators
+        constexpr int G = decltype(g_tag)::value, C = G / GPB, I = C % RM, J = C / RM;
+#pragma unroll
+        for (int e = from_tag(); e < to_tag(); ++e) g4_add_scaled(acc[I][J][e], sum[G & 1][e], scale[J][G % GPB]);
+    };
+    // (half J's codes in the 14 slots from the last chain of the other half on; AT: slots since that began)
+    const auto decode_some = [&](auto j_tag, auto at_tag) {
+        constexpr int AT = decltype(at_tag)::value - DECODE_FROM, N = 14 - DECODE_FROM;
+        if constexpr (AT >= 0 && AT < N) {
+            if constexpr (AT == 0) zeros_of(j_tag);
+            constexpr int X0 = 32 * AT / N, X1 = 32 * (AT + 1) / N;
+            static_for<X1 - X0>([&](auto x) { decode(j_tag, std::integral_constant<int, X0 + decltype(x)::value>{}); });
+        }
+    };
+    uint32_t here = 0; // of the step that is multiplied
+    for (int kb = kb0; kb < kb1; ++kb) {
+        const uint32_t next = S::BUF - here;
+        static_for<SLOTS>([&](auto t_tag) {
+            constexpr int T = decltype(t_tag)::value, C = T / 8, ST = T % 8, I = C % RM, G = T / L;
+            if constexpr (T == MID) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if constexpr (T % L == 0) g4_product_first(a[I][ST], w[ST], sum[G & 1]);
+            else g4_product(a[I][ST], w[ST], sum[G & 1]);
+            // the sum of a group from two slots behind its last product up to where its registers are wanted again
+            constexpr int U = T + SLOTS - L - 1, F = U / L % GROUPS, O = U % L;
+            if constexpr (O < L - 1) fold(std::integral_constant<int, F>{}, std::integral_constant<int, 16 * O / (L - 1)>{}, std::integral_constant<int, 16 * (O + 1) / (L - 1)>{});
+            if constexpr (T == 0) scale_of(I0{});
+            if constexpr (T == 8) scale_of(I1{});
+            decode_some(I1{}, std::integral_constant<int, T - (MID - 8)>{});
+            decode_some(I0{}, std::integral_constant<int, T < 8 ? T + 8 : T - (SLOTS - 8)>{});
+            if constexpr (T >= MID) {
+                constexpr int H = T - MID;
+                if constexpr (H == 0) read_s(next, I0{}), read_w(next, I0{});
+                if constexpr (H == 7) read_s(next, I1{}), read_w(next, I1{});
+                read_a(next, std::integral_constant<int, I>{}, std::integral_constant<int, ST>{});
+                constexpr int C0 = S::COPIES * H / MID, C1 = S::COPIES * (H + 1) / MID;
+                static_for<C1 - C0>([&](auto c) { copy(here, std::integral_constant<int, C0 + decltype(c)::value>{}); });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        copied();
+        here = next;
+    }
+    asm volatile("s_nop 7\n\ts_nop 7" ::: "memory"); // (the last product has to be through)
+    fold(std::integral_constant<int, GROUPS - 1>{}, I0{}, std::integral_constant<int, 16>{});
+    // a load to LDS must not outlive the workgroup
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+    if (parts > 1) { // partial tile in accumulator order: [tile][part][wave][i][j][quarter of 16][lane]
+        v4f* to = reinterpret_cast<v4f*>(g.scratch) + (((size_t)tile * parts + part) * 4 + wave) * (RM * 2 * 4 * 64) + lane;
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    to[((i * 2 + j) * 4 + e) * 64] = v4f{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < RM; ++i) g4_finish<SWIGLU>(g, m0 + (wm * RM + i) * 32, (int64_t)nblk * 2 + wn, acc[i][0], acc[i][1], lane);
+    }
+}
+
+// Sum of the parts of a tile, in their order, and the results.  One wave per 32 rows x 64 places.
+template <int RM, bool SWIGLU>
+__global__ __launch_bounds__(256) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+    const int lane = lane_id();
+    const unsigned tile = blockIdx.x / RM, i = blockIdx.x % RM, wave = wave_id();
+    int mblk, nblk;
+    g4_place(tile, mblocks, nblocks, mblk, nblk);
+    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + ((size_t)tile * parts * 4 + wave) * (RM * 2 * 4 * 64) + i * 512 + lane;
+    float s[2][16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0;
+    for (int p = 0; p < parts; ++p) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const v4f v = from[x * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[x >> 2][4 * (x & 3) + e] += v[e];
+        }
+        from += 4 * RM * 2 * 4 * 64;
+    }
+    g4_finish<SWIGLU>(g, (mblk * 2 + (wave & 1)) * RM * 32 + i * 32, (int64_t)nblk * 2 + (wave >> 1), s[0], s[1], lane);
+}
+
+template <int RM, int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
+    constexpr int LDS = G4Tile<RM, GPB>::LDS;
+    static std::atomic<bool> opted_in[64] = {};
+    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_tile_kernel<RM, GPB, SWIGLU>), opted_in, LDS)) return rc;
+    const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
+    if (tiles * r.parts * 256 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
+    mark(st, "g4_tile_kernel");
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_tile_kernel<RM, GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, r.parts);
+    RKH_CHECK(hipGetLastError());
+    if (r.parts > 1) {
+        mark(st, "g4_join_kernel");
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<RM, SWIGLU>), dim3((unsigned)(tiles * RM)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts);
+        RKH_CHECK(hipGetLastError());
+    }
+    return RKH_OK;
+}
+template <int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
+    return r.rm == 4 ? launch_tiles<4, GPB, SWIGLU>(st, g, r) : r.rm == 2 ? launch_tiles<2, GPB, SWIGLU>(st, g, r) : launch_tiles<1, GPB, SWIGLU>(st, g, r);
+}
+template <int GPB> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
+    return g.swiglu ? launch_tiles<GPB, true>(st, g, r) : launch_tiles<GPB, false>(st, g, r);
+}
+
+} // namespace
+
+#endif // RK_KERNELS_G4_TILE_H

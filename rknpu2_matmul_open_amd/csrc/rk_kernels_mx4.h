@@ -159,6 +159,40 @@ __device__ __forceinline__ int mx_column(int p, int N, int gate_up) {
     return n < F ? n + (p & 32 ? F : 0) : -1;
 }
 
+// ---- what products share
+typedef __attribute__((address_space(3))) uint8_t* mx_lds_ptr;
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm" // m0 is set and clobbered on purpose below
+// 16 bytes per lane from base + off, lane-contiguous to LDS address `to`.  (A load to LDS needs a wait state behind a write of M0.)
+__device__ __forceinline__ void mx_copy(const uint8_t* base, unsigned off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// gate / (1 + exp(-gate)) * up.  exp(x) = 2^(x log2 e): the product's rounded-off part goes in as a factor of its own, so that the
+// error does not grow with x (a few 2^-24); quotient and power by the hardware's reciprocal and exponential, an ulp each.  (The polynomial
+// and the correctly rounded division of the int4 layers' SwiGLU are their interface's bits; in the epilogue of a 256 x 256 tile they took 7 us.)
+__device__ __forceinline__ float mx_silu(float gate, float up) {
+    constexpr float L = 1.44269504088896f, L_REST = 1.92596299e-8f, LN2 = 0.693147180559945f; // log2 e = L + L_REST
+    const float t = -gate * L, rest = fmaf(-gate, L_REST, fmaf(-gate, L, -t));
+    const float power = __builtin_amdgcn_exp2f(t) * (fabsf(gate) < 128.0f ? fmaf(rest, LN2, 1.0f) : 1.0f); // (beyond: 0 or infinity)
+    // (of a quarter: the reciprocal gives zero for what is 2^126 or more, where gate * reciprocal is still a normal number)
+    return 0.25f * gate * __builtin_amdgcn_rcpf(fmaf(0.25f, power, 0.25f)) * up;
+}
+
+// More than 64 KiB of LDS for a kernel, once per device; `opted_in` is the kernel's own.
+int mx_allow_lds(const void* kernel, std::atomic<bool> (&opted_in)[64], int bytes) {
+    int dev = 0;
+    RKH_CHECK(hipGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return RKH_ERR_RUNTIME;
+    if (!opted_in[dev].load(std::memory_order_acquire)) {
+        RKH_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        opted_in[dev].store(true, std::memory_order_release);
+    }
+    return RKH_OK;
+}
+
 } // namespace
 
 #endif // RK_KERNELS_MX4_H

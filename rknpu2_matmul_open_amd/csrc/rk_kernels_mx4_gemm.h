@@ -18,8 +18,6 @@ int launch_mx4_swiglu(hipStream_t st, const rkh_mx4_gemm_args& g);
 
 namespace {
 
-typedef __attribute__((address_space(3))) uint8_t* mx_lds_ptr;
-
 // sum += W * A over 128 k; the scales are byte STEP of the lanes' dwords.
 template <int STEP> __device__ __forceinline__ v4f mx_mfma(const v4i& w, const v4i& a, const v4f& sum, uint32_t ws, uint32_t as) {
     const v8i w8 = {w.x, w.y, w.z, w.w, 0, 0, 0, 0}, a8 = {a.x, a.y, a.z, a.w, 0, 0, 0, 0};
@@ -54,17 +52,6 @@ template <int STEP, bool ACC> __device__ __forceinline__ void mx_mfma_first(cons
 template <bool ACC> __device__ __forceinline__ void mx_settled(v4f& sum) {
     if constexpr (ACC) asm volatile("" : "+a"(sum));
     else asm volatile("" : "+v"(sum));
-}
-
-// gate / (1 + exp(-gate)) * up.  exp(x) = 2^(x log2 e): the product's rounded-off part goes in as a factor of its own, so that the
-// error does not grow with x (a few 2^-24); quotient and power by the hardware's reciprocal and exponential, an ulp each.  (The polynomial
-// and the correctly rounded division of the int4 layers' SwiGLU are their interface's bits; in the epilogue of a 256 x 256 tile they took 7 us.)
-__device__ __forceinline__ float mx_silu(float gate, float up) {
-    constexpr float L = 1.44269504088896f, L_REST = 1.92596299e-8f, LN2 = 0.693147180559945f; // log2 e = L + L_REST
-    const float t = -gate * L, rest = fmaf(-gate, L_REST, fmaf(-gate, L, -t));
-    const float power = __builtin_amdgcn_exp2f(t) * (fabsf(gate) < 128.0f ? fmaf(rest, LN2, 1.0f) : 1.0f); // (beyond: 0 or infinity)
-    // (of a quarter: the reciprocal gives zero for what is 2^126 or more, where gate * reciprocal is still a normal number)
-    return 0.25f * gate * __builtin_amdgcn_rcpf(fmaf(0.25f, power, 0.25f)) * up;
 }
 
 // N (4 or 8) consecutive values to where `to` points, of which `count` exist.  (Instructions that are not yet in the cache cost small
@@ -321,14 +308,6 @@ __global__ __launch_bounds__(MAX_WAVES * 64, RM == 1 ? 4 : 1) void mx4_few_kerne
 //  * the scales of group g + 2, issued in the second step of group g, overwrite those of group g, which were read in the last
 //    step of group g - 1 and waited for by the products of the first step of group g, ahead of the barrier that ended it.
 // Copies beyond the part's K bring its last step again, for the count; nothing reads them.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm" // m0 is set and clobbered on purpose below
-// 16 bytes per lane from base + off, lane-contiguous to LDS address `to`.  (A load to LDS needs a wait state behind a write of M0.)
-__device__ __forceinline__ void mx_copy(const uint8_t* base, unsigned off, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // HALVES: groups that the ring holds.
 template <int RM, int CN, int HALVES> struct MxTile {
     static constexpr int AB = 2 * RM, WB = 2 * CN;               // operands of a step
@@ -715,18 +694,6 @@ MxRoute mx_route(int M, int N, int K, int swiglu) {
     return best;
 }
 size_t mx_scratch(const MxRoute& r) { return r.few || r.parts == 1 ? 0 : (size_t)r.mblocks * r.nblocks * r.parts * r.rm * r.cn * 4096; }
-
-// More than 64 KiB of LDS for a kernel, once per device; `opted_in` is the kernel's own.
-int mx_allow_lds(const void* kernel, std::atomic<bool> (&opted_in)[64], int bytes) {
-    int dev = 0;
-    RKH_CHECK(hipGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return RKH_ERR_RUNTIME;
-    if (!opted_in[dev].load(std::memory_order_acquire)) {
-        RKH_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        opted_in[dev].store(true, std::memory_order_release);
-    }
-    return RKH_OK;
-}
 
 template <int RM, int CN, int NG, int MAX_WAVES, bool SWIGLU, int FUSED, int X>
 int launch_few_as(hipStream_t st, const rkh_mx4_gemm_args& g, const MxRoute& r, int per, int waves) {

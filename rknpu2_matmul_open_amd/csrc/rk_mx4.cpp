@@ -7,7 +7,7 @@
 #include "rk_host.h"
 #include "rk_mx4_shim.h"
 #include "rk_npu_mx4.h"
-#include "rk_rows.h"
+#include "rk_values.h"
 
 using namespace rkhost;
 
@@ -27,20 +27,6 @@ struct rk_npu_mx4_workspace {
 };
 
 namespace {
-
-bool valid_type(int type) { return type >= RK_NPU_MX4_F32 && type <= RK_NPU_MX4_BF16; }
-int64_t type_bytes(int type) { return type == RK_NPU_MX4_F32 ? 4 : 2; }
-bool valid_length(int K) { return K > 0 && K <= INT32_MAX / 1024; }
-
-Span values(const void* p, int type, int64_t rows, int64_t ld, int64_t width) {
-    return Span(p, rows, ld * type_bytes(type), width * type_bytes(type));
-}
-// Pointer and stride of rows of values: aligned to the type, no row on the next one, and all of it addressable.
-bool valid_rows(const void* p, int type, int64_t rows, int64_t ld, int64_t width) {
-    if (rows == 0) return valid_type(type); // (an empty tensor may have no address)
-    return valid_type(type) && p && reinterpret_cast<uintptr_t>(p) % type_bytes(type) == 0 && ld >= width && ld <= (INT64_C(1) << 40) &&
-           ld <= (INT64_C(1) << 56) / rows;
-}
 
 rk_npu_mx4_weights* create_weights(rk_npu_iommu_domain* domain, const rk_npu_mx4_weight_config* config, const uint8_t* codes, const uint8_t* scales,
                                    bool on_host) {

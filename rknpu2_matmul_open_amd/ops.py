@@ -573,3 +573,162 @@ def mx4_ffn_block(gu_ws, gate_up, down_ws, down, stream, branch, weight=None, af
     check(gu_ws.lib.rk_npu_mx4_run_ffn_block_device(gu_ws.h, gate_up.h, down_ws.h, down.h, C.byref(a), C.c_void_p(branch.data_ptr()),
                                                     _channel(next_weight, stream.shape[1], "next_weight", gu_ws.device)), "mx4_ffn_block")
     gu_ws.staged = down_ws.staged = None
+
+
+# ---- G4 layers and the heads' norm and rotation: tensors on the device, as above ----------------
+
+_G4_HALVES = {"torch.float16": capi.MX4_F16, "torch.bfloat16": capi.MX4_BF16, "float16": capi.MX4_F16}
+
+
+def _g4_array(x, shape, types, what, device):
+    """The address of a contiguous tensor or numpy array (device None) of one of the types."""
+    if str(x.dtype) not in types or tuple(x.shape) != shape:
+        raise ValueError("%s: %s of shape %s, got %s %s" % (what, " or ".join(types), shape, x.dtype, tuple(x.shape)))
+    if device is None:
+        if not x.flags.c_contiguous:
+            raise ValueError("%s: a contiguous array" % what)
+        return C.c_void_p(x.ctypes.data)
+    _on_device(x, device)
+    if not x.is_contiguous():
+        raise ValueError("%s: a contiguous tensor" % what)
+    return C.c_void_p(x.data_ptr())
+
+
+class G4Weights:
+    """Group-scaled 4-bit weights [N, K] (gate_up: N = 2F, the gate's rows first) from numpy arrays, or from_device from tensors: codes uint8
+    [N, ceil(K / 2)], scales [N, ceil(K / group)] of float16 or bfloat16 (numpy: bfloat16 as uint16 bits with scale_type=capi.MX4_BF16), zeros uint8
+    [N, ceil(K / group)] or None (8)."""
+
+    def __init__(self, session, K, N, group, codes, scales, zeros=None, gate_up=False, scale_type=None, on_device=False):
+        self.lib, self.K, self.N, self.group, self.gate_up = session.lib, K, N, group, gate_up
+        if group < 1:
+            raise ValueError("groups of %d values" % group)
+        device, groups = _device_of(session) if on_device else None, -(-K // group)
+        if scale_type is None:
+            scale_type = _G4_HALVES.get(str(scales.dtype))
+        if scale_type is None:
+            raise TypeError("scales of float16 or bfloat16: got %s" % scales.dtype)
+        kinds = {capi.MX4_F16: ("torch.float16", "float16", "uint16"), capi.MX4_BF16: ("torch.bfloat16", "uint16")}[scale_type]
+        p = _g4_array(codes, (N, -(-K // 2)), ("torch.uint8", "uint8"), "codes", device)
+        s = _g4_array(scales, (N, groups), kinds, "scales", device)
+        z = None if zeros is None else _g4_array(zeros, (N, groups), ("torch.uint8", "uint8"), "zeros", device)
+        config = capi.G4WeightConfig(K, N, group, 1 if gate_up else 0, scale_type)
+        create = self.lib.rk_npu_g4_weights_create_device if on_device else self.lib.rk_npu_g4_weights_create
+        self.h = create(session.domain, C.byref(config), p, s, z)
+        if not self.h:
+            raise ValueError("rk_npu_g4_weights_create failed")
+
+    @classmethod
+    def from_device(cls, session, K, N, group, codes, scales, zeros=None, gate_up=False):
+        return cls(session, K, N, group, codes, scales, zeros, gate_up, on_device=True)
+
+    def close(self):
+        if self.h:
+            self.lib.rk_npu_g4_weights_free(self.h)
+            self.h = None
+
+
+class G4Workspace:
+    """Workspace for up to max_rows rows of K values and weights of up to N columns (gate / up: 2F)."""
+    device = None # the context's
+
+    def __init__(self, session, max_rows, K, N):
+        self.lib, self.K, self.device = session.lib, K, _device_of(session)
+        self.h = self.lib.rk_npu_g4_workspace_create(session.domain, max_rows, K, N)
+        if not self.h:
+            raise ValueError("rk_npu_g4_workspace_create failed")
+
+    def _run(self, call, weights, a, c, columns):
+        kind, p, ld = _mx4_rows(a, self.K, self.device)
+        c_kind, c_p, c_ld = _mx4_rows(c, columns, self.device)
+        if c.shape[0] != a.shape[0]:
+            raise ValueError("%d rows in, %d out" % (a.shape[0], c.shape[0]))
+        if kind == capi.MX4_F32:
+            raise TypeError("activations of float16 or bfloat16: got %s" % a.dtype)
+        check(call(self.h, weights.h, a.shape[0], kind, p, ld, c_kind, c_p, c_ld), "g4 run")
+
+    def run(self, weights, a, c):
+        """c [rows, N] = a [rows, K] times the weights."""
+        self._run(self.lib.rk_npu_g4_run_device, weights, a, c, weights.N)
+
+    def run_swiglu(self, weights, a, c):
+        """c [rows, F] = silu(a * gate) * (a * up)."""
+        self._run(self.lib.rk_npu_g4_run_swiglu_device, weights, a, c, weights.N // 2)
+
+    def close(self):
+        if self.h:
+            self.lib.rk_npu_g4_workspace_free(self.h)
+            self.h = None
+
+
+def pair_axes(sections, interleaved=False):
+    """Which axis turns which pair, for heads_norm_rotate: sections[i] pairs of axis i, one section behind the other; interleaved: in turn, as long
+    as an axis has pairs left."""
+    if not interleaved:
+        return [axis for axis, n in enumerate(sections) for _ in range(n)]
+    left, table = list(sections), []
+    while any(left):
+        for axis, n in enumerate(left):
+            if n:
+                table.append(axis)
+                left[axis] -= 1
+    return table
+
+
+def heads_args(session, q, k, q_out=None, k_out=None, norm=True, eps=1e-6, q_weight=None, k_weight=None, positions=None, inv_freq=None,
+               pair_axis=None, neighbours=False, rotation_scale=1.0):
+    """rk_npu_heads_args of tensors, which it keeps alive: see heads_norm_rotate."""
+    device = _device_of(session)
+    some = q if q is not None else k
+    if some is None:
+        raise ValueError("queries or keys")
+    rows, _, D = some.shape
+    kind = _MX4_TYPES.get(str(some.dtype))
+    if kind is None:
+        raise TypeError("heads of float32, float16 or bfloat16: got %s" % some.dtype)
+    a = capi.HeadsArgs()
+    session.lib.rk_npu_heads_args_init(C.byref(a), rows, D)
+    a.type, a.norm, a.eps, a.rotation_scale, a.neighbours = kind, 1 if norm else 0, eps, rotation_scale, 1 if neighbours else 0
+    q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
+    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+        if x is None:
+            if out is not None:
+                raise ValueError("%s_out without %s" % (name, name))
+            continue
+        for what, t in ((name, x), (name + "_out", out)):
+            _on_device(t, device)
+            if t.dtype != some.dtype or len(t.shape) != 3 or t.shape[0] != rows or t.shape[2] != D or t.shape[1] != x.shape[1] or (D > 1 and t.stride(2) != 1):
+                raise ValueError("%s: %s [%d, %d, %d] with contiguous heads, got %s %s, strides %s" % (what, some.dtype, rows, x.shape[1], D, t.dtype, tuple(t.shape), t.stride()))
+            setattr(a, what, t.data_ptr())
+            setattr(a, what + "_row", t.stride(0))
+            setattr(a, what + "_head", t.stride(1))
+        setattr(a, name + "_heads", x.shape[1])
+    a.q_weight, a.k_weight = _channel(q_weight, D, "q_weight", device), _channel(k_weight, D, "k_weight", device)
+    a.rotary_dim = 0
+    table = None
+    if inv_freq is not None:
+        pairs = inv_freq.shape[0]
+        a.inv_freq = _channel(inv_freq, pairs, "inv_freq", device)
+        a.rotary_dim = 2 * pairs
+        _on_device(positions, device)
+        if str(positions.dtype) != "torch.int32" or len(positions.shape) not in (1, 2) or positions.shape[-1] != rows or (rows > 1 and positions.stride(-1) != 1):
+            raise ValueError("positions: int32 [%d] or [axes, %d] with contiguous rows, got %s %s" % (rows, rows, positions.dtype, tuple(positions.shape)))
+        a.positions, a.axes = positions.data_ptr(), positions.shape[0] if len(positions.shape) == 2 else 1
+        a.position_axis = positions.stride(0) if len(positions.shape) == 2 else 0
+        if pair_axis is not None:
+            if len(pair_axis) != pairs or any(not 0 <= x < a.axes for x in pair_axis):
+                raise ValueError("pair_axis: an axis 0..%d for each of %d pairs" % (a.axes - 1, pairs))
+            table = (C.c_uint8 * max(1, pairs))(*pair_axis)
+            a.pair_axis = C.addressof(table)
+    elif positions is not None or pair_axis is not None:
+        raise ValueError("positions without inv_freq")
+    a.kept = (q, k, q_out, k_out, q_weight, k_weight, positions, inv_freq, table)
+    return a
+
+
+def heads_norm_rotate(session, q, k, q_out=None, k_out=None, **options):
+    """The norm of query and key heads and their rotation by position (rk_npu_heads_norm_rotate_device): q, k [rows, heads, D], either may be None;
+    outputs of the same shapes, or None: in place.  norm, eps, q_weight and k_weight (float32 [D]); inv_freq float32 [pairs] and positions int32
+    [rows] or [axes, rows], None: no rotation; pair_axis: the axis of each pair (pair_axes); neighbours: pairs (2 i, 2 i + 1) and not (i, i + pairs)."""
+    a = heads_args(session, q, k, q_out, k_out, **options)
+    check(session.lib.rk_npu_heads_norm_rotate_device(session.ctx, C.byref(a)), "heads_norm_rotate")
