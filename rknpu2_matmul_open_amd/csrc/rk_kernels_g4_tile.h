@@ -1,12 +1,12 @@
-// Tiles of G4 products: 64 RM rows x 128 places by four waves (two by two), each RM x 2 accumulators of 32 x 32.  Bound by the matrix pipes and what
+// Tiles of G4 products: 32 RM WM rows x 128 places by 2 WM waves (WM by two), each RM x 2 accumulators of 32 x 32.  Bound by the matrix pipes and what
 // has to be issued beside them.
 //
 // A step is 128 k.  Its activations (rows of 256 bytes), codes and scales are copied global -> LDS directly, two steps ahead of the products and one
 // ahead of the LDS reads:
 //  * a wave's activations of a step live in registers, 8 RM operands that both of its 32-place halves j multiply.  An operand's last product
 //    is one of half 1; behind it, it is replaced by the next step's;
-//  * codes become halves (code - zero) one operand at a time: those of half 1 behind the last products of half 0 that use the same registers, and those
-//    of half 0 of the next step behind the last ones of half 1.  So both ways of issue are used evenly;
+//  * codes become halves (code - zero) one operand at a time, before the half's first products: the first four operands have registers for each half, and
+//    the other four take those of the other half behind its last products;
 //  * a group's products start from zero, and its sum goes into the accumulators, times the scale, while the next group's run.
 // In half-time of step s (between the halves) a wave waits for its copies of step s + 1 and for its LDS reads, and meets the others: from
 // there on LDS holds step s + 1 for all, and nobody reads step s any more, whose place the copies of step s + 2 take.
@@ -22,10 +22,13 @@
 
 namespace {
 
-template <int RM, int GPB> struct G4Tile {
-    static constexpr int ROWS = 64 * RM, HALF = ROWS * 128; // bytes of 64 k
+template <int RM, int WM, int GPB> struct G4Tile {
+    static constexpr int ROWS = 32 * RM * WM, WAVES = 2 * WM, HALF = ROWS * 128; // bytes of 64 k
     static constexpr int W_OFF = 2 * HALF, S_OFF = W_OFF + 8192, S_COPIES = GPB == 4 ? 2 : 1, BUF = S_OFF + S_COPIES * 1024, LDS = 2 * BUF;
-    static constexpr int COPIES = 4 * RM + 3; // of a wave and step: activations, codes, scales
+    static constexpr int XC = 4 * RM, WC = 8 / WAVES, COPIES = XC + WC + 1; // of a wave and step: activations, codes, scales
+    static constexpr int PAIRS = XC / 2 + 2;                                // statements that issue them, two activations' or all codes' at a time
+    static_assert(WC == 1 || WC == 2, "");
+    static constexpr int copies(int statements) { return statements <= XC / 2 ? 2 * statements : XC + WC + statements - XC / 2 - 1; }
     static_assert(LDS <= 160 * 1024, "");
 };
 
@@ -65,33 +68,49 @@ __device__ __forceinline__ void g4_place(unsigned tile, unsigned mblocks, unsign
 }
 
 // Two accumulators of 32 x 32 of rows m0 .. m0 + 31 and the 64 places from `unit` on to results.
-template <bool SWIGLU> __device__ __forceinline__ void g4_finish(const rkh_g4_args& g, int m0, int64_t unit, const float (&s0)[16], const float (&s1)[16], int lane) {
+template <int OUT, bool SWIGLU, bool EXPONENTS>
+__device__ __forceinline__ void g4_finish_as(const rkh_g4_args& g, int m0, int64_t unit, const float (&s0)[16], const float (&s1)[16], int lane) {
+    using T = typename MxType<OUT>::T;
+    typedef T pair __attribute__((ext_vector_type(2)));
+    typedef pair pair_any __attribute__((aligned(sizeof(T))));
     const int64_t n = SWIGLU ? unit * 32 + (lane & 31) : unit * 64 + 2 * (lane & 31);
-    if (n >= g.N) return;
+    const int first = m0 + 4 * (lane >> 5), live = n < g.N ? g.M - first : 0;
+    T* to = static_cast<T*>(g.C) + (size_t)first * g.ldc + n;
+    const bool both = n + 1 < g.N;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        const int m = m0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-        if (m >= g.M) continue;
-        float a = s0[e], b = s1[e];
-        if (g.exponents) {
-            const int ex = g.exponents[m];
-            a = __builtin_amdgcn_ldexpf(a, ex), b = __builtin_amdgcn_ldexpf(b, ex);
+        const int r = 8 * (e >> 2) + (e & 3);
+        if (r < live) {
+            float a = s0[e], b = s1[e];
+            if constexpr (EXPONENTS) {
+                const int ex = g.exponents[first + r];
+                a = __builtin_amdgcn_ldexpf(a, ex), b = __builtin_amdgcn_ldexpf(b, ex);
+            }
+            if constexpr (SWIGLU) *to = (T)mx_silu(a, b);
+            else if (both) *reinterpret_cast<pair_any*>(to) = pair{(T)a, (T)b};
+            else *to = (T)a;
         }
-        if constexpr (SWIGLU) {
-            const float v[1] = {mx_silu(a, b)};
-            g4_put<1>(g, m, n, v);
-        } else {
-            const float v[2] = {a, b};
-            g4_put<2>(g, m, n, v);
-        }
+        to += (e & 3) == 3 ? 5 * g.ldc : g.ldc;
     }
 }
+template <int RM, bool SWIGLU> __device__ __forceinline__ void g4_finish(const rkh_g4_args& g, int m0, int64_t unit, const float (&s)[RM][2][16], int lane) {
+    mx_with_type(g.out_type, [&](auto t) {
+        constexpr int OUT = decltype(t)::value;
+        if (g.exponents) {
+#pragma unroll
+            for (int i = 0; i < RM; ++i) g4_finish_as<OUT, SWIGLU, true>(g, m0 + i * 32, unit, s[i][0], s[i][1], lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < RM; ++i) g4_finish_as<OUT, SWIGLU, false>(g, m0 + i * 32, unit, s[i][0], s[i][1], lane);
+        }
+    });
+}
 
-template <int RM, int GPB, bool SWIGLU>
-__global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
-    using S = G4Tile<RM, GPB>;
+template <int RM, int WM, int GPB, bool SWIGLU>
+__global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+    using S = G4Tile<RM, WM, GPB>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave & 1, wn = wave >> 1;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave % WM, wn = wave / WM;
     const unsigned tiles = (unsigned)mblocks * nblocks, job = (unsigned)xcd_remap(blockIdx.x, (int)(tiles * parts));
     const int part = parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(job / tiles));
     const unsigned tile = job - part * tiles;
@@ -104,29 +123,32 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
     // ---- copies.  Wave-uniform addresses that advance by a step, lane offsets that stay.
     const uint32_t base = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
     const int m0 = mblk * S::ROWS;
-    const uint8_t* x_src = static_cast<const uint8_t*>(g.x) + ((size_t)m0 * g.ldx + (size_t)kb0 * 128) * 2;
+    // (a bias of 1024: offsets of the second copies of pairs are 1024 less, see mx_copy_two)
+    const uint8_t* x_src = static_cast<const uint8_t*>(g.x) + ((size_t)m0 * g.ldx + (size_t)kb0 * 128) * 2 - 1024;
     unsigned x_off[2 * RM]; // of eight rows' 128 bytes; rows beyond M: the last one again
 #pragma unroll
     for (int r = 0; r < 2 * RM; ++r) {
         const int row = min(m0 + (wave * 2 * RM + r) * 8 + (lane >> 3), g.M - 1) - m0;
-        x_off[r] = (unsigned)row * (unsigned)g.ldx * 2 + ((lane & 7) ^ (lane >> 3)) * 16;
+        x_off[r] = (unsigned)row * (unsigned)g.ldx * 2 + ((lane & 7) ^ (lane >> 3)) * 16 + (r & 1 ? 0 : 1024);
     }
-    const uint8_t* w_src[2];
+    const uint8_t* w_src[S::WC];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * 2 + i, places / 16 - 1) * KB + kb0) * 1024;
+    for (int i = 0; i < S::WC; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * S::WC + i, places / 16 - 1) * KB + kb0) * 1024 - i * 1024;
     // (waves copy the same scales, or the same half of them, to one place)
     const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_place = s_lane % (512 * GPB) / (4 * GPB);
     const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)kb0 * places + (size_t)nblk * 128) * GPB * 4;
     const unsigned s_off = (unsigned)min((int64_t)s_place, places - (int64_t)nblk * 128 - (GPB == 1 ? 4 : GPB == 2 ? 2 : 1)) * (4 * GPB);
     const size_t s_step = (size_t)places * GPB * 4;
     int ahead = kb1 - kb0; // steps that are still to be copied
-    const auto copy = [&](uint32_t to, auto c_tag) {
-        constexpr int C = decltype(c_tag)::value;
-        if constexpr (C < 4 * RM) {
-            constexpr int SUB = C / (2 * RM), R = C % (2 * RM);
-            mx_copy(x_src + SUB * 128, x_off[R], base + to + SUB * S::HALF + (wave * 2 * RM + R) * 1024);
-        } else if constexpr (C < 4 * RM + 2) {
-            mx_copy(w_src[C - 4 * RM], lane * 16, base + to + S::W_OFF + (wave * 2 + C - 4 * RM) * 1024);
+    const auto copy = [&](uint32_t to, auto p_tag) {
+        constexpr int P = decltype(p_tag)::value;
+        if constexpr (P < S::XC / 2) {
+            constexpr int SUB = P / RM, R = P % RM * 2;
+            mx_copy_two(x_src + SUB * 128, x_off[R], x_src + SUB * 128, x_off[R + 1], base + to + SUB * S::HALF + (wave * 2 * RM + R) * 1024);
+        } else if constexpr (P == S::XC / 2) {
+            const uint32_t at = base + to + S::W_OFF + wave * S::WC * 1024;
+            if constexpr (S::WC == 2) mx_copy_two(w_src[0], lane * 16, w_src[1], lane * 16, at);
+            else mx_copy(w_src[0], lane * 16, at);
         } else {
             mx_copy(s_src, s_off, base + to + S::S_OFF + (GPB == 4 ? (wave & 1) * 1024 : 0));
         }
@@ -134,7 +156,8 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
     const auto copied = [&]() { // (behind the last step: that one again, which nobody reads)
         if (--ahead > 0) {
             x_src += 256;
-            w_src[0] += 1024, w_src[1] += 1024;
+#pragma unroll
+            for (int i = 0; i < S::WC; ++i) w_src[i] += 1024;
             s_src += s_step;
         }
     };
@@ -145,7 +168,7 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
     for (int s = 0; s < 4; ++s) a_at[s] = (wm * RM * 32 + (lane & 31)) * 128 + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16);
     const uint32_t w_at = S::W_OFF + wn * 4096 + (lane >> 4 & 1) * 2048 + (lane & 15) * 16 + (lane >> 5) * 256;
     const uint32_t s_at = S::S_OFF + (wn * 64 + (lane >> 4 & 1) * 32 + (lane & 15)) * GPB * 4;
-    v4i a[RM][8], w[8];
+    v4i a[RM][8], w[12]; // (of half 0: 0 .. 3 and 8 .. 11, of half 1: 4 .. 11)
     v4i raw[2][2];
     typedef uint32_t words __attribute__((ext_vector_type(GPB)));
     words sd[2];
@@ -172,7 +195,7 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
     asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(magic));
     const auto decode = [&](auto j_tag, auto x_tag) {
         constexpr int J = decltype(j_tag)::value, X = decltype(x_tag)::value, ST = X / 4, R = X % 4;
-        w[ST][R] = (int)g4_pair_here<R>((uint32_t)raw[J][ST & 1][ST >> 1], zero[J][ST * GPB / 8], magic, upper[J]);
+        w[ST < 4 ? 4 * J + ST : 4 + ST][R] = (int)g4_pair_here<R>((uint32_t)raw[J][ST & 1][ST >> 1], zero[J][ST * GPB / 8], magic, upper[J]);
     };
     const auto zeros_of = [&](auto j_tag) {
         constexpr int J = decltype(j_tag)::value;
@@ -185,12 +208,21 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
         for (int n = 0; n < GPB; ++n) scale[J][n] = g4_scale(sd[J][n], g.scale_type);
     };
 
+    // ---- steps.  Slot t is product t of the step and what is issued behind it.  What goes where is spread so that a slot has five or six instructions
+    // beside its product, which are what the product's 32 clocks have room for.
+    constexpr int L = 8 / GPB, GROUPS = 2 * RM * GPB, SLOTS = 16 * RM, MID = 8 * RM; // products of a group, groups and slots of a step
+    // half J's codes, in slots from the start of the other half's last chain: operands 0 .. 3, then 4 .. 7
+    constexpr int CODES_FROM = RM == 4 ? -17 : RM == 2 ? -4 : 4, CODES_THEN = RM == 1 ? 8 : 5, CODES_TO = 14;
+    // copies go out from half-time on, evenly, those of half-time's step + 2 ending some slots ahead of the next one; EARLY of the statements behind a step's end
+    constexpr int COPY_SLOTS = RM == 4 ? 44 : RM == 2 ? 20 : MID, EARLY = S::PAIRS * MID / COPY_SLOTS;
+    constexpr int READS = 18; // (RM = 4) slots that operands of half the rows are read in
+
     // ---- prologue
-    static_for<S::COPIES>([&](auto c) { copy(0, c); });
+    static_for<S::PAIRS>([&](auto p) { copy(0, p); });
     copied();
-    static_for<S::COPIES>([&](auto c) { copy(S::BUF, c); });
-    copied();
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::COPIES) : "memory");
+    static_for<EARLY>([&](auto p) { copy(S::BUF, p); });
+    if constexpr (EARLY == S::PAIRS) copied();
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::copies(EARLY)) : "memory");
     static_for<RM>([&](auto i) { static_for<8>([&](auto s) { read_a(0, i, s); }); });
     read_w(0, I0{}), read_w(0, I1{});
     read_s(0, I0{}), read_s(0, I1{});
@@ -208,20 +240,18 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
 #pragma unroll
     for (int n = 0; n < GPB; ++n) scale[0][n] = scale[1][n] = 0;
 
-    // ---- steps.  Slot t is product t of the step and what is issued behind it.
-    constexpr int L = 8 / GPB, GROUPS = 2 * RM * GPB, SLOTS = 16 * RM, MID = 8 * RM; // products of a group, groups and slots of a step
-    constexpr int DECODE_FROM = RM == 1 ? 4 : 1;                                     // (with RM = 1 the codes have just been read)
     const auto fold = [&](auto g_tag, auto from_tag, auto to_tag) { // elements of group G's sum into the accumulators
         constexpr int G = decltype(g_tag)::value, C = G / GPB, I = C % RM, J = C / RM;
 #pragma unroll
         for (int e = from_tag(); e < to_tag(); ++e) g4_add_scaled(acc[I][J][e], sum[G & 1][e], scale[J][G % GPB]);
     };
-    // (half J's codes in the 14 slots from the last chain of the other half on; AT: slots since that began)
     const auto decode_some = [&](auto j_tag, auto at_tag) {
-        constexpr int AT = decltype(at_tag)::value - DECODE_FROM, N = 14 - DECODE_FROM;
-        if constexpr (AT >= 0 && AT < N) {
-            if constexpr (AT == 0) zeros_of(j_tag);
-            constexpr int X0 = 32 * AT / N, X1 = 32 * (AT + 1) / N;
+        constexpr int AT = decltype(at_tag)::value;
+        if constexpr (AT >= CODES_FROM && AT < CODES_TO) {
+            if constexpr (AT == CODES_FROM) zeros_of(j_tag);
+            constexpr bool FIRST = AT < CODES_THEN;
+            constexpr int FROM = FIRST ? CODES_FROM : CODES_THEN, N = (FIRST ? CODES_THEN : CODES_TO) - FROM, O = FIRST ? 0 : 16;
+            constexpr int X0 = O + 16 * (AT - FROM) / N, X1 = O + 16 * (AT + 1 - FROM) / N;
             static_for<X1 - X0>([&](auto x) { decode(j_tag, std::integral_constant<int, X0 + decltype(x)::value>{}); });
         }
     };
@@ -231,26 +261,39 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
         static_for<SLOTS>([&](auto t_tag) {
             constexpr int T = decltype(t_tag)::value, C = T / 8, ST = T % 8, I = C % RM, G = T / L;
             if constexpr (T == MID) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if constexpr (T % L == 0) g4_product_first(a[I][ST], w[ST], sum[G & 1]);
-            else g4_product(a[I][ST], w[ST], sum[G & 1]);
+            constexpr int J = C / RM, W = ST < 4 ? 4 * J + ST : 4 + ST;
+            if constexpr (T % L == 0) g4_product_first(a[I][ST], w[W], sum[G & 1]);
+            else g4_product(a[I][ST], w[W], sum[G & 1]);
             // the sum of a group from two slots behind its last product up to where its registers are wanted again
             constexpr int U = T + SLOTS - L - 1, F = U / L % GROUPS, O = U % L;
             if constexpr (O < L - 1) fold(std::integral_constant<int, F>{}, std::integral_constant<int, 16 * O / (L - 1)>{}, std::integral_constant<int, 16 * (O + 1) / (L - 1)>{});
             if constexpr (T == 0) scale_of(I0{});
             if constexpr (T == 8) scale_of(I1{});
+            // (a step's slots are both the ones from its own start and the last ones from the step before)
             decode_some(I1{}, std::integral_constant<int, T - (MID - 8)>{});
             decode_some(I0{}, std::integral_constant<int, T < 8 ? T + 8 : T - (SLOTS - 8)>{});
-            if constexpr (T >= MID) {
-                constexpr int H = T - MID;
-                if constexpr (H == 0) read_s(next, I0{}), read_w(next, I0{});
-                if constexpr (H == 7) read_s(next, I1{}), read_w(next, I1{});
+            if constexpr (T == MID) read_s(next, I0{}), read_w(next, I0{});
+            if constexpr (T == MID + 7) read_s(next, I1{}), read_w(next, I1{});
+            if constexpr (RM == 4) { // operands of rows 0 and 1 behind the barrier, of 2 and 3 early in the next step
+                constexpr int N0 = T >= MID + 7 ? T - MID - 7 : T >= 7 && T < 7 + READS ? T - 7 : READS, O = T >= MID ? 0 : 16;
+                if constexpr (N0 < READS) {
+                    constexpr int R0 = O + 16 * N0 / READS, R1 = O + 16 * (N0 + 1) / READS;
+                    static_for<R1 - R0>([&](auto r) {
+                        constexpr int R = R0 + decltype(r)::value;
+                        read_a(T >= MID ? next : here, std::integral_constant<int, R / 8>{}, std::integral_constant<int, R % 8>{});
+                    });
+                }
+            } else if constexpr (T >= MID) { // behind their last products
                 read_a(next, std::integral_constant<int, I>{}, std::integral_constant<int, ST>{});
-                constexpr int C0 = S::COPIES * H / MID, C1 = S::COPIES * (H + 1) / MID;
-                static_for<C1 - C0>([&](auto c) { copy(here, std::integral_constant<int, C0 + decltype(c)::value>{}); });
             }
+            constexpr int H = T >= MID ? T - MID : T + MID; // (SLOTS = 2 MID)
+            if constexpr (H < COPY_SLOTS) {
+                constexpr int P0 = S::PAIRS * H / COPY_SLOTS, P1 = S::PAIRS * (H + 1) / COPY_SLOTS;
+                static_for<P1 - P0>([&](auto p) { copy(T >= MID ? here : next, std::integral_constant<int, P0 + decltype(p)::value>{}); });
+            }
+            if constexpr (H == COPY_SLOTS - 1) copied();
             __builtin_amdgcn_sched_barrier(0);
         });
-        copied();
         here = next;
     }
     asm volatile("s_nop 7\n\ts_nop 7" ::: "memory"); // (the last product has to be through)
@@ -259,7 +302,7 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     if (parts > 1) { // partial tile in accumulator order: [tile][part][wave][i][j][quarter of 16][lane]
-        v4f* to = reinterpret_cast<v4f*>(g.scratch) + (((size_t)tile * parts + part) * 4 + wave) * (RM * 2 * 4 * 64) + lane;
+        v4f* to = reinterpret_cast<v4f*>(g.scratch) + (((size_t)tile * parts + part) * S::WAVES + wave) * (RM * 2 * 4 * 64) + lane;
 #pragma unroll
         for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -268,52 +311,50 @@ __global__ __launch_bounds__(256, 1) void g4_tile_kernel(rkh_g4_args g, int mblo
                 for (int e = 0; e < 4; ++e)
                     to[((i * 2 + j) * 4 + e) * 64] = v4f{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
     } else {
-#pragma unroll
-        for (int i = 0; i < RM; ++i) g4_finish<SWIGLU>(g, m0 + (wm * RM + i) * 32, (int64_t)nblk * 2 + wn, acc[i][0], acc[i][1], lane);
+        g4_finish<RM, SWIGLU>(g, m0 + wm * RM * 32, (int64_t)nblk * 2 + wn, acc, lane);
     }
 }
 
 // Sum of the parts of a tile, in their order, and the results.  One wave per 32 rows x 64 places.
-template <int RM, bool SWIGLU>
-__global__ __launch_bounds__(256) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+template <bool SWIGLU>
+__global__ __launch_bounds__(64) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts, int rm, int wm) {
     const int lane = lane_id();
-    const unsigned tile = blockIdx.x / RM, i = blockIdx.x % RM, wave = wave_id();
+    const unsigned per_tile = rm * wm * 2, tile = blockIdx.x / per_tile, in_tile = blockIdx.x % per_tile, wave = in_tile / rm, i = in_tile % rm;
     int mblk, nblk;
     g4_place(tile, mblocks, nblocks, mblk, nblk);
-    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + ((size_t)tile * parts * 4 + wave) * (RM * 2 * 4 * 64) + i * 512 + lane;
-    float s[2][16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0;
+    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + ((size_t)tile * parts * wm * 2 + wave) * (rm * 512) + i * 512 + lane;
+    float s[1][2][16] = {};
     for (int p = 0; p < parts; ++p) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             const v4f v = from[x * 64];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[x >> 2][4 * (x & 3) + e] += v[e];
+            for (int e = 0; e < 4; ++e) s[0][x >> 2][4 * (x & 3) + e] += v[e];
         }
-        from += 4 * RM * 2 * 4 * 64;
+        from += wm * 2 * rm * 512;
     }
-    g4_finish<SWIGLU>(g, (mblk * 2 + (wave & 1)) * RM * 32 + i * 32, (int64_t)nblk * 2 + (wave >> 1), s[0], s[1], lane);
+    g4_finish<1, SWIGLU>(g, ((mblk * wm + (int)wave % wm) * rm + i) * 32, (int64_t)nblk * 2 + wave / wm, s, lane);
 }
 
-template <int RM, int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
-    constexpr int LDS = G4Tile<RM, GPB>::LDS;
+template <int RM, int WM, int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
+    constexpr int LDS = G4Tile<RM, WM, GPB>::LDS;
     static std::atomic<bool> opted_in[64] = {};
-    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_tile_kernel<RM, GPB, SWIGLU>), opted_in, LDS)) return rc;
+    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_tile_kernel<RM, WM, GPB, SWIGLU>), opted_in, LDS)) return rc;
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
-    if (tiles * r.parts * 256 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
+    if (tiles * r.parts * 128 * WM >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
     mark(st, "g4_tile_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_tile_kernel<RM, GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, r.parts);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_tile_kernel<RM, WM, GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(128 * WM), LDS, st, g, r.mblocks, r.nblocks,
+                       r.parts);
     RKH_CHECK(hipGetLastError());
     if (r.parts > 1) {
         mark(st, "g4_join_kernel");
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<RM, SWIGLU>), dim3((unsigned)(tiles * RM)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * WM * 2)), dim3(64), 0, st, g, r.mblocks, r.nblocks, r.parts, RM, WM);
         RKH_CHECK(hipGetLastError());
     }
     return RKH_OK;
 }
 template <int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
-    return r.rm == 4 ? launch_tiles<4, GPB, SWIGLU>(st, g, r) : r.rm == 2 ? launch_tiles<2, GPB, SWIGLU>(st, g, r) : launch_tiles<1, GPB, SWIGLU>(st, g, r);
+    return r.rm == 4 ? launch_tiles<4, 2, GPB, SWIGLU>(st, g, r) : r.rm == 2 ? launch_tiles<2, 2, GPB, SWIGLU>(st, g, r) : launch_tiles<1, 2, GPB, SWIGLU>(st, g, r);
 }
 template <int GPB> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
     return g.swiglu ? launch_tiles<GPB, true>(st, g, r) : launch_tiles<GPB, false>(st, g, r);

@@ -168,6 +168,11 @@ typedef __attribute__((address_space(3))) uint8_t* mx_lds_ptr;
 __device__ __forceinline__ void mx_copy(const uint8_t* base, unsigned off, uint32_t to) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to) : "memory", "m0");
 }
+// ... and another 16 from base2 + off2 + 1024 to `to` + 1024: the instruction's offset counts on both sides.
+__device__ __forceinline__ void mx_copy_two(const uint8_t* base, unsigned off, const uint8_t* base2, unsigned off2, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024" ::"v"(off), "s"(base), "v"(off2),
+                 "s"(base2), "s"(to) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // gate / (1 + exp(-gate)) * up.  exp(x) = 2^(x log2 e): the product's rounded-off part goes in as a factor of its own, so that the
