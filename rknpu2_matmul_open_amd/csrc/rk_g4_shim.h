@@ -10,8 +10,8 @@
  * is an operand of a 16x16x32 product; dword i of the lanes with q = h and q = h + 2 are two consecutive ones of 32x32x16, whose
  * lane (c + 16 b, h) holds 8 k of 32 places.  Codes beyond K and N are zero.
  *
- * Scales: a dword for each place and internal group of 128 / gpb (gpb = 1, 2, 4: groups in a piece) k: [kb][place][gpb], the scale's
- * 16 bits above 0x6400 + zero point (the half 1024 + zero point).  Beyond K and N the scale is zero.
+ * Scales: a dword for each place and internal group of 128 / gpb (gpb = 1, 2, 4: groups in a piece) k, piece by piece as the codes: [pb][kb][c][gpb], the
+ * scale's 16 bits above 0x6400 + zero point (the half 1024 + zero point).  Beyond K and N the scale is zero.
  *
  * Places of columns, in units of 64 (16-place blocks 0..3 of it): place 16 (2 b + j) + c is column 32 b + 2 c + j of the 64, so that lane c
  * + 16 b of two accumulators j of 32 places has two neighbouring columns.  Gate / up matrices: column 16 b + c of 32, j = 0 of the gate and j = 1 of

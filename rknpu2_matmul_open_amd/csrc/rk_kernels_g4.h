@@ -38,27 +38,16 @@ struct G4Zero {
         high = low + v2h{960, 960};
     }
 };
-template <int R> __device__ __forceinline__ uint32_t g4_pair(uint32_t w, const G4Zero& z) { // codes 2 R and 2 R + 1 of a dword
-    if constexpr (R >= 2) w >>= 8;
-    if constexpr (R & 1) {
-        const v2h v = __builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u);
-        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, v2h{0.0625f16, 0.0625f16}, z.high));
-    } else {
-        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) + z.low);
-    }
-}
-__device__ __forceinline__ v8h g4_halves(uint32_t w, const G4Zero& z) {
-    const v4i v = {(int)g4_pair<0>(w, z), (int)g4_pair<1>(w, z), (int)g4_pair<2>(w, z), (int)g4_pair<3>(w, z)};
-    return __builtin_bit_cast(v8h, v);
-}
-
-// Codes as bf16, zero point not taken off: a byte 0..15 is the e4m3 number code * 2^-9, which the conversion scales by 2^9.  7 instructions for eight.
-// The order is k0 k4 k1 k5 k2 k6 k3 k7; g4_turned_rows gives activations the same.
-__device__ __forceinline__ v8b g4_codes_bf16(uint32_t w) {
-    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
-    const v2b a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)even, 512.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)even, 512.0f, true),
-              c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)odd, 512.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)odd, 512.0f, true);
-    return v8b{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+// Codes as halves or bf16, the zero point not taken off: a byte 0..15 is the e4m3 number code * 2^-9, which the conversion scales by 2^9.  7 instructions for
+// eight.  The order is k0 k4 k1 k5 k2 k6 k3 k7; g4_turned_rows gives activations the same.
+template <int TYPE> __device__ __forceinline__ v4i g4_codes(uint32_t w) {
+    const int even = (int)(w & 0x0f0f0f0fu), odd = (int)((w >> 4) & 0x0f0f0f0fu);
+    if constexpr (TYPE == RKH_MX4_F16)
+        return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, true)),
+                   __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, true))};
+    else
+        return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true)),
+                   __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true))};
 }
 __device__ __forceinline__ v4i g4_turned_rows(const v4i& x) {
     return v4i{(int)__builtin_amdgcn_perm((uint32_t)x.z, (uint32_t)x.x, 0x05040100u), (int)__builtin_amdgcn_perm((uint32_t)x.z, (uint32_t)x.x, 0x07060302u),

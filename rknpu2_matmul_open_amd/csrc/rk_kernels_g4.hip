@@ -36,10 +36,9 @@ __global__ __launch_bounds__(256) void g4_pack_kernel(const uint8_t* codes, cons
         dst[i] = w;
     }
     if (i < scale_words) {
-        const int64_t places = rkh_g4_places(N, gate_up);
         const int g = (int)(i % gpb);
-        const size_t at = i / gpb;
-        const int64_t kb = (int64_t)(at / places), place = (int64_t)(at - (size_t)kb * places), n = column(place >> 4, (int)place & 15);
+        const size_t at = i / gpb, piece = at >> 4;
+        const int64_t block = (int64_t)(piece / KB), kb = (int64_t)(piece - (size_t)block * KB), n = column(block, (int)at & 15);
         const int64_t k = kb * 128 + g * (128 / gpb);
         uint32_t d = 0x6400u;
         if (n >= 0 && k < K) {
@@ -109,163 +108,189 @@ __global__ __launch_bounds__(256) void g4_stage_kernel(const uint16_t* x, int64_
 // ---- few rows ------------------------------------------------------------------------
 // One workgroup multiplies up to 16 rows with 16 CN places; its waves split K into pieces of 128 and are summed through LDS.  Codes go straight into
 // registers, once; so do activations, which every workgroup reads for itself.
-// BOUNCE: up to four rows.  A wave loads a row's 512 values together and turns them into operands through LDS of its own; more rows are
+// ROWS (1, 4, 8 or 16): up to so many rows.  A wave loads a row's 512 values together and turns them into operands through LDS of its own.  0: up to 16 rows,
 // loaded as the operands lie.
-// fp16: products with code - zero.  bf16: products with the code, and the zero point times the group's sum of activations, which a product with ones
-// gives, is taken off the sum.
+// LONG: a wave has more pieces than it loads together; the next ones are on their way while it multiplies.
+// Products are with the code; the zero point times the group's sum of activations, which a product with ones gives, is taken off a group's sum.
 constexpr int FEW_PITCH = 1024 + 16; // bytes of a row of 512 values in LDS
 
-template <int TYPE, int CN, int GPB, bool BOUNCE, bool SWIGLU, int NP, int MAX_WAVES>
+template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES>
 __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W, const uint32_t* scales, const uint16_t* x, int64_t ldx, int M, int K,
                                                                 int per_wave, int workgroups, int waves, rkh_g4_args g) {
-    constexpr bool F16 = TYPE == RKH_MX4_F16;
+    constexpr int ONE = TYPE == RKH_MX4_F16 ? 0x3c003c00 : 0x3f803f80; // two of them
     constexpr int STEPS = 4 / GPB; // 32-k steps of a group
-    static_assert(!SWIGLU || CN == 2, "a gate and an up half");
-    static_assert(!BOUNCE || NP % 4 == 0, "rows are loaded 512 values at a time");
+    static_assert(!SWIGLU || CN % 2 == 0, "gate and up halves");
+    static_assert(!ROWS || NP % 4 == 0, "rows are loaded 512 values at a time");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), c = lane & 15, q = lane >> 4;
     const int KB = (int)rkh_g4_kb(K);
-    const int64_t places = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU);
     const int block0 = xcd_remap(blockIdx.x, workgroups) * CN;
     const int first = wave * per_wave, last = min(first + per_wave, KB);
     const int row = min(c, M - 1); // (operand rows beyond M: the last one again, whose results nobody takes)
     typedef uint32_t words __attribute__((ext_vector_type(GPB)));
 
-    const auto fetch = [&](int m, int k) -> v4i { // (K is a multiple of eight)
-        const v4i v = mx_fetch8<TYPE>(x, (size_t)m * ldx + (k < K ? k : 0)).w[0];
-        return k < K ? v : v4i{0, 0, 0, 0};
+    struct Batch {
+        v4i w[NP][CN], x[ROWS ? ROWS * NP / 4 : NP * 4];
+        words s[NP][CN];
     };
-    v4f acc[CN];
+    // (K is a multiple of eight; what lies beyond it is loaded from a row's start and dropped where it is used: a branch here would wait for
+    // the activations ahead of the codes' loads)
+    const auto fetch = [&](int m, int k) { return mx_fetch8<TYPE>(x, (size_t)m * ldx + (k < K ? k : 0)).w[0]; };
+    const auto within = [&](const v4i& v, int k) { return k < K ? g4_turned_rows(v) : v4i{0, 0, 0, 0}; };
+    const auto load = [&](Batch& b, int from) { // (pieces beyond the last: that one again, which is not multiplied)
+        if constexpr (ROWS) {
 #pragma unroll
-    for (int j = 0; j < CN; ++j) acc[j] = v4f{0, 0, 0, 0};
-    uint8_t* own = lds + wave * (4 * FEW_PITCH);
-
-    for (int from = first; from < last; from += NP) {
-        v4i w[NP][CN], rows[BOUNCE ? NP : NP * 4]; // BOUNCE: [512 values][row]
-        words sd[NP][CN];
-        // everything that the pieces need (of pieces beyond the last: that one again, which is not multiplied)
+            for (int m = 0; m < ROWS * NP / 4; ++m) b.x[m] = fetch(min(m % ROWS, M - 1), (from + m / ROWS * 4) * 128 + lane * 8);
+        } else {
 #pragma unroll
-        for (int i = 0; i < (BOUNCE ? NP : NP * 4); ++i) {
-            if constexpr (!BOUNCE) rows[i] = fetch(row, from * 128 + i * 32 + q * 8);
-            else if ((i & 3) < M) rows[i] = fetch(i & 3, (from + (i & ~3)) * 128 + lane * 8);
+            for (int i = 0; i < NP * 4; ++i) b.x[i] = fetch(row, from * 128 + i * 32 + q * 8);
         }
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             const int kb = min(from + p, KB - 1);
 #pragma unroll
             for (int j = 0; j < CN; ++j) {
-                w[p][j] = *reinterpret_cast<const v4i*>(W + ((size_t)(block0 + j) * KB + kb) * 1024 + lane * 16);
-                sd[p][j] = *reinterpret_cast<const words*>(scales + ((size_t)kb * places + (block0 + j) * 16 + c) * GPB);
+                b.w[p][j] = *reinterpret_cast<const v4i*>(W + ((size_t)(block0 + j) * KB + kb) * 1024 + lane * 16);
+                b.s[p][j] = *reinterpret_cast<const words*>(scales + (((size_t)(block0 + j) * KB + kb) * 16 + c) * GPB);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto product = [](const v4i& rows, const v4i& codes, const v4f& sum) {
+        if constexpr (TYPE == RKH_MX4_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, rows), __builtin_bit_cast(v8h, codes), sum, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, rows), __builtin_bit_cast(v8b, codes), sum, 0, 0, 0);
+    };
+    v4f acc[CN];
+#pragma unroll
+    for (int j = 0; j < CN; ++j) acc[j] = v4f{0, 0, 0, 0};
+    uint8_t* own = lds + wave * (ROWS * FEW_PITCH);
+    const auto multiply = [&](const Batch& b, int from) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
             if (from + p >= last) break;
-            if constexpr (BOUNCE) {
+            if constexpr (ROWS) {
                 if (p % 4 == 0) {
                     __builtin_amdgcn_wave_barrier(); // (a wave's LDS operations complete in order)
 #pragma unroll
-                    for (int m = 0; m < 4; ++m)
-                        if (m < M) *reinterpret_cast<v4i*>(own + m * FEW_PITCH + lane * 16) = F16 ? rows[p + m] : g4_turned_rows(rows[p + m]);
+                    for (int m = 0; m < ROWS; ++m)
+                        *reinterpret_cast<v4i*>(own + m * FEW_PITCH + lane * 16) = within(b.x[p / 4 * ROWS + m], (from + p) * 128 + lane * 8);
                     __builtin_amdgcn_wave_barrier();
                 }
             }
             v4i a[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if constexpr (BOUNCE) a[i] = *reinterpret_cast<const v4i*>(own + row * FEW_PITCH + (p & 3) * 256 + i * 64 + q * 16);
-                else a[i] = F16 ? rows[p * 4 + i] : g4_turned_rows(rows[p * 4 + i]);
+                if constexpr (ROWS) a[i] = *reinterpret_cast<const v4i*>(own + row * FEW_PITCH + (p & 3) * 256 + i * 64 + q * 16);
+                else a[i] = within(b.x[p * 4 + i], (from + p) * 128 + i * 32 + q * 8);
             }
 #pragma unroll
             for (int n = 0; n < GPB; ++n) {
-                if constexpr (F16) {
+                v4f sum = {0, 0, 0, 0};
 #pragma unroll
-                    for (int j = 0; j < CN; ++j) {
-                        G4Zero z;
-                        z.of(sd[p][j][n]);
-                        v4f part = {0, 0, 0, 0};
+                for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) sum = product(a[i], v4i{ONE, ONE, ONE, ONE}, sum);
 #pragma unroll
-                        for (int i = n * STEPS; i < (n + 1) * STEPS; ++i)
-                            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a[i]), g4_halves((uint32_t)w[p][j][i], z), part, 0, 0, 0);
-                        const float s = g4_scale(sd[p][j][n], g.scale_type);
+                for (int j = 0; j < CN; ++j) {
+                    v4f part = {0, 0, 0, 0};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(part[e], s, acc[j][e]);
-                    }
-                } else {
-                    constexpr int ONES = 0x3f803f80;
-                    const v8b ones = __builtin_bit_cast(v8b, (v4i{ONES, ONES, ONES, ONES}));
-                    v4f sum = {0, 0, 0, 0};
+                    for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) part = product(a[i], g4_codes<TYPE>((uint32_t)b.w[p][j][i]), part);
+                    const float s = g4_scale(b.s[p][j][n], g.scale_type), zero = (float)(b.s[p][j][n] & 0xffu);
 #pragma unroll
-                    for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a[i]), ones, sum, 0, 0, 0);
-#pragma unroll
-                    for (int j = 0; j < CN; ++j) {
-                        v4f part = {0, 0, 0, 0};
-#pragma unroll
-                        for (int i = n * STEPS; i < (n + 1) * STEPS; ++i)
-                            part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a[i]), g4_codes_bf16((uint32_t)w[p][j][i]), part, 0, 0, 0);
-                        const float s = g4_scale(sd[p][j][n], g.scale_type), zero = (float)(sd[p][j][n] & 0xffu);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(fmaf(-zero, sum[e], part[e]), s, acc[j][e]);
-                    }
+                    for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(fmaf(-zero, sum[e], part[e]), s, acc[j][e]);
                 }
             }
         }
+    };
+    Batch now;
+    load(now, first);
+    if constexpr (!LONG) {
+        multiply(now, first);
+    } else {
+        for (int from = first;;) {
+            Batch next;
+            if (from + NP < last) load(next, from + NP);
+            multiply(now, from);
+            if ((from += NP) >= last) break;
+            now = next;
+        }
     }
 
-    // the waves' sums, added in order
-    v4f* sums = reinterpret_cast<v4f*>(lds + (BOUNCE ? waves * 4 * FEW_PITCH : 0));
+    // the waves' sums, added in order: a thread takes one result (SwiGLU: both halves of one)
+    float* sums = reinterpret_cast<float*>(lds + waves * ROWS * FEW_PITCH);
 #pragma unroll
-    for (int j = 0; j < CN; ++j) sums[(wave * CN + j) * 64 + lane] = acc[j];
+    for (int j = 0; j < CN; ++j) *reinterpret_cast<v4f*>(sums + (wave * CN + j) * 256 + lane * 4) = acc[j];
     __syncthreads();
-    if (wave != 0) return;
-    v4f s[CN];
-#pragma unroll
-    for (int j = 0; j < CN; ++j) {
-        s[j] = sums[j * 64 + lane];
-        for (int o = 1; o < waves; ++o) s[j] += sums[(o * CN + j) * 64 + lane];
-    }
-    const int64_t n = g4_column(block0, c, SWIGLU);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int m = 4 * q + e;
-        if (m >= M) break;
-        float v[CN];
-#pragma unroll
-        for (int j = 0; j < CN; ++j) v[j] = g.exponents ? __builtin_amdgcn_ldexpf(s[j][e], g.exponents[m]) : s[j][e];
-        if constexpr (SWIGLU) {
-            const float y[1] = {mx_silu(v[0], v[1])};
-            g4_put<1>(g, m, n, y);
-        } else {
-            g4_put<CN>(g, m, n, v);
-        }
+    const auto total = [&](int i) {
+        float s = sums[i];
+#pragma unroll 4
+        for (int o = 1; o < waves; ++o) s += sums[o * CN * 256 + i];
+        return s;
+    };
+    for (int i = threadIdx.x; i < (SWIGLU ? CN / 2 : CN) * 256; i += waves * 64) {
+        const int m = (i >> 6 & 3) * 4 + (i & 3), at = SWIGLU ? (i >> 8) * 512 + (i & 255) : i;
+        if (m >= M) continue;
+        const int ex = g.exponents ? g.exponents[m] : 0;
+        const float a = __builtin_amdgcn_ldexpf(total(at), ex);
+        const float v[1] = {SWIGLU ? mx_silu(a, __builtin_amdgcn_ldexpf(total(at + 256), ex)) : a};
+        g4_put<1>(g, m, g4_column(block0 + (at >> 8), i >> 2 & 15, SWIGLU), v);
     }
 }
 
 constexpr int FEW_ROWS = 16;
 
-template <int TYPE, int CN, int GPB, bool BOUNCE, bool SWIGLU, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
+// What a workgroup of the few-row kernel takes.  Where both sides were measured (bf16, one scale in 128, weights from HBM, us):
+//   rows at a time as they are in LDS, or as operands (ROWS 0): 8 x 4096 x 4096 4.4 and 6.6, 16 x 4096 x 4096 5.1 and 6.7;
+//   columns: activations are read by every workgroup, so more rows want more columns, where enough workgroups are left.  1 x 14336 x 4096 16 columns 7.9, 32
+//   8.1, 64 9.1; 4 rows of it 9.0, 8.3, 9.4; 8 rows 10.3, 10.6, 9.8 and, as operands, 64 columns 9.2; 16 rows 17.2, 12.4 and, as operands, 10.0;
+//   4 x 4096 x 4096 16 columns 4.4, 32 4.7;
+//   K in parts, which takes a second launch: 8 x 4096 x 14336 11.2 -> 12.4 at best, 16 rows of it 15.2 -> 13.4.
+struct FewShape {
+    int rows, cn, most; // LDS rows of a wave (0: none), blocks of 16 places, most waves
+};
+// (more than eight waves leave 128 registers for a lane, which is too few for two blocks or many groups and rows at once)
+FewShape few_shape(int M, int64_t blocks, int KB, int gpb, bool swiglu) {
+    if (KB <= 32 && ((M > 8 && blocks >= 512) || (M > 4 && blocks >= 768))) return {0, 4, 16};
+    const int rows = M == 1 ? 1 : M <= 4 ? 4 : M <= 8 ? 8 : 16;
+    const bool two = swiglu || (rows == 4 && blocks >= 768 && KB <= 32);
+    return {rows, two ? 2 : 1, two || rows == 16 || (rows == 8 && gpb == 4) ? 8 : 16};
+}
+
+template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
     const int KB = (int)rkh_g4_kb(g.K), waves = (KB + per - 1) / per;
     const int64_t workgroups = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / (16 * CN);
     if (workgroups * waves * 64 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
-    const size_t bytes = (size_t)waves * (CN * 1024 + (BOUNCE ? 4 * FEW_PITCH : 0));
-    const auto kernel = g4_few_kernel<TYPE, CN, GPB, BOUNCE, SWIGLU, NP, MAX_WAVES>;
+    constexpr size_t BYTES = CN * 1024 + ROWS * FEW_PITCH; // of a wave
+    static_assert(MAX_WAVES * BYTES <= 160 * 1024, "");
+    const auto kernel = g4_few_kernel<TYPE, CN, GPB, ROWS, SWIGLU, LONG, NP, MAX_WAVES>;
     static std::atomic<bool> opted_in[64] = {};
     if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(kernel), opted_in, 160 * 1024)) return rc;
     mark(st, "g4_few_kernel");
-    hipLaunchKernelGGL(kernel, dim3((unsigned)workgroups), dim3(waves * 64), bytes, st, g.W, g.w_scale, static_cast<const uint16_t*>(g.x), g.ldx, g.M, g.K, per,
-                       (int)workgroups, waves, g);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)workgroups), dim3(waves * 64), waves * BYTES, st, g.W, g.w_scale, static_cast<const uint16_t*>(g.x), g.ldx, g.M, g.K,
+                       per, (int)workgroups, waves, g);
     RKH_CHECK(hipGetLastError());
     return RKH_OK;
 }
-template <int TYPE, int GPB> int launch_few(hipStream_t st, const rkh_g4_args& g) {
+template <int TYPE, int GPB, bool SWIGLU> int launch_few(hipStream_t st, const rkh_g4_args& g) {
     const int KB = (int)rkh_g4_kb(g.K);
-    const auto per = [&](int waves, int np) { return std::max((KB + waves - 1) / waves, std::min(np, (KB + 3) / 4)); }; // pieces of a wave
-    if (g.swiglu) return g.M <= 4 ? launch_few<TYPE, 2, GPB, true, true, 4, 8>(st, g, per(8, 4)) : launch_few<TYPE, 2, GPB, false, true, 2, 8>(st, g, per(8, 4));
-    return g.M <= 4 ? launch_few<TYPE, 1, GPB, true, false, 4, 16>(st, g, per(16, 4)) : launch_few<TYPE, 1, GPB, false, false, 2, 16>(st, g, per(16, 4));
+    const FewShape shape = few_shape(g.M, rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / 16, KB, GPB, SWIGLU);
+    // pieces of a wave: up to four (as operands: two) that are loaded together, eight waves where they go round, and as many as there are waves for
+    const int np = shape.rows ? 4 : 2, per = std::max((KB + shape.most - 1) / shape.most, std::min(np, (KB + 7) / 8));
+    if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, false, 2, 16>(st, g, per);
+    const auto go = [&](auto is_long) {
+        constexpr bool LONG = decltype(is_long)::value;
+        constexpr int CN = SWIGLU ? 2 : 1, MOST = SWIGLU ? 8 : 16;
+        if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, LONG, 4, MOST>(st, g, per);
+        if constexpr (!SWIGLU && !LONG) {
+            if (shape.cn == 2) return launch_few<TYPE, 2, GPB, 4, SWIGLU, LONG, 4, 8>(st, g, per);
+        }
+        if (shape.rows == 4) return launch_few<TYPE, CN, GPB, 4, SWIGLU, LONG, 4, MOST>(st, g, per);
+        if (shape.rows == 8) return launch_few<TYPE, CN, GPB, 8, SWIGLU, LONG, 4, GPB == 4 ? 8 : MOST>(st, g, per);
+        return launch_few<TYPE, CN, GPB, 16, SWIGLU, LONG, 4, 8>(st, g, per);
+    };
+    return per > 4 ? go(std::true_type{}) : go(std::false_type{});
 }
 template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
-    return g.gpb == 1 ? launch_few<TYPE, 1>(st, g) : g.gpb == 2 ? launch_few<TYPE, 2>(st, g) : launch_few<TYPE, 4>(st, g);
+    if (g.swiglu) return g.gpb == 1 ? launch_few<TYPE, 1, true>(st, g) : g.gpb == 2 ? launch_few<TYPE, 2, true>(st, g) : launch_few<TYPE, 4, true>(st, g);
+    return g.gpb == 1 ? launch_few<TYPE, 1, false>(st, g) : g.gpb == 2 ? launch_few<TYPE, 2, false>(st, g) : launch_few<TYPE, 4, false>(st, g);
 }
 
 // ---- which kernel ------------------------------------------------------------------
@@ -349,7 +374,8 @@ int rkh_g4_run(void* stream, const rkh_g4_args* args) {
 }
 void rkh_g4_route(int M, int N, int K, int gpb, int swiglu, int* kernel, int* rows, int* columns, int* parts) {
     if (M <= FEW_ROWS) {
-        *kernel = 0, *rows = 16, *columns = swiglu ? 32 : 16, *parts = 1;
+        *kernel = 0, *rows = 16, *parts = 1;
+        *columns = 16 * few_shape(M, rkh_g4_places(swiglu ? 2 * (int64_t)N : N, swiglu) / 16, (int)rkh_g4_kb(K), gpb, swiglu).cn;
         return;
     }
     const rkk::G4Route r = g4_route(M, N, K, gpb, swiglu);

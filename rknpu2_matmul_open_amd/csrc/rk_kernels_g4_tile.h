@@ -134,11 +134,10 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
     const uint8_t* w_src[S::WC];
 #pragma unroll
     for (int i = 0; i < S::WC; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * S::WC + i, places / 16 - 1) * KB + kb0) * 1024 - i * 1024;
-    // (waves copy the same scales, or the same half of them, to one place)
-    const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_place = s_lane % (512 * GPB) / (4 * GPB);
-    const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)kb0 * places + (size_t)nblk * 128) * GPB * 4;
-    const unsigned s_off = (unsigned)min((int64_t)s_place, places - (int64_t)nblk * 128 - (GPB == 1 ? 4 : GPB == 2 ? 2 : 1)) * (4 * GPB);
-    const size_t s_step = (size_t)places * GPB * 4;
+    // (waves copy the same scales, or the same half of them, to one place: of each block of 16 places a piece of 64 GPB bytes)
+    const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_at_tile = s_lane % (512 * GPB);
+    const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)nblk * 8 * KB + kb0) * (64 * GPB);
+    const unsigned s_off = (unsigned)min((int64_t)(s_at_tile / (64 * GPB)), places / 16 - 1 - (int64_t)nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
     int ahead = kb1 - kb0; // steps that are still to be copied
     const auto copy = [&](uint32_t to, auto p_tag) {
         constexpr int P = decltype(p_tag)::value;
@@ -158,7 +157,7 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
             x_src += 256;
 #pragma unroll
             for (int i = 0; i < S::WC; ++i) w_src[i] += 1024;
-            s_src += s_step;
+            s_src += 64 * GPB;
         }
     };
 
@@ -167,7 +166,7 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
 #pragma unroll
     for (int s = 0; s < 4; ++s) a_at[s] = (wm * RM * 32 + (lane & 31)) * 128 + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16);
     const uint32_t w_at = S::W_OFF + wn * 4096 + (lane >> 4 & 1) * 2048 + (lane & 15) * 16 + (lane >> 5) * 256;
-    const uint32_t s_at = S::S_OFF + (wn * 64 + (lane >> 4 & 1) * 32 + (lane & 15)) * GPB * 4;
+    const uint32_t s_at = S::S_OFF + (wn * 64 + (lane >> 4 & 1) * 32 + (lane & 15)) * GPB * 4; // [block][c][gpb], as copied
     v4i a[RM][8], w[12]; // (of half 0: 0 .. 3 and 8 .. 11, of half 1: 4 .. 11)
     v4i raw[2][2];
     typedef uint32_t words __attribute__((ext_vector_type(GPB)));
