@@ -67,44 +67,38 @@ __device__ __forceinline__ void g4_place(unsigned tile, unsigned mblocks, unsign
     nblk = __builtin_amdgcn_readfirstlane((int)col);
 }
 
-// Two accumulators of 32 x 32 of rows m0 .. m0 + 31 and the 64 places from `unit` on to results.
-template <int OUT, bool SWIGLU, bool EXPONENTS>
-__device__ __forceinline__ void g4_finish_as(const rkh_g4_args& g, int m0, int64_t unit, const float (&s0)[16], const float (&s1)[16], int lane) {
+// Four rows from `first` on of a lane's two columns (SwiGLU: of both halves of one) from accumulators of 32 x 32 to results; n: the first column.
+template <int OUT, bool SWIGLU, bool EXPONENTS> __device__ __forceinline__ void g4_finish4(const rkh_g4_args& g, int first, int64_t n, const float* s0, const float* s1) {
     using T = typename MxType<OUT>::T;
     typedef T pair __attribute__((ext_vector_type(2)));
     typedef pair pair_any __attribute__((aligned(sizeof(T))));
-    const int64_t n = SWIGLU ? unit * 32 + (lane & 31) : unit * 64 + 2 * (lane & 31);
-    const int first = m0 + 4 * (lane >> 5), live = n < g.N ? g.M - first : 0;
     T* to = static_cast<T*>(g.C) + (size_t)first * g.ldc + n;
+    const int live = n < g.N ? g.M - first : 0;
     const bool both = n + 1 < g.N;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int r = 8 * (e >> 2) + (e & 3);
-        if (r < live) {
+    for (int e = 0; e < 4; ++e) {
+        if (e < live) {
             float a = s0[e], b = s1[e];
             if constexpr (EXPONENTS) {
-                const int ex = g.exponents[first + r];
+                const int ex = g.exponents[first + e];
                 a = __builtin_amdgcn_ldexpf(a, ex), b = __builtin_amdgcn_ldexpf(b, ex);
             }
             if constexpr (SWIGLU) *to = (T)mx_silu(a, b);
             else if (both) *reinterpret_cast<pair_any*>(to) = pair{(T)a, (T)b};
             else *to = (T)a;
         }
-        to += (e & 3) == 3 ? 5 * g.ldc : g.ldc;
+        to += g.ldc;
     }
 }
-template <int RM, bool SWIGLU> __device__ __forceinline__ void g4_finish(const rkh_g4_args& g, int m0, int64_t unit, const float (&s)[RM][2][16], int lane) {
+template <bool SWIGLU, class F> __device__ __forceinline__ void g4_with_finish(const rkh_g4_args& g, F&& f) {
     mx_with_type(g.out_type, [&](auto t) {
         constexpr int OUT = decltype(t)::value;
-        if (g.exponents) {
-#pragma unroll
-            for (int i = 0; i < RM; ++i) g4_finish_as<OUT, SWIGLU, true>(g, m0 + i * 32, unit, s[i][0], s[i][1], lane);
-        } else {
-#pragma unroll
-            for (int i = 0; i < RM; ++i) g4_finish_as<OUT, SWIGLU, false>(g, m0 + i * 32, unit, s[i][0], s[i][1], lane);
-        }
+        if (g.exponents) f([&](int first, int64_t n, const float* s0, const float* s1) { g4_finish4<OUT, SWIGLU, true>(g, first, n, s0, s1); });
+        else f([&](int first, int64_t n, const float* s0, const float* s1) { g4_finish4<OUT, SWIGLU, false>(g, first, n, s0, s1); });
     });
 }
+// A lane's first column of the 64 places from `unit` on.
+template <bool SWIGLU> __device__ __forceinline__ int64_t g4_lane_column(int64_t unit, int lane) { return SWIGLU ? unit * 32 + (lane & 31) : unit * 64 + 2 * (lane & 31); }
 
 template <int RM, int WM, int GPB, bool SWIGLU>
 __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
@@ -310,29 +304,31 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
                 for (int e = 0; e < 4; ++e)
                     to[((i * 2 + j) * 4 + e) * 64] = v4f{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
     } else {
-        g4_finish<RM, SWIGLU>(g, m0 + wm * RM * 32, (int64_t)nblk * 2 + wn, acc, lane);
+        const int64_t n = g4_lane_column<SWIGLU>((int64_t)nblk * 2 + wn, lane);
+        g4_with_finish<SWIGLU>(g, [&](auto&& finish4) {
+#pragma unroll
+            for (int i = 0; i < RM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) finish4(m0 + (wm * RM + i) * 32 + 8 * e + 4 * (lane >> 5), n, &acc[i][0][4 * e], &acc[i][1][4 * e]);
+        });
     }
 }
 
-// Sum of the parts of a tile, in their order, and the results.  One wave per 32 rows x 64 places.
+// Sum of the parts of a tile, in their order, and the results.  One wave per quarter of 32 rows x 64 places.
 template <bool SWIGLU>
-__global__ __launch_bounds__(64) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts, int rm, int wm) {
-    const int lane = lane_id();
+__global__ __launch_bounds__(256) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts, int rm, int wm) {
+    const int lane = lane_id(), e = wave_id();
     const unsigned per_tile = rm * wm * 2, tile = blockIdx.x / per_tile, in_tile = blockIdx.x % per_tile, wave = in_tile / rm, i = in_tile % rm;
     int mblk, nblk;
     g4_place(tile, mblocks, nblocks, mblk, nblk);
-    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + ((size_t)tile * parts * wm * 2 + wave) * (rm * 512) + i * 512 + lane;
-    float s[1][2][16] = {};
-    for (int p = 0; p < parts; ++p) {
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            const v4f v = from[x * 64];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[0][x >> 2][4 * (x & 3) + e] += v[e];
-        }
-        from += wm * 2 * rm * 512;
-    }
-    g4_finish<1, SWIGLU>(g, ((mblk * wm + (int)wave % wm) * rm + i) * 32, (int64_t)nblk * 2 + wave / wm, s, lane);
+    const size_t step = (size_t)wm * 2 * rm * 512;
+    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + tile * parts * step + (wave * rm + i) * 512 + e * 64 + lane;
+    v4f s0 = from[0], s1 = from[256];
+#pragma unroll 4
+    for (int p = 1; p < parts; ++p) s0 += from[p * step], s1 += from[p * step + 256];
+    const float a[4] = {s0.x, s0.y, s0.z, s0.w}, b[4] = {s1.x, s1.y, s1.z, s1.w};
+    const int64_t n = g4_lane_column<SWIGLU>((int64_t)nblk * 2 + wave / wm, lane);
+    g4_with_finish<SWIGLU>(g, [&](auto&& finish4) { finish4(((mblk * wm + (int)(wave % wm)) * rm + i) * 32 + 8 * e + 4 * (lane >> 5), n, a, b); });
 }
 
 template <int RM, int WM, int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
@@ -347,7 +343,7 @@ template <int RM, int WM, int GPB, bool SWIGLU> int launch_tiles(hipStream_t st,
     RKH_CHECK(hipGetLastError());
     if (r.parts > 1) {
         mark(st, "g4_join_kernel");
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * WM * 2)), dim3(64), 0, st, g, r.mblocks, r.nblocks, r.parts, RM, WM);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * WM * 2)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts, RM, WM);
         RKH_CHECK(hipGetLastError());
     }
     return RKH_OK;
