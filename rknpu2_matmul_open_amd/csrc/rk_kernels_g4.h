@@ -13,7 +13,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 namespace rkk {
 // rk_kernels_g4_tile*.hip, by internal groups in a piece (compiling all of them in one unit takes minutes)
-struct G4Route { // of tiles
+struct G4Route { // tiles of 32 rm rows x 128 places
     int rm, parts, mblocks, nblocks;
 };
 int launch_g4_tiles1(hipStream_t st, const rkh_g4_args& g, const G4Route& r);

@@ -295,34 +295,41 @@ template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
 
 // ---- which kernel ------------------------------------------------------------------
 constexpr int G4_CUS = 256; // compute units that a launch is cut for
-// Tiles of 64 rm rows x 128 places: what a step of 128 k takes in each, us
-struct G4Shape { int rm; float step, end; };
-constexpr G4Shape G4_SHAPES[] = {{4, 1.3f, 3.0f}, {2, 0.8f, 2.0f}, {1, 0.5f, 1.5f}};
-constexpr float G4_TILES_US = 3.0f, G4_JOIN_US = 3.0f, G4_JOIN_RATE = 4.5e6f;
+
+// Tiles of 32 rm rows x 128 places: what a step of 128 k takes when every compute unit has one, what a launch has beside its steps, and what another round has, us;
+// how many share a compute unit.  From 64 x 14336 x 4096 (32 rows: 17.3), 512 x 4096 x 4096 (64: 26.7; 128 in two parts: 28.7), 512 x 14336 x 4096 (256: 61) and
+// their like with K = 14336.
+struct G4Shape { int rm; float step, launch, round; int share; };
+constexpr G4Shape G4_SHAPES[] = {{8, 1.75f, 5.0f, 4.0f, 1}, {4, 1.1f, 5.0f, 2.0f, 1}, {2, 0.7f, 4.3f, 0.5f, 2}, {1, 0.4f, 4.3f, 0.5f, 2}};
+constexpr float G4_JOIN_US = 3.5f, G4_JOIN_RATE = 1.2e7f; // a launch that adds parts, and its bytes per us
 constexpr int G4_MOST_PARTS = 16;
 
-rkk::G4Route g4_route(int M, int N, int K, int gpb, int swiglu) {
-    (void)gpb;
+// The tiles that are expected to take the least time.  Where both sides of a choice were measured, us: 64 x 4096 x 4096 32 rows in four parts 11.6, 64 rows in
+// eight 13.5, 32 rows in one 16.3; 128 x 11008 x 4096 64 rows 22.3, 128 rows in two parts 24.8; 256 x 4096 x 4096 64 rows in two parts 20.9, in one 22.8, 128 rows
+// 29.8; 512 x 4096 x 4096 64 rows 26.7, 128 rows in two parts 28.7, 256 rows 48; 512 x 14336 x 4096 256 rows 61, 64 rows 72; 4096 x 14336 x 4096 442 and 518.
+rkk::G4Route g4_route(int M, int N, int K, int swiglu) {
     const int64_t places = rkh_g4_places(swiglu ? 2 * (int64_t)N : N, swiglu), KB = rkh_g4_kb(K);
     rkk::G4Route best{};
     float least = FLT_MAX;
     for (const G4Shape& s : G4_SHAPES) {
-        if (s.rm > 1 && M <= 32 * s.rm) continue; // (half of the rows would be none)
+        if (s.rm > 1 && M <= 16 * s.rm) continue; // (half of the rows would be none)
         rkk::G4Route r{};
         r.rm = s.rm, r.parts = 1;
-        r.mblocks = (M + 64 * s.rm - 1) / (64 * s.rm);
+        r.mblocks = (M + 32 * s.rm - 1) / (32 * s.rm);
         r.nblocks = (int)((places + 127) / 128);
         const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
-        float us = G4_TILES_US + (tiles + G4_CUS - 1) / G4_CUS * (KB * s.step + s.end);
+        // (tiles that share a compute unit fill the last round, those that do not wait for it)
+        const float rounds = s.share > 1 ? std::max(1.0f, (float)tiles / G4_CUS) : (float)((tiles + G4_CUS - 1) / G4_CUS);
+        float us = s.launch + rounds * KB * s.step + (rounds - 1) * s.round;
         if (us < least) least = us, best = r;
         for (int64_t parts = 2; parts <= KB / 2 && parts <= G4_MOST_PARTS && tiles * parts <= G4_CUS; ++parts) {
-            us = G4_TILES_US + (KB + parts - 1) / parts * s.step + s.end + G4_JOIN_US + (float)M * places * 8 * parts / G4_JOIN_RATE;
+            us = s.launch + (KB + parts - 1) / parts * s.step + G4_JOIN_US + (float)M * places * 8 * parts / G4_JOIN_RATE;
             if (us < least) least = us, best = r, best.parts = (int)parts;
         }
     }
     return best;
 }
-size_t g4_scratch(const rkk::G4Route& r) { return r.parts == 1 ? 0 : (size_t)r.mblocks * r.nblocks * r.parts * r.rm * 64 * 128 * 4; }
+size_t g4_scratch(const rkk::G4Route& r) { return r.parts == 1 ? 0 : (size_t)r.mblocks * r.nblocks * r.parts * r.rm * 32 * 128 * 4; }
 
 } // namespace
 
@@ -368,7 +375,7 @@ int rkh_g4_run(void* stream, const rkh_g4_args* args) {
         if (few) g.K = (int)g.ldx; // (zeros there, in the rows as in the codes)
     }
     if (few) return g.x_type == RKH_MX4_F16 ? launch_few<RKH_MX4_F16>(st, g) : launch_few<RKH_MX4_BF16>(st, g);
-    rkk::G4Route r = g4_route(g.M, g.N, g.K, g.gpb, g.swiglu);
+    rkk::G4Route r = g4_route(g.M, g.N, g.K, g.swiglu);
     if (g4_scratch(r) > (g.scratch ? g.scratch_bytes : 0)) r.parts = 1;
     return g.gpb == 1 ? rkk::launch_g4_tiles1(st, g, r) : g.gpb == 2 ? rkk::launch_g4_tiles2(st, g, r) : rkk::launch_g4_tiles4(st, g, r);
 }
@@ -378,13 +385,13 @@ void rkh_g4_route(int M, int N, int K, int gpb, int swiglu, int* kernel, int* ro
         *columns = 16 * few_shape(M, rkh_g4_places(swiglu ? 2 * (int64_t)N : N, swiglu) / 16, (int)rkh_g4_kb(K), gpb, swiglu).cn;
         return;
     }
-    const rkk::G4Route r = g4_route(M, N, K, gpb, swiglu);
-    *kernel = 1, *rows = 64 * r.rm, *columns = 128, *parts = r.parts;
+    const rkk::G4Route r = g4_route(M, N, K, swiglu);
+    *kernel = 1, *rows = 32 * r.rm, *columns = 128, *parts = r.parts;
 }
-size_t rkh_g4_scratch_bytes(int M, int N, int K, int gpb, int swiglu) { return M <= FEW_ROWS ? 0 : g4_scratch(g4_route(M, N, K, gpb, swiglu)); }
+size_t rkh_g4_scratch_bytes(int M, int N, int K, int swiglu) { return M <= FEW_ROWS ? 0 : g4_scratch(g4_route(M, N, K, swiglu)); }
 // (g4_route: a part for each compute unit at most, tiles no larger than the rows ask for)
 size_t rkh_g4_scratch_most(int max_rows, int K) {
-    return max_rows > FEW_ROWS && rkh_g4_kb(K) >= 4 ? (size_t)G4_CUS * 64 * 128 * 4 * (max_rows > 128 ? 4 : max_rows > 64 ? 2 : 1) : 0;
+    return max_rows > FEW_ROWS && rkh_g4_kb(K) >= 4 ? (size_t)G4_CUS * 32 * 128 * 4 * (max_rows > 128 ? 8 : max_rows > 64 ? 4 : max_rows > 32 ? 2 : 1) : 0;
 }
 
 } // extern "C"

@@ -1,5 +1,6 @@
-// Tiles of G4 products: 32 RM WM rows x 128 places by 2 WM waves (WM by two), each RM x 2 accumulators of 32 x 32.  Bound by the matrix pipes and what
-// has to be issued beside them.
+// Tiles of G4 products.
+//
+// Many rows: 256 rows x 128 places by four waves (two by two), each 4 x 2 accumulators of 32 x 32.  Bound by power, and by what one wave has to issue.
 //
 // A step is 128 k.  Its activations (rows of 256 bytes), codes and scales are copied global -> LDS directly, two steps ahead of the products and one
 // ahead of the LDS reads:
@@ -11,8 +12,8 @@
 // In half-time of step s (between the halves) a wave waits for its copies of step s + 1 and for its LDS reads, and meets the others: from
 // there on LDS holds step s + 1 for all, and nobody reads step s any more, whose place the copies of step s + 2 take.
 //
-// Places in LDS: a row's 128 bytes of 64 k are eight pieces of 16 bytes, of which piece c lies at place c ^ (row & 7); eight lanes then read
-// eight rows without a conflict, and a copy still fetches whole 128-byte lines.
+// Places in LDS: a row's 128 bytes of 64 k are eight pieces of 16 bytes, of which piece c lies at place c ^ (row / 2 & 7); sixteen lanes then read
+// sixteen rows from all 64 banks, and a copy still fetches whole 128-byte lines.
 #ifndef RK_KERNELS_G4_TILE_H
 #define RK_KERNELS_G4_TILE_H
 
@@ -22,13 +23,12 @@
 
 namespace {
 
-template <int RM, int WM, int GPB> struct G4Tile {
-    static constexpr int ROWS = 32 * RM * WM, WAVES = 2 * WM, HALF = ROWS * 128; // bytes of 64 k
+template <int GPB> struct G4Tile {
+    static constexpr int RM = 4, ROWS = 64 * RM, HALF = ROWS * 128; // HALF: bytes of 64 k
     static constexpr int W_OFF = 2 * HALF, S_OFF = W_OFF + 8192, S_COPIES = GPB == 4 ? 2 : 1, BUF = S_OFF + S_COPIES * 1024, LDS = 2 * BUF;
-    static constexpr int XC = 4 * RM, WC = 8 / WAVES, COPIES = XC + WC + 1; // of a wave and step: activations, codes, scales
-    static constexpr int PAIRS = XC / 2 + 2;                                // statements that issue them, two activations' or all codes' at a time
-    static_assert(WC == 1 || WC == 2, "");
-    static constexpr int copies(int statements) { return statements <= XC / 2 ? 2 * statements : XC + WC + statements - XC / 2 - 1; }
+    // copies of a wave and step: activations, codes, scales; and the statements that issue them, two at a time but the last
+    static constexpr int XC = 4 * RM, COPIES = XC + 3, PAIRS = XC / 2 + 2;
+    static constexpr int copies(int statements) { return statements < PAIRS ? 2 * statements : COPIES; }
     static_assert(LDS <= 160 * 1024, "");
 };
 
@@ -100,11 +100,12 @@ template <bool SWIGLU, class F> __device__ __forceinline__ void g4_with_finish(c
 // A lane's first column of the 64 places from `unit` on.
 template <bool SWIGLU> __device__ __forceinline__ int64_t g4_lane_column(int64_t unit, int lane) { return SWIGLU ? unit * 32 + (lane & 31) : unit * 64 + 2 * (lane & 31); }
 
-template <int RM, int WM, int GPB, bool SWIGLU>
-__global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
-    using S = G4Tile<RM, WM, GPB>;
+template <int GPB, bool SWIGLU>
+__global__ __launch_bounds__(256) void g4_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+    using S = G4Tile<GPB>;
+    constexpr int RM = S::RM;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave % WM, wn = wave / WM;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave & 1, wn = wave >> 1;
     const unsigned tiles = (unsigned)mblocks * nblocks, job = (unsigned)xcd_remap(blockIdx.x, (int)(tiles * parts));
     const int part = parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(job / tiles));
     const unsigned tile = job - part * tiles;
@@ -123,11 +124,11 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
 #pragma unroll
     for (int r = 0; r < 2 * RM; ++r) {
         const int row = min(m0 + (wave * 2 * RM + r) * 8 + (lane >> 3), g.M - 1) - m0;
-        x_off[r] = (unsigned)row * (unsigned)g.ldx * 2 + ((lane & 7) ^ (lane >> 3)) * 16 + (r & 1 ? 0 : 1024);
+        x_off[r] = (unsigned)row * (unsigned)g.ldx * 2 + ((lane & 7) ^ ((r & 1) * 4 + (lane >> 4))) * 16 + (r & 1 ? 0 : 1024);
     }
-    const uint8_t* w_src[S::WC];
+    const uint8_t* w_src[2];
 #pragma unroll
-    for (int i = 0; i < S::WC; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * S::WC + i, places / 16 - 1) * KB + kb0) * 1024 - i * 1024;
+    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * 2 + i, places / 16 - 1) * KB + kb0) * 1024 - i * 1024;
     // (waves copy the same scales, or the same half of them, to one place: of each block of 16 places a piece of 64 GPB bytes)
     const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_at_tile = s_lane % (512 * GPB);
     const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)nblk * 8 * KB + kb0) * (64 * GPB);
@@ -139,9 +140,7 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
             constexpr int SUB = P / RM, R = P % RM * 2;
             mx_copy_two(x_src + SUB * 128, x_off[R], x_src + SUB * 128, x_off[R + 1], base + to + SUB * S::HALF + (wave * 2 * RM + R) * 1024);
         } else if constexpr (P == S::XC / 2) {
-            const uint32_t at = base + to + S::W_OFF + wave * S::WC * 1024;
-            if constexpr (S::WC == 2) mx_copy_two(w_src[0], lane * 16, w_src[1], lane * 16, at);
-            else mx_copy(w_src[0], lane * 16, at);
+            mx_copy_two(w_src[0], lane * 16, w_src[1], lane * 16, base + to + S::W_OFF + wave * 2048);
         } else {
             mx_copy(s_src, s_off, base + to + S::S_OFF + (GPB == 4 ? (wave & 1) * 1024 : 0));
         }
@@ -149,8 +148,7 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
     const auto copied = [&]() { // (behind the last step: that one again, which nobody reads)
         if (--ahead > 0) {
             x_src += 256;
-#pragma unroll
-            for (int i = 0; i < S::WC; ++i) w_src[i] += 1024;
+            w_src[0] += 1024, w_src[1] += 1024;
             s_src += 64 * GPB;
         }
     };
@@ -158,7 +156,7 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
     // ---- LDS reads
     uint32_t a_at[4]; // step s of a row's 64 k: s % 4
 #pragma unroll
-    for (int s = 0; s < 4; ++s) a_at[s] = (wm * RM * 32 + (lane & 31)) * 128 + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16);
+    for (int s = 0; s < 4; ++s) a_at[s] = (wm * RM * 32 + (lane & 31)) * 128 + (((2 * s + (lane >> 5)) ^ (lane >> 1 & 7)) * 16);
     const uint32_t w_at = S::W_OFF + wn * 4096 + (lane >> 4 & 1) * 2048 + (lane & 15) * 16 + (lane >> 5) * 256;
     const uint32_t s_at = S::S_OFF + (wn * 64 + (lane >> 4 & 1) * 32 + (lane & 15)) * GPB * 4; // [block][c][gpb], as copied
     v4i a[RM][8], w[12]; // (of half 0: 0 .. 3 and 8 .. 11, of half 1: 4 .. 11)
@@ -205,16 +203,15 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
     // beside its product, which are what the product's 32 clocks have room for.
     constexpr int L = 8 / GPB, GROUPS = 2 * RM * GPB, SLOTS = 16 * RM, MID = 8 * RM; // products of a group, groups and slots of a step
     // half J's codes, in slots from the start of the other half's last chain: operands 0 .. 3, then 4 .. 7
-    constexpr int CODES_FROM = RM == 4 ? -17 : RM == 2 ? -4 : 4, CODES_THEN = RM == 1 ? 8 : 5, CODES_TO = 14;
+    constexpr int CODES_FROM = -17, CODES_THEN = 5, CODES_TO = 14;
     // copies go out from half-time on, evenly, those of half-time's step + 2 ending some slots ahead of the next one; EARLY of the statements behind a step's end
-    constexpr int COPY_SLOTS = RM == 4 ? 44 : RM == 2 ? 20 : MID, EARLY = S::PAIRS * MID / COPY_SLOTS;
-    constexpr int READS = 18; // (RM = 4) slots that operands of half the rows are read in
+    constexpr int COPY_SLOTS = 44, EARLY = S::PAIRS * MID / COPY_SLOTS;
+    constexpr int READS = 18; // slots that operands of half the rows are read in
 
     // ---- prologue
     static_for<S::PAIRS>([&](auto p) { copy(0, p); });
     copied();
     static_for<EARLY>([&](auto p) { copy(S::BUF, p); });
-    if constexpr (EARLY == S::PAIRS) copied();
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::copies(EARLY)) : "memory");
     static_for<RM>([&](auto i) { static_for<8>([&](auto s) { read_a(0, i, s); }); });
     read_w(0, I0{}), read_w(0, I1{});
@@ -267,17 +264,14 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
             decode_some(I0{}, std::integral_constant<int, T < 8 ? T + 8 : T - (SLOTS - 8)>{});
             if constexpr (T == MID) read_s(next, I0{}), read_w(next, I0{});
             if constexpr (T == MID + 7) read_s(next, I1{}), read_w(next, I1{});
-            if constexpr (RM == 4) { // operands of rows 0 and 1 behind the barrier, of 2 and 3 early in the next step
-                constexpr int N0 = T >= MID + 7 ? T - MID - 7 : T >= 7 && T < 7 + READS ? T - 7 : READS, O = T >= MID ? 0 : 16;
-                if constexpr (N0 < READS) {
-                    constexpr int R0 = O + 16 * N0 / READS, R1 = O + 16 * (N0 + 1) / READS;
-                    static_for<R1 - R0>([&](auto r) {
-                        constexpr int R = R0 + decltype(r)::value;
-                        read_a(T >= MID ? next : here, std::integral_constant<int, R / 8>{}, std::integral_constant<int, R % 8>{});
-                    });
-                }
-            } else if constexpr (T >= MID) { // behind their last products
-                read_a(next, std::integral_constant<int, I>{}, std::integral_constant<int, ST>{});
+            // operands of rows 0 and 1 behind the barrier, of 2 and 3 early in the next step
+            constexpr int N0 = T >= MID + 7 ? T - MID - 7 : T >= 7 && T < 7 + READS ? T - 7 : READS, R = T >= MID ? 0 : 16;
+            if constexpr (N0 < READS) {
+                constexpr int R0 = R + 16 * N0 / READS, R1 = R + 16 * (N0 + 1) / READS;
+                static_for<R1 - R0>([&](auto r) {
+                    constexpr int X = R0 + decltype(r)::value;
+                    read_a(T >= MID ? next : here, std::integral_constant<int, X / 8>{}, std::integral_constant<int, X % 8>{});
+                });
             }
             constexpr int H = T >= MID ? T - MID : T + MID; // (SLOTS = 2 MID)
             if constexpr (H < COPY_SLOTS) {
@@ -295,7 +289,7 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     if (parts > 1) { // partial tile in accumulator order: [tile][part][wave][i][j][quarter of 16][lane]
-        v4f* to = reinterpret_cast<v4f*>(g.scratch) + (((size_t)tile * parts + part) * S::WAVES + wave) * (RM * 2 * 4 * 64) + lane;
+        v4f* to = reinterpret_cast<v4f*>(g.scratch) + (((size_t)tile * parts + part) * 4 + wave) * (RM * 2 * 4 * 64) + lane;
 #pragma unroll
         for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -316,40 +310,296 @@ __global__ __launch_bounds__(128 * WM) void g4_tile_kernel(rkh_g4_args g, int mb
 
 // Sum of the parts of a tile, in their order, and the results.  One wave per quarter of 32 rows x 64 places.
 template <bool SWIGLU>
-__global__ __launch_bounds__(256) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts, int rm, int wm) {
+__global__ __launch_bounds__(256) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+    constexpr int RM = G4Tile<1>::RM;
     const int lane = lane_id(), e = wave_id();
-    const unsigned per_tile = rm * wm * 2, tile = blockIdx.x / per_tile, in_tile = blockIdx.x % per_tile, wave = in_tile / rm, i = in_tile % rm;
+    const unsigned tile = blockIdx.x / (4 * RM), in_tile = blockIdx.x % (4 * RM), wave = in_tile / RM, i = in_tile % RM;
     int mblk, nblk;
     g4_place(tile, mblocks, nblocks, mblk, nblk);
-    const size_t step = (size_t)wm * 2 * rm * 512;
-    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + tile * parts * step + (wave * rm + i) * 512 + e * 64 + lane;
+    constexpr size_t step = 4 * RM * 512;
+    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + tile * parts * step + (wave * RM + i) * 512 + e * 64 + lane;
     v4f s0 = from[0], s1 = from[256];
 #pragma unroll 4
     for (int p = 1; p < parts; ++p) s0 += from[p * step], s1 += from[p * step + 256];
     const float a[4] = {s0.x, s0.y, s0.z, s0.w}, b[4] = {s1.x, s1.y, s1.z, s1.w};
-    const int64_t n = g4_lane_column<SWIGLU>((int64_t)nblk * 2 + wave / wm, lane);
-    g4_with_finish<SWIGLU>(g, [&](auto&& finish4) { finish4(((mblk * wm + (int)(wave % wm)) * rm + i) * 32 + 8 * e + 4 * (lane >> 5), n, a, b); });
+    const int64_t n = g4_lane_column<SWIGLU>((int64_t)nblk * 2 + (wave >> 1), lane);
+    g4_with_finish<SWIGLU>(g, [&](auto&& finish4) { finish4(((mblk * 2 + (int)(wave & 1)) * RM + i) * 32 + 8 * e + 4 * (lane >> 5), n, a, b); });
 }
 
-template <int RM, int WM, int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
-    constexpr int LDS = G4Tile<RM, WM, GPB>::LDS;
+template <int GPB, bool SWIGLU> int launch_big_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
+    constexpr int LDS = G4Tile<GPB>::LDS, RM = G4Tile<GPB>::RM;
     static std::atomic<bool> opted_in[64] = {};
-    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_tile_kernel<RM, WM, GPB, SWIGLU>), opted_in, LDS)) return rc;
+    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_tile_kernel<GPB, SWIGLU>), opted_in, LDS)) return rc;
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
-    if (tiles * r.parts * 128 * WM >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
+    if (tiles * r.parts * 256 >= MX_TOO_MANY_THREADS || (r.parts > 1 && tiles * RM * 4 * 256 >= MX_TOO_MANY_THREADS)) return RKH_ERR_RUNTIME;
     mark(st, "g4_tile_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_tile_kernel<RM, WM, GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(128 * WM), LDS, st, g, r.mblocks, r.nblocks,
-                       r.parts);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_tile_kernel<GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, r.parts);
     RKH_CHECK(hipGetLastError());
     if (r.parts > 1) {
         mark(st, "g4_join_kernel");
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * WM * 2)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts, RM, WM);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * 4)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts);
         RKH_CHECK(hipGetLastError());
     }
     return RKH_OK;
 }
+
+// ---- tiles of few rows -----------------------------------------------------------------
+// 32 RM rows x 128 places by four waves, each all of the rows and 32 places: nobody makes the same codes into halves twice, which is what tiles of few rows are
+// bound by (128 x 128 x 128 two by two 2020 clocks, this way {STEP128}), for twice the reads of activations.
+//  * A step's activations live in registers as above, each replaced by the next step's behind its product; the next step's codes become halves in
+//    registers of their own, so that two steps make one turn of the loop.
+//  * At the start of step s a wave waits for its copies of step s + 1 and for its LDS reads, and meets the others: nobody reads step s any more, and the
+//    copies of step s + BUFFERS take its place.  Steps are short, and memory answers after a microsecond: as many are under way as LDS holds.
+template <int RM, int GPB> struct G4Rows {
+    static constexpr int ROWS = 32 * RM, HALF = ROWS * 128, W_OFF = 2 * HALF, S_OFF = W_OFF + 8192, S_COPIES = GPB == 4 ? 2 : 1, BUF = S_OFF + S_COPIES * 1024,
+                         BUFFERS = RM == 1 ? 4 : 3, LDS = BUFFERS * BUF;
+    static constexpr int COPIES = 2 * RM + 3; // of a wave and step: activations, codes, scales
+    static_assert(LDS <= 160 * 1024, "");
+};
+
+// Four rows from `first` on of a lane's column n to results.  (SwiGLU: lanes 16 .. 31 and 48 .. 63 hold what goes with the gates of the 16 before.)
+template <int OUT, bool SWIGLU, bool EXPONENTS> __device__ __forceinline__ void g4_rows_finish4(const rkh_g4_args& g, int first, int64_t n, int lane, const float* s) {
+    using T = typename MxType<OUT>::T;
+    T* to = static_cast<T*>(g.C) + (size_t)first * g.ldc + n;
+    const int live = n < g.N && (!SWIGLU || !(lane & 16)) ? g.M - first : 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float v = s[e];
+        if constexpr (EXPONENTS) v = __builtin_amdgcn_ldexpf(v, g.exponents[min(first + e, g.M - 1)]);
+        if constexpr (SWIGLU) v = mx_silu(v, __shfl_xor(v, 16));
+        if (e < live) *to = (T)v;
+        to += g.ldc;
+    }
+}
+template <bool SWIGLU, class F> __device__ __forceinline__ void g4_with_rows_finish(const rkh_g4_args& g, int block0, int lane, F&& f) {
+    const int64_t n = g4_column(block0 + (lane >> 4 & 1), lane & 15, SWIGLU);
+    mx_with_type(g.out_type, [&](auto t) {
+        constexpr int OUT = decltype(t)::value;
+        if (g.exponents) f([&](int first, const float* s) { g4_rows_finish4<OUT, SWIGLU, true>(g, first, n, lane, s); });
+        else f([&](int first, const float* s) { g4_rows_finish4<OUT, SWIGLU, false>(g, first, n, lane, s); });
+    });
+}
+
+template <int RM, int GPB, bool SWIGLU>
+__global__ __launch_bounds__(256) void g4_rows_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+    using S = G4Rows<RM, GPB>;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+    const unsigned tiles = (unsigned)mblocks * nblocks, job = (unsigned)xcd_remap(blockIdx.x, (int)(tiles * parts));
+    const int part = parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(job / tiles));
+    const unsigned tile = job - part * tiles;
+    int mblk, nblk;
+    g4_place(tile, mblocks, nblocks, mblk, nblk);
+    const int KB = (int)rkh_g4_kb(g.K);
+    const int kb0 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * part / parts)), kb1 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * (part + 1) / parts));
+    const int64_t places = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU);
+
+    // ---- copies
+    const uint32_t base = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
+    const int m0 = mblk * S::ROWS;
+    const uint8_t* x_src = static_cast<const uint8_t*>(g.x) + ((size_t)m0 * g.ldx + (size_t)kb0 * 128) * 2;
+    unsigned x_off[RM]; // of eight rows' 128 bytes; rows beyond M: the last one again
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+        const int row = min(m0 + (wave * RM + r) * 8 + (lane >> 3), g.M - 1) - m0;
+        x_off[r] = (unsigned)row * (unsigned)g.ldx * 2 + ((lane & 7) ^ (((wave * RM + r) & 1) * 4 + (lane >> 4))) * 16;
+    }
+    const uint8_t* w_src[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * 2 + i, places / 16 - 1) * KB + kb0) * 1024 - i * 1024;
+    const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_at_tile = s_lane % (512 * GPB);
+    const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)nblk * 8 * KB + kb0) * (64 * GPB);
+    const unsigned s_off = (unsigned)min((int64_t)(s_at_tile / (64 * GPB)), places / 16 - 1 - (int64_t)nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
+    int ahead = kb1 - kb0; // steps that are still to be copied
+    const auto copy = [&](uint32_t to, auto p_tag) { // statement P: activations of eight rows, 64 k and 64 k; codes; scales
+        constexpr int P = decltype(p_tag)::value;
+        if constexpr (P < RM) {
+            mx_copy(x_src, x_off[P], base + to + (wave * RM + P) * 1024);
+            mx_copy(x_src + 128, x_off[P], base + to + S::HALF + (wave * RM + P) * 1024);
+        } else if constexpr (P == RM) {
+            mx_copy_two(w_src[0], lane * 16, w_src[1], lane * 16, base + to + S::W_OFF + wave * 2048);
+        } else {
+            mx_copy(s_src, s_off, base + to + S::S_OFF + (GPB == 4 ? (wave & 1) * 1024 : 0));
+        }
+    };
+    const auto copied = [&]() { // (behind the last step: that one again, which nobody reads)
+        if (--ahead > 0) {
+            x_src += 256;
+            w_src[0] += 1024, w_src[1] += 1024;
+            s_src += 64 * GPB;
+        }
+    };
+
+    // ---- LDS reads
+    uint32_t a_at[4]; // step s of a row's 64 k: s % 4
+#pragma unroll
+    for (int s = 0; s < 4; ++s) a_at[s] = (lane & 31) * 128 + (((2 * s + (lane >> 5)) ^ (lane >> 1 & 7)) * 16);
+    const uint32_t w_at = S::W_OFF + wave * 2048 + (lane >> 4 & 1) * 1024 + (lane & 15) * 16 + (lane >> 5) * 256;
+    const uint32_t s_at = S::S_OFF + (wave * 32 + (lane & 31)) * GPB * 4;
+    v4i a[RM][8], w[2][8], raw[2];
+    typedef uint32_t words __attribute__((ext_vector_type(GPB)));
+    words sd;
+    float scale[2][GPB];
+    const auto read_a = [&](uint32_t from, auto i_tag, auto s_tag) {
+        constexpr int I = decltype(i_tag)::value, ST = decltype(s_tag)::value;
+        a[I][ST] = *reinterpret_cast<const v4i*>(lds + from + a_at[ST & 3] + (ST >> 2) * S::HALF + I * 4096);
+    };
+    const auto read_w = [&](uint32_t from) {
+        raw[0] = *reinterpret_cast<const v4i*>(lds + from + w_at);
+        raw[1] = *reinterpret_cast<const v4i*>(lds + from + w_at + 512);
+        sd = *reinterpret_cast<const words*>(lds + from + s_at);
+    };
+
+    // ---- codes to operands: pair x (0 .. 31) of a step's eight
+    G4Zero zero[GPB];
+    uint32_t magic, upper = 0;
+    asm volatile("v_mov_b32 %0, 0x64006400" : "=v"(magic));
+    const auto decode = [&](auto p_tag, auto x_tag) {
+        constexpr int P = decltype(p_tag)::value, X = decltype(x_tag)::value, ST = X / 4, R = X % 4;
+        if constexpr (X == 0) {
+#pragma unroll
+            for (int n = 0; n < GPB; ++n) zero[n].of(sd[n]);
+        }
+        w[P][ST][R] = (int)g4_pair_here<R>((uint32_t)raw[ST & 1][ST >> 1], zero[ST * GPB / 8], magic, upper);
+    };
+    const auto scale_of = [&](auto p_tag) {
+        constexpr int P = decltype(p_tag)::value;
+#pragma unroll
+        for (int n = 0; n < GPB; ++n) scale[P][n] = g4_scale(sd[n], g.scale_type);
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+
+    // ---- prologue
+    static_for<S::BUFFERS>([&](auto b) {
+        static_for<RM + 2>([&](auto p) { copy(decltype(b)::value * S::BUF, p); });
+        copied();
+    });
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S::BUFFERS - 1) * S::COPIES) : "memory");
+    static_for<RM>([&](auto i) { static_for<8>([&](auto s) { read_a(0, i, s); }); });
+    read_w(0);
+    static_for<32>([&](auto x) { decode(I0{}, x); });
+    scale_of(I0{});
+
+    float acc[RM][16];
+    v16f sum[2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i) acc[i][e] = 0;
+        sum[0][e] = sum[1][e] = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < GPB; ++n) scale[1][n] = 0;
+
+    constexpr int L = 8 / GPB, GROUPS = RM * GPB, SLOTS = 8 * RM; // products of a group, groups and slots of a step
+    constexpr int CODES_FROM = RM == 1 ? 4 : 6;                   // (codes are read in slot 0)
+    const auto fold = [&](auto p_tag, auto g_tag, auto from_tag, auto to_tag) { // elements of the sum of group G of a step of parity P into the accumulators
+        constexpr int P = decltype(p_tag)::value, G = decltype(g_tag)::value;
+#pragma unroll
+        for (int e = from_tag(); e < to_tag(); ++e) g4_add_scaled(acc[G / GPB][e], sum[(P * GROUPS + G) & 1][e], scale[P][G % GPB]);
+    };
+    uint32_t next = S::BUF, here = 0; // of the next step and this one
+    const auto step = [&](auto p_tag) {
+        constexpr int P = decltype(p_tag)::value;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::BUFFERS - 2) * S::COPIES) : "memory");
+        static_for<SLOTS>([&](auto t_tag) {
+            constexpr int T = decltype(t_tag)::value, ST = T % 8, I = T / 8, G = P * GROUPS + T / L;
+            if constexpr (T % L == 0) g4_product_first(a[I][ST], w[P][ST], sum[G & 1]);
+            else g4_product(a[I][ST], w[P][ST], sum[G & 1]);
+            // the sum of a group from two slots behind its last product up to where its registers are wanted again
+            constexpr int U = T + 2 * SLOTS - L - 1, O = U % L, F = (P * GROUPS + U / L) % (2 * GROUPS);
+            if constexpr (O < L - 1)
+                fold(std::integral_constant<int, F / GROUPS>{}, std::integral_constant<int, F % GROUPS>{}, std::integral_constant<int, 16 * O / (L - 1)>{},
+                     std::integral_constant<int, 16 * (O + 1) / (L - 1)>{});
+            if constexpr (T == 0) read_w(next);
+            if constexpr (T >= CODES_FROM) {
+                constexpr int N = SLOTS - CODES_FROM, X0 = 32 * (T - CODES_FROM) / N, X1 = 32 * (T + 1 - CODES_FROM) / N;
+                static_for<X1 - X0>([&](auto x) { decode(std::integral_constant<int, 1 - P>{}, std::integral_constant<int, X0 + decltype(x)::value>{}); });
+            }
+            read_a(next, std::integral_constant<int, I>{}, std::integral_constant<int, ST>{});
+            if constexpr (T == SLOTS - 1) scale_of(std::integral_constant<int, 1 - P>{}); // (the step before has been added with its own)
+            constexpr int P0 = (RM + 2) * T / SLOTS, P1 = (RM + 2) * (T + 1) / SLOTS;
+            static_for<P1 - P0>([&](auto p) { copy(here, std::integral_constant<int, P0 + decltype(p)::value>{}); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        copied();
+        here = next;
+        next = next == (S::BUFFERS - 1) * S::BUF ? 0 : next + S::BUF;
+    };
+    const auto last = [&](auto p_tag) {
+        asm volatile("s_nop 7\n\ts_nop 7" ::: "memory"); // (the last product has to be through)
+        fold(p_tag, std::integral_constant<int, GROUPS - 1>{}, I0{}, std::integral_constant<int, 16>{});
+    };
+    int left = kb1 - kb0;
+    for (; left >= 2; left -= 2) {
+        step(I0{});
+        step(I1{});
+    }
+    if (left) {
+        step(I0{});
+        last(I0{});
+    } else {
+        last(I1{});
+    }
+    // a load to LDS must not outlive the workgroup
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+    if (parts > 1) { // partial tile in accumulator order: [tile][part][wave][i][quarter of 16][lane]
+        v4f* to = reinterpret_cast<v4f*>(g.scratch) + (((size_t)tile * parts + part) * 4 + wave) * (RM * 4 * 64) + lane;
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[(i * 4 + e) * 64] = v4f{acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]};
+    } else {
+        g4_with_rows_finish<SWIGLU>(g, nblk * 8 + wave * 2, lane, [&](auto&& finish4) {
+#pragma unroll
+            for (int i = 0; i < RM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) finish4(m0 + i * 32 + 8 * e + 4 * (lane >> 5), &acc[i][4 * e]);
+        });
+    }
+}
+
+// Sum of the parts, in their order, and the results.  One workgroup per 32 rows x 32 places, one wave per quarter of its accumulator.
+template <bool SWIGLU> __global__ __launch_bounds__(256) void g4_rows_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts, int rm) {
+    const int lane = lane_id(), e = wave_id();
+    const unsigned per_tile = rm * 4, tile = blockIdx.x / per_tile, in_tile = blockIdx.x % per_tile, wave = in_tile / rm, i = in_tile % rm;
+    int mblk, nblk;
+    g4_place(tile, mblocks, nblocks, mblk, nblk);
+    const size_t step = (size_t)rm * 1024;
+    const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + tile * parts * step + (wave * rm + i) * 256 + e * 64 + lane;
+    v4f s = from[0];
+#pragma unroll 4
+    for (int p = 1; p < parts; ++p) s += from[p * step];
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    g4_with_rows_finish<SWIGLU>(g, nblk * 8 + wave * 2, lane, [&](auto&& finish4) { finish4((mblk * rm + (int)i) * 32 + 8 * e + 4 * (lane >> 5), v); });
+}
+
+template <int RM, int GPB, bool SWIGLU> int launch_rows_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
+    constexpr int LDS = G4Rows<RM, GPB>::LDS;
+    static std::atomic<bool> opted_in[64] = {};
+    if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_rows_tile_kernel<RM, GPB, SWIGLU>), opted_in, LDS)) return rc;
+    const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
+    if (tiles * r.parts * 256 >= MX_TOO_MANY_THREADS || (r.parts > 1 && tiles * RM * 4 * 256 >= MX_TOO_MANY_THREADS)) return RKH_ERR_RUNTIME;
+    mark(st, "g4_rows_tile_kernel");
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_rows_tile_kernel<RM, GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, r.parts);
+    RKH_CHECK(hipGetLastError());
+    if (r.parts > 1) {
+        mark(st, "g4_rows_join_kernel");
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_rows_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * 4)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts, RM);
+        RKH_CHECK(hipGetLastError());
+    }
+    return RKH_OK;
+}
+
 template <int GPB, bool SWIGLU> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
-    return r.rm == 4 ? launch_tiles<4, 2, GPB, SWIGLU>(st, g, r) : r.rm == 2 ? launch_tiles<2, 2, GPB, SWIGLU>(st, g, r) : launch_tiles<1, 2, GPB, SWIGLU>(st, g, r);
+    switch (r.rm) {
+    case 8: return launch_big_tiles<GPB, SWIGLU>(st, g, r);
+    case 4: return launch_rows_tiles<4, GPB, SWIGLU>(st, g, r);
+    case 2: return launch_rows_tiles<2, GPB, SWIGLU>(st, g, r);
+    default: return launch_rows_tiles<1, GPB, SWIGLU>(st, g, r);
+    }
 }
 template <int GPB> int launch_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
     return g.swiglu ? launch_tiles<GPB, true>(st, g, r) : launch_tiles<GPB, false>(st, g, r);
