@@ -345,7 +345,7 @@ template <int GPB, bool SWIGLU> int launch_big_tiles(hipStream_t st, const rkh_g
 
 // ---- tiles of few rows -----------------------------------------------------------------
 // 32 RM rows x 128 places by four waves, each all of the rows and 32 places: nobody makes the same codes into halves twice, which is what tiles of few rows are
-// bound by (128 x 128 x 128 two by two 2020 clocks, this way {STEP128}), for twice the reads of activations.
+// bound by (128 x 128 x 128 two by two 2020 clocks, this way 1100 - 1700), for twice the reads of activations.
 //  * A step's activations live in registers as above, each replaced by the next step's behind its product; the next step's codes become halves in
 //    registers of their own, so that two steps make one turn of the loop.
 //  * At the start of step s a wave waits for its copies of step s + 1 and for its LDS reads, and meets the others: nobody reads step s any more, and the

@@ -1,8 +1,9 @@
 // The norm of attention heads and their rotation by position: z = rms(x) * w, pairs of z turned by position * inv_freq, one pass over the rows.
 //
-// Bound by memory for many rows, by one workgroup's round trips for few.  A workgroup takes some rows: it first makes their cosines and sines,
-// which all heads share, in LDS; then groups of lanes take a head each.  A lane holds both values of the pairs that it turns, so nothing is
-// exchanged but the sum of squares.
+// Bound by memory for many rows, by one workgroup's round trips for few.  A thread keeps its place in its head through some rows, so that weights and
+// addresses are fetched and made once; it holds both values of the pairs that it turns, so that nothing is exchanged but the sum of squares.  The rows' cosines
+// and sines, which all heads share, are made in LDS while the rows are on their way.
+// 8192 rows of 40 heads of 128 (bf16, norm): 34 us, 4.9 TB/s; two rows a workgroup 38, one 51; with half of the values a thread, and heads dealt out one by one, 52 us.
 #include <algorithm>
 
 #include "rk_heads_shim.h"
@@ -10,21 +11,34 @@
 
 namespace {
 
-constexpr int HEADS_THREADS = 256;
+constexpr int HEADS_MOST_THREADS = 256;
 
-// PAIRS (4 or 1) pairs of neighbouring indices a unit, UNITS units a lane, LANES lanes a head.
+// Sum over aligned groups of `lanes` lanes, a power of two; every lane of a group gets the same bits.
+__device__ __forceinline__ float heads_sum(float x, int lanes) {
+    const auto add = [&](auto ctrl) { x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xF, 0xF, true)); };
+    if (lanes > 1) add(std::integral_constant<int, 0xB1>{});  // lanes 1 0 3 2
+    if (lanes > 2) add(std::integral_constant<int, 0x4E>{});  // lanes 2 3 0 1
+    if (lanes > 4) add(std::integral_constant<int, 0x141>{}); // 7 .. 0 of eight
+    if (lanes > 8) add(std::integral_constant<int, 0x140>{}); // 15 .. 0 of sixteen
+    if (lanes > 16) x += __shfl_xor(x, 16);
+    if (lanes > 32) x += __shfl_xor(x, 32);
+    return x;
+}
+
+// PAIRS (8, 4 or 1) pairs of neighbouring indices a unit, UNITS units a thread, `lanes` threads a head, heads_each heads and ROWS rows a workgroup.
 // Unit u < R / 2 / PAIRS: pairs PAIRS u .., the rest of the units 2 PAIRS of the values behind R.
-template <int TYPE, int PAIRS, int UNITS, int AT_ONCE, bool NEIGHBOURS>
-__global__ __launch_bounds__(HEADS_THREADS) void heads_kernel(rkh_heads_args a, int lanes, int rows_each) {
+template <int TYPE, int PAIRS, int UNITS, int ROWS, bool NEIGHBOURS>
+__global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_args a, int lanes, int heads_each, int chunks) {
     using T = typename MxType<TYPE>::T;
     typedef T vec __attribute__((ext_vector_type(PAIRS)));
     typedef vec vec_any __attribute__((aligned(sizeof(T))));
     extern __shared__ __attribute__((aligned(16))) float turns[]; // [row][cos of a pair .., sin of a pair ..]
-    const int row0 = a.first + (int)blockIdx.x * rows_each, rows = min(rows_each, a.rows - row0), P = a.R / 2;
-    const int P4 = (P + 3) & ~3; // (16-byte places for units of four)
-    const int heads = a.q_heads + a.k_heads, lane = threadIdx.x % lanes, groups = HEADS_THREADS / lanes;
+    const int block = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - block * chunks;
+    const int row0 = a.first + block * ROWS, P = a.R / 2, P4 = (P + 3) & ~3; // (16-byte places)
+    const int lane = (int)threadIdx.x & (lanes - 1), slot = (int)threadIdx.x / lanes, head = chunk * heads_each + slot, heads = a.q_heads + a.k_heads;
+    const bool live = slot < heads_each && head < heads, is_q = head < a.q_heads;
 
-    // what a lane's units are: places of the first and the second PAIRS values, and how many of each exist
+    // where a thread's units are: places of the first and the second PAIRS values, and whether they exist
     int first_at[UNITS], second_at[UNITS], pair[UNITS];
     bool turned[UNITS], any[UNITS], both[UNITS];
     const int turned_units = P / PAIRS;
@@ -40,58 +54,40 @@ __global__ __launch_bounds__(HEADS_THREADS) void heads_kernel(rkh_heads_args a, 
             first_at[u] = a.R + 2 * PAIRS * (unit - turned_units);
             second_at[u] = first_at[u] + PAIRS;
         }
-        any[u] = first_at[u] < a.D; // (units of four end with the head)
-        both[u] = any[u] && second_at[u] < a.D;
+        any[u] = live && first_at[u] < a.D; // (units of several pairs end with the head)
+        both[u] = live && second_at[u] < a.D;
+        // (what does not exist is read where something does, and dropped)
+        first_at[u] = any[u] ? first_at[u] : 0, second_at[u] = both[u] ? second_at[u] : 0;
     }
+    const int h = live ? is_q ? head : head - a.q_heads : 0;
+    const bool from_q = live ? is_q : a.q_heads > 0;
+    const int64_t row_stride = from_q ? a.q_row : a.k_row, out_stride = from_q ? a.q_out_row : a.k_out_row;
+    const T* from = static_cast<const T*>(from_q ? a.q : a.k) + h * (from_q ? a.q_head : a.k_head);
+    T* to = static_cast<T*>(from_q ? a.q_out : a.k_out) + h * (from_q ? a.q_out_head : a.k_out_head);
 
-    // items: heads of the rows, dealt to the groups; AT_ONCE of a group are loaded together
-    struct Item { int row, head; };
-    const auto next = [&](Item& i) {
-        i.head += groups;
-        while (i.head >= heads) i.head -= heads, ++i.row;
-    };
-    const auto base = [&](const Item& i, const void* q, const void* k, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head) {
-        const bool is_q = i.head < a.q_heads;
-        const int64_t at = is_q ? (int64_t)(row0 + i.row) * q_row + i.head * q_head : (int64_t)(row0 + i.row) * k_row + (i.head - a.q_heads) * k_head;
-        return static_cast<T*>(const_cast<void*>(is_q ? q : k)) + at;
-    };
-    vec x[AT_ONCE][UNITS][2] = {};
-    const auto load = [&](Item i) {
+    vec x[ROWS][UNITS][2]; // (rows beyond the last: that one again)
 #pragma unroll
-        for (int n = 0; n < AT_ONCE; ++n) {
-            if (i.row < rows) {
-                const T* p = base(i, a.q, a.k, a.q_row, a.q_head, a.k_row, a.k_head);
+    for (int r = 0; r < ROWS; ++r) {
+        const T* p = from + (int64_t)min(row0 + r, a.rows - 1) * row_stride;
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u) {
-                    if (any[u]) x[n][u][0] = *reinterpret_cast<const vec_any*>(p + first_at[u]);
-                    if (both[u]) x[n][u][1] = *reinterpret_cast<const vec_any*>(p + second_at[u]);
-                }
-            }
-            next(i);
+        for (int u = 0; u < UNITS; ++u) {
+            x[r][u][0] = *reinterpret_cast<const vec_any*>(p + first_at[u]);
+            x[r][u][1] = *reinterpret_cast<const vec_any*>(p + second_at[u]);
         }
-    };
-    Item item{0, (int)threadIdx.x / lanes};
-    while (item.head >= heads) item.head -= heads, ++item.row;
-    load(item);
-
-    float q_weight[UNITS][2][PAIRS], k_weight[UNITS][2][PAIRS];
-    if (a.norm) {
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < PAIRS; ++e) {
-                    const bool is = h ? both[u] : any[u];
-                    const int at = (h ? second_at[u] : first_at[u]) + e;
-                    q_weight[u][h][e] = is && a.q_weight && a.q_heads ? a.q_weight[at] : 1.0f;
-                    k_weight[u][h][e] = is && a.k_weight && a.k_heads ? a.k_weight[at] : 1.0f;
-                }
     }
+    float weight[UNITS][2][PAIRS];
+    const float* w = from_q ? a.q_weight : a.k_weight;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+        for (int e = 0; e < PAIRS; ++e) {
+            weight[u][0][e] = w ? w[first_at[u] + e] : 1.0f;
+            weight[u][1][e] = w ? w[second_at[u] + e] : 1.0f;
+        }
 
     // angles in turns, reduced in 64 bits: what is left, -1/2 .. 1/2, has no use for more than 32
-    for (int i = threadIdx.x; i < rows * P; i += HEADS_THREADS) {
-        const int row = i / P, p = i - row * P;
+    for (int i = threadIdx.x; i < min(ROWS, a.rows - row0) * P; i += blockDim.x) {
+        const int row = ROWS == 1 ? 0 : (int)((unsigned)i / (unsigned)P), p = i - row * P;
         const int axis = (int)(a.axis_of[p >> 4] >> (2 * (p & 15))) & 3;
         const double angle = (double)a.positions[axis * a.position_axis + row0 + row] * (double)a.inv_freq[p] * 0.15915494309189533577;
         float sine, cosine;
@@ -101,65 +97,55 @@ __global__ __launch_bounds__(HEADS_THREADS) void heads_kernel(rkh_heads_args a, 
     }
     __syncthreads();
 
-    while (item.row < rows) {
-        Item i = item;
 #pragma unroll
-        for (int n = 0; n < AT_ONCE; ++n) {
-            // (lanes of a group stay together; what a group beyond the last item reduces is nobody's)
-            float v[UNITS][2][PAIRS], sum = 0;
+    for (int r = 0; r < ROWS; ++r) {
+        if (row0 + r >= a.rows) break;
+        float v[UNITS][2][PAIRS], sum = 0;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int e = 0; e < PAIRS; ++e) {
+                    v[u][s][e] = (float)x[r][u][s][e];
+                    const float counted = PAIRS > 1 || (s ? both[u] : any[u]) ? v[u][s][e] : 0.0f;
+                    sum = fmaf(counted, counted, sum);
+                }
+        if (a.norm) {
+            // (units of several pairs exist as a whole or not at all)
+            if (PAIRS > 1 && !any[0]) sum = 0;
+            const float factor = mx_norm_factor(heads_sum(sum, lanes), a.D, a.eps);
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int e = 0; e < PAIRS; ++e) {
-                        v[u][h][e] = (h ? both[u] : any[u]) ? (float)x[n][u][h][e] : 0.0f;
-                        sum = fmaf(v[u][h][e], v[u][h][e], sum);
-                    }
-            const bool is_q = i.head < a.q_heads;
-            if (a.norm) {
-                for (int off = 1; off < lanes; off <<= 1) sum += __shfl_xor(sum, off);
-                const float factor = mx_norm_factor(sum, a.D, a.eps);
+                    for (int e = 0; e < PAIRS; ++e) v[u][s][e] = v[u][s][e] * factor * weight[u][s][e];
+        }
+        T* row_to = to + (int64_t)(row0 + r) * out_stride;
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u)
+        for (int u = 0; u < UNITS; ++u) {
+            if (turned[u]) {
+                const float* cosine = turns + r * 2 * P4 + pair[u];
+                const float* sine = cosine + P4;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < PAIRS; ++e) v[u][h][e] = v[u][h][e] * factor * (is_q ? q_weight[u][h][e] : k_weight[u][h][e]);
-            }
-            if (i.row < rows) {
-                T* to = base(i, a.q_out, a.k_out, a.q_out_row, a.q_out_head, a.k_out_row, a.k_out_head);
-#pragma unroll
-                for (int u = 0; u < UNITS; ++u) {
-                    if (turned[u]) {
-                        const float* cosine = turns + i.row * 2 * P4 + pair[u];
-                        const float* sine = cosine + P4;
-                        float c[PAIRS], s[PAIRS];
-#pragma unroll
-                        for (int e = 0; e < PAIRS; ++e) c[e] = cosine[e], s[e] = sine[e];
-#pragma unroll
-                        for (int e = 0; e < PAIRS; ++e) {
-                            // neighbours: the unit's values one after the other, pair e at 2 e and 2 e + 1
-                            float& first = NEIGHBOURS ? v[u][2 * e / PAIRS][2 * e % PAIRS] : v[u][0][e];
-                            float& second = NEIGHBOURS ? v[u][(2 * e + 1) / PAIRS][(2 * e + 1) % PAIRS] : v[u][1][e];
-                            const float p = first, q = second;
-                            first = fmaf(p, c[e], -(q * s[e]));
-                            second = fmaf(q, c[e], p * s[e]);
-                        }
-                    }
-                    vec y[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < PAIRS; ++e) y[h][e] = (T)v[u][h][e];
-                    if (any[u]) *reinterpret_cast<vec_any*>(to + first_at[u]) = y[0];
-                    if (both[u]) *reinterpret_cast<vec_any*>(to + second_at[u]) = y[1];
+                for (int e = 0; e < PAIRS; ++e) {
+                    // neighbours: the unit's values one after the other, pair e at 2 e and 2 e + 1
+                    float& first = NEIGHBOURS ? v[u][2 * e / PAIRS][2 * e % PAIRS] : v[u][0][e];
+                    float& second = NEIGHBOURS ? v[u][(2 * e + 1) / PAIRS][(2 * e + 1) % PAIRS] : v[u][1][e];
+                    const float p = first, q = second;
+                    first = fmaf(p, cosine[e], -(q * sine[e]));
+                    second = fmaf(q, cosine[e], p * sine[e]);
                 }
             }
-            next(i);
+            vec y[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int e = 0; e < PAIRS; ++e) y[s][e] = (T)v[u][s][e];
+            if (any[u]) __builtin_nontemporal_store(y[0], reinterpret_cast<vec_any*>(row_to + first_at[u]));
+            if (both[u]) __builtin_nontemporal_store(y[1], reinterpret_cast<vec_any*>(row_to + second_at[u]));
         }
-        item = i;
-        load(item);
     }
 }
 
@@ -168,30 +154,35 @@ __global__ __launch_bounds__(HEADS_THREADS) void heads_kernel(rkh_heads_args a, 
 extern "C" int rkh_heads(void* stream, const rkh_heads_args* args) {
     rkh_heads_args a = *args;
     const hipStream_t st = (hipStream_t)stream;
-    // four pairs at a time where they come in fours, and so do the values behind them; one otherwise
-    const bool fours = a.D % 8 == 0 && a.R % 8 == 0;
-    const int units = fours ? a.D / 8 : a.R / 2 + (a.D - a.R + 1) / 2;
+    // 16 bytes of each half at a time where heads and what is turned of them come in such units, 16 bytes of both, or single pairs
+    const auto whole = [&](int pairs) { return a.D % (2 * pairs) == 0 && a.R % (2 * pairs) == 0; };
+    const int pairs = a.type != RKH_MX4_F32 && whole(8) ? 8 : whole(4) ? 4 : 1;
+    const int units = pairs > 1 ? a.D / (2 * pairs) : a.R / 2 + (a.D - a.R + 1) / 2;
     int lanes = 1;
     while (lanes < units && lanes < 64) lanes *= 2;
-    const int per_lane = (units + lanes - 1) / lanes;
-    const int heads = a.q_heads + a.k_heads;
-    const int rows_each = std::max<int64_t>(1, std::min<int64_t>(8, 2048 / ((int64_t)heads * lanes)));
+    const int per_lane = (units + lanes - 1) / lanes; // (several pairs: one, D being 512 at most)
+    const int heads = a.q_heads + a.k_heads, most_heads = HEADS_MOST_THREADS / lanes, chunks = (heads + most_heads - 1) / most_heads;
+    const int heads_each = (heads + chunks - 1) / chunks, threads = (int)rkh_align_up((int64_t)heads_each * lanes, 64);
+    // several rows a workgroup where that leaves enough of them
+    const bool many = per_lane == 1 && (int64_t)a.rows * chunks >= 4096;
+    const int rows_each = many ? 4 : 1;
     const size_t lds = (size_t)rows_each * 2 * ((a.R / 2 + 3) & ~3) * 4;
-    const int64_t most = (INT64_C(1) << 31) / HEADS_THREADS * rows_each; // rows of a launch
+    const int64_t most = std::max<int64_t>(1, (INT64_C(1) << 31) / threads / chunks) * rows_each; // rows of a launch, which holds fewer than 2^32 threads
     for (int64_t first = 0; first < args->rows; first += most) {
         a.first = (int)first;
         a.rows = (int)std::min<int64_t>(args->rows, first + most);
-        const dim3 grid((unsigned)((a.rows - first + rows_each - 1) / rows_each));
+        const dim3 grid((unsigned)((a.rows - first + rows_each - 1) / rows_each * chunks));
         mark(st, "heads_kernel");
         mx_with_type(a.type, [&](auto t) {
-            constexpr int TYPE = decltype(t)::value;
+            constexpr int TYPE = decltype(t)::value, WIDE = TYPE == RKH_MX4_F32 ? 4 : 8;
             const auto go = [&](auto n) {
                 constexpr bool N = decltype(n)::value;
-                const auto kernel = fours           ? heads_kernel<TYPE, 4, 1, 4, N>
-                                    : per_lane == 1 ? heads_kernel<TYPE, 1, 1, 4, N>
-                                    : per_lane == 2 ? heads_kernel<TYPE, 1, 2, 2, N>
+                const auto kernel = pairs == 8      ? many ? heads_kernel<TYPE, WIDE, 1, 4, N> : heads_kernel<TYPE, WIDE, 1, 1, N>
+                                    : pairs == 4    ? many ? heads_kernel<TYPE, 4, 1, 4, N> : heads_kernel<TYPE, 4, 1, 1, N>
+                                    : per_lane == 1 ? many ? heads_kernel<TYPE, 1, 1, 4, N> : heads_kernel<TYPE, 1, 1, 1, N>
+                                    : per_lane == 2 ? heads_kernel<TYPE, 1, 2, 1, N>
                                                     : heads_kernel<TYPE, 1, 4, 1, N>;
-                hipLaunchKernelGGL(kernel, grid, dim3(HEADS_THREADS), lds, st, a, lanes, rows_each);
+                hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), lds, st, a, lanes, heads_each, chunks);
             };
             if (a.neighbours) go(std::true_type{});
             else go(std::false_type{});
