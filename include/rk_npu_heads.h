@@ -8,7 +8,7 @@
  *         phi = positions[axis of i][t] * inv_freq[i]
  *         a' = rotation_scale * (a cos phi - b sin phi),   b' = rotation_scale * (b cos phi + a sin phi)
  *     z[R] .. z[D - 1] as they are
- * computed in fp32 and rounded once.  The angle is reduced in fp64, so that far positions (all 32 bits) lose nothing that fp32 holds.
+ * computed in fp32 and rounded once.  The angle is reduced in fp64: far positions (all 32 bits) are off by 2^-21 at most.
  * Squares are added in fp32, without scaling; a NaN makes its head NaN where there is a norm, and otherwise the pair.
  *
  * Positions have up to four axes (time, height, width, ..), and a table says by which one a pair is turned: sections of pairs one behind

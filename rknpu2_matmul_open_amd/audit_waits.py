@@ -283,7 +283,7 @@ def audit_function(name, lines):
     return violations
 
 
-def audit_text(asm_text, only=("gemm_wk_kernel", "gemm_wk_big_kernel", "gemm_stream_kernel", "mx4_tile_kernel", "mx4_big_kernel", "g4_tile_kernel")):
+def audit_text(asm_text, only=("gemm_wk_kernel", "gemm_wk_big_kernel", "gemm_stream_kernel", "mx4_tile_kernel", "mx4_big_kernel", "g4_tile_kernel", "g4_rows_tile_kernel")):
     """Violations in every kernel of an assembly file whose (mangled) name contains one of `only`."""
     violations, checked = [], 0
     lines = asm_text.splitlines() + [".Lfunc_end:"]
