@@ -30,7 +30,10 @@ class Layer:
             self.zeros[rng.random((N, groups)) < 0.9] %= 16
         t = device(s, kind)
         self.scales, self.group = host(t), group
-        codes = device(ref.pack(self.code))
+        packed = ref.pack(self.code)
+        if K % 2:
+            packed[:, -1] |= 0xa0 # (what is beyond a row counts for nothing)
+        codes = device(packed)
         ready()
         self.w = ops.G4Weights.from_device(sess, K, N, group, codes, t, None if self.zeros is None else device(self.zeros), gate_up=gate_up)
         self.values, self.sizes = (f(self.code, self.scales, self.zeros, group) for f in (ref.weights, ref.sizes))
