@@ -4,6 +4,7 @@
 // addresses are fetched and made once; it holds both values of the pairs that it turns, so that nothing is exchanged but the sum of squares.  The rows' cosines
 // and sines, which all heads share, are made in LDS while the rows are on their way.
 // 8192 rows of 40 heads of 128 (bf16, norm): 34 us, 4.9 TB/s; two rows a workgroup 38, one 51; with half of the values a thread, and heads dealt out one by one, 52 us.
+// 8192 rows of 20 heads of 90, 60 of them turned: bf16 18.8 us, fp32 30.3; a pair a time 31.3 and 35.6.
 #include <algorithm>
 
 #include "rk_heads_shim.h"
@@ -12,6 +13,9 @@
 namespace {
 
 constexpr int HEADS_MOST_THREADS = 256;
+
+// Places for a row's cosines, and its sines: those of the units' pairs one behind the other.
+__host__ __device__ constexpr int heads_table(int R) { return (R / 2 + 7) & ~7; }
 
 // Sum over aligned groups of `lanes` lanes, a power of two; every lane of a group gets the same bits.
 __device__ __forceinline__ float heads_sum(float x, int lanes) {
@@ -26,89 +30,106 @@ __device__ __forceinline__ float heads_sum(float x, int lanes) {
 }
 
 // PAIRS (8, 4 or 1) pairs of neighbouring indices a unit, UNITS units a thread, `lanes` threads a head, heads_each heads and ROWS rows a workgroup.
-// Unit u < R / 2 / PAIRS: pairs PAIRS u .., the rest of the units 2 PAIRS of the values behind R.
-template <int TYPE, int PAIRS, int UNITS, int ROWS, bool NEIGHBOURS>
+// The first units are turned: PAIRS pairs, from pair PAIRS u on; the others are 2 PAIRS of the values behind R.
+// RAGGED: what is turned, or the rest, is not in whole units.  The last unit of either begins earlier, so that it is whole, and keeps only what it does not share
+// with the one before; where there is no one before, it reaches beyond and keeps only its own.
+template <int TYPE, int PAIRS, int UNITS, int ROWS, bool NEIGHBOURS, bool RAGGED>
 __global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_args a, int lanes, int heads_each, int chunks) {
     using T = typename MxType<TYPE>::T;
     typedef T vec __attribute__((ext_vector_type(PAIRS)));
     typedef vec vec_any __attribute__((aligned(sizeof(T))));
     extern __shared__ __attribute__((aligned(16))) float turns[]; // [row][cos of a pair .., sin of a pair ..]
     const int block = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - block * chunks;
-    const int row0 = a.first + block * ROWS, P = a.R / 2, P4 = (P + 3) & ~3; // (16-byte places)
+    const int row0 = a.first + block * ROWS, P = a.R / 2, table = heads_table(a.R);
     const int lane = (int)threadIdx.x & (lanes - 1), slot = (int)threadIdx.x / lanes, head = chunk * heads_each + slot, heads = a.q_heads + a.k_heads;
     const bool live = slot < heads_each && head < heads, is_q = head < a.q_heads;
 
-    // where a thread's units are: places of the first and the second PAIRS values, and whether they exist
-    int first_at[UNITS], second_at[UNITS], pair[UNITS];
-    bool turned[UNITS], any[UNITS], both[UNITS];
-    const int turned_units = P / PAIRS;
+    // where a thread's units are: places of the first and the second PAIRS values, and which of those it keeps
+    int at[UNITS][2], from_e[UNITS][2], to_e[UNITS][2], turn[UNITS];
+    bool turned[UNITS], shares[UNITS][2]; // (whether all of the PAIRS values are of its kind)
+    const int turned_units = (P + PAIRS - 1) / PAIRS;
+    const auto first_pair = [&](int unit) { return RAGGED ? max(0, min(unit * PAIRS, P - PAIRS)) : unit * PAIRS; };
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
         const int unit = lane + u * lanes;
         turned[u] = unit < turned_units;
-        pair[u] = turned[u] ? unit * PAIRS : 0;
+        turn[u] = turned[u] ? unit * PAIRS : 0;
         if (turned[u]) {
-            first_at[u] = NEIGHBOURS ? 2 * PAIRS * unit : PAIRS * unit;
-            second_at[u] = NEIGHBOURS ? first_at[u] + PAIRS : P + PAIRS * unit;
+            const int pair = first_pair(unit), own = unit * PAIRS - pair, end = min(P - pair, PAIRS); // first, first and last kept of the unit
+            at[u][0] = NEIGHBOURS ? 2 * pair : pair;
+            at[u][1] = NEIGHBOURS ? at[u][0] + PAIRS : P + pair;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                from_e[u][s] = NEIGHBOURS ? 2 * own - s * PAIRS : own;
+                to_e[u][s] = NEIGHBOURS ? 2 * end - s * PAIRS : end;
+            }
         } else {
-            first_at[u] = a.R + 2 * PAIRS * (unit - turned_units);
-            second_at[u] = first_at[u] + PAIRS;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int first = a.R + PAIRS * (2 * (unit - turned_units) + s);
+                at[u][s] = RAGGED ? min(first, a.D - PAIRS) : first;
+                from_e[u][s] = first - at[u][s]; // (PAIRS and more: nothing)
+                to_e[u][s] = first < a.D ? PAIRS : 0;
+            }
         }
-        any[u] = live && first_at[u] < a.D; // (units of several pairs end with the head)
-        both[u] = live && second_at[u] < a.D;
         // (what does not exist is read where something does, and dropped)
-        first_at[u] = any[u] ? first_at[u] : 0, second_at[u] = both[u] ? second_at[u] : 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            shares[u][s] = turned[u] ? P >= PAIRS : at[u][s] >= a.R;
+            if (!live || at[u][s] + PAIRS > a.D) at[u][s] = to_e[u][s] = 0;
+        }
     }
+    const auto keeps = [&](int u, int s, int e) { return RAGGED ? e >= from_e[u][s] && e < to_e[u][s] : to_e[u][s] > 0; };
     const int h = live ? is_q ? head : head - a.q_heads : 0;
     const bool from_q = live ? is_q : a.q_heads > 0;
     const int64_t row_stride = from_q ? a.q_row : a.k_row, out_stride = from_q ? a.q_out_row : a.k_out_row;
     const T* from = static_cast<const T*>(from_q ? a.q : a.k) + h * (from_q ? a.q_head : a.k_head);
     T* to = static_cast<T*>(from_q ? a.q_out : a.k_out) + h * (from_q ? a.q_out_head : a.k_out_head);
 
-    // (single pairs of neighbours: both values at once, where no unit is half of one; 8192 rows of 20 heads of 90 in fp32 36.7 -> 33.3 us)
-    typedef T two __attribute__((ext_vector_type(2)));
-    typedef two two_any __attribute__((aligned(sizeof(T))));
-    const bool at_once = PAIRS == 1 && NEIGHBOURS && a.D % 2 == 0;
     vec x[ROWS][UNITS][2]; // (rows beyond the last: that one again)
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
         const T* p = from + (int64_t)min(row0 + r, a.rows - 1) * row_stride;
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            if (at_once) {
-                const two v = *reinterpret_cast<const two_any*>(p + first_at[u]);
-                x[r][u][0][0] = v[0], x[r][u][1][0] = v[1];
-                continue;
-            }
-            x[r][u][0] = *reinterpret_cast<const vec_any*>(p + first_at[u]);
-            x[r][u][1] = *reinterpret_cast<const vec_any*>(p + second_at[u]);
-        }
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) x[r][u][s] = *reinterpret_cast<const vec_any*>(p + at[u][s]);
     }
-    float weight[UNITS][2][PAIRS];
+    typedef float fvec __attribute__((ext_vector_type(PAIRS)));
+    typedef fvec fvec_any __attribute__((aligned(4)));
+    fvec weight[UNITS][2];
     const float* w = from_q ? a.q_weight : a.k_weight;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-        for (int e = 0; e < PAIRS; ++e) {
-            weight[u][0][e] = w ? w[first_at[u] + e] : 1.0f;
-            weight[u][1][e] = w ? w[second_at[u] + e] : 1.0f;
-        }
+        for (int s = 0; s < 2; ++s) weight[u][s] = w ? *reinterpret_cast<const fvec_any*>(w + at[u][s]) : fvec(1.0f);
 
     // angles in turns, reduced in 64 bits: what is left, -1/2 .. 1/2, has no use for more than 32
-    for (int i = threadIdx.x; i < min(ROWS, a.rows - row0) * P; i += blockDim.x) {
-        const int row = ROWS == 1 ? 0 : (int)((unsigned)i / (unsigned)P), p = i - row * P;
+    const int turns_of_row = turned_units * PAIRS;
+    for (int i = threadIdx.x; i < min(ROWS, a.rows - row0) * turns_of_row; i += blockDim.x) {
+        const int row = ROWS == 1 ? 0 : (int)((unsigned)i / (unsigned)turns_of_row), at_row = i - row * turns_of_row;
+        const int p = RAGGED ? min(first_pair(at_row / PAIRS) + at_row % PAIRS, P - 1) : at_row;
         const int axis = (int)(a.axis_of[p >> 4] >> (2 * (p & 15))) & 3;
         const double angle = (double)a.positions[axis * a.position_axis + row0 + row] * (double)a.inv_freq[p] * 0.15915494309189533577;
         float sine, cosine;
         sincospif((float)(2.0 * (angle - rint(angle))), &sine, &cosine);
-        turns[row * 2 * P4 + p] = cosine * a.rotation_scale;
-        turns[row * 2 * P4 + P4 + p] = sine * a.rotation_scale;
+        turns[row * 2 * table + at_row] = cosine * a.rotation_scale;
+        turns[row * 2 * table + table + at_row] = sine * a.rotation_scale;
     }
     __syncthreads();
 
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
         if (row0 + r >= a.rows) break;
+        if constexpr (RAGGED && PAIRS > 1) { // all of the row has been read before any of it is written
+            typedef int words __attribute__((ext_vector_type(PAIRS * sizeof(T) / 4)));
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                words first = __builtin_bit_cast(words, x[r][u][0]), second = __builtin_bit_cast(words, x[r][u][1]);
+                asm volatile("" : "+v"(first), "+v"(second));
+                x[r][u][0] = __builtin_bit_cast(vec, first), x[r][u][1] = __builtin_bit_cast(vec, second);
+            }
+        }
         float v[UNITS][2][PAIRS], sum = 0;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
@@ -117,12 +138,10 @@ __global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_arg
 #pragma unroll
                 for (int e = 0; e < PAIRS; ++e) {
                     v[u][s][e] = (float)x[r][u][s][e];
-                    const float counted = PAIRS > 1 || (s ? both[u] : any[u]) ? v[u][s][e] : 0.0f;
+                    const float counted = keeps(u, s, e) ? v[u][s][e] : 0.0f;
                     sum = fmaf(counted, counted, sum);
                 }
         if (a.norm) {
-            // (units of several pairs exist as a whole or not at all)
-            if (PAIRS > 1 && !any[0]) sum = 0;
             const float factor = mx_norm_factor(heads_sum(sum, lanes), a.D, a.eps);
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)
@@ -135,8 +154,8 @@ __global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_arg
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             if (turned[u]) {
-                const float* cosine = turns + r * 2 * P4 + pair[u];
-                const float* sine = cosine + P4;
+                const float* cosine = turns + r * 2 * table + turn[u];
+                const float* sine = cosine + table;
 #pragma unroll
                 for (int e = 0; e < PAIRS; ++e) {
                     // neighbours: the unit's values one after the other, pair e at 2 e and 2 e + 1
@@ -152,12 +171,21 @@ __global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_arg
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int e = 0; e < PAIRS; ++e) y[s][e] = (T)v[u][s][e];
-            if (at_once) {
-                if (any[u]) __builtin_nontemporal_store(two{y[0][0], y[1][0]}, reinterpret_cast<two_any*>(row_to + first_at[u]));
-                continue;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                T* p = row_to + at[u][s];
+                // (ragged: streaming stores of parts of lines take three times as long; values that two units share are stored twice, the same)
+                if constexpr (!RAGGED) {
+                    if (to_e[u][s] > 0) __builtin_nontemporal_store(y[s], reinterpret_cast<vec_any*>(p));
+                } else if (to_e[u][s] <= 0 || from_e[u][s] >= PAIRS) {
+                } else if (shares[u][s]) {
+                    *reinterpret_cast<vec_any*>(p) = y[s];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < PAIRS; ++e)
+                        if (keeps(u, s, e)) p[e] = y[s][e];
+                }
             }
-            if (any[u]) __builtin_nontemporal_store(y[0], reinterpret_cast<vec_any*>(row_to + first_at[u]));
-            if (both[u]) __builtin_nontemporal_store(y[1], reinterpret_cast<vec_any*>(row_to + second_at[u]));
         }
     }
 }
@@ -167,20 +195,20 @@ __global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_arg
 extern "C" int rkh_heads(void* stream, const rkh_heads_args* args) {
     rkh_heads_args a = *args;
     const hipStream_t st = (hipStream_t)stream;
-    // 16 bytes of each half at a time where heads and what is turned of them come in such units, 16 bytes of both, or single pairs
-    const auto whole = [&](int pairs) { return a.D % (2 * pairs) == 0 && a.R % (2 * pairs) == 0; };
-    const int pairs = a.type != RKH_MX4_F32 && whole(8) ? 8 : whole(4) ? 4 : 1;
-    const int units = pairs > 1 ? a.D / (2 * pairs) : a.R / 2 + (a.D - a.R + 1) / 2;
+    // 16 bytes of each half at a time, of both for the shortest heads, or single pairs
+    const int pairs = a.type != RKH_MX4_F32 && a.D >= 16 ? 8 : a.D >= 8 ? 4 : 1;
+    const bool ragged = a.R % (2 * pairs) || (a.D - a.R) % (2 * pairs);
+    const int units = (a.R / 2 + pairs - 1) / pairs + (a.D - a.R + 2 * pairs - 1) / (2 * pairs);
     int lanes = 1;
     while (lanes < units && lanes < 64) lanes *= 2;
-    const int per_lane = (units + lanes - 1) / lanes; // (several pairs: one, D being 512 at most)
+    const int per_lane = (units + lanes - 1) / lanes; // (two for ragged heads of nearly 512 values)
     const int heads = a.q_heads + a.k_heads, most_heads = HEADS_MOST_THREADS / lanes, chunks = (heads + most_heads - 1) / most_heads;
     const int heads_each = (heads + chunks - 1) / chunks, threads = (int)rkh_align_up((int64_t)heads_each * lanes, 64);
     // several rows a workgroup where that leaves enough of them (one row / four: 256 rows of 40 heads of 128 in bf16 4.2 / 5.5 us, 1000 rows 8.5 / 7.5; 1521
     // rows of 20 heads of 96 in fp32 12.1 / 7.4)
     const bool many = per_lane == 1 && (int64_t)a.rows * chunks >= 1024;
     const int rows_each = many ? 4 : 1;
-    const size_t lds = (size_t)rows_each * 2 * ((a.R / 2 + 3) & ~3) * 4;
+    const size_t lds = (size_t)rows_each * 2 * heads_table(a.R) * 4;
     const int64_t most = std::max<int64_t>(1, (INT64_C(1) << 31) / threads / chunks) * rows_each; // rows of a launch, which holds fewer than 2^32 threads
     for (int64_t first = 0; first < args->rows; first += most) {
         a.first = (int)first;
@@ -189,17 +217,16 @@ extern "C" int rkh_heads(void* stream, const rkh_heads_args* args) {
         mark(st, "heads_kernel");
         mx_with_type(a.type, [&](auto t) {
             constexpr int TYPE = decltype(t)::value, WIDE = TYPE == RKH_MX4_F32 ? 4 : 8;
-            const auto go = [&](auto n) {
-                constexpr bool N = decltype(n)::value;
-                const auto kernel = pairs == 8      ? many ? heads_kernel<TYPE, WIDE, 1, 4, N> : heads_kernel<TYPE, WIDE, 1, 1, N>
-                                    : pairs == 4    ? many ? heads_kernel<TYPE, 4, 1, 4, N> : heads_kernel<TYPE, 4, 1, 1, N>
-                                    : per_lane == 1 ? many ? heads_kernel<TYPE, 1, 1, 4, N> : heads_kernel<TYPE, 1, 1, 1, N>
-                                    : per_lane == 2 ? heads_kernel<TYPE, 1, 2, 1, N>
-                                                    : heads_kernel<TYPE, 1, 4, 1, N>;
+            const auto go = [&](auto n, auto rg) {
+                constexpr bool N = decltype(n)::value, RG = decltype(rg)::value;
+                const auto kernel = pairs == 8      ? many ? heads_kernel<TYPE, WIDE, 1, 4, N, RG> : heads_kernel<TYPE, WIDE, 1, 1, N, RG>
+                                    : pairs == 1    ? many ? heads_kernel<TYPE, 1, 1, 4, N, true> : heads_kernel<TYPE, 1, 1, 1, N, true>
+                                    : per_lane == 1 ? many ? heads_kernel<TYPE, 4, 1, 4, N, RG> : heads_kernel<TYPE, 4, 1, 1, N, RG>
+                                                    : heads_kernel<TYPE, 4, 2, 1, N, true>;
                 hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), lds, st, a, lanes, heads_each, chunks);
             };
-            if (a.neighbours) go(std::true_type{});
-            else go(std::false_type{});
+            if (a.neighbours) ragged ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+            else ragged ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
         });
         RKH_CHECK(hipGetLastError());
     }

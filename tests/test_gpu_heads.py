@@ -76,7 +76,8 @@ CASES = [(1, 32, 8, 128, 128, "bf16", {}), (1, 1, 0, 1, 0, "f32", {}), (3, 0, 2,
          (3, 300, 70, 3, 2, "f16", {}), (5000, 2, 1, 64, 64, "f32", {}), (4099, 1, 1, 15, 8, "bf16", {}), (2049, 40, 8, 128, 128, "bf16", {}),
          (1026, 40, 8, 128, 96, "f32", dict(neighbours=True, axes=2)), (4101, 3, 2, 130, 128, "f16", {}), (4097, 1, 0, 200, 24, "f16", dict(norm=False, neighbours=True)),
          (6, 2, 2, 255, 254, "f32", {}), (6, 2, 2, 300, 200, "f16", dict(neighbours=True)), (4100, 4, 4, 40, 8, "f32", dict(neighbours=True)),
-         (4200, 4, 4, 24, 8, "bf16", dict(neighbours=True))]
+         (4200, 4, 4, 24, 8, "bf16", dict(neighbours=True)), (2100, 9, 3, 70, 66, "bf16", {}), (2100, 9, 3, 70, 66, "f32", dict(neighbours=True, axes=2)), (2100, 9, 3, 128, 10, "f16", {}),
+         (2100, 5, 1, 512, 2, "f32", {}), (2100, 9, 3, 90, 0, "bf16", {})]
 
 
 @pytest.mark.parametrize("rows,q_heads,k_heads,D,R,kind,more", CASES)
@@ -91,6 +92,19 @@ def test_norm_and_rotation(sess, rows, q_heads, k_heads, D, R, kind, more):
     case.call(sess, *here)
     done(sess)
     assert all(a is None or torch.equal(a, b) for a, b in zip(outs, here))
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_heads_and_turned_parts_of_every_length(sess, kind, neighbours):
+    """Turned and not in any number of values, in place: what no unit holds as a whole is turned and left out once."""
+    pairs = [(D, R) for D in range(1, 42) for R in range(0, D + 1, 2)] + [(D, R) for D in (127, 128, 200, 509, 511, 512) for R in (0, 2, 14, 18, 74, 126, 2 * (D // 2) - 2, 2 * (D // 2)) if R <= D]
+    for D, R in pairs:
+        case = Case(3, 2, 1, D, R, kind, neighbours=neighbours, norm=D % 3 != 0)
+        q, k = case.q.clone(), case.k.clone()
+        case.call(sess, q, k)
+        done(sess)
+        case.check(q, k)
 
 
 @pytest.mark.parametrize("kind,D,R,shift", [("bf16", 128, 128, 0), ("f16", 64, 32, 1), ("f32", 72, 72, 3), ("bf16", 33, 10, 5)])
