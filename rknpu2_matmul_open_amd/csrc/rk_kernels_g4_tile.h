@@ -58,15 +58,36 @@ template <int R> __device__ __forceinline__ uint32_t g4_pair_here(uint32_t w, co
     return v;
 }
 
-// Where a tile lies: column sweeps over groups of row blocks, so that concurrently running tiles share weights in L2.
-__device__ __forceinline__ void g4_place(unsigned tile, unsigned mblocks, unsigned nblocks, int& mblk, int& nblk) {
-    constexpr unsigned GM = 4;
-    const unsigned per_group = GM * nblocks, grp = tile / per_group, first_m = grp * GM, gm = min(mblocks - first_m, GM);
-    const unsigned in_group = tile - grp * per_group, col = in_group / gm;
-    mblk = __builtin_amdgcn_readfirstlane((int)(first_m + in_group - col * gm));
-    nblk = __builtin_amdgcn_readfirstlane((int)col);
-}
+// What a launch of tiles covers, and the numbers that its workgroups would divide by.  (With divisions, of 64 bits among them, a workgroup of 32 rows had its
+// first address after 2000 clocks and not after 1200, and 32 x 4096 x 4096 took 11.8 us, now 10.4.)
+struct G4Grid {
+    int mblocks, nblocks, parts;
+    int blocks;                   // of 16 places
+    int each, more;               // pieces of K of a part; the first `more` have one more
+    MxDivider tiles, group, last; // .. by tiles, by those of a group of row blocks, by the row blocks of the last group
+    static constexpr int GROUP = 4; // row blocks that are swept together
 
+    static G4Grid of(const rkk::G4Route& r, const rkh_g4_args& g) {
+        const int KB = (int)rkh_g4_kb(g.K), left = r.mblocks % GROUP;
+        return {r.mblocks, r.nblocks, r.parts, (int)(rkh_g4_places(g.swiglu ? 2 * (int64_t)g.N : g.N, g.swiglu) / 16), KB / r.parts, KB % r.parts,
+                MxDivider::of((uint32_t)(r.mblocks * r.nblocks)), MxDivider::of((uint32_t)(GROUP * r.nblocks)), MxDivider::of((uint32_t)(left ? left : GROUP))};
+    }
+    // Where a tile lies: column sweeps over groups of row blocks, so that concurrently running tiles share weights in L2.
+    __device__ __forceinline__ void place(unsigned tile, int& mblk, int& nblk) const {
+        const unsigned grp = group.divide(tile), first_m = grp * GROUP, in_group = tile - grp * GROUP * nblocks;
+        const bool whole = mblocks - first_m >= GROUP;
+        const unsigned of_last = last.divide(in_group), col = whole ? in_group / GROUP : of_last;
+        mblk = __builtin_amdgcn_readfirstlane((int)(first_m + in_group - col * (whole ? (unsigned)GROUP : mblocks - first_m)));
+        nblk = __builtin_amdgcn_readfirstlane((int)col);
+    }
+    __device__ __forceinline__ void job(unsigned at, unsigned& tile, int& part) const {
+        const unsigned in_order = (unsigned)xcd_remap((int)at, mblocks * nblocks * parts);
+        part = __builtin_amdgcn_readfirstlane((int)tiles.divide(in_order));
+        tile = in_order - part * mblocks * nblocks;
+    }
+    __device__ __forceinline__ int begin(int part) const { return part * each + min(part, more); }
+    __device__ __forceinline__ int KB() const { return begin(parts); }
+};
 // Four rows from `first` on of a lane's two columns (SwiGLU: of both halves of one) from accumulators of 32 x 32 to results; n: the first column.
 template <int OUT, bool SWIGLU, bool EXPONENTS> __device__ __forceinline__ void g4_finish4(const rkh_g4_args& g, int first, int64_t n, const float* s0, const float* s1) {
     using T = typename MxType<OUT>::T;
@@ -101,19 +122,17 @@ template <bool SWIGLU, class F> __device__ __forceinline__ void g4_with_finish(c
 template <bool SWIGLU> __device__ __forceinline__ int64_t g4_lane_column(int64_t unit, int lane) { return SWIGLU ? unit * 32 + (lane & 31) : unit * 64 + 2 * (lane & 31); }
 
 template <int GPB, bool SWIGLU>
-__global__ __launch_bounds__(256) void g4_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+__global__ __launch_bounds__(256) void g4_tile_kernel(G4Grid t, rkh_g4_args g) {
     using S = G4Tile<GPB>;
     constexpr int RM = S::RM;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wm = wave & 1, wn = wave >> 1;
-    const unsigned tiles = (unsigned)mblocks * nblocks, job = (unsigned)xcd_remap(blockIdx.x, (int)(tiles * parts));
-    const int part = parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(job / tiles));
-    const unsigned tile = job - part * tiles;
-    int mblk, nblk;
-    g4_place(tile, mblocks, nblocks, mblk, nblk);
-    const int KB = (int)rkh_g4_kb(g.K);
-    const int kb0 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * part / parts)), kb1 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * (part + 1) / parts));
-    const int64_t places = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU);
+    const int parts = t.parts, KB = t.KB();
+    unsigned tile;
+    int part, mblk, nblk;
+    t.job(blockIdx.x, tile, part);
+    t.place(tile, mblk, nblk);
+    const int kb0 = t.begin(part), kb1 = t.begin(part + 1);
 
     // ---- copies.  Wave-uniform addresses that advance by a step, lane offsets that stay.
     const uint32_t base = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
@@ -128,11 +147,11 @@ __global__ __launch_bounds__(256) void g4_tile_kernel(rkh_g4_args g, int mblocks
     }
     const uint8_t* w_src[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * 2 + i, places / 16 - 1) * KB + kb0) * 1024 - i * 1024;
+    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min(nblk * 8 + wave * 2 + i, t.blocks - 1) * KB + kb0) * 1024 - i * 1024;
     // (waves copy the same scales, or the same half of them, to one place: of each block of 16 places a piece of 64 GPB bytes)
     const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_at_tile = s_lane % (512 * GPB);
     const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)nblk * 8 * KB + kb0) * (64 * GPB);
-    const unsigned s_off = (unsigned)min((int64_t)(s_at_tile / (64 * GPB)), places / 16 - 1 - (int64_t)nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
+    const unsigned s_off = (unsigned)min((int)(s_at_tile / (64 * GPB)), t.blocks - 1 - nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
     int ahead = kb1 - kb0; // steps that are still to be copied
     const auto copy = [&](uint32_t to, auto p_tag) {
         constexpr int P = decltype(p_tag)::value;
@@ -310,12 +329,13 @@ __global__ __launch_bounds__(256) void g4_tile_kernel(rkh_g4_args g, int mblocks
 
 // Sum of the parts of a tile, in their order, and the results.  One wave per quarter of 32 rows x 64 places.
 template <bool SWIGLU>
-__global__ __launch_bounds__(256) void g4_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+__global__ __launch_bounds__(256) void g4_join_kernel(G4Grid t, rkh_g4_args g) {
     constexpr int RM = G4Tile<1>::RM;
     const int lane = lane_id(), e = wave_id();
     const unsigned tile = blockIdx.x / (4 * RM), in_tile = blockIdx.x % (4 * RM), wave = in_tile / RM, i = in_tile % RM;
+    const int parts = t.parts;
     int mblk, nblk;
-    g4_place(tile, mblocks, nblocks, mblk, nblk);
+    t.place(tile, mblk, nblk);
     constexpr size_t step = 4 * RM * 512;
     const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + tile * parts * step + (wave * RM + i) * 512 + e * 64 + lane;
     v4f s0 = from[0], s1 = from[256];
@@ -332,12 +352,13 @@ template <int GPB, bool SWIGLU> int launch_big_tiles(hipStream_t st, const rkh_g
     if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_tile_kernel<GPB, SWIGLU>), opted_in, LDS)) return rc;
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
     if (tiles * r.parts * 256 >= MX_TOO_MANY_THREADS || (r.parts > 1 && tiles * RM * 4 * 256 >= MX_TOO_MANY_THREADS)) return RKH_ERR_RUNTIME;
+    const G4Grid t = G4Grid::of(r, g);
     mark(st, "g4_tile_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_tile_kernel<GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, r.parts);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_tile_kernel<GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, t, g);
     RKH_CHECK(hipGetLastError());
     if (r.parts > 1) {
         mark(st, "g4_join_kernel");
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * 4)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * 4)), dim3(256), 0, st, t, g);
         RKH_CHECK(hipGetLastError());
     }
     return RKH_OK;
@@ -381,18 +402,16 @@ template <bool SWIGLU, class F> __device__ __forceinline__ void g4_with_rows_fin
 }
 
 template <int RM, int GPB, bool SWIGLU>
-__global__ __launch_bounds__(256) void g4_rows_tile_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts) {
+__global__ __launch_bounds__(256) void g4_rows_tile_kernel(G4Grid t, rkh_g4_args g) {
     using S = G4Rows<RM, GPB>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
-    const unsigned tiles = (unsigned)mblocks * nblocks, job = (unsigned)xcd_remap(blockIdx.x, (int)(tiles * parts));
-    const int part = parts == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(job / tiles));
-    const unsigned tile = job - part * tiles;
-    int mblk, nblk;
-    g4_place(tile, mblocks, nblocks, mblk, nblk);
-    const int KB = (int)rkh_g4_kb(g.K);
-    const int kb0 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * part / parts)), kb1 = __builtin_amdgcn_readfirstlane((int)((int64_t)KB * (part + 1) / parts));
-    const int64_t places = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU);
+    const int parts = t.parts, KB = t.KB();
+    unsigned tile;
+    int part, mblk, nblk;
+    t.job(blockIdx.x, tile, part);
+    t.place(tile, mblk, nblk);
+    const int kb0 = t.begin(part), kb1 = t.begin(part + 1);
 
     // ---- copies
     const uint32_t base = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
@@ -406,10 +425,10 @@ __global__ __launch_bounds__(256) void g4_rows_tile_kernel(rkh_g4_args g, int mb
     }
     const uint8_t* w_src[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min((int64_t)nblk * 8 + wave * 2 + i, places / 16 - 1) * KB + kb0) * 1024 - i * 1024;
+    for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min(nblk * 8 + wave * 2 + i, t.blocks - 1) * KB + kb0) * 1024 - i * 1024;
     const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_at_tile = s_lane % (512 * GPB);
     const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)nblk * 8 * KB + kb0) * (64 * GPB);
-    const unsigned s_off = (unsigned)min((int64_t)(s_at_tile / (64 * GPB)), places / 16 - 1 - (int64_t)nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
+    const unsigned s_off = (unsigned)min((int)(s_at_tile / (64 * GPB)), t.blocks - 1 - nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
     int ahead = kb1 - kb0; // steps that are still to be copied
     const auto copy = [&](uint32_t to, auto p_tag) { // statement P: activations of eight rows, 64 k and 64 k; codes; scales
         constexpr int P = decltype(p_tag)::value;
@@ -562,11 +581,12 @@ __global__ __launch_bounds__(256) void g4_rows_tile_kernel(rkh_g4_args g, int mb
 }
 
 // Sum of the parts, in their order, and the results.  One workgroup per 32 rows x 32 places, one wave per quarter of its accumulator.
-template <bool SWIGLU> __global__ __launch_bounds__(256) void g4_rows_join_kernel(rkh_g4_args g, int mblocks, int nblocks, int parts, int rm) {
+template <bool SWIGLU> __global__ __launch_bounds__(256) void g4_rows_join_kernel(G4Grid t, int rm_bits, rkh_g4_args g) {
     const int lane = lane_id(), e = wave_id();
-    const unsigned per_tile = rm * 4, tile = blockIdx.x / per_tile, in_tile = blockIdx.x % per_tile, wave = in_tile / rm, i = in_tile % rm;
+    const unsigned rm = 1u << rm_bits, tile = blockIdx.x >> (2 + rm_bits), wave = blockIdx.x >> rm_bits & 3, i = blockIdx.x & (rm - 1);
+    const int parts = t.parts;
     int mblk, nblk;
-    g4_place(tile, mblocks, nblocks, mblk, nblk);
+    t.place(tile, mblk, nblk);
     const size_t step = (size_t)rm * 1024;
     const v4f* from = reinterpret_cast<const v4f*>(g.scratch) + tile * parts * step + (wave * rm + i) * 256 + e * 64 + lane;
     v4f s = from[0];
@@ -582,12 +602,13 @@ template <int RM, int GPB, bool SWIGLU> int launch_rows_tiles(hipStream_t st, co
     if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(&g4_rows_tile_kernel<RM, GPB, SWIGLU>), opted_in, LDS)) return rc;
     const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
     if (tiles * r.parts * 256 >= MX_TOO_MANY_THREADS || (r.parts > 1 && tiles * RM * 4 * 256 >= MX_TOO_MANY_THREADS)) return RKH_ERR_RUNTIME;
+    const G4Grid t = G4Grid::of(r, g);
     mark(st, "g4_rows_tile_kernel");
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_rows_tile_kernel<RM, GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, g, r.mblocks, r.nblocks, r.parts);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_rows_tile_kernel<RM, GPB, SWIGLU>), dim3((unsigned)(tiles * r.parts)), dim3(256), LDS, st, t, g);
     RKH_CHECK(hipGetLastError());
     if (r.parts > 1) {
         mark(st, "g4_rows_join_kernel");
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_rows_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * 4)), dim3(256), 0, st, g, r.mblocks, r.nblocks, r.parts, RM);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(g4_rows_join_kernel<SWIGLU>), dim3((unsigned)(tiles * RM * 4)), dim3(256), 0, st, t, RM / 2, g);
         RKH_CHECK(hipGetLastError());
     }
     return RKH_OK;

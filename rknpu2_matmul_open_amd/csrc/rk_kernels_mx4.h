@@ -19,6 +19,18 @@ typedef uint16_t u16_any __attribute__((aligned(1)));
 // pieces of so many workgroups of 256.
 constexpr int64_t MX_TOO_MANY_THREADS = INT64_C(1) << 32, MX_MOST_GROUPS = MX_TOO_MANY_THREADS / 2 / 256;
 
+// n / d for n below 2^28 by a multiplication: kernels that take microseconds have no time for divisions.
+struct MxDivider {
+    uint32_t factor;
+    int shift;
+    static MxDivider of(uint32_t d) { // 2^shift / d rounded up, which is off by less than 2^-28 of it
+        int bits = 0;
+        while ((UINT64_C(1) << bits) < d) ++bits;
+        return {(uint32_t)(((UINT64_C(1) << (28 + bits)) + d - 1) / d), 28 + bits};
+    }
+    __device__ __forceinline__ unsigned divide(unsigned n) const { return (unsigned)((uint64_t)n * factor >> shift); }
+};
+
 template <int TYPE> struct MxType;
 template <> struct MxType<RKH_MX4_F32> { using T = float; };
 template <> struct MxType<RKH_MX4_F16> { using T = _Float16; };
