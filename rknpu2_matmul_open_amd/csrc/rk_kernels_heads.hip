@@ -29,19 +29,19 @@ __device__ __forceinline__ float heads_sum(float x, int lanes) {
     return x;
 }
 
-// PAIRS (8, 4 or 1) pairs of neighbouring indices a unit, UNITS units a thread, `lanes` threads a head, heads_each heads and ROWS rows a workgroup.
+// PAIRS (8, 4 or 1) pairs of neighbouring indices a unit, UNITS units a thread, 2^lane_bits threads a head, heads_each heads and ROWS rows a workgroup.
 // The first units are turned: PAIRS pairs, from pair PAIRS u on; the others are 2 PAIRS of the values behind R.
 // RAGGED: what is turned, or the rest, is not in whole units.  The last unit of either begins earlier, so that it is whole, and keeps only what it does not share
 // with the one before; where there is no one before, it reaches beyond and keeps only its own.
 template <int TYPE, int PAIRS, int UNITS, int ROWS, bool NEIGHBOURS, bool RAGGED>
-__global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_args a, int lanes, int heads_each, int chunks) {
+__global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_args a, int lane_bits, int heads_each, int chunks, MxDivider by_chunks, MxDivider by_turns) {
     using T = typename MxType<TYPE>::T;
     typedef T vec __attribute__((ext_vector_type(PAIRS)));
     typedef vec vec_any __attribute__((aligned(sizeof(T))));
     extern __shared__ __attribute__((aligned(16))) float turns[]; // [row][cos of a pair .., sin of a pair ..]
-    const int block = (int)blockIdx.x / chunks, chunk = (int)blockIdx.x - block * chunks;
+    const int block = (int)by_chunks.divide(blockIdx.x), chunk = (int)blockIdx.x - block * chunks;
     const int row0 = a.first + block * ROWS, P = a.R / 2, table = heads_table(a.R);
-    const int lane = (int)threadIdx.x & (lanes - 1), slot = (int)threadIdx.x / lanes, head = chunk * heads_each + slot, heads = a.q_heads + a.k_heads;
+    const int lanes = 1 << lane_bits, lane = (int)threadIdx.x & (lanes - 1), slot = (int)threadIdx.x >> lane_bits, head = chunk * heads_each + slot, heads = a.q_heads + a.k_heads;
     const bool live = slot < heads_each && head < heads, is_q = head < a.q_heads;
 
     // where a thread's units are: places of the first and the second PAIRS values, and which of those it keeps
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(HEADS_MOST_THREADS) void heads_kernel(rkh_heads_arg
     // angles in turns, reduced in 64 bits: what is left, -1/2 .. 1/2, has no use for more than 32
     const int turns_of_row = turned_units * PAIRS;
     for (int i = threadIdx.x; i < min(ROWS, a.rows - row0) * turns_of_row; i += blockDim.x) {
-        const int row = ROWS == 1 ? 0 : (int)((unsigned)i / (unsigned)turns_of_row), at_row = i - row * turns_of_row;
+        const int row = ROWS == 1 ? 0 : (int)by_turns.divide(i), at_row = i - row * turns_of_row;
         const int p = RAGGED ? min(first_pair(at_row / PAIRS) + at_row % PAIRS, P - 1) : at_row;
         const int axis = (int)(a.axis_of[p >> 4] >> (2 * (p & 15))) & 3;
         const double angle = (double)a.positions[axis * a.position_axis + row0 + row] * (double)a.inv_freq[p] * 0.15915494309189533577;
@@ -199,8 +199,9 @@ extern "C" int rkh_heads(void* stream, const rkh_heads_args* args) {
     const int pairs = a.type != RKH_MX4_F32 && a.D >= 16 ? 8 : a.D >= 8 ? 4 : 1;
     const bool ragged = a.R % (2 * pairs) || (a.D - a.R) % (2 * pairs);
     const int units = (a.R / 2 + pairs - 1) / pairs + (a.D - a.R + 2 * pairs - 1) / (2 * pairs);
-    int lanes = 1;
-    while (lanes < units && lanes < 64) lanes *= 2;
+    int lane_bits = 0;
+    while (1 << lane_bits < units && lane_bits < 6) ++lane_bits;
+    const int lanes = 1 << lane_bits;
     const int per_lane = (units + lanes - 1) / lanes; // (two for ragged heads of nearly 512 values)
     const int heads = a.q_heads + a.k_heads, most_heads = HEADS_MOST_THREADS / lanes, chunks = (heads + most_heads - 1) / most_heads;
     const int heads_each = (heads + chunks - 1) / chunks, threads = (int)rkh_align_up((int64_t)heads_each * lanes, 64);
@@ -208,6 +209,7 @@ extern "C" int rkh_heads(void* stream, const rkh_heads_args* args) {
     // rows of 20 heads of 96 in fp32 12.1 / 7.4)
     const bool many = per_lane == 1 && (int64_t)a.rows * chunks >= 1024;
     const int rows_each = many ? 4 : 1;
+    const MxDivider by_chunks = MxDivider::of(chunks), by_turns = MxDivider::of(std::max(1, (a.R / 2 + pairs - 1) / pairs * pairs));
     const size_t lds = (size_t)rows_each * 2 * heads_table(a.R) * 4;
     const int64_t most = std::max<int64_t>(1, (INT64_C(1) << 31) / threads / chunks) * rows_each; // rows of a launch, which holds fewer than 2^32 threads
     for (int64_t first = 0; first < args->rows; first += most) {
@@ -223,7 +225,7 @@ extern "C" int rkh_heads(void* stream, const rkh_heads_args* args) {
                                     : pairs == 1    ? many ? heads_kernel<TYPE, 1, 1, 4, N, true> : heads_kernel<TYPE, 1, 1, 1, N, true>
                                     : per_lane == 1 ? many ? heads_kernel<TYPE, 4, 1, 4, N, RG> : heads_kernel<TYPE, 4, 1, 1, N, RG>
                                                     : heads_kernel<TYPE, 4, 2, 1, N, true>;
-                hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), lds, st, a, lanes, heads_each, chunks);
+                hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), lds, st, a, lane_bits, heads_each, chunks, by_chunks, by_turns);
             };
             if (a.neighbours) ragged ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
             else ragged ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
