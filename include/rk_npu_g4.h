@@ -9,7 +9,8 @@
  *
  * code - zero is multiplied as the integer that it is; products are exact, sums have 32 bits, each group's sum is scaled in fp32, and the result
  * is rounded once.  No weight is rounded.  Rows are independent of each other; a row that holds an infinity or a NaN has
- * infinities and NaN as its results.  Scales are finite numbers.
+ * infinities and NaN as its results, and so may one whose sums of code * A, which are taken ahead of the scale, are beyond fp32 (bf16 values from
+ * 2^116 on).  Scales are finite numbers.
  *
  * All pointers are device pointers unless said otherwise; the calls enqueue on the context's stream and return, under the rules
  * for *_device calls in rk_npu_hip.h (rk_npu_hip_sync() waits, stream capture records them, a workspace is BUSY only while a

@@ -52,7 +52,7 @@ void rk_npu_heads_args_init(rk_npu_heads_args* args, int rows, int head_dim) {
 int rk_npu_heads_norm_rotate_device(rk_npu_ctx* ctx, const rk_npu_heads_args* a) {
     if (!ctx || !a || a->struct_size != sizeof(*a)) return RK_NPU_ERR_PARAM;
     const int D = a->head_dim, R = a->rotary_dim;
-    if (a->rows < 0 || D < 1 || D > RKH_HEADS_MOST_DIM || a->q_heads < 0 || a->k_heads < 0 || a->q_heads > 1 << 20 || a->k_heads > 1 << 20 || !valid_type(a->type) ||
+    if (a->rows < 0 || a->rows > INT_MAX - 15 || D < 1 || D > RKH_HEADS_MOST_DIM || a->q_heads < 0 || a->k_heads < 0 || a->q_heads > 1 << 20 || a->k_heads > 1 << 20 || !valid_type(a->type) ||
         R < 0 || R > D || R % 2 || a->axes < 1 || a->axes > 4)
         return RK_NPU_ERR_PARAM;
     if (a->norm ? !(a->eps >= 0.0f) : (a->q_weight || a->k_weight)) return RK_NPU_ERR_PARAM;

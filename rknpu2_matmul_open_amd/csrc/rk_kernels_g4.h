@@ -61,16 +61,10 @@ __host__ __device__ __forceinline__ int64_t g4_column(int64_t block, int c, bool
     return gate_up ? unit * 32 + 16 * b + c : unit * 64 + 32 * b + 2 * c + j;
 }
 
-// One or two neighbouring results of row m from column n on.
-template <int N> __device__ __forceinline__ void g4_put(const rkh_g4_args& g, int m, int64_t n, const float (&v)[N]) {
-    mx_with_type(g.out_type, [&](auto t) {
-        using T = typename MxType<decltype(t)::value>::T;
-        typedef T pair __attribute__((ext_vector_type(2)));
-        typedef pair pair_any __attribute__((aligned(sizeof(T))));
-        T* to = static_cast<T*>(g.C) + (size_t)m * g.ldc + n;
-        if (N == 2 && n + 1 < g.N) *reinterpret_cast<pair_any*>(to) = pair{(T)v[0], (T)v[N - 1]};
-        else if (n < g.N) *to = (T)v[0];
-    });
+// The result of row m and column n.
+__device__ __forceinline__ void g4_put(const rkh_g4_args& g, int m, int64_t n, float v) {
+    if (n >= g.N) return;
+    mx_with_type(g.out_type, [&](auto t) { mx_store1<decltype(t)::value>(g.C, (size_t)m * g.ldc + n, v); });
 }
 
 } // namespace

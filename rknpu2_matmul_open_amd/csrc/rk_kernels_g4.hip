@@ -239,8 +239,8 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
         if (m >= M) continue;
         const int ex = g.exponents ? g.exponents[m] : 0;
         const float a = __builtin_amdgcn_ldexpf(total(at), ex);
-        const float v[1] = {SWIGLU ? mx_silu(a, __builtin_amdgcn_ldexpf(total(at + 256), ex)) : a};
-        g4_put<1>(g, m, g4_column(block0 + (at >> 8), i >> 2 & 15, SWIGLU), v);
+        const float v = SWIGLU ? mx_silu(a, __builtin_amdgcn_ldexpf(total(at + 256), ex)) : a;
+        g4_put(g, m, g4_column(block0 + (at >> 8), i >> 2 & 15, SWIGLU), v);
     }
 }
 

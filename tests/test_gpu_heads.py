@@ -231,6 +231,15 @@ def test_captured_calls_replay_what_the_eager_call_gives(sess, rows):
     sess.lib.rk_npu_hip_graph_free(graph)
 
 
+def test_batches_of_no_rows_write_nothing(sess):
+    case = Case(3, 2, 1, 64, 64, "bf16")
+    q, k = case.q.clone(), case.k.clone()
+    ready()
+    ops.heads_norm_rotate(sess, q[:0], k[:0], q_weight=case.wq, positions=case.positions[:, :0], inv_freq=case.inv_freq)
+    done(sess)
+    assert torch.equal(q, case.q) and torch.equal(k, case.k)
+
+
 def test_refusals(sess):
     lib, bad = sess.lib, capi.RK_NPU_ERR_PARAM
     rows, D = 4, 16
@@ -249,7 +258,7 @@ def test_refusals(sess):
         return lib.rk_npu_heads_norm_rotate_device(ctx, C.byref(a))
     table = (C.c_uint8 * 4)(0, 1, 0, 0)
     q, k = case.q.data_ptr(), case.k.data_ptr()
-    for wrong in (dict(ctx=None), dict(struct_size=8), dict(rows=-1), dict(head_dim=0), dict(head_dim=513, rotary_dim=0, q_row=2000, q_head=600, k_row=600), dict(q_heads=-1), dict(k_heads=-1),
+    for wrong in (dict(ctx=None), dict(struct_size=8), dict(rows=-1), dict(rows=2 ** 31 - 1, q_row=D, q_head=2 ** 36, q_out_row=D, q_out_head=2 ** 36, k_heads=0), dict(head_dim=0), dict(head_dim=513, rotary_dim=0, q_row=2000, q_head=600, k_row=600), dict(q_heads=-1), dict(k_heads=-1),
                   dict(q_heads=1 << 21), dict(type=3), dict(type=-1), dict(rotary_dim=7), dict(rotary_dim=-2), dict(rotary_dim=18), dict(axes=0), dict(axes=5), dict(eps=-1.0),
                   dict(eps=float("nan")), dict(norm=0), dict(q=None), dict(k_out=None), dict(q=q + 1), dict(q_head=D - 1), dict(q_row=2 * D - 1), dict(k_row=D - 1),
                   dict(q_out_row=D), dict(q_row=1 << 62), dict(q_row=-32), dict(positions=None), dict(inv_freq=None), dict(positions=case.positions.data_ptr() + 2),
