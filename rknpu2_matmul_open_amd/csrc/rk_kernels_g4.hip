@@ -119,11 +119,11 @@ __global__ __launch_bounds__(256) void g4_stage_kernel(const uint16_t* x, int64_
 // registers, once; so do activations, which every workgroup reads for itself.
 // ROWS (1, 4, 8 or 16): up to so many rows.  A wave loads a row's 512 values together and turns them into operands through LDS of its own.  0: up to 16 rows,
 // loaded as the operands lie.
-// LONG: a wave has more pieces than it loads together; the next ones are on their way while it multiplies.
 // Products are with the code; the zero point times the group's sum of activations, which a product with ones gives, is taken off a group's sum.
 constexpr int FEW_PITCH = 1024 + 16; // bytes of a row of 512 values in LDS
+constexpr int few_area(int rows, int cn) { return rows * FEW_PITCH > cn * 1024 ? rows * FEW_PITCH : cn * 1024; }
 
-template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES>
+template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, int NP, int MAX_WAVES>
 __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W, const uint32_t* scales, const uint16_t* x, int64_t ldx, int M, int K,
                                                                 int per_wave, int workgroups, int waves, rkh_g4_args g) {
     constexpr int ONE = TYPE == RKH_MX4_F16 ? 0x3c003c00 : 0x3f803f80; // two of them
@@ -142,10 +142,17 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
         v4i w[NP][CN], x[ROWS ? ROWS * NP / 4 : NP * 4];
         words s[NP][CN];
     };
-    // (K is a multiple of eight; what lies beyond it is loaded from a row's start and dropped where it is used: a branch here would wait for
-    // the activations ahead of the codes' loads)
-    const auto fetch = [&](int m, int k) { return mx_fetch8<TYPE>(x, (size_t)m * ldx + (k < K ? k : 0)).w[0]; };
+    // (What lies beyond K, eight at least, is loaded from a row's last eight values and dropped where it is used: a branch here would wait for the activations
+    // ahead of the codes' loads.)
+    const auto fetch = [&](int m, int k) { return mx_fetch8<TYPE>(x, (size_t)m * ldx + min(k, K - 8)).w[0]; };
     const auto within = [&](const v4i& v, int k) { return k < K ? g4_turned_rows(v) : v4i{0, 0, 0, 0}; };
+    const auto moved = [&](const v4i& v, int k) { // where K ends within eight values: the last eight to their places
+        const int beyond = k < K ? max(k + 8 - K, 0) : 0, bits = 16 * (beyond & 3);
+        uint64_t low = (uint64_t)(uint32_t)v.y << 32 | (uint32_t)v.x, high = (uint64_t)(uint32_t)v.w << 32 | (uint32_t)v.z;
+        if (beyond >= 4) low = high, high = 0;
+        low = low >> bits | (high << 1) << (63 - bits), high >>= bits;
+        return v4i{(int)low, (int)(low >> 32), (int)high, (int)(high >> 32)};
+    };
     const auto load = [&](Batch& b, int from) { // (pieces beyond the last: that one again, which is not multiplied)
         if constexpr (ROWS) {
 #pragma unroll
@@ -172,7 +179,8 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
     v4f acc[CN];
 #pragma unroll
     for (int j = 0; j < CN; ++j) acc[j] = v4f{0, 0, 0, 0};
-    uint8_t* own = lds + wave * (ROWS * FEW_PITCH);
+    constexpr int AREA = few_area(ROWS, CN); // a wave's part of LDS: its activations, and in the end its sums
+    uint8_t* own = lds + wave * AREA;
     const auto multiply = [&](const Batch& b, int from) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
@@ -209,29 +217,33 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
             }
         }
     };
-    Batch now;
-    load(now, first);
-    if constexpr (!LONG) {
-        multiply(now, first);
-    } else {
-        for (int from = first;;) {
-            Batch next;
-            if (from + NP < last) load(next, from + NP);
-            multiply(now, from);
-            if ((from += NP) >= last) break;
-            now = next;
+    // (one batch of registers: other waves' loads are on their way meanwhile.  With the next batch's loads ahead of the products, which leaves room for half of
+    // the waves, 1 x 11008 x 14336 took 23.6 us, this way 17.7, and 8 x 4096 x 14336 10.3, 9.2)
+    for (int from = first;;) {
+        Batch b;
+        load(b, from);
+        if (ROWS < 16 && K % 8 && (from + NP) * 128 > K) { // (of sixteen rows it costs the loads' order 1.4 us of 12.3: those are staged)
+            if constexpr (ROWS) {
+#pragma unroll
+                for (int m = 0; m < ROWS * NP / 4; ++m) b.x[m] = moved(b.x[m], (from + m / ROWS * 4) * 128 + lane * 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NP * 4; ++i) b.x[i] = moved(b.x[i], from * 128 + i * 32 + q * 8);
+            }
         }
+        multiply(b, from);
+        if ((from += NP) >= last) break;
     }
 
     // the waves' sums, added in order: a thread takes one result (SwiGLU: both halves of one)
-    float* sums = reinterpret_cast<float*>(lds + waves * ROWS * FEW_PITCH);
 #pragma unroll
-    for (int j = 0; j < CN; ++j) *reinterpret_cast<v4f*>(sums + (wave * CN + j) * 256 + lane * 4) = acc[j];
+    for (int j = 0; j < CN; ++j) *reinterpret_cast<v4f*>(own + j * 1024 + lane * 16) = acc[j];
     __syncthreads();
     const auto total = [&](int i) {
-        float s = sums[i];
+        const float* from = reinterpret_cast<const float*>(lds) + i;
+        float s = *from;
 #pragma unroll 4
-        for (int o = 1; o < waves; ++o) s += sums[o * CN * 256 + i];
+        for (int o = 1; o < waves; ++o) s += from[o * (AREA / 4)];
         return s;
     };
     for (int i = threadIdx.x; i < (SWIGLU ? CN / 2 : CN) * 256; i += waves * 64) {
@@ -245,31 +257,35 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
 }
 
 constexpr int FEW_ROWS = 16;
+constexpr int G4_CUS = 256; // compute units that a launch is cut for
 
-// What a workgroup of the few-row kernel takes.  Where both sides were measured (bf16, one scale in 128, weights from HBM, us):
-//   rows at a time as they are in LDS, or as operands (ROWS 0): 8 x 4096 x 4096 4.4 and 6.6, 16 x 4096 x 4096 5.1 and 6.7;
-//   columns: activations are read by every workgroup, so more rows want more columns, where enough workgroups are left.  1 x 14336 x 4096 16 columns 7.9, 32
-//   8.1, 64 9.1; 4 rows of it 9.0, 8.3, 9.4; 8 rows 10.3, 10.6, 9.8 and, as operands, 64 columns 9.2; 16 rows 17.2, 12.4 and, as operands, 10.0;
-//   4 x 4096 x 4096 16 columns 4.4, 32 4.7;
-//   K in parts, which takes a second launch: 8 x 4096 x 14336 11.2 -> 12.4 at best, 16 rows of it 15.2 -> 13.4.
+// What a workgroup of the few-row kernel takes.  Where both sides were measured (fp16, one scale in 128, the weights of four layers in turn, us):
+//   rows at a time as they are in LDS, or as operands (ROWS 0) with 64 columns a workgroup, where there are columns for that: 16 rows x 8192 columns x K = 4096
+//   10.7 and 7.8, x 8192 13.5 and 13.7; x 11008 columns x 14336 33.3 and 27.8; 8 rows x 14336 x 8192 14.9 and 13.0, x 8192 x 8192 9.1 and 11.6; 4 rows x 14336
+//   x 14336 26.0 and 22.8, x 8192 12.2 and 12.5;
+//   waves, where there are more workgroups than compute units and several share one: 8 rows x 8192 x 8192 16 waves 10.2, 8 9.1, 4 10.8; 16 rows x 6144 x 14336
+//   8 waves 21.5, 4 18.0; 4 rows x 8192 x 14336 16 waves 12.1, 8 13.1; where there are not: 8 rows x 4096 x 14336 16 waves 8.8, 8 9.4, 4 10.8;
+//   columns of four rows: x 14336 x 4096 16 columns 9.0, 32 8.3, x 4096 x 4096 4.4 and 4.7;
+//   K in parts, which takes a second launch: 8 x 4096 x 14336 8.8 -> 12 at best.
 struct FewShape {
     int rows, cn, most; // LDS rows of a wave (0: none), blocks of 16 places, most waves
 };
 // (more than eight waves leave 128 registers for a lane, which is too few for two blocks or many groups and rows at once)
 FewShape few_shape(int M, int64_t blocks, int KB, int gpb, bool swiglu) {
-    if (KB <= 32 && ((M > 8 && blocks >= 512) || (M > 4 && blocks >= 768))) return {0, 4, 16};
+    if ((M > 4 && blocks >= 640) || (M > 8 && blocks >= 512 && KB <= 32) || (M > 1 && blocks >= 768 && KB > 64)) return {0, 4, 16};
     const int rows = M == 1 ? 1 : M <= 4 ? 4 : M <= 8 ? 8 : 16;
-    const bool two = swiglu || (rows == 4 && blocks >= 768 && KB <= 32);
-    return {rows, two ? 2 : 1, two || rows == 16 || (rows == 8 && gpb == 4) ? 8 : 16};
+    const int cn = swiglu || (rows == 4 && blocks >= 768 && KB <= 32) ? 2 : 1;
+    const bool shared = blocks / cn > G4_CUS;
+    return {rows, cn, rows == 16 ? shared ? 4 : 8 : cn == 2 || (rows == 8 && (shared || gpb == 4)) ? 8 : 16};
 }
 
-template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
+template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
     const int KB = (int)rkh_g4_kb(g.K), waves = (KB + per - 1) / per;
     const int64_t workgroups = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / (16 * CN);
     if (workgroups * waves * 64 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
-    constexpr size_t BYTES = CN * 1024 + ROWS * FEW_PITCH; // of a wave
+    constexpr size_t BYTES = few_area(ROWS, CN); // of a wave
     static_assert(MAX_WAVES * BYTES <= 160 * 1024, "");
-    const auto kernel = g4_few_kernel<TYPE, CN, GPB, ROWS, SWIGLU, LONG, NP, MAX_WAVES>;
+    const auto kernel = g4_few_kernel<TYPE, CN, GPB, ROWS, SWIGLU, NP, MAX_WAVES>;
     static std::atomic<bool> opted_in[64] = {};
     if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(kernel), opted_in, 160 * 1024)) return rc;
     mark(st, "g4_few_kernel");
@@ -283,19 +299,15 @@ template <int TYPE, int GPB, bool SWIGLU> int launch_few(hipStream_t st, const r
     const FewShape shape = few_shape(g.M, rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / 16, KB, GPB, SWIGLU);
     // pieces of a wave: up to four (as operands: two) that are loaded together, eight waves where they go round, and as many as there are waves for
     const int np = shape.rows ? 4 : 2, per = std::max((KB + shape.most - 1) / shape.most, std::min(np, (KB + 7) / 8));
-    if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, false, 2, 16>(st, g, per);
-    const auto go = [&](auto is_long) {
-        constexpr bool LONG = decltype(is_long)::value;
-        constexpr int CN = SWIGLU ? 2 : 1, MOST = SWIGLU ? 8 : 16;
-        if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, LONG, 4, MOST>(st, g, per);
-        if constexpr (!SWIGLU && !LONG) {
-            if (shape.cn == 2) return launch_few<TYPE, 2, GPB, 4, SWIGLU, LONG, 4, 8>(st, g, per);
-        }
-        if (shape.rows == 4) return launch_few<TYPE, CN, GPB, 4, SWIGLU, LONG, 4, MOST>(st, g, per);
-        if (shape.rows == 8) return launch_few<TYPE, CN, GPB, 8, SWIGLU, LONG, 4, GPB == 4 ? 8 : MOST>(st, g, per);
-        return launch_few<TYPE, CN, GPB, 16, SWIGLU, LONG, 4, 8>(st, g, per);
-    };
-    return per > 4 ? go(std::true_type{}) : go(std::false_type{});
+    if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, 2, 16>(st, g, per);
+    constexpr int CN = SWIGLU ? 2 : 1, MOST = SWIGLU ? 8 : 16;
+    if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, 4, MOST>(st, g, per);
+    if constexpr (!SWIGLU) {
+        if (shape.cn == 2) return launch_few<TYPE, 2, GPB, 4, SWIGLU, 4, 8>(st, g, per);
+    }
+    if (shape.rows == 4) return launch_few<TYPE, CN, GPB, 4, SWIGLU, 4, MOST>(st, g, per);
+    if (shape.rows == 8) return launch_few<TYPE, CN, GPB, 8, SWIGLU, 4, GPB == 4 ? 8 : MOST>(st, g, per);
+    return launch_few<TYPE, CN, GPB, 16, SWIGLU, 4, 8>(st, g, per);
 }
 template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
     if (g.swiglu) return g.gpb == 1 ? launch_few<TYPE, 1, true>(st, g) : g.gpb == 2 ? launch_few<TYPE, 2, true>(st, g) : launch_few<TYPE, 4, true>(st, g);
@@ -303,8 +315,6 @@ template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
 }
 
 // ---- which kernel ------------------------------------------------------------------
-constexpr int G4_CUS = 256; // compute units that a launch is cut for
-
 // Tiles of 32 rm rows x 128 places: what a step of 128 k takes when every compute unit has one, what a launch has beside its steps, and what another round has, us;
 // how many share a compute unit.  From 64 x 14336 x 4096 (32 rows: 17.3), 512 x 4096 x 4096 (64: 26.7; 128 in two parts: 28.7), 512 x 14336 x 4096 (256: 61) and
 // their like with K = 14336.
@@ -360,10 +370,10 @@ int rkh_g4_run(void* stream, const rkh_g4_args* args) {
     if (!args->M || !args->N) return RKH_OK;
     const hipStream_t st = (hipStream_t)stream;
     rkh_g4_args g = *args;
-    // few rows are taken as they are when they are whole pieces of eight values; tiles copy fp16 rows to LDS that are whole pieces of 128, 16-byte
+    // few rows are taken as they are when they are whole pieces of eight values, or eight rows at most and values at least; tiles copy fp16 rows to LDS that are whole pieces of 128, 16-byte
     // aligned and less than 2^32 bytes of a tile apart
     const bool few = g.M <= FEW_ROWS;
-    const bool as_is = few ? g.K % 8 == 0
+    const bool as_is = few ? g.K % 8 == 0 || (g.K >= 8 && g.M <= 8)
                            : g.x_type == RKH_MX4_F16 && g.K % 128 == 0 && g.ldx % 8 == 0 && g.ldx <= 1 << 22 && reinterpret_cast<uintptr_t>(g.x) % 16 == 0;
     if (as_is) {
         g.exponents = nullptr;
