@@ -272,7 +272,7 @@ struct FewShape {
 };
 // (more than eight waves leave 128 registers for a lane, which is too few for two blocks or many groups and rows at once)
 FewShape few_shape(int M, int64_t blocks, int KB, int gpb, bool swiglu) {
-    if ((M > 4 && blocks >= 640) || (M > 8 && blocks >= 512 && KB <= 32) || (M > 1 && blocks >= 768 && KB > 64)) return {0, 4, 16};
+    if ((M > 4 && blocks >= 640) || (M > 8 && blocks >= 512 && KB <= 32) || (M > 1 && blocks >= 768 && KB > 64)) return {0, 4, gpb == 4 ? 8 : 16};
     const int rows = M == 1 ? 1 : M <= 4 ? 4 : M <= 8 ? 8 : 16;
     const int cn = swiglu || (rows == 4 && blocks >= 768 && KB <= 32) ? 2 : 1;
     const bool shared = blocks / cn > G4_CUS;
@@ -299,7 +299,7 @@ template <int TYPE, int GPB, bool SWIGLU> int launch_few(hipStream_t st, const r
     const FewShape shape = few_shape(g.M, rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / 16, KB, GPB, SWIGLU);
     // pieces of a wave: up to four (as operands: two) that are loaded together, eight waves where they go round, and as many as there are waves for
     const int np = shape.rows ? 4 : 2, per = std::max((KB + shape.most - 1) / shape.most, std::min(np, (KB + 7) / 8));
-    if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, 2, 16>(st, g, per);
+    if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, 2, GPB == 4 ? 8 : 16>(st, g, per);
     constexpr int CN = SWIGLU ? 2 : 1, MOST = SWIGLU ? 8 : 16;
     if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, 4, MOST>(st, g, per);
     if constexpr (!SWIGLU) {
