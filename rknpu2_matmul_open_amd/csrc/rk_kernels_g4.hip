@@ -264,7 +264,8 @@ constexpr int G4_CUS = 256; // compute units that a launch is cut for
 //   10.7 and 7.8, x 8192 13.5 and 13.7; x 11008 columns x 14336 33.3 and 27.8; 8 rows x 14336 x 8192 14.9 and 13.0, x 8192 x 8192 9.1 and 11.6; 4 rows x 14336
 //   x 14336 26.0 and 22.8, x 8192 12.2 and 12.5;
 //   waves, where there are more workgroups than compute units and several share one: 8 rows x 8192 x 8192 16 waves 10.2, 8 9.1, 4 10.8; 16 rows x 6144 x 14336
-//   8 waves 21.5, 4 18.0; 4 rows x 8192 x 14336 16 waves 12.1, 8 13.1; where there are not: 8 rows x 4096 x 14336 16 waves 8.8, 8 9.4, 4 10.8;
+//   8 waves 21.5, 4 18.0; 4 rows x 8192 x 14336 16 waves 12.1, 8 13.1; 1 row of it with groups of 32 18.6,
+//   16.1; where there are not: 8 rows x 4096 x 14336 16 waves 8.8, 8 9.4, 4 10.8;
 //   columns of four rows: x 14336 x 4096 16 columns 9.0, 32 8.3, x 4096 x 4096 4.4 and 4.7;
 //   K in parts, which takes a second launch: 8 x 4096 x 14336 8.8 -> 12 at best.
 struct FewShape {
@@ -276,7 +277,7 @@ FewShape few_shape(int M, int64_t blocks, int KB, int gpb, bool swiglu) {
     const int rows = M == 1 ? 1 : M <= 4 ? 4 : M <= 8 ? 8 : 16;
     const int cn = swiglu || (rows == 4 && blocks >= 768 && KB <= 32) ? 2 : 1;
     const bool shared = blocks / cn > G4_CUS;
-    return {rows, cn, rows == 16 ? shared ? 4 : 8 : cn == 2 || (rows == 8 && (shared || gpb == 4)) ? 8 : 16};
+    return {rows, cn, rows == 16 ? shared ? 4 : 8 : cn == 2 || (shared && (rows == 8 || gpb == 4)) || (rows == 8 && gpb == 4) ? 8 : 16};
 }
 
 template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
