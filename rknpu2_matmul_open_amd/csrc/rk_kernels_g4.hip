@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void g4_stage_kernel(const uint16_t* x, int64_
 constexpr int FEW_PITCH = 1024 + 16; // bytes of a row of 512 values in LDS
 constexpr int few_area(int rows, int cn) { return rows * FEW_PITCH > cn * 1024 ? rows * FEW_PITCH : cn * 1024; }
 
-template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, int NP, int MAX_WAVES>
+template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES>
 __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W, const uint32_t* scales, const uint16_t* x, int64_t ldx, int M, int K,
                                                                 int per_wave, int workgroups, int waves, rkh_g4_args g) {
     constexpr int ONE = TYPE == RKH_MX4_F16 ? 0x3c003c00 : 0x3f803f80; // two of them
@@ -217,8 +217,9 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
             }
         }
     };
-    // (one batch of registers: other waves' loads are on their way meanwhile.  With the next batch's loads ahead of the products, which leaves room for half of
-    // the waves, 1 x 11008 x 14336 took 23.6 us, this way 17.7, and 8 x 4096 x 14336 10.3, 9.2)
+    // LONG: a wave has more pieces than it loads together.  (One batch of registers: other waves' loads are on their way meanwhile.  With the next batch's loads
+    // ahead of the products, which leaves room for half of the waves, 1 x 11008 x 14336 took 23.6 us, this way 17.7, and 8 x 4096 x 14336 10.3, 8.9.  Written
+    // as a loop where there is one batch, the kernel has ten registers more: SwiGLU of 1 x 14336 x 4096 13.2 -> 14.1.)
     for (int from = first;;) {
         Batch b;
         load(b, from);
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
             }
         }
         multiply(b, from);
-        if ((from += NP) >= last) break;
+        if (!LONG || (from += NP) >= last) break;
     }
 
     // the waves' sums, added in order: a thread takes one result (SwiGLU: both halves of one)
@@ -280,13 +281,13 @@ FewShape few_shape(int M, int64_t blocks, int KB, int gpb, bool swiglu) {
     return {rows, cn, rows == 16 ? shared ? 4 : 8 : cn == 2 || (shared && (rows == 8 || gpb == 4)) || (rows == 8 && gpb == 4) ? 8 : 16};
 }
 
-template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
+template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
     const int KB = (int)rkh_g4_kb(g.K), waves = (KB + per - 1) / per;
     const int64_t workgroups = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / (16 * CN);
     if (workgroups * waves * 64 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
     constexpr size_t BYTES = few_area(ROWS, CN); // of a wave
     static_assert(MAX_WAVES * BYTES <= 160 * 1024, "");
-    const auto kernel = g4_few_kernel<TYPE, CN, GPB, ROWS, SWIGLU, NP, MAX_WAVES>;
+    const auto kernel = g4_few_kernel<TYPE, CN, GPB, ROWS, SWIGLU, LONG, NP, MAX_WAVES>;
     static std::atomic<bool> opted_in[64] = {};
     if (const int rc = mx_allow_lds(reinterpret_cast<const void*>(kernel), opted_in, 160 * 1024)) return rc;
     mark(st, "g4_few_kernel");
@@ -300,15 +301,19 @@ template <int TYPE, int GPB, bool SWIGLU> int launch_few(hipStream_t st, const r
     const FewShape shape = few_shape(g.M, rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / 16, KB, GPB, SWIGLU);
     // pieces of a wave: up to four (as operands: two) that are loaded together, eight waves where they go round, and as many as there are waves for
     const int np = shape.rows ? 4 : 2, per = std::max((KB + shape.most - 1) / shape.most, std::min(np, (KB + 7) / 8));
-    if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, 2, GPB == 4 ? 8 : 16>(st, g, per);
-    constexpr int CN = SWIGLU ? 2 : 1, MOST = SWIGLU ? 8 : 16;
-    if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, 4, MOST>(st, g, per);
-    if constexpr (!SWIGLU) {
-        if (shape.cn == 2) return launch_few<TYPE, 2, GPB, 4, SWIGLU, 4, 8>(st, g, per);
-    }
-    if (shape.rows == 4) return launch_few<TYPE, CN, GPB, 4, SWIGLU, 4, MOST>(st, g, per);
-    if (shape.rows == 8) return launch_few<TYPE, CN, GPB, 8, SWIGLU, 4, GPB == 4 ? 8 : MOST>(st, g, per);
-    return launch_few<TYPE, CN, GPB, 16, SWIGLU, 4, 8>(st, g, per);
+    const auto go = [&](auto is_long) {
+        constexpr bool LONG = decltype(is_long)::value;
+        if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, LONG, 2, GPB == 4 ? 8 : 16>(st, g, per);
+        constexpr int CN = SWIGLU ? 2 : 1, MOST = SWIGLU ? 8 : 16;
+        if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, LONG, 4, MOST>(st, g, per);
+        if constexpr (!SWIGLU && !LONG) {
+            if (shape.cn == 2) return launch_few<TYPE, 2, GPB, 4, SWIGLU, LONG, 4, 8>(st, g, per);
+        }
+        if (shape.rows == 4) return launch_few<TYPE, CN, GPB, 4, SWIGLU, LONG, 4, MOST>(st, g, per);
+        if (shape.rows == 8) return launch_few<TYPE, CN, GPB, 8, SWIGLU, LONG, 4, GPB == 4 ? 8 : MOST>(st, g, per);
+        return launch_few<TYPE, CN, GPB, 16, SWIGLU, LONG, 4, 8>(st, g, per);
+    };
+    return per > np ? go(std::true_type{}) : go(std::false_type{});
 }
 template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
     if (g.swiglu) return g.gpb == 1 ? launch_few<TYPE, 1, true>(st, g) : g.gpb == 2 ? launch_few<TYPE, 2, true>(st, g) : launch_few<TYPE, 4, true>(st, g);
