@@ -585,8 +585,8 @@ def _g4_array(x, shape, types, what, device):
     if str(x.dtype) not in types or tuple(x.shape) != shape:
         raise ValueError("%s: %s of shape %s, got %s %s" % (what, " or ".join(types), shape, x.dtype, tuple(x.shape)))
     if device is None:
-        if not x.flags.c_contiguous:
-            raise ValueError("%s: a contiguous array" % what)
+        if not hasattr(x, "ctypes") or not x.flags.c_contiguous:
+            raise ValueError("%s: a contiguous numpy array (tensors: from_device)" % what)
         return C.c_void_p(x.ctypes.data)
     _on_device(x, device)
     if not x.is_contiguous():
@@ -710,6 +710,8 @@ def heads_args(session, q, k, q_out=None, k_out=None, norm=True, eps=1e-6, q_wei
         pairs = inv_freq.shape[0]
         a.inv_freq = _channel(inv_freq, pairs, "inv_freq", device)
         a.rotary_dim = 2 * pairs
+        if positions is None:
+            raise ValueError("inv_freq without positions")
         _on_device(positions, device)
         if str(positions.dtype) != "torch.int32" or len(positions.shape) not in (1, 2) or positions.shape[-1] != rows or (rows > 1 and positions.stride(-1) != 1):
             raise ValueError("positions: int32 [%d] or [axes, %d] with contiguous rows, got %s %s" % (rows, rows, positions.dtype, tuple(positions.shape)))

@@ -41,6 +41,8 @@ def test_weights_are_checked():
         with pytest.raises(ValueError):
             ops.G4Weights(s, K, N, group, codes, scales)
     with pytest.raises(ValueError):
+        ops.G4Weights(s, K, N, group, torch.zeros((N, 38), dtype=torch.uint8), np.zeros((N, 3), np.float16))
+    with pytest.raises(ValueError):
         ops.G4Weights(s, K, N, 0, np.zeros((N, 38), np.uint8), np.zeros((N, 3), np.float16))
     assert len(s.lib.calls) == 4
 
@@ -91,6 +93,7 @@ def test_heads_are_checked():
                  lambda: ops.heads_norm_rotate(s, t(4), None, k_out=t(2)), lambda: ops.heads_norm_rotate(s, t(4, index=0), t(2)),
                  lambda: ops.heads_norm_rotate(s, t(4), t(2), k_out=t(2, index=0)), lambda: ops.heads_norm_rotate(s, t(4), t(2), q_weight=channel(15)),
                  lambda: ops.heads_norm_rotate(s, t(4), t(2), k_weight=channel(D, index=0)), lambda: ops.heads_norm_rotate(s, t(4), t(2), positions=pos(rows)),
+                 lambda: ops.heads_norm_rotate(s, t(4), t(2), inv_freq=channel(8)), lambda: ops.heads_norm_rotate(s, t(4), t(2), pair_axis=[0] * 8),
                  lambda: ops.heads_norm_rotate(s, t(4), t(2), positions=pos(rows - 1), inv_freq=channel(8)),
                  lambda: ops.heads_norm_rotate(s, t(4), t(2), positions=pos(rows, dtype=torch.int64), inv_freq=channel(8)),
                  lambda: ops.heads_norm_rotate(s, t(4), t(2), positions=pos(rows, index=0), inv_freq=channel(8)),
