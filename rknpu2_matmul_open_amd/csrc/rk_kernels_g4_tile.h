@@ -60,6 +60,31 @@ template <int R> __device__ __forceinline__ uint32_t g4_pair_here(uint32_t w, co
     return v;
 }
 
+// The same for the four pairs of a dword, for a wave that has nothing to wait for in between.
+__device__ __forceinline__ v4i g4_dword_here(uint32_t w, const G4Zero& z, uint32_t magic) {
+    uint32_t v0, v1, v2, v3, upper;
+    asm volatile("v_and_or_b32 %0, %5, %6, %8\n\tv_and_or_b32 %1, %5, %7, %8\n\tv_lshrrev_b32 %4, 8, %5\n\tv_pk_add_f16 %0, %0, %9\n\tv_pk_fma_f16 %1, %1, %11, %10\n\t"
+                 "v_and_or_b32 %2, %4, %6, %8\n\tv_and_or_b32 %3, %4, %7, %8\n\tv_pk_add_f16 %2, %2, %9\n\tv_pk_fma_f16 %3, %3, %11, %10"
+                 : "=&v"(v0), "=&v"(v1), "=&v"(v2), "=&v"(v3), "=&v"(upper)
+                 : "v"(w), "s"(0x000f000fu), "s"(0x00f000f0u), "v"(magic), "v"(z.low), "v"(z.high), "s"(0x2c002c00u));
+    return v4i{(int)v0, (int)v1, (int)v2, (int)v3};
+}
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm" // m0 is set and clobbered on purpose below
+// mx_copy to `to` + `more`, which M0 takes as the sum that it is.
+__device__ __forceinline__ void g4_copy(const uint8_t* base, unsigned off, uint32_t to, uint32_t more) {
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to), "s"(more) : "memory", "m0", "scc");
+}
+template <int MORE> __device__ __forceinline__ void g4_copy(const uint8_t* base, unsigned off, uint32_t to) {
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to), "n"(MORE) : "memory", "m0", "scc");
+}
+// mx_copy_two
+__device__ __forceinline__ void g4_copy_two(const uint8_t* base, const uint8_t* base2, unsigned off, uint32_t to, uint32_t more) {
+    asm volatile("s_add_u32 m0, %3, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\tglobal_load_lds_dwordx4 %0, %2 offset:1024" ::"v"(off), "s"(base), "s"(base2),
+                 "s"(to), "s"(more) : "memory", "m0", "scc");
+}
+#pragma clang diagnostic pop
+
 // What a launch of tiles covers, and the numbers that its workgroups would divide by.  (With divisions, of 64 bits among them, a workgroup of 32 rows had its
 // first address after 2000 clocks and not after 1200, and 32 x 4096 x 4096 took 11.8 us, now 10.4.)
 struct G4Grid {
@@ -421,6 +446,7 @@ __global__ __launch_bounds__(256) void g4_rows_tile_kernel(G4Grid t, rkh_g4_args
     const uint32_t base = (uint32_t)(uintptr_t)(mx_lds_ptr)lds;
     const int m0 = mblk * S::ROWS;
     const uint8_t* x_src = static_cast<const uint8_t*>(g.x) + ((size_t)m0 * g.ldx + (size_t)kb0 * 128) * 2;
+    const uint8_t* x_src2 = x_src + 128;
     unsigned x_off[RM]; // of eight rows' 128 bytes; rows beyond M: the last one again
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
@@ -432,25 +458,29 @@ __global__ __launch_bounds__(256) void g4_rows_tile_kernel(G4Grid t, rkh_g4_args
     for (int i = 0; i < 2; ++i) w_src[i] = g.W + ((size_t)min(nblk * 8 + wave * 2 + i, t.blocks - 1) * KB + kb0) * 1024 - i * 1024;
     const unsigned s_lane = (GPB == 4 ? (wave & 1) * 1024 : 0) + lane * 16, s_at_tile = s_lane % (512 * GPB);
     const uint8_t* s_src = reinterpret_cast<const uint8_t*>(g.w_scale) + ((size_t)nblk * 8 * KB + kb0) * (64 * GPB);
-    const unsigned s_off = (unsigned)min((int)(s_at_tile / (64 * GPB)), t.blocks - 1 - nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
+    const unsigned s_first = (unsigned)min((int)(s_at_tile / (64 * GPB)), t.blocks - 1 - nblk * 8) * (unsigned)KB * (64 * GPB) + s_at_tile % (64 * GPB);
+    unsigned w_off = lane * 16, s_off = s_first;
+    const uint32_t x_to = base + wave * RM * 1024, w_to = base + S::W_OFF + wave * 2048, s_to = base + S::S_OFF + (GPB == 4 ? (wave & 1) * 1024 : 0);
     int ahead = kb1 - kb0; // steps that are still to be copied
     const auto copy = [&](uint32_t to, auto p_tag) { // statement P: activations of eight rows, 64 k and 64 k; codes; scales
         constexpr int P = decltype(p_tag)::value;
         if constexpr (P < RM) {
-            mx_copy(x_src, x_off[P], base + to + (wave * RM + P) * 1024);
-            mx_copy(x_src + 128, x_off[P], base + to + S::HALF + (wave * RM + P) * 1024);
+            g4_copy<P * 1024>(x_src, x_off[P], to + x_to);
+            g4_copy<S::HALF + P * 1024>(x_src2, x_off[P], to + x_to);
         } else if constexpr (P == RM) {
-            mx_copy_two(w_src[0], lane * 16, w_src[1], lane * 16, base + to + S::W_OFF + wave * 2048);
+            g4_copy_two(w_src[0], w_src[1], w_off, to, w_to);
         } else {
-            mx_copy(s_src, s_off, base + to + S::S_OFF + (GPB == 4 ? (wave & 1) * 1024 : 0));
+            g4_copy(s_src, s_off, to, s_to);
         }
     };
+    // (a wave issues an instruction every five clocks, scalar ones among them: lanes' offsets advance, not addresses)
     const auto copied = [&]() { // (behind the last step: that one again, which nobody reads)
-        if (--ahead > 0) {
-            x_src += 256;
-            w_src[0] += 1024, w_src[1] += 1024;
-            s_src += 64 * GPB;
-        }
+        const bool more = --ahead > 0;
+        const unsigned x_by = more ? 256 : 0, w_by = more ? 1024 : 0, s_by = more ? 64 * GPB : 0;
+#pragma unroll
+        for (int r = 0; r < RM; ++r) x_off[r] += x_by;
+        w_off += w_by;
+        s_off += s_by;
     };
 
     // ---- LDS reads
@@ -484,6 +514,14 @@ __global__ __launch_bounds__(256) void g4_rows_tile_kernel(G4Grid t, rkh_g4_args
             for (int n = 0; n < GPB; ++n) zero[n].of(sd[n]);
         }
         w[P][ST][R] = (int)g4_pair_here<R>((uint32_t)raw[ST & 1][ST >> 1], zero[ST * GPB / 8], magic, upper);
+    };
+    const auto decode_dword = [&](auto p_tag, auto st_tag) {
+        constexpr int P = decltype(p_tag)::value, ST = decltype(st_tag)::value;
+        if constexpr (ST == 0) {
+#pragma unroll
+            for (int n = 0; n < GPB; ++n) zero[n].of(sd[n]);
+        }
+        w[P][ST] = g4_dword_here((uint32_t)raw[ST & 1][ST >> 1], zero[ST * GPB / 8], magic);
     };
     const auto scale_of = [&](auto p_tag) {
         constexpr int P = decltype(p_tag)::value;
@@ -536,7 +574,10 @@ __global__ __launch_bounds__(256) void g4_rows_tile_kernel(G4Grid t, rkh_g4_args
                 fold(std::integral_constant<int, F / GROUPS>{}, std::integral_constant<int, F % GROUPS>{}, std::integral_constant<int, 16 * O / (L - 1)>{},
                      std::integral_constant<int, 16 * (O + 1) / (L - 1)>{});
             if constexpr (T == 0) read_w(next);
-            if constexpr (T >= CODES_FROM) {
+            if constexpr (RM <= 2 && T >= CODES_FROM) {
+                constexpr int N = SLOTS - CODES_FROM, X0 = 8 * (T - CODES_FROM) / N, X1 = 8 * (T + 1 - CODES_FROM) / N;
+                static_for<X1 - X0>([&](auto x) { decode_dword(std::integral_constant<int, 1 - P>{}, std::integral_constant<int, X0 + decltype(x)::value>{}); });
+            } else if constexpr (T >= CODES_FROM) {
                 constexpr int N = SLOTS - CODES_FROM, X0 = 32 * (T - CODES_FROM) / N, X1 = 32 * (T + 1 - CODES_FROM) / N;
                 static_for<X1 - X0>([&](auto x) { decode(std::integral_constant<int, 1 - P>{}, std::integral_constant<int, X0 + decltype(x)::value>{}); });
             }
