@@ -321,17 +321,28 @@ template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
 }
 
 // ---- which kernel ------------------------------------------------------------------
-// Tiles of 32 rm rows x 128 places: what a step of 128 k takes when every compute unit has one, what a launch has beside its steps, and what another round has, us;
-// how many share a compute unit.  From 64 x 14336 x 4096 (32 rows: 17.3), 512 x 4096 x 4096 (64: 26.7; 128 in two parts: 28.7), 512 x 14336 x 4096 (256: 61) and
-// their like with K = 14336.
-struct G4Shape { int rm; float step, launch, round; int share; };
-constexpr G4Shape G4_SHAPES[] = {{8, 1.75f, 5.0f, 4.0f, 1}, {4, 1.1f, 5.0f, 2.0f, 1}, {2, 0.7f, 4.3f, 0.5f, 2}, {1, 0.4f, 4.3f, 0.5f, 2}};
-constexpr float G4_JOIN_US = 3.5f, G4_JOIN_RATE = 1.2e7f; // a launch that adds parts, and its bytes per us
+// Tiles of 32 rm rows x 128 places: us of a step of 128 k where up to half of the compute units have a tile, where all have one, and, for tiles of which two share a
+// unit, where few and where all have two.  (What all units do at once they do slower.)  From products of K = 4096 and groups of 128, us, with 32, 64, 128 and 256 rows:
+//   128 x 8192 15.7 19.7 28.5;  x 11008 23.7 20.3 28.7;  x 28672 49.8 39.9 39.4;  256 x 4096 15.7 19.5 29.3 48;  x 5504 23.9 20.3 29.6;  x 8192 27.4 22.8 29.7 48.1;
+//   512 x 8192 51.6 40.5 39.8 48.8;  x 11008 72.1 57.2 67.6 54.2;  x 14336 87.5 73.2 73.3 61.3;  1024 x 14336 170 132 147 123;  2048 x 8192 - 149 154 133.
+//   And of K = 1024: 1000 x 4096 - 15.1 14.6 18.5;  4096 x 4096 - 49.6 52.0 45.5.
+struct G4Shape { int rm; float few, all, some_two, all_two; int share; float launch, round; }; // launch, round: what a launch has beside its steps, and what another round has
+constexpr G4Shape G4_SHAPES[] = {{8, 1.31f, 1.90f, 0, 0, 1, 7.0f, 5.0f},
+                                 {4, 0.75f, 1.09f, 0, 0, 1, 5.0f, 3.5f},
+                                 {2, 0.465f, 0.575f, 0.90f, 1.105f, 2, 4.6f, 2.0f},
+                                 {1, 0.33f, 0.36f, 0.61f, 0.73f, 2, 4.0f, 1.0f}};
+constexpr float G4_JOIN_US = 2.4f, G4_JOIN_RATE = 1.2e7f; // a launch that adds parts, and its bytes per us
 constexpr int G4_MOST_PARTS = 16;
 
-// The tiles that are expected to take the least time.  Where both sides of a choice were measured, us: 64 x 4096 x 4096 32 rows in four parts 11.6, 64 rows in
-// eight 13.5, 32 rows in one 16.3; 128 x 11008 x 4096 64 rows 22.3, 128 rows in two parts 24.8; 256 x 4096 x 4096 64 rows in two parts 20.9, in one 22.8, 128 rows
-// 29.8; 512 x 4096 x 4096 64 rows 26.7, 128 rows in two parts 28.7, 256 rows 48; 512 x 14336 x 4096 256 rows 61, 64 rows 72; 4096 x 14336 x 4096 442 and 518.
+float g4_steps_us(const G4Shape& s, int64_t tiles, int64_t steps) {
+    const int64_t round = (int64_t)G4_CUS * s.share, whole = tiles / round, rest = tiles % round;
+    const auto step = [&](int64_t n) {
+        return n <= G4_CUS ? s.few + (s.all - s.few) * std::max(0.0f, n * 2.0f / G4_CUS - 1) : s.some_two + (s.all_two - s.some_two) * ((float)n / G4_CUS - 1);
+    };
+    return s.launch + steps * (whole * (whole ? step(round) : 0) + (rest ? step(rest) : 0)) + s.round * (whole + (rest > 0) - 1);
+}
+
+// The tiles that are expected to take the least time.  (K in parts, us: 64 x 4096 x 4096 32 rows in four parts 9.7, in one 15.3; 128 x 4096 x 4096 in two 12.6.)
 rkk::G4Route g4_route(int M, int N, int K, int swiglu) {
     const int64_t places = rkh_g4_places(swiglu ? 2 * (int64_t)N : N, swiglu), KB = rkh_g4_kb(K);
     rkk::G4Route best{};
@@ -343,12 +354,10 @@ rkk::G4Route g4_route(int M, int N, int K, int swiglu) {
         r.mblocks = (M + 32 * s.rm - 1) / (32 * s.rm);
         r.nblocks = (int)((places + 127) / 128);
         const int64_t tiles = (int64_t)r.mblocks * r.nblocks;
-        // (tiles that share a compute unit fill the last round, those that do not wait for it)
-        const float rounds = s.share > 1 ? std::max(1.0f, (float)tiles / G4_CUS) : (float)((tiles + G4_CUS - 1) / G4_CUS);
-        float us = s.launch + rounds * KB * s.step + (rounds - 1) * s.round;
+        float us = g4_steps_us(s, tiles, KB);
         if (us < least) least = us, best = r;
         for (int64_t parts = 2; parts <= KB / 2 && parts <= G4_MOST_PARTS && tiles * parts <= G4_CUS; ++parts) {
-            us = s.launch + (KB + parts - 1) / parts * s.step + G4_JOIN_US + (float)M * places * 8 * parts / G4_JOIN_RATE;
+            us = g4_steps_us(s, tiles * parts, (KB + parts - 1) / parts) + G4_JOIN_US + (float)M * places * 8 * parts / G4_JOIN_RATE;
             if (us < least) least = us, best = r, best.parts = (int)parts;
         }
     }
