@@ -127,7 +127,7 @@ rk_npu_g4_workspace* rk_npu_g4_workspace_create(rk_npu_iommu_domain* domain, int
     const size_t scratch = rkh_g4_scratch_most(max_rows, K);
     const OnDevice device(domain->ctx->device);
     std::lock_guard<std::mutex> lock(domain->ctx->submit_mutex);
-    if (ws->staged.alloc(ws->owner, rkh_g4_staged_bytes(max_rows, K), false) || ws->exponents.alloc(ws->owner, (size_t)max_rows * 4, false) ||
+    if (ws->staged.alloc(ws->owner, rkh_g4_staged_bytes(max_rows, K), false) || ws->exponents.alloc(ws->owner, (size_t)rkh_align_up(max_rows, 256) * 4, false) ||
         (scratch && ws->scratch.alloc(ws->owner, scratch, false)))
         return nullptr;
     return ws.release();

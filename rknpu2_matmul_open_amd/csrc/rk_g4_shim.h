@@ -56,7 +56,7 @@ typedef struct rkh_g4_args {
     void* C;
     int64_t ldc;
     uint16_t* staged;    /* staged rows, where a product needs them */
-    int* exponents;      /* of M rows                               */
+    int* exponents;      /* of M rows, and room for whole tiles of 256 */
     float* scratch;      /* partial tiles of a K split over workgroups */
     size_t scratch_bytes;
 } rkh_g4_args;

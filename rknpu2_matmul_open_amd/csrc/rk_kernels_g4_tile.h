@@ -115,8 +115,15 @@ struct G4Grid {
     __device__ __forceinline__ int begin(int part) const { return part * each + min(part, more); }
     __device__ __forceinline__ int KB() const { return begin(parts); }
 };
+// The exponents of four rows from `first` on.  (All of them are fetched ahead of the first store, behind which a load would wait: 1622 x 1335 x 1536 of bf16 32.7 us
+// with a load a row, now EXPONENTS_US.)
+template <bool EXPONENTS> __device__ __forceinline__ v4i g4_exponents4(const rkh_g4_args& g, int first) {
+    if constexpr (EXPONENTS) return *reinterpret_cast<const v4i*>(g.exponents + first);
+    else return v4i{0, 0, 0, 0};
+}
 // Four rows from `first` on of a lane's two columns (SwiGLU: of both halves of one) from accumulators of 32 x 32 to results; n: the first column.
-template <int OUT, bool SWIGLU, bool EXPONENTS> __device__ __forceinline__ void g4_finish4(const rkh_g4_args& g, int first, int64_t n, const float* s0, const float* s1) {
+template <int OUT, bool SWIGLU, bool EXPONENTS>
+__device__ __forceinline__ void g4_finish4(const rkh_g4_args& g, int first, int64_t n, const float* s0, const float* s1, const v4i& exponents) {
     using T = typename MxType<OUT>::T;
     typedef T pair __attribute__((ext_vector_type(2)));
     typedef pair pair_any __attribute__((aligned(sizeof(T))));
@@ -127,10 +134,7 @@ template <int OUT, bool SWIGLU, bool EXPONENTS> __device__ __forceinline__ void 
     for (int e = 0; e < 4; ++e) {
         if (e < live) {
             float a = s0[e], b = s1[e];
-            if constexpr (EXPONENTS) {
-                const int ex = g.exponents[first + e];
-                a = __builtin_amdgcn_ldexpf(a, ex), b = __builtin_amdgcn_ldexpf(b, ex);
-            }
+            if constexpr (EXPONENTS) a = __builtin_amdgcn_ldexpf(a, exponents[e]), b = __builtin_amdgcn_ldexpf(b, exponents[e]);
             if constexpr (SWIGLU) *to = (T)mx_silu(a, b);
             else if (both) *reinterpret_cast<pair_any*>(to) = pair{(T)a, (T)b};
             else *to = (T)a;
@@ -141,8 +145,13 @@ template <int OUT, bool SWIGLU, bool EXPONENTS> __device__ __forceinline__ void 
 template <bool SWIGLU, class F> __device__ __forceinline__ void g4_with_finish(const rkh_g4_args& g, F&& f) {
     mx_with_type(g.out_type, [&](auto t) {
         constexpr int OUT = decltype(t)::value;
-        if (g.exponents) f([&](int first, int64_t n, const float* s0, const float* s1) { g4_finish4<OUT, SWIGLU, true>(g, first, n, s0, s1); });
-        else f([&](int first, int64_t n, const float* s0, const float* s1) { g4_finish4<OUT, SWIGLU, false>(g, first, n, s0, s1); });
+        const auto go = [&](auto with) {
+            constexpr bool EXPONENTS = decltype(with)::value;
+            f([&](int first) { return g4_exponents4<EXPONENTS>(g, first); },
+              [&](int first, int64_t n, const float* s0, const float* s1, const v4i& exponents) { g4_finish4<OUT, SWIGLU, EXPONENTS>(g, first, n, s0, s1, exponents); });
+        };
+        if (g.exponents) go(std::true_type{});
+        else go(std::false_type{});
     });
 }
 // A lane's first column of the 64 places from `unit` on.
@@ -345,11 +354,13 @@ __global__ __launch_bounds__(256) void g4_tile_kernel(G4Grid t, rkh_g4_args g) {
                     to[((i * 2 + j) * 4 + e) * 64] = v4f{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
     } else {
         const int64_t n = g4_lane_column<SWIGLU>((int64_t)nblk * 2 + wn, lane);
-        g4_with_finish<SWIGLU>(g, [&](auto&& finish4) {
+        const auto first = [&](int x) { return m0 + (wm * RM + x / 4) * 32 + 8 * (x % 4) + 4 * (lane >> 5); };
+        g4_with_finish<SWIGLU>(g, [&](auto&& exponents4, auto&& finish4) {
+            v4i exponents[RM * 4];
 #pragma unroll
-            for (int i = 0; i < RM; ++i)
+            for (int x = 0; x < RM * 4; ++x) exponents[x] = exponents4(first(x));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) finish4(m0 + (wm * RM + i) * 32 + 8 * e + 4 * (lane >> 5), n, &acc[i][0][4 * e], &acc[i][1][4 * e]);
+            for (int x = 0; x < RM * 4; ++x) finish4(first(x), n, &acc[x / 4][0][x % 4 * 4], &acc[x / 4][1][x % 4 * 4], exponents[x]);
         });
     }
 }
@@ -370,7 +381,8 @@ __global__ __launch_bounds__(256) void g4_join_kernel(G4Grid t, rkh_g4_args g) {
     for (int p = 1; p < parts; ++p) s0 += from[p * step], s1 += from[p * step + 256];
     const float a[4] = {s0.x, s0.y, s0.z, s0.w}, b[4] = {s1.x, s1.y, s1.z, s1.w};
     const int64_t n = g4_lane_column<SWIGLU>((int64_t)nblk * 2 + (wave >> 1), lane);
-    g4_with_finish<SWIGLU>(g, [&](auto&& finish4) { finish4(((mblk * 2 + (int)(wave & 1)) * RM + i) * 32 + 8 * e + 4 * (lane >> 5), n, a, b); });
+    const int first = ((mblk * 2 + (int)(wave & 1)) * RM + i) * 32 + 8 * e + 4 * (lane >> 5);
+    g4_with_finish<SWIGLU>(g, [&](auto&& exponents4, auto&& finish4) { finish4(first, n, a, b, exponents4(first)); });
 }
 
 template <int GPB, bool SWIGLU> int launch_big_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
@@ -408,14 +420,15 @@ template <int RM, int GPB> struct G4Rows {
 };
 
 // Four rows from `first` on of a lane's column n to results.  (SwiGLU: lanes 16 .. 31 and 48 .. 63 hold what goes with the gates of the 16 before.)
-template <int OUT, bool SWIGLU, bool EXPONENTS> __device__ __forceinline__ void g4_rows_finish4(const rkh_g4_args& g, int first, int64_t n, int lane, const float* s) {
+template <int OUT, bool SWIGLU, bool EXPONENTS>
+__device__ __forceinline__ void g4_rows_finish4(const rkh_g4_args& g, int first, int64_t n, int lane, const float* s, const v4i& exponents) {
     using T = typename MxType<OUT>::T;
     T* to = static_cast<T*>(g.C) + (size_t)first * g.ldc + n;
     const int live = n < g.N && (!SWIGLU || !(lane & 16)) ? g.M - first : 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         float v = s[e];
-        if constexpr (EXPONENTS) v = __builtin_amdgcn_ldexpf(v, g.exponents[min(first + e, g.M - 1)]);
+        if constexpr (EXPONENTS) v = __builtin_amdgcn_ldexpf(v, exponents[e]);
         if constexpr (SWIGLU) v = mx_silu(v, __shfl_xor(v, 16));
         if (e < live) *to = (T)v;
         to += g.ldc;
@@ -425,8 +438,13 @@ template <bool SWIGLU, class F> __device__ __forceinline__ void g4_with_rows_fin
     const int64_t n = g4_column(block0 + (lane >> 4 & 1), lane & 15, SWIGLU);
     mx_with_type(g.out_type, [&](auto t) {
         constexpr int OUT = decltype(t)::value;
-        if (g.exponents) f([&](int first, const float* s) { g4_rows_finish4<OUT, SWIGLU, true>(g, first, n, lane, s); });
-        else f([&](int first, const float* s) { g4_rows_finish4<OUT, SWIGLU, false>(g, first, n, lane, s); });
+        const auto go = [&](auto with) {
+            constexpr bool EXPONENTS = decltype(with)::value;
+            f([&](int first) { return g4_exponents4<EXPONENTS>(g, first); },
+              [&](int first, const float* s, const v4i& exponents) { g4_rows_finish4<OUT, SWIGLU, EXPONENTS>(g, first, n, lane, s, exponents); });
+        };
+        if (g.exponents) go(std::true_type{});
+        else go(std::false_type{});
     });
 }
 
@@ -616,11 +634,13 @@ __global__ __launch_bounds__(256) void g4_rows_tile_kernel(G4Grid t, rkh_g4_args
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[(i * 4 + e) * 64] = v4f{acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]};
     } else {
-        g4_with_rows_finish<SWIGLU>(g, nblk * 8 + wave * 2, lane, [&](auto&& finish4) {
+        const auto first = [&](int x) { return m0 + x / 4 * 32 + 8 * (x % 4) + 4 * (lane >> 5); };
+        g4_with_rows_finish<SWIGLU>(g, nblk * 8 + wave * 2, lane, [&](auto&& exponents4, auto&& finish4) {
+            v4i exponents[RM * 4];
 #pragma unroll
-            for (int i = 0; i < RM; ++i)
+            for (int x = 0; x < RM * 4; ++x) exponents[x] = exponents4(first(x));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) finish4(m0 + i * 32 + 8 * e + 4 * (lane >> 5), &acc[i][4 * e]);
+            for (int x = 0; x < RM * 4; ++x) finish4(first(x), &acc[x / 4][x % 4 * 4], exponents[x]);
         });
     }
 }
@@ -638,7 +658,8 @@ template <bool SWIGLU> __global__ __launch_bounds__(256) void g4_rows_join_kerne
 #pragma unroll 4
     for (int p = 1; p < parts; ++p) s += from[p * step];
     const float v[4] = {s.x, s.y, s.z, s.w};
-    g4_with_rows_finish<SWIGLU>(g, nblk * 8 + wave * 2, lane, [&](auto&& finish4) { finish4((mblk * rm + (int)i) * 32 + 8 * e + 4 * (lane >> 5), v); });
+    const int first = (mblk * rm + (int)i) * 32 + 8 * e + 4 * (lane >> 5);
+    g4_with_rows_finish<SWIGLU>(g, nblk * 8 + wave * 2, lane, [&](auto&& exponents4, auto&& finish4) { finish4(first, v, exponents4(first)); });
 }
 
 template <int RM, int GPB, bool SWIGLU> int launch_rows_tiles(hipStream_t st, const rkh_g4_args& g, const rkk::G4Route& r) {
