@@ -116,7 +116,7 @@ struct G4Grid {
     __device__ __forceinline__ int KB() const { return begin(parts); }
 };
 // The exponents of four rows from `first` on.  (All of them are fetched ahead of the first store, behind which a load would wait: 1622 x 1335 x 1536 of bf16 32.7 us
-// with a load a row, now EXPONENTS_US.)
+// with a load a row, now 26.3.)
 template <bool EXPONENTS> __device__ __forceinline__ v4i g4_exponents4(const rkh_g4_args& g, int first) {
     if constexpr (EXPONENTS) return *reinterpret_cast<const v4i*>(g.exponents + first);
     else return v4i{0, 0, 0, 0};
