@@ -330,11 +330,22 @@ template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
 //   128 x 8192 15.7 19.7 28.5;  x 11008 23.7 20.3 28.7;  x 28672 49.8 39.9 39.4;  256 x 4096 15.7 19.5 29.3 48;  x 5504 23.9 20.3 29.6;  x 8192 27.4 22.8 29.7 48.1;
 //   512 x 8192 51.6 40.5 39.8 48.8;  x 11008 72.1 57.2 67.6 54.2;  x 14336 87.5 73.2 73.3 61.3;  1024 x 14336 170 132 147 123;  2048 x 8192 - 149 154 133.
 //   And of K = 1024: 1000 x 4096 - 15.1 14.6 18.5;  4096 x 4096 - 49.6 52.0 45.5.
+//   With groups of 32: 256 x 4096 x 4096 19.2 26.3 42.1 73.7;  512 x 16384 x 4096 110 89 91 85;  1600 x 1280 x 1536 14.0 12.7 19.7 32.9;  of 64: 17.1 21.5 32.0 55.6;
+//   100 79 78 73;  12.6 11.7 16.1 26.0.
 struct G4Shape { int rm; float few, all, some_two, all_two; int share; float launch, round; }; // launch, round: what a launch has beside its steps, and what another round has
-constexpr G4Shape G4_SHAPES[] = {{8, 1.31f, 1.90f, 0, 0, 1, 7.0f, 5.0f},
-                                 {4, 0.75f, 1.09f, 0, 0, 1, 5.0f, 3.5f},
-                                 {2, 0.465f, 0.575f, 0.90f, 1.105f, 2, 4.6f, 2.0f},
-                                 {1, 0.33f, 0.36f, 0.61f, 0.73f, 2, 4.0f, 1.0f}};
+constexpr G4Shape G4_SHAPES[3][4] = {// one, two and four groups in a step
+                                     {{8, 1.31f, 1.90f, 0, 0, 1, 7.0f, 5.0f},
+                                      {4, 0.75f, 1.09f, 0, 0, 1, 5.0f, 3.5f},
+                                      {2, 0.465f, 0.575f, 0.90f, 1.105f, 2, 4.6f, 2.0f},
+                                      {1, 0.33f, 0.36f, 0.61f, 0.73f, 2, 4.0f, 1.0f}},
+                                     {{8, 1.53f, 2.07f, 0, 0, 1, 7.0f, 5.0f},
+                                      {4, 0.85f, 1.09f, 0, 0, 1, 5.0f, 3.5f},
+                                      {2, 0.53f, 0.61f, 0.92f, 1.13f, 2, 4.6f, 2.0f},
+                                      {1, 0.38f, 0.41f, 0.66f, 0.76f, 2, 4.0f, 1.0f}},
+                                     {{8, 2.10f, 2.44f, 0, 0, 1, 7.0f, 5.0f},
+                                      {4, 1.16f, 1.31f, 0, 0, 1, 5.0f, 3.5f},
+                                      {2, 0.68f, 0.72f, 1.08f, 1.33f, 2, 4.6f, 2.0f},
+                                      {1, 0.44f, 0.475f, 0.70f, 0.83f, 2, 4.0f, 1.0f}}};
 constexpr float G4_JOIN_US = 2.4f, G4_JOIN_RATE = 1.2e7f; // a launch that adds parts, and its bytes per us
 constexpr int G4_MOST_PARTS = 16;
 
@@ -347,11 +358,11 @@ float g4_steps_us(const G4Shape& s, int64_t tiles, int64_t steps) {
 }
 
 // The tiles that are expected to take the least time.  (K in parts, us: 64 x 4096 x 4096 32 rows in four parts 9.7, in one 15.3; 128 x 4096 x 4096 in two 12.6.)
-rkk::G4Route g4_route(int M, int N, int K, int swiglu) {
+rkk::G4Route g4_route(int M, int N, int K, int gpb, int swiglu) {
     const int64_t places = rkh_g4_places(swiglu ? 2 * (int64_t)N : N, swiglu), KB = rkh_g4_kb(K);
     rkk::G4Route best{};
     float least = FLT_MAX;
-    for (const G4Shape& s : G4_SHAPES) {
+    for (const G4Shape& s : G4_SHAPES[gpb / 2]) {
         if (s.rm > 1 && M <= 16 * s.rm) continue; // (half of the rows would be none)
         rkk::G4Route r{};
         r.rm = s.rm, r.parts = 1;
@@ -413,7 +424,7 @@ int rkh_g4_run(void* stream, const rkh_g4_args* args) {
         if (few) g.K = (int)g.ldx; // (zeros there, in the rows as in the codes)
     }
     if (few) return g.x_type == RKH_MX4_F16 ? launch_few<RKH_MX4_F16>(st, g) : launch_few<RKH_MX4_BF16>(st, g);
-    rkk::G4Route r = g4_route(g.M, g.N, g.K, g.swiglu);
+    rkk::G4Route r = g4_route(g.M, g.N, g.K, g.gpb, g.swiglu);
     if (g4_scratch(r) > (g.scratch ? g.scratch_bytes : 0)) r.parts = 1;
     return g.gpb == 1 ? rkk::launch_g4_tiles1(st, g, r) : g.gpb == 2 ? rkk::launch_g4_tiles2(st, g, r) : rkk::launch_g4_tiles4(st, g, r);
 }
@@ -423,10 +434,10 @@ void rkh_g4_route(int M, int N, int K, int gpb, int swiglu, int* kernel, int* ro
         *columns = 16 * few_shape(M, rkh_g4_places(swiglu ? 2 * (int64_t)N : N, swiglu) / 16, (int)rkh_g4_kb(K), gpb, swiglu).cn;
         return;
     }
-    const rkk::G4Route r = g4_route(M, N, K, swiglu);
+    const rkk::G4Route r = g4_route(M, N, K, gpb, swiglu);
     *kernel = 1, *rows = 32 * r.rm, *columns = 128, *parts = r.parts;
 }
-size_t rkh_g4_scratch_bytes(int M, int N, int K, int swiglu) { return M <= FEW_ROWS ? 0 : g4_scratch(g4_route(M, N, K, swiglu)); }
+size_t rkh_g4_scratch_bytes(int M, int N, int K, int gpb, int swiglu) { return M <= FEW_ROWS ? 0 : g4_scratch(g4_route(M, N, K, gpb, swiglu)); }
 // (g4_route: a part for each compute unit at most, tiles no larger than the rows ask for)
 size_t rkh_g4_scratch_most(int max_rows, int K) {
     return max_rows > FEW_ROWS && rkh_g4_kb(K) >= 4 ? (size_t)G4_CUS * 32 * 128 * 4 * (max_rows > 128 ? 8 : max_rows > 64 ? 4 : max_rows > 32 ? 2 : 1) : 0;

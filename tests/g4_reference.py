@@ -59,6 +59,6 @@ SHAPES = [(1, 1, 1, 32), (1, 33, 31, 64), (1, 128, 4096, 128), (1, 70, 1001, 32)
           (4, 12300, 256, 64), (3, 1999, 2050, 50016), (5, 48, 8200, 32), (5, 12300, 520, 32), (8, 100, 8320, 128), (8, 65, 640, 320), (8, 31, 9000, 64), (9, 8200, 512, 128),
           (9, 129, 500, 64), (16, 48, 14336, 32), (16, 96, 4104, 160), (16, 8200, 1001, 64), (13, 257, 33, 32), (17, 1, 1, 32), (17, 64, 128, 128), (32, 100, 33, 64), (33, 130, 1000, 32),
           (61, 1999, 2050, 64), (64, 700, 4096, 128), (65, 257, 640, 192), (64, 96, 8192, 32), (130, 11008, 256, 64), (300, 300, 14336, 128), (33, 11800, 130, 32),
-          (260, 13000, 200, 160), (200, 15490, 136, 64), (360, 5600, 280, 64), (1346, 129, 2366, 128), (300, 12400, 160, 32), (1025, 6000, 384, 128), (2100, 5900, 300, 64), (77, 15000, 500, 32), (1025, 1800, 1030, 32), (129, 1000, 8192, 256)]
+          (260, 13000, 200, 160), (200, 15490, 136, 64), (360, 5600, 280, 64), (871, 2330, 262, 128), (1370, 263, 3534, 32), (1346, 129, 2366, 128), (300, 12400, 160, 32), (1025, 6000, 384, 128), (2100, 5900, 300, 64), (77, 15000, 500, 32), (1025, 1800, 1030, 32), (129, 1000, 8192, 256)]
 SWIGLU = [(1, 1, 1, 32), (1, 64, 96, 64), (1, 33, 4608, 32), (1, 40, 4360, 128), (3, 300, 4100, 64), (4, 40, 520, 160), (7, 100, 640, 32), (8, 33, 8200, 128), (16, 250, 640, 128), (16, 40, 4400, 32),
-          (12, 4100, 264, 64), (17, 32, 64, 32), (31, 70, 1000, 64), (64, 500, 4096, 128), (33, 11800, 130, 32), (71, 15740, 140, 64), (300, 300, 14336, 32), (700, 3000, 264, 128), (160, 13500, 100, 128)]
+          (12, 4100, 264, 64), (17, 32, 64, 32), (31, 70, 1000, 64), (64, 500, 4096, 128), (33, 11800, 130, 32), (71, 15740, 140, 64), (300, 300, 14336, 32), (700, 3000, 264, 128), (489, 2152, 269, 128), (160, 13500, 100, 128)]

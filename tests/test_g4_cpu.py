@@ -83,18 +83,19 @@ def test_route_covers_every_row_and_column_and_its_scratch_is_what_the_parts_nee
     seen = set()
     for _ in range(4000):
         M, N, K = (int(np.exp(rng.uniform(0, np.log(top)))) for top in (9000, 40000, 40000))
-        kernel, rows, columns, parts = _route(lib, M, N, K, int(rng.choice([1, 2, 4])), swiglu)
+        gpb = int(rng.choice([1, 2, 4]))
+        kernel, rows, columns, parts = _route(lib, M, N, K, gpb, swiglu)
         places = 2 * (-(-N // 32) * 32) if swiglu else -(-N // 64) * 64
         seen.add((kernel, rows, parts > 1))
         assert rows > 0 and 1 <= parts <= max(1, -(-K // 128) // 2), (M, N, K)
         if kernel == 0:
             assert M <= 16 == rows and parts == 1 and places % columns == 0 and (not swiglu or columns % 32 == 0)
-            assert lib.rkh_g4_scratch_bytes(M, N, K, swiglu) == 0
+            assert lib.rkh_g4_scratch_bytes(M, N, K, gpb, swiglu) == 0
             continue
         assert M > 16 and rows in (32, 64, 128, 256) and columns == 128
         tiles = -(-M // rows) * -(-places // columns)
         want = tiles * parts * rows * columns * 4 if parts > 1 else 0
-        assert lib.rkh_g4_scratch_bytes(M, N, K, swiglu) == want, (M, N, K)
+        assert lib.rkh_g4_scratch_bytes(M, N, K, gpb, swiglu) == want, (M, N, K)
         # what a workspace of as many rows has, and one of more
         assert want <= lib.rkh_g4_scratch_most(M, K) <= lib.rkh_g4_scratch_most(M + 5, K), (M, N, K)
     assert {(0, 16, False), (1, 32, False), (1, 32, True), (1, 64, False), (1, 64, True), (1, 128, True), (1, 256, False), (1, 256, True)} <= seen, seen
