@@ -1,8 +1,8 @@
 // Tiles of G4 products.
 //
 // Many rows: 256 rows x 128 places by four waves (two by two), each 4 x 2 accumulators of 32 x 32.  Bound by power, and by what one wave has to issue: about
-// 2950 clocks a step, 2090 of them products; variants with 2800 took no less time, as the clock fell.  4096 x 14336 x 4096 461 us, 1.04 PFLOP/s (a library's
-// product of halves of this size, which has no codes to turn into halves, 417); 512 rows of SwiGLU with groups of 64 128 us, 0.93.
+// 2950 clocks a step, 2090 of them products; variants with 2800 took no less time, as the clock fell.  4096 x 14336 x 4096 429 us, 1.12 PFLOP/s (a library's
+// product of halves of this size, which has no codes to turn into halves, 417); 512 rows of SwiGLU with groups of 64 130 us, 0.92.
 //
 // A step is 128 k.  Its activations (rows of 256 bytes), codes and scales are copied global -> LDS directly, two steps ahead of the products and one
 // ahead of the LDS reads:
@@ -406,8 +406,9 @@ template <int GPB, bool SWIGLU> int launch_big_tiles(hipStream_t st, const rkh_g
 // ---- tiles of few rows -----------------------------------------------------------------
 // 32 RM rows x 128 places by four waves, each all of the rows and 32 places: nobody makes the same codes into halves twice, which is what tiles of few rows are
 // bound by (128 x 128 x 128 two by two 2020 clocks, this way 1100 - 1700), for twice the reads of activations.  A wave issues some 150 instructions a step of 32
-// rows in 970 clocks, 260 of them products, and two waves on a SIMD 1500: 128 x 11008 x 4096 23.4 us.  Of those, without: codes made into halves 17.5, sums added
-// 23.7, LDS reads 23.3, copies 22.7 (of 25.2 in that run).  Neither more steps under way nor codes spread over more of the products change it.
+// rows, one in five clocks at best, and eight of them are products: 128 x 8192 x 4096 in 32 rows 15.2 us, in 64 rows 19.7, x 11008 23.7 and 19.9.  Without codes made into
+// halves 32 rows x 8192 took 13.2 of 18.4, without LDS reads 16.3, without copies 15.4, without sums added 16.3 (all before the last steps).  Neither more steps under
+// way nor codes spread over more of the products change it.
 //  * A step's activations live in registers as above, each replaced by the next step's behind its product; the next step's codes become halves in
 //    registers of their own, so that two steps make one turn of the loop.
 //  * At the start of step s a wave waits for its copies of step s + 1 and for its LDS reads, and meets the others: nobody reads step s any more, and the
