@@ -419,3 +419,35 @@ def test_rows_further_apart_than_32_bits(sess, M, kind):
     assert np.array_equal(host(out), host(torch.from_numpy(a @ layer.values.T).to(HALVES[kind])))
     ws.close()
     layer.close()
+
+
+def test_two_threads(sess):
+    """With a workspace each, both get their products; with one, a call is made or refused as BUSY, and nothing else."""
+    import threading
+    rng = np.random.default_rng(8)
+    M, N, K = 40, 200, 1000
+    layer = Layer(sess, rng, N, K, 64)
+    a = [rng.integers(-4, 5, (M, K)).astype(np.float64) for _ in range(2)]
+    x = [rows_of(v, "bf16") for v in a]
+    for shared in (False, True):
+        spaces = [ops.G4Workspace(sess, M, K, N) for _ in range(2)]
+        outs, codes = [torch.zeros((M, N), device="cuda") for _ in range(2)], [set(), set()]
+        ready()
+
+        def loop(i):
+            ws = spaces[0 if shared else i]
+            for _ in range(200):
+                codes[i].add(sess.lib.rk_npu_g4_run_device(ws.h, layer.w.h, M, capi.MX4_BF16, x[i].data_ptr(), x[i].stride(0), capi.MX4_F32, outs[i].data_ptr(), N))
+        threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        done(sess)
+        for i in range(2):
+            assert codes[i] <= ({0, capi.RK_NPU_ERR_BUSY} if shared else {0})
+            if 0 in codes[i]:
+                assert np.array_equal(host(outs[i]), a[i] @ layer.values.T)
+        for ws in spaces:
+            ws.close()
+    layer.close()
