@@ -28,8 +28,8 @@ __device__ __forceinline__ float g4_scale(uint32_t d, int type) {
     return type == RKH_MX4_BF16 ? __uint_as_float(d & 0xffff0000u) : (float)__builtin_bit_cast(_Float16, (uint16_t)(d >> 16));
 }
 
-// code - zero as halves, exactly.  A code under the exponent of 1024 is the half 1024 + code, four bits further up 1024 + 16 code: one addition, or
-// one multiplication and addition, of neighbours in a dword.  9 instructions for eight weights.
+// code - zero as halves, exactly.  A code under the exponent of 1024 is the half 1024 + code, four bits further up 1024 + 16 code (a known way from
+// integers to floating point): one addition, or one multiplication and addition, of neighbours in a dword.  9 instructions for eight weights.
 struct G4Zero {
     v2h low, high; // -(1024 + zero), -(64 + zero)
     __device__ __forceinline__ void of(uint32_t scale_dword) {
@@ -38,16 +38,27 @@ struct G4Zero {
         high = low + v2h{960, 960};
     }
 };
-// Codes as halves or bf16, the zero point not taken off: a byte 0..15 is the e4m3 number code * 2^-9, which the conversion scales by 2^9.  7 instructions for
+// The exponents, in a vector register: as a constant they would be a literal, and masking and joining two instructions.
+__device__ __forceinline__ uint32_t g4_exponents() {
+    uint32_t v;
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(v));
+    return v;
+}
+// The eight weights of a dword, in their order.
+__device__ __forceinline__ v4i g4_halves(uint32_t w, const G4Zero& zero, uint32_t exponents) {
+    const auto low = [&](uint32_t u) { return __builtin_bit_cast(int, __builtin_bit_cast(v2h, (u & 0x000f000fu) | exponents) + zero.low); };
+    const auto high = [&](uint32_t u) {
+        const v2h sixteenth = {0.0625f, 0.0625f};
+        return __builtin_bit_cast(int, __builtin_elementwise_fma(__builtin_bit_cast(v2h, (u & 0x00f000f0u) | exponents), sixteenth, zero.high));
+    };
+    return v4i{low(w), high(w), low(w >> 8), high(w >> 8)};
+}
+// Codes as bf16, the zero point not taken off: a byte 0..15 is the e4m3 number code * 2^-9, which the conversion scales by 2^9.  7 instructions for
 // eight.  The order is k0 k4 k1 k5 k2 k6 k3 k7; g4_turned_rows gives activations the same.
-template <int TYPE> __device__ __forceinline__ v4i g4_codes(uint32_t w) {
+__device__ __forceinline__ v4i g4_codes(uint32_t w) {
     const int even = (int)(w & 0x0f0f0f0fu), odd = (int)((w >> 4) & 0x0f0f0f0fu);
-    if constexpr (TYPE == RKH_MX4_F16)
-        return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(even, 512.0f, true)),
-                   __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(odd, 512.0f, true))};
-    else
-        return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true)),
-                   __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true))};
+    return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(even, 512.0f, true)),
+               __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(odd, 512.0f, true))};
 }
 __device__ __forceinline__ v4i g4_turned_rows(const v4i& x) {
     return v4i{(int)__builtin_amdgcn_perm((uint32_t)x.z, (uint32_t)x.x, 0x05040100u), (int)__builtin_amdgcn_perm((uint32_t)x.z, (uint32_t)x.x, 0x07060302u),

@@ -1,7 +1,11 @@
 // Group-scaled 4-bit (G4) layers: weights laid out, rows staged for the tiles, products of few rows, and which kernel takes a product.
 //
-// C[m, n] = sum over groups of scale[n, g] * (sum over k in g of (code - zero) * x[m, k]).  code - zero is a small integer and exact in 16 bits, so the
-// matrix cores' products with 16-bit activations are exact and their sums have 32 bits; the scales multiply sums, and no weight is rounded.
+// C[m, n] = sum over groups of scale[n, g] * (sum over k in g of (code - zero) * x[m, k]).  Codes and code - zero are small integers and exact in 16 bits, so the
+// matrix cores' products with 16-bit activations are exact and their sums have 32 bits; the scales multiply sums, and no weight is rounded.  What is multiplied:
+//   fp16 rows, as many as there are: code - zero.
+//   bf16 rows, up to 16: the code; the zero point times the group's sum of activations is taken off the group's sum.  Both have 32 bits, so the roundings of terms
+//   (code + zero) |x| stay, also where code and zero are equal.
+//   bf16 rows, more: code - zero, with the row as halves (g4_stage_kernel), which is the row itself down to 2^-31 of its largest value.
 #include <algorithm>
 
 #include "rk_kernels_g4.h"
@@ -125,14 +129,17 @@ __global__ __launch_bounds__(256) void g4_stage_kernel(const uint16_t* x, int64_
 // loaded as the operands lie.
 // One row is bound by the weights' way from HBM (1 x 14336 x 4096 7.2 us where caches help, 7.7 where they do not: 4 TB/s), more rows by the activations' from L2 as well
 // (8 x 4096 x 14336 8.9 to 10.6).
-// Products are with the code; the zero point times the group's sum of activations, which a product with ones gives, is taken off a group's sum.
+// fp16 rows are multiplied with code - zero.  bf16 rows with the code, and the zero point times the group's sum of activations, which a product with ones gives, is taken off
+// a group's sum: bf16 has no packed additions, so that code - zero takes 17 instructions for eight weights by way of fp32, not 7, and one row x 14336 x 4096
+// 8.7 us and not 7.8, SwiGLU of it 15.2 and not 13.1, 8 x 4096 x 14336 11.6 and not 11.1.
 constexpr int FEW_PITCH = 1024 + 16; // bytes of a row of 512 values in LDS
 constexpr int few_area(int rows, int cn) { return rows * FEW_PITCH > cn * 1024 ? rows * FEW_PITCH : cn * 1024; }
 
 template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES>
 __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W, const uint32_t* scales, const uint16_t* x, int64_t ldx, int M, int K,
                                                                 int per_wave, int workgroups, int waves, rkh_g4_args g) {
-    constexpr int ONE = TYPE == RKH_MX4_F16 ? 0x3c003c00 : 0x3f803f80; // two of them
+    constexpr bool HALVES = TYPE == RKH_MX4_F16;
+    constexpr int ONE = 0x3f803f80; // two of bf16
     constexpr int STEPS = 4 / GPB; // 32-k steps of a group
     static_assert(!SWIGLU || CN % 2 == 0, "gate and up halves");
     static_assert(!ROWS || NP % 4 == 0, "rows are loaded 512 values at a time");
@@ -151,7 +158,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
     // (What lies beyond K, eight at least, is loaded from a row's last eight values and dropped where it is used: a branch here would wait for the activations
     // ahead of the codes' loads.)
     const auto fetch = [&](int m, int k) { return mx_fetch8<TYPE>(x, (size_t)m * ldx + min(k, K - 8)).w[0]; };
-    const auto within = [&](const v4i& v, int k) { return k < K ? g4_turned_rows(v) : v4i{0, 0, 0, 0}; };
+    const auto within = [&](const v4i& v, int k) { return k < K ? HALVES ? v : g4_turned_rows(v) : v4i{0, 0, 0, 0}; };
     const auto moved = [&](const v4i& v, int k) { // where K ends within eight values: the last eight to their places
         const int beyond = k < K ? max(k + 8 - K, 0) : 0, bits = 16 * (beyond & 3);
         uint64_t low = (uint64_t)(uint32_t)v.y << 32 | (uint32_t)v.x, high = (uint64_t)(uint32_t)v.w << 32 | (uint32_t)v.z;
@@ -182,6 +189,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
         if constexpr (TYPE == RKH_MX4_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, rows), __builtin_bit_cast(v8h, codes), sum, 0, 0, 0);
         else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, rows), __builtin_bit_cast(v8b, codes), sum, 0, 0, 0);
     };
+    const uint32_t exponents = g4_exponents();
     v4f acc[CN];
 #pragma unroll
     for (int j = 0; j < CN; ++j) acc[j] = v4f{0, 0, 0, 0};
@@ -209,16 +217,29 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
 #pragma unroll
             for (int n = 0; n < GPB; ++n) {
                 v4f sum = {0, 0, 0, 0};
+                if constexpr (!HALVES) {
 #pragma unroll
-                for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) sum = product(a[i], v4i{ONE, ONE, ONE, ONE}, sum);
+                    for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) sum = product(a[i], v4i{ONE, ONE, ONE, ONE}, sum);
+                }
 #pragma unroll
                 for (int j = 0; j < CN; ++j) {
+                    const uint32_t d = b.s[p][j][n];
+                    const float s = g4_scale(d, g.scale_type);
                     v4f part = {0, 0, 0, 0};
+                    if constexpr (HALVES) {
+                        G4Zero zero;
+                        zero.of(d);
 #pragma unroll
-                    for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) part = product(a[i], g4_codes<TYPE>((uint32_t)b.w[p][j][i]), part);
-                    const float s = g4_scale(b.s[p][j][n], g.scale_type), zero = (float)(b.s[p][j][n] & 0xffu);
+                        for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) part = product(a[i], g4_halves((uint32_t)b.w[p][j][i], zero, exponents), part);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(fmaf(-zero, sum[e], part[e]), s, acc[j][e]);
+                        for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(part[e], s, acc[j][e]);
+                    } else {
+                        const float zero = (float)(d & 0xffu);
+#pragma unroll
+                        for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) part = product(a[i], g4_codes((uint32_t)b.w[p][j][i]), part);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(fmaf(-zero, sum[e], part[e]), s, acc[j][e]);
+                    }
                 }
             }
         }
