@@ -7,10 +7,16 @@
  *
  *     w[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group],    C[m, n] = sum over k of A[m, k] w[n, k]
  *
- * code - zero is multiplied as the integer that it is; products are exact, sums have 32 bits, each group's sum is scaled in fp32, and the result
- * is rounded once.  No weight is rounded.  Rows are independent of each other; a row that holds an infinity or a NaN has
- * infinities and NaN as its results, and so may one whose sums of code * A, which are taken ahead of the scale, are beyond fp32 (bf16 values from
- * 2^116 on).  Scales are finite numbers.
+ * No weight is rounded: products are of small integers and exact, sums have 32 bits, each group's sum is scaled in fp32, and the result is rounded
+ * once.  What is multiplied:
+ *   fp16 rows: code - zero, with A as it is.
+ *   bf16 rows, more than 16 of them: code - zero, with the row as fp16 times a power of two.  A is as it is down to 2^-31 of its row's largest
+ *     magnitude; what is smaller is off by up to 2^-39 of that magnitude.
+ *   bf16 rows, up to 16: the code, and zero times the group's sum of A is taken off the group's sum in fp32, whose roundings are those of terms
+ *     (code + zero) |A|, also where the weight is zero; or as more rows.
+ * So fp16 rows have results that differ by the order of fp32 sums alone, however many there are, and bf16 rows ones that differ by the above, too.
+ * Rows are independent of each other; a row that holds an infinity or a NaN has infinities and NaN as its results, and so may one
+ * whose sums ahead of the scale are beyond fp32: up to 128 terms of up to 255 |A|, bf16 values from 2^113 on.  Scales are finite numbers.
  *
  * All pointers are device pointers unless said otherwise; the calls enqueue on the context's stream and return, under the rules
  * for *_device calls in rk_npu_hip.h (rk_npu_hip_sync() waits, stream capture records them, a workspace is BUSY only while a

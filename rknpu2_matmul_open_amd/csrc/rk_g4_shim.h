@@ -17,8 +17,8 @@
  * + 16 b of two accumulators j of 32 places has two neighbouring columns.  Gate / up matrices: column 16 b + c of 32, j = 0 of the gate and j = 1 of
  * the up half.
  *
- * Staged rows: fp16, row-major, Kp = 128 KB values apart, zeros beyond K; bf16 rows times 2^e(row) (exact for all that is not 2^-38 of the row's
- * largest), the exponents in an array of their own.
+ * Staged rows: fp16, row-major, Kp = 128 KB values apart, zeros beyond K; bf16 rows times 2^e(row) (exact for all that is not below 2^-31 of the
+ * row's largest), the exponents in an array of their own.
  */
 #ifndef RK_G4_SHIM_H
 #define RK_G4_SHIM_H

@@ -63,8 +63,10 @@ __global__ __launch_bounds__(256) void g4_pack_kernel(const uint8_t* codes, cons
 }
 
 // ---- rows for the tiles ---------------------------------------------------------------
-// One workgroup per row, or a wave (ROWS = 4) where rows are short: 2457 x 768 with SwiGLU behind it 21.6 -> 19.1 us.  bf16: the row's largest finite magnitude is moved to 2^14 .. 2^15, where eight bits fit a half down to 2^-38 of it (what is
-// smaller than that is rounded to a multiple of 2^-39 of it); infinities and NaN stay what they are.
+// One workgroup per row, or a wave (ROWS = 4) where rows are short: 2457 x 768 with SwiGLU behind it 21.6 -> 19.1 us.
+// bf16: the row's largest finite magnitude is moved to 2^14 .. 2^15.  A half's smallest step is 2^-24, where the eight bits of a value of 2^-17 end, so all that is 2^-31 of the
+// largest or more stays as it is.  What is smaller is rounded to a multiple of 2^-24, by 2^-25 or 2^-39 of the largest at most.  (As bf16, code - zero would take
+// twice the instructions, which are what tiles are bound by.)  Infinities and NaN stay what they are.
 template <bool BF16, int ROWS>
 __global__ __launch_bounds__(256) void g4_stage_kernel(const uint16_t* x, int64_t ldx, int M, int K, uint16_t* staged, int* exponents, int first) {
     constexpr int THREADS = 256 / ROWS, STRIDE = THREADS * 8; // of a row

@@ -1,13 +1,15 @@
 """What G4 products make of a row's values: which are multiplied exactly, whatever else the row holds, and that nothing but a row's own values counts.
 
-fp16 rows are multiplied with code - zero as they are.
+fp16 rows are multiplied with code - zero as they are.  bf16 rows of up to 16 are multiplied with the code, and zero times the group's sum is taken off; more of them are
+staged as halves: exact down to 2^-31 of the row's largest value (that is moved to 2^14 .. 2^15, and the eight bits of a value of 2^-17 end at 2^-24, a half's smallest step),
+off by half of a step, 2^-39 of the largest value's power of two, below.
 """
 import numpy as np
 import pytest
 
 from rknpu2_matmul_open_amd import ops
 from tests import g4_reference as ref
-from tests.test_gpu_g4 import Layer, rows_of
+from tests.test_gpu_g4 import Layer, row_bound, rows_of
 from tests.test_gpu_mx4 import device, done, host, poisoned, ready, untouched
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +55,47 @@ def test_large_fp16_values_under_weights_of_zero_count_for_nothing(sess, M, K, g
     got = run(sess, layer, rows_of(a, "f16"), N, K)
     assert np.array_equal(got, want), np.abs(got - want).max()
     layer.close()
+
+
+@pytest.mark.parametrize("K", [1024, 264, 999])
+@pytest.mark.parametrize("M", [17, 40, 100, 200])
+def test_staged_bf16_rows_are_exact_down_to_2_31_of_their_largest_value(sess, M, K):
+    """The largest value counts for nothing; the others are 128 .. 255 times 2^-38 of its power of two, which fp32 adds exactly in any order, and then of 2^-39 .. 2^-48."""
+    rng = np.random.default_rng(M + K)
+    N = 70
+    layer = Silent(sess, rng, N, K, 64)
+    assert 2.0 * 255 * np.abs(layer.values).sum(1).max() < 2 ** 24
+    for largest, below in ((1.0, 38), (1.9921875, 38), (1.0, 39), (1.9921875, 39), (1.5, 41), (1.0, 44), (1.0, 48)):
+        power = np.exp2(rng.integers(-60, 100, (M, 1)))
+        a = rng.integers(128, 256, (M, K)) * rng.choice([-1.0, 1.0], (M, K)) * 2.0 ** -below * power
+        a[:, layer.where] = 0.0
+        want = a @ layer.values.T
+        a[:, layer.where] = largest * power * rng.choice([-1.0, 1.0], (M, len(layer.where)))
+        got = run(sess, layer, rows_of(a, "bf16"), N, K)
+        if below == 38:
+            assert np.array_equal(got, want), (largest, np.abs(got / want - 1).max())
+        else: # (halves of 2^-25 and its multiples: sums of them are exact as well)
+            far = np.abs(got - want) - 2.0 ** -39 * power * np.abs(layer.values).sum(1)
+            assert far.max() <= 0, (largest, below)
+    layer.close()
+
+
+@pytest.mark.parametrize("M", [1, 4, 8, 16, 17, 40, 200])
+def test_bf16_sums_are_finite_up_to_2_113(sess, M):
+    """A group of 128 values below 2^113 of one sign under zero points of 255: its sums stay below 2^128, in either form."""
+    rng = np.random.default_rng(M)
+    N, K, group = 70, 640, 128
+    code, zeros = rng.integers(0, 16, (N, K)), np.full((N, K // group), 255, np.uint8)
+    scales = np.exp2(rng.integers(-9, -5, (N, K // group)))
+    w = ops.G4Weights(sess, K, N, group, ref.pack(code), scales.astype(np.float16), zeros)
+    values, sizes = (f(code, scales, zeros, group) for f in (ref.weights, ref.sizes))
+
+    class Holder:
+        pass
+    layer = Holder()
+    layer.w = w
+    a = rng.integers(128, 256, (M, K)) * 2.0 ** 105 * rng.choice([-1.0, 1.0], (M, 1))
+    got, want = run(sess, layer, rows_of(a, "bf16"), N, K), a @ values.T
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= row_bound(a, sizes, K) + ref.HALF_STEP["f32"] * np.abs(want)).all()
+    w.close()
