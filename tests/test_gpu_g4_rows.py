@@ -6,6 +6,7 @@ off by half of a step, 2^-39 of the largest value's power of two, below.
 """
 import numpy as np
 import pytest
+import torch
 
 from rknpu2_matmul_open_amd import ops
 from tests import g4_reference as ref
@@ -99,3 +100,56 @@ def test_bf16_sums_are_finite_up_to_2_113(sess, M):
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= row_bound(a, sizes, K) + ref.HALF_STEP["f32"] * np.abs(want)).all()
     w.close()
+
+
+SHAPES = [(1, 200, 4096, 128), (8, 200, 4096, 32), (8, 4096, 14336, 128), (16, 12300, 640, 64), (40, 700, 4096, 64), (64, 96, 8192, 32), (100, 300, 1001, 128), (300, 300, 14336, 128),
+          (300, 6000, 520, 32)]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", SHAPES)
+def test_rows_keep_their_bits_beside_any_others_and_from_call_to_call(sess, M, N, K, group, kind):
+    """A third of the rows stays; the others are replaced by rows of other sizes, with infinities and NaN among them.  The first rows are multiplied again at the end."""
+    rng = np.random.default_rng(M + N)
+    layer = Layer(sess, rng, N, K, group, exact=False)
+    kept = np.arange(M) % 3 == 0
+    a = rng.standard_normal((M, K)) * np.exp2(rng.integers(-6, 3, (M, 1)))
+    first = run(sess, layer, rows_of(a, kind), N, K)
+    assert np.isfinite(first).all()
+    for turn in range(3):
+        b = rng.standard_normal((M, K)) * np.exp2(rng.integers(-12, 9, (M, 1)))
+        b[:, rng.integers(0, K, 8)] *= 50
+        b[kept] = a[kept]
+        x = rows_of(b, kind)
+        for r in np.flatnonzero(~kept)[turn::4]:
+            x[r, int(rng.integers(0, K))] = float(rng.choice([np.nan, np.inf, -np.inf]))
+        assert np.array_equal(run(sess, layer, x, N, K)[kept], first[kept])
+    assert np.array_equal(run(sess, layer, rows_of(a, kind), N, K), first)
+    layer.close()
+
+
+def test_passes_over_long_k_repeat_bit_for_bit(sess):
+    """Eight rows of bf16 x 4096 x 14336: sixteen waves a workgroup, which load twice.  Layers in turn, nothing waiting in between."""
+    rng = np.random.default_rng(14)
+    M, N, K, group = 8, 4096, 14336, 128
+    layers = [Layer(sess, rng, N, K, group, exact=False) for _ in range(2)]
+    x = [rows_of(rng.standard_normal((M, K)) * np.where(rng.random((M, K)) < 0.005, 20, 1), "bf16") for _ in layers]
+    ws = ops.G4Workspace(sess, M, K, N)
+    outs = [torch.zeros((M, N), device="cuda") for _ in layers]
+    first = None
+    for turn in range(40):
+        for c in outs:
+            c.fill_(77)
+        ready()
+        for _ in range(3):
+            for layer, a, c in zip(layers, x, outs):
+                ws.run(layer.w, a, c)
+        done(sess)
+        if first is None:
+            first = [c.clone() for c in outs]
+            for layer, a, c in zip(layers, x, first):
+                want = host(a) @ layer.values.T
+                assert (np.abs(host(c) - want) <= ref.sum_bound(host(a), layer.sizes, K) + ref.HALF_STEP["f32"] * np.abs(want)).all()
+        assert all(torch.equal(a, b) for a, b in zip(first, outs)), turn
+    for h in (ws, *layers):
+        h.close()
