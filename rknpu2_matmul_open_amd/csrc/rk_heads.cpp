@@ -23,12 +23,11 @@ struct Heads {
     int64_t width() const { return heads == 1 || rows == 1 ? D : rows_hold_heads() ? (heads - 1) * head + D : (rows - 1) * row + D; }
     bool valid() const {
         if (empty()) return true;
-        const int64_t most = INT64_C(1) << 40;
+        const int64_t most = INT64_C(1) << 40, all = INT64_C(1) << 56;
         if (!p || reinterpret_cast<uintptr_t>(p) % type_bytes(type) || (rows > 1 && (row < D || row > most)) || (heads > 1 && (head < D || head > most))) return false;
-        // neither the inner extent nor the whole may leave 2^56 values
-        const int64_t inner = width(), n = outer(), step = pitch();
-        if (inner > (INT64_C(1) << 56) || inner < 0) return false;
-        return n == 1 || (step >= inner && step <= (INT64_C(1) << 56) / n);
+        // neither the inner extent nor the whole may leave 2^56 values: looked at ahead of the products, which 64 bits need not hold otherwise
+        if ((rows > 1 && row > all / rows) || (heads > 1 && head > all / heads)) return false;
+        return outer() == 1 || (pitch() >= width() && pitch() <= all / outer());
     }
     Span span() const { return empty() ? Span() : Span(p, outer(), pitch() * type_bytes(type), width() * type_bytes(type)); }
     bool is(const Heads& o) const { return p == o.p && (rows == 1 || row == o.row) && (heads == 1 || head == o.head); }
