@@ -40,6 +40,7 @@ rk_npu_g4_weights* create_weights(rk_npu_iommu_domain* domain, const rk_npu_g4_w
     w->config.gate_up = gate_up;
     rk_npu_ctx* ctx = domain->ctx;
     const OnDevice device(ctx->device);
+    if (!device) return nullptr;
     std::lock_guard<std::mutex> lock(ctx->submit_mutex);
     const size_t groups = (size_t)N * (((int64_t)K + config->group - 1) / config->group);
     DeviceBuffer raw, raw_scales, raw_zeros;
@@ -92,6 +93,7 @@ int run(rk_npu_g4_workspace* ws, const rk_npu_g4_weights* w, bool swiglu, int ro
     g.scratch = ws->scratch.as<float>();
     g.scratch_bytes = ws->scratch.bytes();
     const OnDevice device(ws->owner.ctx->device);
+    if (!device) return RK_NPU_ERR_SUBMIT;
     std::lock_guard<std::mutex> submit(ws->owner.ctx->submit_mutex);
     return map_error(rkh_g4_run(ws->owner.ctx->stream, &g));
 }
@@ -126,6 +128,7 @@ rk_npu_g4_workspace* rk_npu_g4_workspace_create(rk_npu_iommu_domain* domain, int
     ws->N = N;
     const size_t scratch = rkh_g4_scratch_most(max_rows, K);
     const OnDevice device(domain->ctx->device);
+    if (!device) return nullptr;
     std::lock_guard<std::mutex> lock(domain->ctx->submit_mutex);
     if (ws->staged.alloc(ws->owner, rkh_g4_staged_bytes(max_rows, K), false) || ws->exponents.alloc(ws->owner, (size_t)rkh_align_up(max_rows, 256) * 4, false) ||
         (scratch && ws->scratch.alloc(ws->owner, scratch, false)))

@@ -105,6 +105,7 @@ int rk_npu_heads_norm_rotate_device(rk_npu_ctx* ctx, const rk_npu_heads_args* a)
     h.positions = a->positions;
     h.position_axis = a->position_axis;
     const OnDevice device(ctx->device);
+    if (!device) return RK_NPU_ERR_SUBMIT;
     std::lock_guard<std::mutex> submit(ctx->submit_mutex);
     return map_error(rkh_heads(ctx->stream, &h));
 }

@@ -68,8 +68,9 @@ int rkh_device_count(void);
 int rkh_open(int device, void** stream_out, char* name_out, int name_len, int* cu_count,
              int* clock_khz);
 void rkh_close(int device, void* stream);
-/* Makes `device` the calling thread's current one for a while: returns what was, which leaving restores (-1: nothing to do). */
-int rkh_enter_device(int device);
+/* Makes `device` the calling thread's current one for a while: *before is what was, which leaving restores (-1: nothing to do).  Where it
+ * cannot be made current, nothing may be launched. */
+int rkh_enter_device(int device, int* before);
 void rkh_leave_device(int before);
 int rkh_malloc(int device, void** ptr, size_t bytes);
 void rkh_free(int device, void* ptr);

@@ -114,16 +114,17 @@ private:
 };
 
 // The context's device is the calling thread's current one for as long as this lives (kernels have attributes per device, and are
-// launched on the current one).
+// launched on the current one); false where it could not be made current.
 class OnDevice {
 public:
-    explicit OnDevice(int device) : before_(rkh_enter_device(device)) {}
+    explicit OnDevice(int device) : rc_(rkh_enter_device(device, &before_)) {}
     ~OnDevice() { rkh_leave_device(before_); }
     OnDevice(const OnDevice&) = delete;
     OnDevice& operator=(const OnDevice&) = delete;
+    explicit operator bool() const { return rc_ == RKH_OK; }
 
 private:
-    int before_;
+    int before_ = -1, rc_;
 };
 
 // Non-reentrancy guard of a workspace: try-lock semantics, BUSY on contention.

@@ -1219,10 +1219,14 @@ void rkh_set_marker(rkh_marker_fn fn, void* user) {
     g_marker_on.store(fn != nullptr, std::memory_order_release);
 }
 
-int rkh_enter_device(int device) {
-    int before = -1;
-    if (hipGetDevice(&before) != hipSuccess || before == device || hipSetDevice(device) != hipSuccess) return -1;
-    return before;
+int rkh_enter_device(int device, int* before) {
+    int now = -1;
+    *before = -1;
+    RKH_CHECK(hipGetDevice(&now));
+    if (now == device) return RKH_OK;
+    RKH_CHECK(hipSetDevice(device));
+    *before = now;
+    return RKH_OK;
 }
 void rkh_leave_device(int before) {
     if (before >= 0) (void)hipSetDevice(before);

@@ -10,7 +10,7 @@ static int g_launches;
 
 extern "C" {
 int rkh_heads(void*, const rkh_heads_args*) { return ++g_launches, RKH_OK; }
-int rkh_enter_device(int) { return -1; }
+int rkh_enter_device(int, int* before) { return *before = -1, RKH_OK; }
 void rkh_leave_device(int) {}
 }
 
