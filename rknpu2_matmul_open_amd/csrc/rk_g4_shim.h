@@ -64,6 +64,8 @@ int rkh_g4_run(void* stream, const rkh_g4_args* args);
 /* What rkh_g4_run does for a shape, by arithmetic alone: the kernel (0: few rows, 1: tiles), rows and columns (SwiGLU: of both halves) of a
  * workgroup and the parts that K is split into.  N as in the args. */
 void rkh_g4_route(int M, int N, int K, int gpb, int swiglu, int* kernel, int* rows, int* columns, int* parts);
+/* ... and of up to 16 rows which few-row kernel: rows that it is made for (0: it loads operands), columns and waves of a workgroup, and whether a wave loads more than once. */
+void rkh_g4_few_route(int M, int N, int K, int gpb, int swiglu, int* rows, int* columns, int* waves, int* again);
 size_t rkh_g4_scratch_bytes(int M, int N, int K, int gpb, int swiglu);
 /* ... and the most that any product of up to max_rows rows of K values needs. */
 size_t rkh_g4_scratch_most(int max_rows, int K);

@@ -310,8 +310,20 @@ FewShape few_shape(int M, int64_t blocks, int KB, int gpb, bool swiglu) {
     return {rows, cn, rows == 16 ? shared ? 4 : 8 : cn == 2 || (shared && (rows == 8 || gpb == 4)) || (rows == 8 && gpb == 4) ? 8 : 16};
 }
 
-template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, int per) {
-    const int KB = (int)rkh_g4_kb(g.K), waves = (KB + per - 1) / per;
+// ... and its waves: pieces of K that one loads together, and has in all.
+struct FewPlan {
+    FewShape shape;
+    int together, per, waves;
+};
+FewPlan few_plan(int M, int64_t blocks, int KB, int gpb, bool swiglu) {
+    const FewShape shape = few_shape(M, blocks, KB, gpb, swiglu);
+    // pieces of a wave: up to four (as operands: two) that are loaded together, eight waves where they go round, and as many as there are waves for
+    const int together = shape.rows ? 4 : 2, per = std::max((KB + shape.most - 1) / shape.most, std::min(together, (KB + 7) / 8));
+    return {shape, together, per, (KB + per - 1) / per};
+}
+
+template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, int MAX_WAVES> int launch_few(hipStream_t st, const rkh_g4_args& g, const FewPlan& plan) {
+    const int per = plan.per, waves = plan.waves;
     const int64_t workgroups = rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / (16 * CN);
     if (workgroups * waves * 64 >= MX_TOO_MANY_THREADS) return RKH_ERR_RUNTIME;
     constexpr size_t BYTES = few_area(ROWS, CN); // of a wave
@@ -326,23 +338,21 @@ template <int TYPE, int CN, int GPB, int ROWS, bool SWIGLU, bool LONG, int NP, i
     return RKH_OK;
 }
 template <int TYPE, int GPB, bool SWIGLU> int launch_few(hipStream_t st, const rkh_g4_args& g) {
-    const int KB = (int)rkh_g4_kb(g.K);
-    const FewShape shape = few_shape(g.M, rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / 16, KB, GPB, SWIGLU);
-    // pieces of a wave: up to four (as operands: two) that are loaded together, eight waves where they go round, and as many as there are waves for
-    const int np = shape.rows ? 4 : 2, per = std::max((KB + shape.most - 1) / shape.most, std::min(np, (KB + 7) / 8));
+    const FewPlan plan = few_plan(g.M, rkh_g4_places(SWIGLU ? 2 * (int64_t)g.N : g.N, SWIGLU) / 16, (int)rkh_g4_kb(g.K), GPB, SWIGLU);
+    const FewShape& shape = plan.shape;
     const auto go = [&](auto is_long) {
         constexpr bool LONG = decltype(is_long)::value;
-        if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, LONG, 2, GPB == 4 ? 8 : 16>(st, g, per);
+        if (!shape.rows) return launch_few<TYPE, 4, GPB, 0, SWIGLU, LONG, 2, GPB == 4 ? 8 : 16>(st, g, plan);
         constexpr int CN = SWIGLU ? 2 : 1, MOST = SWIGLU ? 8 : 16;
-        if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, LONG, 4, MOST>(st, g, per);
+        if (shape.rows == 1) return launch_few<TYPE, CN, GPB, 1, SWIGLU, LONG, 4, MOST>(st, g, plan);
         if constexpr (!SWIGLU && !LONG) {
-            if (shape.cn == 2) return launch_few<TYPE, 2, GPB, 4, SWIGLU, LONG, 4, 8>(st, g, per);
+            if (shape.cn == 2) return launch_few<TYPE, 2, GPB, 4, SWIGLU, LONG, 4, 8>(st, g, plan);
         }
-        if (shape.rows == 4) return launch_few<TYPE, CN, GPB, 4, SWIGLU, LONG, 4, MOST>(st, g, per);
-        if (shape.rows == 8) return launch_few<TYPE, CN, GPB, 8, SWIGLU, LONG, 4, GPB == 4 ? 8 : MOST>(st, g, per);
-        return launch_few<TYPE, CN, GPB, 16, SWIGLU, LONG, 4, 8>(st, g, per);
+        if (shape.rows == 4) return launch_few<TYPE, CN, GPB, 4, SWIGLU, LONG, 4, MOST>(st, g, plan);
+        if (shape.rows == 8) return launch_few<TYPE, CN, GPB, 8, SWIGLU, LONG, 4, GPB == 4 ? 8 : MOST>(st, g, plan);
+        return launch_few<TYPE, CN, GPB, 16, SWIGLU, LONG, 4, 8>(st, g, plan);
     };
-    return per > np ? go(std::true_type{}) : go(std::false_type{});
+    return plan.per > plan.together ? go(std::true_type{}) : go(std::false_type{});
 }
 template <int TYPE> int launch_few(hipStream_t st, const rkh_g4_args& g) {
     if (g.swiglu) return g.gpb == 1 ? launch_few<TYPE, 1, true>(st, g) : g.gpb == 2 ? launch_few<TYPE, 2, true>(st, g) : launch_few<TYPE, 4, true>(st, g);
@@ -461,6 +471,10 @@ void rkh_g4_route(int M, int N, int K, int gpb, int swiglu, int* kernel, int* ro
     }
     const rkk::G4Route r = g4_route(M, N, K, gpb, swiglu);
     *kernel = 1, *rows = 32 * r.rm, *columns = 128, *parts = r.parts;
+}
+void rkh_g4_few_route(int M, int N, int K, int gpb, int swiglu, int* rows, int* columns, int* waves, int* again) {
+    const FewPlan plan = few_plan(M, rkh_g4_places(swiglu ? 2 * (int64_t)N : N, swiglu) / 16, (int)rkh_g4_kb(K), gpb, swiglu != 0);
+    *rows = plan.shape.rows, *columns = 16 * plan.shape.cn, *waves = plan.waves, *again = plan.per > plan.together;
 }
 size_t rkh_g4_scratch_bytes(int M, int N, int K, int gpb, int swiglu) { return M <= FEW_ROWS ? 0 : g4_scratch(g4_route(M, N, K, gpb, swiglu)); }
 // (g4_route: a part for each compute unit at most, tiles no larger than the rows ask for)
