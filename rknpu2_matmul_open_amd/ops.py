@@ -606,8 +606,8 @@ class G4Weights:
         device, groups = _device_of(session) if on_device else None, -(-K // group)
         if scale_type is None:
             scale_type = _G4_HALVES.get(str(scales.dtype))
-        if scale_type is None:
-            raise TypeError("scales of float16 or bfloat16: got %s" % scales.dtype)
+        if scale_type not in (capi.MX4_F16, capi.MX4_BF16):
+            raise TypeError("scales of float16 or bfloat16: got %s%s" % (scales.dtype, "" if scale_type is None else ", scale_type %r" % (scale_type,)))
         kinds = {capi.MX4_F16: ("torch.float16", "float16", "uint16"), capi.MX4_BF16: ("torch.bfloat16", "uint16")}[scale_type]
         p = _g4_array(codes, (N, -(-K // 2)), ("torch.uint8", "uint8"), "codes", device)
         s = _g4_array(scales, (N, groups), kinds, "scales", device)
