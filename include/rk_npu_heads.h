@@ -8,7 +8,8 @@
  *         phi = positions[axis of i][t] * inv_freq[i]
  *         a' = rotation_scale * (a cos phi - b sin phi),   b' = rotation_scale * (b cos phi + a sin phi)
  *     z[R] .. z[D - 1] as they are
- * computed in fp32 and rounded once.  The angle is reduced in fp64: far positions (all 32 bits) are off by 2^-21 at most.
+ * computed in fp32 and rounded once.  The angle is made and reduced in fp64 and then rounded to fp32: off by less than 2^-23 near zero, and by less than 2^-20 for
+ * positions of all 32 bits, where inv_freq is 1 or less (products beyond 2^31 lose bits of the angle as fp64 does).
  * Squares are added in fp32, without scaling; a NaN makes its head NaN where there is a norm, and otherwise the pair.
  *
  * Positions have up to four axes (time, height, width, ..), and a table says by which one a pair is turned: sections of pairs one behind

@@ -45,7 +45,7 @@ __device__ __forceinline__ void g4_product_first(const v4i& a, const v4i& w, v16
     asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(sum) : "a"(a), "v"(w));
 }
 __device__ __forceinline__ void g4_add_scaled(float& acc, float sum, float scale) { asm volatile("v_fmac_f32_e32 %0, %1, %2" : "+v"(acc) : "v"(sum), "v"(scale)); }
-// g4_pair; `magic` is 0x64006400 in a vector register.  (One statement: between two of them the compiler puts a wait state for a hazard that these
+// Pair R of g4_halves; `magic` is g4_exponents.  (One statement: between two of them the compiler puts a wait state for a hazard that these
 // instructions do not have.)  R = 2 leaves the codes, shifted by eight bits, in `upper` for R = 3.
 template <int R> __device__ __forceinline__ uint32_t g4_pair_here(uint32_t w, const G4Zero& z, uint32_t magic, uint32_t& upper) {
     uint32_t v;

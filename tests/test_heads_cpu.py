@@ -14,8 +14,8 @@ CSRC = os.path.join(ROOT, "rknpu2_matmul_open_amd", "csrc")
 @pytest.fixture(scope="module")
 def answers(tmp_path_factory):
     exe = tmp_path_factory.mktemp("heads") / "heads_calls"
-    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=undefined", "-I" + CSRC, "-I" + os.path.join(ROOT, "include"), "-o", str(exe),
-                           os.path.join(ROOT, "tests", "heads_calls_cpu.cpp"), os.path.join(CSRC, "rk_heads.cpp")])
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=undefined", "-I" + CSRC, "-I" + os.path.join(ROOT, "include"),
+                           "-o", str(exe), os.path.join(ROOT, "tests", "heads_calls_cpu.cpp"), os.path.join(CSRC, "rk_heads.cpp")])
 
     def ask(cases):
         text = "\n".join(" ".join(map(str, c)) for c in cases)
