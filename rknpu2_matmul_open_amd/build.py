@@ -66,9 +66,9 @@ def check_toolchain(hipcc):
 
 
 def build(verbose=True, audit=True):
-    """Compiles and links the library.  audit: also compile the two inline-assembly load units to
-    device assembly (alongside the objects) and check the hand-placed waits in it, see
-    audit_waits.py; a violation fails the build (RK_NPU_HIP_SKIP_WAIT_AUDIT=1 skips the check)."""
+    """Compiles and links the library.  audit: also compile the inline-assembly units to
+    device assembly (alongside the objects) and check the hand-placed waits in it, and the 64-bit shifts of the
+    linked library, see audit_waits.py; a violation fails the build (RK_NPU_HIP_SKIP_WAIT_AUDIT=1 skips the checks)."""
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     check_toolchain(hipcc)
     audit = audit and os.environ.get("RK_NPU_HIP_SKIP_WAIT_AUDIT") != "1"
@@ -114,8 +114,20 @@ def build(verbose=True, audit=True):
                                % (len(violations), checked))
         if verbose:
             sys.stderr.write("[build] wait audit: %d kernels, no violation\n" % checked)
-    cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-lpthread"]
+    linked = LIB + ".new"
+    cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", linked] + objs + ["-lpthread"]
     subprocess.check_call(cmd)
+    if audit:
+        violations, checked = audit_waits.audit_shifts(linked)
+        if violations or not checked:
+            for line in violations[:20]:
+                sys.stderr.write("[build] shift audit: %s\n" % line)
+            os.remove(linked)
+            raise RuntimeError("shift audit: %d 64-bit shifts in %d kernels take their amount from a wave's last register"
+                               % (len(violations), checked))
+        if verbose:
+            sys.stderr.write("[build] shift audit: %d kernels, no violation\n" % checked)
+    os.replace(linked, LIB)
     return LIB
 
 

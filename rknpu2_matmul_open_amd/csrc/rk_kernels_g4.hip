@@ -161,12 +161,16 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
     // ahead of the codes' loads.)
     const auto fetch = [&](int m, int k) { return mx_fetch8<TYPE>(x, (size_t)m * ldx + min(k, K - 8)).w[0]; };
     const auto within = [&](const v4i& v, int k) { return k < K ? HALVES ? v : g4_turned_rows(v) : v4i{0, 0, 0, 0}; };
-    const auto moved = [&](const v4i& v, int k) { // where K ends within eight values: the last eight to their places
-        const int beyond = k < K ? max(k + 8 - K, 0) : 0, bits = 16 * (beyond & 3);
-        uint64_t low = (uint64_t)(uint32_t)v.y << 32 | (uint32_t)v.x, high = (uint64_t)(uint32_t)v.w << 32 | (uint32_t)v.z;
-        if (beyond >= 4) low = high, high = 0;
-        low = low >> bits | (high << 1) << (63 - bits), high >>= bits;
-        return v4i{(int)low, (int)(low >> 32), (int)high, (int)(high >> 32)};
+    // Where K ends within eight values: the last eight to their places, by four values, by two and by one.  (A 64-bit shift by a register reads a pair of registers
+    // for the amount; where that is the last one a wave has, it reads v0 instead: rows of 4140 values were shifted by the lane's number.  audit_waits looks for these.)
+    const auto moved = [&](v4i v, int k) {
+        const int beyond = k < K ? max(k + 8 - K, 0) : 0;
+        const bool four = beyond & 4, two = beyond & 2;
+        v = v4i{four ? v.z : v.x, four ? v.w : v.y, four ? 0 : v.z, four ? 0 : v.w};
+        v = v4i{two ? v.y : v.x, two ? v.z : v.y, two ? v.w : v.z, two ? 0 : v.w};
+        const uint32_t bits = (beyond & 1) * 16;
+        return v4i{(int)__builtin_amdgcn_alignbit((uint32_t)v.y, (uint32_t)v.x, bits), (int)__builtin_amdgcn_alignbit((uint32_t)v.z, (uint32_t)v.y, bits),
+                   (int)__builtin_amdgcn_alignbit((uint32_t)v.w, (uint32_t)v.z, bits), (int)((uint32_t)v.w >> bits)};
     };
     const auto load = [&](Batch& b, int from) { // (pieces beyond the last: that one again, which is not multiplied)
         if constexpr (ROWS) {
@@ -210,14 +214,14 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void g4_few_kernel(const uint8_t* W
                     __builtin_amdgcn_wave_barrier();
                 }
             }
-            v4i a[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (ROWS) a[i] = *reinterpret_cast<const v4i*>(own + row * FEW_PITCH + (p & 3) * 256 + i * 64 + q * 16);
-                else a[i] = within(b.x[p * 4 + i], (from + p) * 128 + i * 32 + q * 8);
-            }
 #pragma unroll
             for (int n = 0; n < GPB; ++n) {
+                v4i a[4];
+#pragma unroll
+                for (int i = n * STEPS; i < (n + 1) * STEPS; ++i) {
+                    if constexpr (ROWS) a[i] = *reinterpret_cast<const v4i*>(own + row * FEW_PITCH + (p & 3) * 256 + i * 64 + q * 16);
+                    else a[i] = within(b.x[p * 4 + i], (from + p) * 128 + i * 32 + q * 8);
+                }
                 v4f sum = {0, 0, 0, 0};
                 if constexpr (!HALVES) {
 #pragma unroll
