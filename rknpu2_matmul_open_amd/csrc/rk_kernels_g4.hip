@@ -129,8 +129,8 @@ __global__ __launch_bounds__(256) void g4_stage_kernel(const uint16_t* x, int64_
 // registers, once; so do activations, which every workgroup reads for itself.
 // ROWS (1, 4, 8 or 16): up to so many rows.  A wave loads a row's 512 values together and turns them into operands through LDS of its own.  0: up to 16 rows,
 // loaded as the operands lie.
-// One row is bound by the weights' way from HBM (1 x 14336 x 4096 7.2 us where caches help, 7.7 where they do not: 4 TB/s), more rows by the activations' from L2 as well
-// (8 x 4096 x 14336 8.9 to 10.6).
+// One row is bound by the weights' way from HBM (1 x 14336 x 4096 7.2 us where caches help, 7.8 to 8.1 where they do not: 3.8 TB/s, where a launch that only reads takes 5.9),
+// more rows by the activations' from L2 as well (8 x 4096 x 14336 8.9, 11.1).
 // fp16 rows are multiplied with code - zero.  bf16 rows with the code, and the zero point times the group's sum of activations, which a product with ones gives, is taken off
 // a group's sum: bf16 has no packed additions, so that code - zero takes 17 instructions for eight weights by way of fp32, not 7, and one row x 14336 x 4096
 // 8.7 us and not 7.8, SwiGLU of it 15.2 and not 13.1, 8 x 4096 x 14336 11.6 and not 11.1.
